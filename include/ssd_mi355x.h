@@ -191,6 +191,81 @@ int ssd_tree_attention_bf16(const uint16_t* q, int64_t ldq, int M, int heads, in
                             float scale, float* ws, int64_t ws_floats, uint16_t* out, int64_t ldo,
                             hipStream_t stream);
 
+/* ---------------------------------------------------------- 8-bit KV cache
+ * One layer of a batch of sequences' caches. Every row (sequence, slot, kv head) of K and of V is
+ * head_dim e4m3 codes and one exponent byte b: value = code * 2^(b - 127), the least power of two that
+ * keeps the row's largest finite magnitude within 448 (b >= 27), so a row rounds once, to four
+ * significant bits, and its stored values are bf16 values. Values that are not finite are stored as NaN.
+ * k, v: [n_seq][kv_heads] regions of max_len * head_dim bytes; k_exp, v_exp: regions of max_len bytes;
+ * max_len a multiple of 64, head_dim 64 or 128, all arrays 16-byte aligned. A region is a sequence of
+ * 64-slot blocks in the attention's operand order, offsets of slot s (within the region):
+ *   K[s][d]: ((s/16)*(hd/64) + d/64)*1024 + (((d/16)%4)*16 + s%16)*16 + d%16;
+ *   V[s][d]: ((s/64)*(hd/16) + d/16)*1024 + (((s/4)%4)*16 + d%16)*16 + ((s/32)%2)*8 + ((s/16)%2)*4 + s%4;
+ *   exponent: (s/64)*64 + ((s/4)%4)*16 + ((s/16)%4)*4 + s%4.
+ * (Python: ssd.engine.kv_cache.KVCacheQ8.) The reference keeps a bf16 cache for one sequence
+ * (ssd/engine/kv_cache.py:21-73). Host struct, read during the call only. */
+typedef struct SsdKvQ8 {
+  uint8_t* k;
+  uint8_t* v;
+  uint8_t* k_exp;
+  uint8_t* v_exp;
+  int32_t n_seq, kv_heads, head_dim;
+  int64_t max_len;
+} SsdKvQ8;
+
+/* Rotary positions: fp32 tables [rows][rot_dim / 2] of cos and sin (scaling for long contexts lives in
+ * the tables). The first rot_dim (a multiple of 16) dims of a head turn in pairs (i, i + rot_dim / 2),
+ * or (2i, 2i + 1) when interleaved; the rest stay. Positions outside [0, rows) use the nearest row.
+ * Generalises the rotate_half RoPE of ssd/models/subnetwork_draft.py:213,218. */
+typedef struct SsdRope {
+  const float* cos;
+  const float* sin;
+  int64_t rows;
+  int32_t rot_dim, interleaved;
+} SsdRope;
+
+/* y[m] = x[m] rotated to row_pos[m], heads of head_dim (64 or 128), products in fp32, one rounding to bf16.
+ * y may be x. Rows 16-byte aligned. M = 0 does nothing. */
+int ssd_rope_bf16(const SsdRope* rope, const int32_t* row_pos, const uint16_t* x, int64_t ldx, int M, int heads,
+                  int head_dim, uint16_t* y, int64_t ldy, hipStream_t stream);
+
+/* Row m's K (rotated in fp32 first when rope is given) and V of every kv head quantised into the cache at
+ * (row_seq[m], row_slot[m]); rows outside the cache are not written. The rows of one call name different
+ * places. With q: its rows are rotated into q_out in the same launch (copied without rope). rope, row_pos and q
+ * may be NULL (rope and row_pos together). M = 0 does nothing. The 8-bit counterpart of
+ * KVCache.update (ssd/engine/kv_cache.py:32-43). */
+int ssd_kv_q8_write_bf16(const SsdKvQ8* cache, const uint16_t* k, int64_t ldk, const uint16_t* v, int64_t ldv, int M,
+                         const int32_t* row_seq, const int32_t* row_slot, const SsdRope* rope, const int32_t* row_pos,
+                         const uint16_t* q, int64_t ldq, int heads, uint16_t* q_out, int64_t ldo, hipStream_t stream);
+
+/* The stored values of (row_seq[m], row_slot[m]) as bf16 rows [kv_heads * head_dim]: exact; zeros for
+ * places outside the cache. M = 0 does nothing. */
+int ssd_kv_q8_read_bf16(const SsdKvQ8* cache, int M, const int32_t* row_seq, const int32_t* row_slot, uint16_t* k,
+                        int64_t ldk, uint16_t* v, int64_t ldv, hipStream_t stream);
+
+/* KVCache.keep_positions (ssd/engine/kv_cache.py:54-70) for a batch: in every layer (the cache's arrays hold `layers`
+ * layers back to back) sequence s's slots src[s][0 .. n[s]) move to [start[s], start[s] + n[s]), all sources read
+ * before any destination is written, codes and exponents as they are. n[s] counts up to n_max <= 64 are
+ * followed, moves from or to slots outside the cache are skipped. start, n: [n_seq]; src: [n_seq][n_max]. */
+int ssd_kv_q8_compact(const SsdKvQ8* cache, int layers, const int32_t* start, const int32_t* src, const int32_t* n,
+                      int n_max, hipStream_t stream);
+
+/* Tree attention over the 8-bit cache for a batch: sequence s owns rows [row_begin[s], row_begin[s + 1]) (device
+ * int32 [n_seq + 1], increasing, at most rows_max <= 64 rows each), and row t attends slots [0, prefix[t]) then
+ * anc[t][0 .. depth[t]) of its sequence, as ssd_tree_attention_bf16 does. A row that attends nothing gets zeros;
+ * rows outside [row_begin[0], row_begin[n_seq]) are left as they were. l_max >= every prefix + depth (host bound;
+ * keys at logical positions from l_max on are not attended). Keys are folded in a fixed order: within a span of
+ * `span` logical positions (a multiple of 64) block by block, then span by span, so a row's result depends on
+ * its query, its keys and span alone -- not on the other rows, the other sequences or the slots its ancestors
+ * sit in: a verify row equals the autoregressive step at its position bit for bit.
+ * heads / kv_heads any whole ratio. ws: ssd_attn_q8_ws_floats(...) floats, 16-byte aligned, no clearing needed; calls
+ * that overlap in time must not share it. */
+int64_t ssd_attn_q8_ws_floats(int M, int heads, int head_dim, int64_t l_max, int span);
+int ssd_tree_attention_q8(const SsdKvQ8* cache, const uint16_t* q, int64_t ldq, int M, int heads, const int32_t* row_begin,
+                          const int32_t* prefix, const int32_t* depth, const int32_t* anc, int rows_max, int l_max,
+                          int span, float scale, float* ws, int64_t ws_floats, uint16_t* out, int64_t ldo,
+                          hipStream_t stream);
+
 /* ---------------------------------------------------------------- rows */
 /* HF LlamaRMSNorm / bridge RMSNorm (ssd/models/bridges.py:33-37; subnetwork_draft.py:216,245,344). */
 int ssd_rmsnorm_bf16(const uint16_t* x, int64_t ldx, int M, int D, const uint16_t* w, float eps, uint16_t* y,
@@ -367,6 +442,23 @@ int ssd_accept_sample(const SsdTree* tree, const float* P, int64_t ldp, const fl
                       int rows, int max_kids, uint64_t seed, uint64_t counter, void* ws, int64_t ws_bytes,
                       int committed, int32_t* result, int32_t* keep_src, int32_t* n_keep, int32_t* root_token,
                       hipStream_t stream);
+
+/* Speculative verification of one drafted chain per sequence from given random numbers (sample_verify,
+ * ssd/engine/verify.py:60-95, with one child per node, for a batch). P: target rows, row i of sequence s at
+ * P + s * ldp_seq + i * ldp (i <= k_max), Q: draft rows (i < k_max) alike; fp32, nonnegative, V columns, need not
+ * be normalised as long as P and Q rows have the same mass. draft[s][i] (row stride k_max) is the i-th drafted
+ * token, n_draft[s] (NULL: k_max; clamped to [0, k_max]) their count. Token i is accepted while
+ * u[s][i] * Q_i[x_i] < P_i[x_i] (products of 64 bits; a token outside [0, V) is refused). After n accepted tokens
+ * the next one is drawn from max(P_n - Q_n, 0) -- from P_n when every draft was accepted or that has no mass --
+ * as the least y whose cumulative mass exceeds u_next[s] * total, all sums in 64 bits; a row without mass gives
+ * -1. out_n[s] = n; out_tok[s][k_max + 1] = the accepted tokens, the next one, then -1.
+ * ws: ssd_verify_chain_ws_bytes(n_seq, V) bytes, 8-byte aligned, no clearing needed; calls that overlap in time
+ * must not share it. k_max <= 64, V <= 2^24. */
+int64_t ssd_verify_chain_ws_bytes(int n_seq, int V);
+int ssd_verify_chain(const float* P, int64_t ldp_seq, int64_t ldp, const float* Q, int64_t ldq_seq, int64_t ldq, int V,
+                     int n_seq, int k_max, const int32_t* draft, const int32_t* n_draft, const float* u,
+                     const float* u_next, void* ws, int64_t ws_bytes, int32_t* out_tok, int32_t* out_n,
+                     hipStream_t stream);
 
 /* Batched acceptance trials for the statistical check of the acceptance rule at scale (no
  * counterpart in the reference, whose loop is verify.py:60-95 on the CPU): `trials` independent

@@ -86,6 +86,15 @@ class SsdPrefillBuffers(C.Structure):
         ("cache_cap", I64), ("logits", P)]
 
 
+class SsdKvQ8(C.Structure):
+    _fields_ = [(n, P) for n in ("k", "v", "k_exp", "v_exp")] + [("n_seq", C.c_int32), ("kv_heads", C.c_int32),
+                                                                ("head_dim", C.c_int32), ("max_len", I64)]
+
+
+class SsdRope(C.Structure):
+    _fields_ = [("cos", P), ("sin", P), ("rows", I64), ("rot_dim", C.c_int32), ("interleaved", C.c_int32)]
+
+
 _PROTOS = {
     "ssd_last_error": (C.c_char_p, []),
     "ssd_abi_version": (I32, []),
@@ -106,6 +115,14 @@ _PROTOS = {
     "ssd_attn_max_depth": (I32, []),
     "ssd_tree_attention_bf16": (I32, [P, I64, I32, I32, I32, I32, P, P, I64, P, P, P, I32, I32, F32, P, I64, P,
                                       I64, P]),
+    "ssd_rope_bf16": (I32, [C.POINTER(SsdRope), P, P, I64, I32, I32, I32, P, I64, P]),
+    "ssd_kv_q8_write_bf16": (I32, [C.POINTER(SsdKvQ8), P, I64, P, I64, I32, P, P, C.POINTER(SsdRope), P, P, I64, I32, P,
+                                   I64, P]),
+    "ssd_kv_q8_read_bf16": (I32, [C.POINTER(SsdKvQ8), I32, P, P, P, I64, P, I64, P]),
+    "ssd_kv_q8_compact": (I32, [C.POINTER(SsdKvQ8), I32, P, P, P, I32, P]),
+    "ssd_attn_q8_ws_floats": (I64, [I32, I32, I32, I64, I32]),
+    "ssd_tree_attention_q8": (I32, [C.POINTER(SsdKvQ8), P, I64, I32, I32, P, P, P, P, I32, I32, I32, F32, P, I64, P,
+                                    I64, P]),
     "ssd_rmsnorm_bf16": (I32, [P, I64, I32, I32, P, F32, P, I64, P]),
     "ssd_embed_bf16": (I32, [P, I32, P, I64, I32, P, I64, P]),
     "ssd_kv_compact_bf16": (I32, [P, P, I32, I32, I32, I64, I32, P, P, I32, P, P]),
@@ -141,6 +158,8 @@ _PROTOS = {
     "ssd_sample_top64_bf16": (I32, [P, I64, I32, I32, F32, F32, U64, U64, P, P, I64, P]),
     "ssd_accept_sample": (I32, [C.POINTER(SsdTree), P, I64, P, I64, I32, I32, I32, U64, U64, P, I64, I32, P, P, P, P,
                                 P]),
+    "ssd_verify_chain_ws_bytes": (I64, [I32, I32]),
+    "ssd_verify_chain": (I32, [P, I64, I64, P, I64, I64, I32, I32, I32, P, P, P, P, P, I64, P, P, P]),
     "ssd_accept_sample_trials": (I32, [P, I64, P, I64, I32, P, P, I32, C.POINTER(C.c_int32), U64, U64, I32, P, P, P]),
     "ssd_forward": (I32, [C.POINTER(SsdModel), C.POINTER(SsdPlan), C.POINTER(SsdBuffers), C.POINTER(SsdRows), I32,
                           I32, I32, I32, I32, P]),

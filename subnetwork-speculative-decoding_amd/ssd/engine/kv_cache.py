@@ -19,7 +19,7 @@ from typing import Optional
 
 import torch
 
-from ssd import ops
+from ssd import _lib, ops
 
 
 class KVCache:
@@ -108,3 +108,108 @@ class KVCache:
 
     def reset(self) -> None:
         self.seq_len = 0
+
+
+class KVCacheQ8:
+    """KV caches of ``sequences`` sequences in 8 bits: e4m3 codes and one power-of-two exponent per (slot, kv head) of
+    K and of V, 2 * (head_dim + 1) bytes a slot and head against the bf16 cache's 4 * head_dim. Arrays
+    [layers, sequences, kv_heads, capacity * head_dim] (codes) and [..., capacity] (exponents), capacity the next
+    multiple of 64, in the operand order documented at SsdKvQ8 in the C header. head_dim 64 or 128.
+
+    Rows are quantised as they are written (``write``, K rotated in the same launch), every stored value is a bf16
+    value, so ``read`` returns exactly what ``attend`` uses. Lengths are the caller's: rows name their sequence and slot.
+    ``span`` (keys per record of the attention, a multiple of 64) is part of the arithmetic: rows of two caches agree
+    bit for bit when their keys, queries and spans do. None: ``default_span``."""
+
+    def __init__(self, num_slots: int, max_length: int, kv_heads: int, head_dim: int, device, sequences: int = 1,
+                 span: Optional[int] = None):
+        if head_dim not in (64, 128):
+            raise ValueError(f"KVCacheQ8: head_dim {head_dim} unsupported (64, 128)")
+        if min(num_slots, max_length, kv_heads, sequences) < 1:
+            raise ValueError("KVCacheQ8: layers, max_length, kv_heads and sequences must be positive")
+        if span is not None and (span < 64 or span % 64):
+            raise ValueError(f"KVCacheQ8: span {span} must be a multiple of 64")
+        self.num_slots, self.max_length = num_slots, max_length
+        self.kv_heads, self.head_dim, self.sequences = kv_heads, head_dim, sequences
+        self.capacity = (max_length + 63) // 64 * 64
+        self.span = self.default_span(sequences, kv_heads, self.capacity) if span is None else span
+        lead = (num_slots, sequences, kv_heads)
+        codes = dict(dtype=torch.uint8, device=device)
+        self.k = torch.zeros(*lead, self.capacity * head_dim, **codes)
+        self.v = torch.zeros_like(self.k)
+        self.k_exp = torch.full((*lead, self.capacity), 127, **codes)
+        self.v_exp = torch.full_like(self.k_exp, 127)
+        self.device = self.k.device
+        self._layers = [_lib.SsdKvQ8(self.k[i].data_ptr(), self.v[i].data_ptr(), self.k_exp[i].data_ptr(),
+                                     self.v_exp[i].data_ptr(), sequences, kv_heads, head_dim, self.capacity)
+                        for i in range(num_slots)]
+        for d in self._layers:
+            d.device = self.device
+
+    @staticmethod
+    def default_span(sequences: int, kv_heads: int, capacity: int) -> int:
+        return 256
+
+    def layer(self, i: int) -> _lib.SsdKvQ8:
+        """The descriptor of layer ``i`` for the ops that take a cache."""
+        return self._layers[i]
+
+    def write(self, i: int, k: torch.Tensor, v: torch.Tensor, seq: torch.Tensor, slot: torch.Tensor, rope=None, pos=None,
+              interleaved: bool = False, q: Optional[torch.Tensor] = None,
+              q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+        """Rows k, v [M, kv_heads * head_dim] (any row stride) into layer ``i`` at (seq[m], slot[m]) (int32 on the device,
+        all places different; rows outside the cache are not written). ``rope``: (cos, sin) tables of
+        ``models.llama.rope_tables_f32``, K rotated to ``pos`` before it is quantised; with ``q`` [M, heads * head_dim]
+        its rows are rotated too and returned (in ``q_out`` if given, which may be ``q``)."""
+        heads = 0
+        if q is not None:
+            heads = q.shape[1] // self.head_dim
+            if q.shape[1] % self.head_dim:
+                raise ValueError(f"q has {q.shape[1]} columns, not a multiple of head_dim {self.head_dim}")
+            if q_out is None:
+                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        ops.kv_q8_write(self._layers[i], k, v, k.shape[0], seq, slot, rope, pos, interleaved, q, heads, q_out)
+        return q_out
+
+    def load(self, i: int, cache: KVCache, length: int, seq: int = 0, start: int = 0) -> None:
+        """Slots [start, length) of a bf16 cache's layer ``i`` (a prompt's, after its prefill) into sequence ``seq``."""
+        if not 0 <= start <= length <= self.max_length or not 0 <= seq < self.sequences:
+            raise ValueError(f"KVCacheQ8.load: slots [{start}, {length}) or sequence {seq} outside the cache")
+        k, v = (x[:, start:].transpose(0, 1).flatten(1) for x in cache.read(i, length))
+        slot = torch.arange(start, length, dtype=torch.int32, device=self.device)
+        self.write(i, k, v, torch.full_like(slot, seq), slot)
+
+    def read(self, i: int, seq: torch.Tensor, slot: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        """K, V [M, kv_heads * head_dim] bf16 of layer ``i`` at (seq[m], slot[m]); zeros for places outside the cache."""
+        m, cols = seq.numel(), self.kv_heads * self.head_dim
+        k, v = torch.empty(2, m, cols, dtype=torch.bfloat16, device=self.device)
+        ops.kv_q8_read(self._layers[i], m, seq, slot, k, v)
+        return k, v
+
+    def attend_floats(self, m: int, heads: int, l_max: int) -> int:
+        """Workspace floats of ``attend`` for ``m`` rows."""
+        return ops.attn_q8_ws_floats(m, heads, self.head_dim, l_max, self.span)
+
+    def attend(self, i: int, q: torch.Tensor, row_begin: torch.Tensor, prefix: torch.Tensor, depth: torch.Tensor,
+               anc: torch.Tensor, rows_max: int, l_max: int, out: Optional[torch.Tensor] = None,
+               ws: Optional[torch.Tensor] = None, scale: Optional[float] = None) -> torch.Tensor:
+        """Tree attention of q [M, heads * head_dim] over layer ``i``: sequence s owns rows row_begin[s] ..
+        row_begin[s + 1] (at most rows_max <= 64), row t attends slots [0, prefix[t]) then anc[t, :depth[t]]; zeros for
+        rows that attend nothing; rows of no sequence are left as ``out`` has them. l_max bounds prefix + depth. ``ws``: fp32, attend_floats(M, heads, l_max) (None: allocated here)."""
+        m, cols = q.shape
+        if cols % self.head_dim:
+            raise ValueError(f"q has {cols} columns, not a multiple of head_dim {self.head_dim}")
+        if out is None:
+            out = torch.empty(m, cols, dtype=q.dtype, device=q.device)
+        if ws is None:
+            ws = torch.empty(max(self.attend_floats(m, cols // self.head_dim, l_max), 4), dtype=torch.float32,
+                             device=q.device)
+        return ops.tree_attention_q8(self._layers[i], q, m, cols // self.head_dim, row_begin, prefix, depth, anc, rows_max,
+                                     l_max, self.span, ws, out, scale)
+
+    def compact_device(self, start: torch.Tensor, src: torch.Tensor, n: torch.Tensor) -> None:
+        """In every layer, sequence s's slots src[s, :n[s]] move to [start[s], start[s] + n[s]) (int32 on the device; src
+        [sequences, n_max <= 64]): the accepted paths of a verified batch, one launch."""
+        if src.dim() != 2 or src.shape[0] != self.sequences:
+            raise ValueError(f"src must be [{self.sequences}, n_max], got {tuple(src.shape)}")
+        ops.kv_q8_compact(self._layers[0], self.num_slots, start, src, n, src.shape[1])

@@ -8,6 +8,8 @@ tree). These functions keep the reference's host-level signatures for callers th
 
 from __future__ import annotations
 
+from typing import Optional
+
 import torch
 
 from ssd import ops
@@ -98,3 +100,24 @@ def sample_verify(tree: DraftTree, target_logits: torch.Tensor, temperature: flo
     n_new = r[0]
     accepted = [s - 1 for s in keep_src[1:n_new].tolist()]
     return accepted, r[n_new]
+
+
+def verify_chain(P: torch.Tensor, Q: torch.Tensor, draft: torch.Tensor, u: torch.Tensor, u_next: torch.Tensor,
+                 n_draft: Optional[torch.Tensor] = None, ws: Optional[torch.Tensor] = None) -> tuple:
+    """Speculative verification of a batch of drafted chains from given random numbers, on the device and without a
+    host round trip (``ssd_verify_chain``; sample_verify with one child per node). P [B, K + 1, V] and Q [B, K, V]:
+    warped target and draft distributions (fp32); draft [B, K] int32 tokens, the first n_draft [B] of each valid
+    (None: all); u [B, K] and u_next [B] uniforms in [0, 1). Returns (accepted counts [B], tokens [B, K + 1]:
+    the accepted ones, the next one, then -1), int32. ``ws``: uint8 workspace of
+    ops.verify_chain_ws_bytes(B, V) bytes (None: allocated here)."""
+    if P.dim() != 3:
+        raise ValueError(f"P must be [B, K + 1, V], got {tuple(P.shape)}")
+    B, rows, V = P.shape
+    if rows < 1 or V < 1:
+        raise ValueError(f"P must be [B, K + 1, V], got {tuple(P.shape)}")
+    i32 = dict(dtype=torch.int32, device=P.device)
+    tok, n = torch.empty(B, rows, **i32), torch.empty(B, **i32)
+    if ws is None:
+        ws = torch.empty(max(ops.verify_chain_ws_bytes(B, V), 16), dtype=torch.uint8, device=P.device)
+    ops.verify_chain(P, Q, draft, u, u_next, n_draft, tok, n, ws)
+    return n, tok

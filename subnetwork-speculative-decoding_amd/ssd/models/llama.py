@@ -21,6 +21,7 @@ generated directly on the GPU for synthetic benchmarks (``synthetic``), never du
 
 from __future__ import annotations
 
+import math
 import types
 from dataclasses import dataclass
 from typing import Optional
@@ -135,6 +136,42 @@ def rope_inv_freq(hd: int, theta: float, scaling: Optional[tuple] = None) -> tor
     blend = (1 - s) * scaled / f + s * scaled
     mid = (wavelen >= high_cut) & (wavelen <= low_cut)
     return torch.where(mid, blend, scaled)
+
+
+def rope_tables_f32(positions: int, rot_dim: int, theta: float, device, scaling: Optional[dict] = None) -> tuple:
+    """cos/sin [positions, rot_dim / 2] in fp32 for ``ops.rope`` and the 8-bit cache's write, from frequencies and angles
+    in 64 bits (at position 10^6 an fp32 angle is off by 0.03). ``scaling`` (HF's keys, ``rope_type``): "linear"
+    (factor), "llama3" (factor, low_freq_factor, high_freq_factor, original_max_position_embeddings) or "yarn"
+    (factor, original_max_position_embeddings; optional beta_fast, beta_slow, attention_factor): YaRN's ramp between
+    the dims that turn beta_fast and beta_slow times in the original context, cos and sin times 0.1 ln(factor) + 1."""
+    if rot_dim < 2 or rot_dim % 2 or positions < 1:
+        raise ValueError(f"rope_tables_f32: bad positions={positions} rot_dim={rot_dim}")
+    i = torch.arange(rot_dim // 2, dtype=torch.float64)
+    inv = theta ** (-2.0 * i / rot_dim)
+    gain, kind = 1.0, "default" if scaling is None else scaling.get("rope_type", scaling.get("type"))
+    if kind == "linear":
+        inv = inv / float(scaling["factor"])
+    elif kind == "llama3":
+        f, ctx = float(scaling["factor"]), float(scaling["original_max_position_embeddings"])
+        lo, hi = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
+        keep = ((ctx * inv / (2 * math.pi) - lo) / (hi - lo)).clamp(0, 1)
+        inv = (1 - keep) * inv / f + keep * inv
+    elif kind == "yarn":
+        f, ctx = float(scaling["factor"]), float(scaling["original_max_position_embeddings"])
+
+        def dim(turns):
+            return rot_dim * math.log(ctx / (turns * 2 * math.pi)) / (2 * math.log(theta))
+
+        lo = max(math.floor(dim(float(scaling.get("beta_fast") or 32.0))), 0)
+        hi = min(math.ceil(dim(float(scaling.get("beta_slow") or 1.0))), rot_dim - 1)
+        slow = ((i - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
+        inv = inv * (1 - slow) + inv / f * slow
+        given = scaling.get("attention_factor")
+        gain = 0.1 * math.log(f) + 1.0 if given is None and f > 1 else float(given or 1.0)
+    elif kind != "default":
+        raise ValueError(f"rope_type {kind!r} is not supported (default, linear, llama3, yarn)")
+    ang = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * inv.to(device)
+    return (ang.cos() * gain).float(), (ang.sin() * gain).float()
 
 
 def rope_tables(positions: int, hd: int, theta: float, device,
