@@ -254,11 +254,11 @@ int ssd_kv_q8_compact(const SsdKvQ8* cache, int layers, const int32_t* start, co
  * int32 [n_seq + 1], increasing, at most rows_max <= 64 rows each), and row t attends slots [0, prefix[t]) then
  * anc[t][0 .. depth[t]) of its sequence, as ssd_tree_attention_bf16 does. A row that attends nothing gets zeros;
  * rows outside [row_begin[0], row_begin[n_seq]) are left as they were. l_max >= every prefix + depth (host bound;
- * keys at logical positions from l_max on are not attended). Keys are folded in a fixed order: within a span of
- * `span` logical positions (a multiple of 64) block by block, then span by span, so a row's result depends on
+ * keys at logical positions from l_max on are not attended). Keys are folded in a fixed order (blocks of 64 within a
+ * span of `span` logical positions, a multiple of 64; four spans a group; the groups), so a row's result depends on
  * its query, its keys and span alone -- not on the other rows, the other sequences or the slots its ancestors
  * sit in: a verify row equals the autoregressive step at its position bit for bit.
- * heads / kv_heads any whole ratio. ws: ssd_attn_q8_ws_floats(...) floats, 16-byte aligned, no clearing needed; calls
+ * heads / kv_heads any whole ratio; scale > 0. ws: ssd_attn_q8_ws_floats(...) floats, 16-byte aligned, no clearing needed; calls
  * that overlap in time must not share it. */
 int64_t ssd_attn_q8_ws_floats(int M, int heads, int head_dim, int64_t l_max, int span);
 int ssd_tree_attention_q8(const SsdKvQ8* cache, const uint16_t* q, int64_t ldq, int M, int heads, const int32_t* row_begin,

@@ -78,8 +78,8 @@ def rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos: torch.Tenso
 
 # ------------------------------------------------------------------------------------------------- attention
 def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, row_begin, prefix, depth, anc, scale=None):
-    """q [M, heads, hd]; k, v [sequences, kv_heads, slots, hd] (the stored values). Returns (out [M, heads, hd] doubles,
-    bound on what rounding the weights to bf16 moves: sum of w |v| / 2^8). NaN rows: those of no sequence."""
+    """q [M, heads, hd]; k, v [sequences, kv_heads, slots, hd] (the stored values). Returns (out, sum of
+    w |v|), [M, heads, hd] doubles each. NaN rows: those of no sequence."""
     M, heads, hd = q.shape
     rep = heads // k.shape[1]
     scale = hd ** -0.5 if scale is None else scale

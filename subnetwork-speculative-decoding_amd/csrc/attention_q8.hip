@@ -2,28 +2,29 @@
 // row t attends cache slots [0, prefix[t]), then its ancestors' slots in depth order).
 //
 // Arithmetic of a row (the same whatever shares the call): its keys, by logical position, are cut into 64-key
-// blocks and spans of whole blocks. A span is folded block by block with a running maximum m, sum l and
-// output O (fp32); the spans' records (m, l, O) are folded in order. Keys every row of a sequence attends
-// -- whole blocks below the sequence's smallest prefix -- are folded by q8_shared_kernel for all rows at
-// once; the rest of a row's keys (its last block or two: committed slots, then ancestors) by q8_tail_kernel,
-// one workgroup per (row, kv head), which takes up the span where the shared kernel left it and then folds
-// the records. The record holds the fold's own registers, so the cut between the kernels leaves no trace.
+// blocks, spans of whole blocks and groups of four spans. A span is folded block by block with a running
+// reference m, sum l and output O (fp32); the spans of a group, then the groups, are added with weights from
+// their largest m. First launch: groups that every row of a sequence attends whole are folded for all its rows at
+// once, a row's other groups by a workgroup of its own; each (row, head, group) leaves a record (m, l, O).
+// Second launch: the groups' sum. Contexts of few groups take one launch that does both.
 //
-// S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32_bf16: codes become bf16 exactly (v_cvt_scalef32_pk_bf16_fp8);
-// K's exponents multiply the scores, V's the probabilities before they are rounded to bf16 (both exact), so
-// that rounding -- relative, 2^-9 -- is the only one below fp32. l is summed by the MFMA too, from the rounded
-// probabilities (an A operand of 2^-(V exponent)), so the weights that O is made of add up to l exactly.
+// S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32_bf16: codes become bf16 exactly (v_cvt_scalef32_pk_bf16_fp8,
+// with K's exponents as its scale); V's exponents multiply the probabilities before those are rounded to bf16
+// (exact), so that rounding -- 2^-8 of a weight at most -- is the only one below fp32. l is summed by the MFMA too, from
+// the rounded probabilities (an A operand of 2^-(V exponent)), so the weights O is made of add up to l exactly.
 #include "kv_q8.h"
 
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 namespace ssd {
 
 constexpr int QA_BLK = 64;
 constexpr int QA_MAXD = 32;   // gathered tree slots per row
 constexpr int QA_ROWS = 64;   // rows per sequence
+constexpr int QA_GRP = 4;     // spans per group
 
 int q8_check(const SsdKvQ8* c, const char* what);
 
@@ -34,10 +35,11 @@ struct AttnQ8Args {
   int64_t max_len;
   int n_seq, kv, heads, rep, M;
   const int *row_begin, *prefix, *depth, *anc;
-  int l_max, span_blk, n_spans, tiles;
+  int l_max, span_blk, n_grps;
+  int units, sets, tiles_per_set;  // launch geometry of the shared groups
   float scale_log2;
-  float* ws_o;    // [row][head][span][HD]: O
-  float2* ws_ml;  // [row][head][span]: (m, l)
+  float* ws_o;    // [row][head][group][HD]: O
+  float2* ws_ml;  // [row][head][group]: (m, l)
   bf16_t* out;
   int64_t ldo;
 };
@@ -46,7 +48,8 @@ template <int HD>
 struct Q8Frags {
   u32x4_t k[4][HD / 64];
   u32x4_t v[HD / 16];
-  u32x4_t kx, vx;  // exponent bytes of keys 16 kt + 4g + e: byte e of word kt
+  u32x4_t kx;  // K's exponents, the block's layout seen from the key's lane: byte j % 4 of word kt is key 16 kt + j
+  u32x4_t vx;  // V's exponents of keys 16 kt + 4g + e: byte e of word kt
 };
 
 template <int HD>
@@ -56,21 +59,13 @@ struct Q8State {
   f32x4_t o[HD / 16];   // O[row j][16 dt + 4g + e]
 };
 
-template <int HD>
-__device__ __forceinline__ void q8_reset(Q8State<HD>& s) {
-  s.m = -INFINITY;
-  s.l = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int dt = 0; dt < HD / 16; ++dt) s.o[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-}
-
-// Two words (8 codes) -> an MFMA operand.
-__device__ __forceinline__ bf16x8_t q8_bf16x8(uint32_t a, uint32_t b) {
+// Two words (8 codes) times a power of two -> an MFMA operand.
+__device__ __forceinline__ bf16x8_t q8_bf16x8(uint32_t a, uint32_t b, float scale) {
   u32x4_t r;
-  r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.f, false));
-  r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.f, true));
-  r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.f, false));
-  r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.f, true));
+  r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, scale, false));
+  r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, scale, true));
+  r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, scale, false));
+  r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, scale, true));
   return bits_bf16x8(r);
 }
 
@@ -83,61 +78,86 @@ __device__ __forceinline__ float q8_max32(float v) {
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
-// Folds one block into the state of a 16-row tile. valid: bit 4 kt + e says whether key 16 kt + 4g + e is
-// attended (masked instance only; codes and exponents of the others are 0 and 127).
-template <int HD, bool MASKED>
-__device__ __forceinline__ void q8_fold(const Q8Frags<HD>& f, const u32x4_t (&qf)[HD / 32], uint32_t valid, float scale_log2,
-                                        Q8State<HD>& st) {
-  // products and sums stay separate: the masked and unmasked instances must round alike
-#pragma clang fp contract(off)
-  f32x4_t s[4];
-#pragma unroll
-  for (int kt = 0; kt < 4; ++kt) s[kt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int p = 0; p < HD / 64; ++p)
-#pragma unroll
-    for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-      for (int kt = 0; kt < 4; ++kt)
-        s[kt] = mfma16x16x32(q8_bf16x8(f.k[kt][p][2 * hf], f.k[kt][p][2 * hf + 1]), bits_bf16x8(qf[2 * p + hf]), s[kt]);
-  float sv[16], mx = -INFINITY;
-#pragma unroll
-  for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      float v = s[kt][e] * (q8_scale((f.kx[kt] >> (8 * e)) & 0xffu) * scale_log2);
-      if (MASKED) v = ((valid >> (kt * 4 + e)) & 1u) ? v : -INFINITY;
-      sv[kt * 4 + e] = v;
-      mx = fmaxf(mx, v);
-    }
-  mx = q8_max32(q8_max16(mx));
-  const float m = fmaxf(st.m, mx);
-  const float ms = m == -INFINITY ? 0.f : m;  // nothing attended so far: every p is 0
-  const float alpha = __builtin_amdgcn_exp2f(st.m - ms);
-  st.m = m;
-  uint32_t pw[2][4], iv[2][4];
+// Folds one block into the states of T 16-row tiles; every operand is converted once for all of them, right before
+// the MFMAs that take it. valid: bit 4 kt + e says whether key 16 kt + 4g + e is attended (masked instance only;
+// V codes of the others are 0 and their exponents 127). FIRST: the states are empty. The reference m follows the
+// maximum only when that has grown by more than 2^8 (probabilities up to 2^8 are as exact as those up to 1):
+// after a span's first block the sums are hardly ever rescaled. Whether a row rescales is the row's own doing; that
+// a wave skips the products when none of its rows does changes nothing (they would be by 1).
+template <int HD, int T, bool MASKED, bool FIRST>
+__device__ __forceinline__ void q8_fold(const Q8Frags<HD>& f, const u32x4_t (&qf)[T][HD / 32], uint32_t valid, float scale_log2,
+                                        int j, Q8State<HD> (&st)[T]) {
+  f32x4_t s[T][4];
 #pragma unroll
   for (int kt = 0; kt < 4; ++kt) {
+    const float ks = q8_scale(f.kx[kt] >> (8 * (j & 3)) & 0xffu);
 #pragma unroll
-    for (int e = 0; e < 4; e += 2) {
-      const float p0 = __builtin_amdgcn_exp2f(sv[kt * 4 + e] - ms) * q8_scale((f.vx[kt] >> (8 * e)) & 0xffu);
-      const float p1 = __builtin_amdgcn_exp2f(sv[kt * 4 + e + 1] - ms) * q8_scale((f.vx[kt] >> (8 * e + 8)) & 0xffu);
-      pw[kt >> 1][(kt & 1) * 2 + e / 2] = pack_bf16x2(p0, p1);
-    }
-    const uint32_t w = 0xfefefefeu - f.vx[kt];  // bytes of 2^-(exponent)
-    iv[kt >> 1][(kt & 1) * 2] = (w & 0xffu) << 7 | (w & 0xff00u) << 15;
-    iv[kt >> 1][(kt & 1) * 2 + 1] = (w & 0xff0000u) >> 9 | (w & 0xff000000u) >> 1;
+    for (int t = 0; t < T; ++t) s[t][kt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int p = 0; p < HD / 64; ++p)
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const bf16x8_t ka = q8_bf16x8(f.k[kt][p][2 * hf], f.k[kt][p][2 * hf + 1], ks);
+#pragma unroll
+        for (int t = 0; t < T; ++t) s[t][kt] = mfma16x16x32(ka, bits_bf16x8(qf[t][2 * p + hf]), s[t][kt]);
+      }
   }
-  st.l *= alpha;
+  uint32_t pw[T][2][4];
 #pragma unroll
-  for (int dt = 0; dt < HD / 16; ++dt) st.o[dt] *= alpha;
+  for (int t = 0; t < T; ++t) {
+    float mx = -INFINITY;
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (MASKED) s[t][kt][e] = ((valid >> (kt * 4 + e)) & 1u) ? s[t][kt][e] : -INFINITY;
+        mx = fmaxf(mx, s[t][kt][e]);
+      }
+    mx = q8_max32(q8_max16(mx)) * scale_log2;  // scale_log2 >= 0
+    const float m = FIRST || mx > st[t].m + 8.f ? mx : st[t].m;
+    const float ms = m == -INFINITY ? 0.f : m;  // nothing attended so far: every p is 0
+    if (!FIRST) {
+      if (__any(m != st[t].m)) {
+        const float alpha = __builtin_amdgcn_exp2f(st[t].m - ms);
+        st[t].l *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < HD / 16; ++dt) st[t].o[dt] *= alpha;
+      }
+    }
+    st[t].m = m;
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+      for (int e = 0; e < 4; e += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[t][kt][e], scale_log2, -ms)) * q8_scale((f.vx[kt] >> (8 * e)) & 0xffu);
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(s[t][kt][e + 1], scale_log2, -ms)) * q8_scale((f.vx[kt] >> (8 * e + 8)) & 0xffu);
+        pw[t][kt >> 1][(kt & 1) * 2 + e / 2] = pack_bf16x2(p0, p1);
+      }
+  }
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
-    const bf16x8_t pb = bits_bf16x8(u32x4_t{pw[c][0], pw[c][1], pw[c][2], pw[c][3]});
-    st.l = mfma16x16x32(bits_bf16x8(u32x4_t{iv[c][0], iv[c][1], iv[c][2], iv[c][3]}), pb, st.l);
+    u32x4_t iv;
 #pragma unroll
-    for (int dt = 0; dt < HD / 16; ++dt)
-      st.o[dt] = mfma16x16x32(q8_bf16x8(f.v[dt][2 * c], f.v[dt][2 * c + 1]), pb, st.o[dt]);
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t x = 0xfefefefeu - f.vx[2 * c + i];  // bytes of 2^-(exponent)
+      iv[2 * i] = (x & 0xffu) << 7 | (x & 0xff00u) << 15;
+      iv[2 * i + 1] = (x & 0xff0000u) >> 9 | (x & 0xff000000u) >> 1;
+    }
+    const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      const bf16x8_t pb = bits_bf16x8(u32x4_t{pw[t][c][0], pw[t][c][1], pw[t][c][2], pw[t][c][3]});
+      st[t].l = mfma16x16x32(bits_bf16x8(iv), pb, FIRST && c == 0 ? zero : st[t].l);
+    }
+#pragma unroll
+    for (int dt = 0; dt < HD / 16; ++dt) {
+      const bf16x8_t va = q8_bf16x8(f.v[dt][2 * c], f.v[dt][2 * c + 1], 1.f);
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+        const bf16x8_t pb = bits_bf16x8(u32x4_t{pw[t][c][0], pw[t][c][1], pw[t][c][2], pw[t][c][3]});
+        st[t].o[dt] = mfma16x16x32(va, pb, FIRST && c == 0 ? zero : st[t].o[dt]);
+      }
+    }
   }
 }
 
@@ -161,195 +181,462 @@ __device__ __forceinline__ void q8_load_block(Q8Frags<HD>& f, const uint8_t* K, 
     for (int p = 0; p < HD / 64; ++p) f.k[kt][p] = *(const u32x4_t*)(kb + (kt * (HD / 64) + p) * 1024);
 #pragma unroll
   for (int dt = 0; dt < HD / 16; ++dt) f.v[dt] = *(const u32x4_t*)(vb + dt * 1024);
-  f.kx = *(const u32x4_t*)(Kx + (size_t)blk * 64 + (lane >> 4) * 16);
+  f.kx = *(const u32x4_t*)(Kx + (size_t)blk * 64 + (lane >> 2 & 3) * 16);
   f.vx = *(const u32x4_t*)(Vx + (size_t)blk * 64 + (lane >> 4) * 16);
 }
 
-template <int HD>
-__device__ __forceinline__ void q8_store_state(const AttnQ8Args& a, size_t rec, const Q8State<HD>& st, int g) {
-  float* o = a.ws_o + rec * HD + 4 * g;
-#pragma unroll
-  for (int dt = 0; dt < HD / 16; ++dt) *(f32x4_t*)(o + dt * 16) = st.o[dt];
-  a.ws_ml[rec] = make_float2(st.m, st.l[0]);
+// Smallest value over the wave's 64 lanes (row exchanges by DPP, then the swaps across rows).
+__device__ __forceinline__ int wave_min(int v) {
+  v = min(v, __builtin_amdgcn_mov_dpp(v, 0xb1, 0xf, 0xf, true));   // lane ^ 1
+  v = min(v, __builtin_amdgcn_mov_dpp(v, 0x4e, 0xf, 0xf, true));   // lane ^ 2
+  v = min(v, __builtin_amdgcn_mov_dpp(v, 0x141, 0xf, 0xf, true));  // the other half of 8
+  v = min(v, __builtin_amdgcn_mov_dpp(v, 0x140, 0xf, 0xf, true));  // the other half of 16
+  auto r = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
+  v = min((int)r[0], (int)r[1]);
+  r = __builtin_amdgcn_permlane32_swap((uint32_t)v, (uint32_t)v, false, false);
+  return min((int)r[0], (int)r[1]);
 }
 
-template <int HD>
-__device__ __forceinline__ void q8_load_state(const AttnQ8Args& a, size_t rec, Q8State<HD>& st, int g) {
-  const float* o = a.ws_o + rec * HD + 4 * g;
-#pragma unroll
-  for (int dt = 0; dt < HD / 16; ++dt) st.o[dt] = *(const f32x4_t*)(o + dt * 16);
-  const float2 ml = a.ws_ml[rec];
-  st.m = ml.x;
-  st.l = f32x4_t{ml.y, ml.y, ml.y, ml.y};
-}
-
-// Rows [r0, r1) of a sequence and the number of its blocks that every row attends. Called by whole waves.
-__device__ __forceinline__ int q8_shared_blocks(const AttnQ8Args& a, int seq, int lane, int& r0, int& r1) {
+// Rows [r0, r1) of a sequence.
+__device__ __forceinline__ void q8_rows(const AttnQ8Args& a, int seq, int& r0, int& r1) {
   r0 = min(max(a.row_begin[seq], 0), a.M);
   r1 = min(max(a.row_begin[seq + 1], r0), min(a.M, r0 + QA_ROWS));
-  int p = lane < r1 - r0 ? a.prefix[r0 + lane] : INT32_MAX;
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) p = min(p, __shfl_xor(p, o));
+}
+
+// The number of blocks that every row of the sequence attends. Called by whole waves.
+__device__ __forceinline__ int q8_shared_blocks(const AttnQ8Args& a, int r0, int r1, int lane) {
+  const int p = wave_min(lane < r1 - r0 ? a.prefix[r0 + lane] : INT32_MAX);
   return min(max(p, 0), a.l_max) / QA_BLK;
 }
 
-// Shared keys: one wave per (sequence, kv head, span, 16-row tile).
-template <int HD>
-__global__ __launch_bounds__(64) void q8_shared_kernel(AttnQ8Args a) {
-  const int lane = threadIdx.x, j = lane & 15, g = lane >> 4;
-  int id = blockIdx.x;
-  const int tile = id % a.tiles;
-  id /= a.tiles;
-  const int kvh = id % a.kv;
-  id /= a.kv;
-  const int span = id % a.n_spans, seq = id / a.n_spans;
-  int r0, r1;
-  const int nb = q8_shared_blocks(a, seq, lane, r0, r1);
-  const int b0 = span * a.span_blk, b1 = min(nb, b0 + a.span_blk), n_rows = (r1 - r0) * a.rep;
-  if (r1 <= r0 || b0 >= b1 || tile * 16 >= n_rows) return;
-  const size_t reg = ((size_t)seq * a.kv + kvh) * a.max_len;
-  const int R = min(tile * 16 + j, n_rows - 1);  // rows past the last repeat it and store the same record
-  const int row = r0 + R / a.rep, h = kvh * a.rep + R % a.rep;
-  u32x4_t qf[HD / 32];
-  q8_load_q<HD>(qf, a.Q + (size_t)row * a.ldq + (size_t)h * HD, g);
-  Q8State<HD> st;
-  q8_reset(st);
-  for (int b = b0; b < b1; ++b) {
-    Q8Frags<HD> f;
-    q8_load_block<HD>(f, a.K + reg * HD, a.V + reg * HD, a.Kx + reg, a.Vx + reg, b, lane);
-    q8_fold<HD, false>(f, qf, 0, a.scale_log2, st);
-  }
-  q8_store_state<HD>(a, ((size_t)row * a.heads + h) * a.n_spans + span, st, g);
+__device__ __forceinline__ float q8_weight(float m, float top) {
+  return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
 }
 
-// A row's own keys and the fold of its records: one workgroup per (sequence, row, kv head), 4 waves.
+// The four spans of a group meet in LDS: area for one 16-row tile (rows of a tile are query heads).
 template <int HD>
-__global__ __launch_bounds__(256) void q8_tail_kernel(AttnQ8Args a, int rows_max) {
+struct alignas(16) Q8Spans {
+  float o[QA_GRP][16][HD + 4];
+  float m[QA_GRP][16], l[QA_GRP][16];
+};
+
+// Wave w leaves its span's state; one without keys leaves (-inf, 0, 0).
+template <int HD>
+__device__ __forceinline__ void q8_publish(Q8Spans<HD>& lds, int w, int j, int g, bool have, const Q8State<HD>& st) {
+  lds.m[w][j] = have ? st.m : -INFINITY;  // the four lanes of row j write the same values
+  lds.l[w][j] = have ? st.l[0] : 0.f;
+#pragma unroll
+  for (int dt = 0; dt < HD / 16; ++dt) *(f32x4_t*)&lds.o[w][j][dt * 16 + 4 * g] = have ? st.o[dt] : f32x4_t{0.f, 0.f, 0.f, 0.f};
+}
+
+// Row rr's record, dims 4 dc .. + 4 of every 64: the largest reference first, then the weighted sums in order.
+template <int HD>
+struct Q8Record {
+  float m, l;
+  f32x4_t o[HD / 64];
+};
+template <int HD>
+__device__ __forceinline__ Q8Record<HD> q8_merge(const Q8Spans<HD>& lds, int rr, int dc) {
+  Q8Record<HD> r;
+  r.m = -INFINITY, r.l = 0.f;
+#pragma unroll
+  for (int i = 0; i < HD / 64; ++i) r.o[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int s = 0; s < QA_GRP; ++s) r.m = fmaxf(r.m, lds.m[s][rr]);
+#pragma unroll
+  for (int s = 0; s < QA_GRP; ++s) {
+    const float wgt = q8_weight(lds.m[s][rr], r.m);
+    r.l = fmaf(lds.l[s][rr], wgt, r.l);
+#pragma unroll
+    for (int i = 0; i < HD / 64; ++i) {
+      const f32x4_t x = *(const f32x4_t*)&lds.o[s][rr][i * 64 + dc * 4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r.o[i][e] = fmaf(x[e], wgt, r.o[i][e]);
+    }
+  }
+  return r;
+}
+
+template <int HD>
+__device__ __forceinline__ void q8_store_record(const AttnQ8Args& a, size_t rec, int dc, const Q8Record<HD>& r) {
+#pragma unroll
+  for (int i = 0; i < HD / 64; ++i) *(f32x4_t*)(a.ws_o + rec * HD + i * 64 + dc * 4) = r.o[i];
+  if (dc == 0) a.ws_ml[rec] = make_float2(r.m, r.l);
+}
+
+// Shared groups. Workgroup (sequence, group, kv head, set of row tiles): wave w folds span w of the group for T tiles
+// of 16 query rows, so that each block's K and V are loaded and converted once for T tiles. The sets of one
+// (sequence, group, kv head) are ids 8 apart: one XCD, whose L2 they share.
+template <int HD, int T>
+__device__ __forceinline__ void q8_shared_group(const AttnQ8Args& a, int id, Q8Spans<HD> (&lds)[T]) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, j = lane & 15, g = lane >> 4;
-  const int kvh = blockIdx.x % a.kv, seq = blockIdx.x / a.kv / rows_max, place = blockIdx.x / a.kv % rows_max;
-  __shared__ int s_anc[QA_MAXD];
-  __shared__ uint8_t s_v[QA_MAXD][HD];          // the ancestors' V codes
-  __shared__ uint8_t s_x[2][QA_MAXD];           // and exponents (K, V)
+  const int rest = id >> 3, set = rest % a.sets;
+  int u = rest / a.sets * 8 + (id & 7);
+  if (u >= a.units) return;
+  const int kvh = u % a.kv;
+  u /= a.kv;
+  const int grp = u % a.n_grps, seq = u / a.n_grps;
   int r0, r1;
-  const int nb = q8_shared_blocks(a, seq, lane, r0, r1);
-  const int row = r0 + place;
-  if (row >= r1) return;
-  const int P = min(max(a.prefix[row], 0), a.l_max);
-  const int L = min(P + min(max(a.depth[row], 0), QA_MAXD), a.l_max), D = L - P;
+  q8_rows(a, seq, r0, r1);
+  const int n_rows = (r1 - r0) * a.rep, tile0 = set * a.tiles_per_set;
+  if (r1 <= r0 || tile0 * 16 >= n_rows) return;
+  if ((grp + 1) * QA_GRP * a.span_blk > q8_shared_blocks(a, r0, r1, lane)) return;  // the rows' own
   const size_t reg = ((size_t)seq * a.kv + kvh) * a.max_len;
-  const uint8_t *K = a.K + reg * HD, *V = a.V + reg * HD, *Kx = a.Kx + reg, *Vx = a.Vx + reg;
-  const int n_blk = (L + QA_BLK - 1) / QA_BLK, n_sp = (n_blk + a.span_blk - 1) / a.span_blk;
+  u32x4_t qf[T][HD / 32];
+  Q8State<HD> st[T];
+#pragma unroll
+  for (int t = 0; t < T; ++t) {  // rows past the last repeat it
+    const int R = min((tile0 + min(t, a.tiles_per_set - 1)) * 16 + j, n_rows - 1);
+    q8_load_q<HD>(qf[t], a.Q + (size_t)(r0 + R / a.rep) * a.ldq + (size_t)(kvh * a.rep + R % a.rep) * HD, g);
+  }
+  const int b0 = (grp * QA_GRP + w) * a.span_blk;
+  Q8Frags<HD> f;
+  q8_load_block<HD>(f, a.K + reg * HD, a.V + reg * HD, a.Kx + reg, a.Vx + reg, b0, lane);
+  q8_fold<HD, T, false, true>(f, qf, 0, a.scale_log2, j, st);
+  for (int b = b0 + 1; b < b0 + a.span_blk; ++b) {
+    q8_load_block<HD>(f, a.K + reg * HD, a.V + reg * HD, a.Kx + reg, a.Vx + reg, b, lane);
+    q8_fold<HD, T, false, false>(f, qf, 0, a.scale_log2, j, st);
+  }
+#pragma unroll
+  for (int t = 0; t < T; ++t) q8_publish<HD>(lds[t], w, j, g, true, st[t]);
+  __syncthreads();
+  const int rr = threadIdx.x >> 4, dc = threadIdx.x & 15;
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+    const int R = (tile0 + t) * 16 + rr;
+    if (t < a.tiles_per_set && R < n_rows) {
+      const size_t head = (size_t)(r0 + R / a.rep) * a.heads + kvh * a.rep + R % a.rep;
+      q8_store_record<HD>(a, head * a.n_grps + grp, dc, q8_merge<HD>(lds[t], rr, dc));
+    }
+  }
+}
+
+// One block of a row's own keys: positions below P are cache slots, those in [P, L) the ancestors' slots.
+template <int HD>
+struct alignas(16) Q8Anc {
+  int slot[QA_MAXD];            // -1: not attended
+  uint8_t v[QA_MAXD][HD];       // V codes
+  uint8_t x[2][QA_MAXD];        // exponents (K, V)
+};
+
+template <int HD>
+__device__ __forceinline__ uint32_t q8_load_own(Q8Frags<HD>& f, const uint8_t* K, const uint8_t* V, const uint8_t* Kx,
+                                                const uint8_t* Vx, int b, int P, int L, const Q8Anc<HD>& anc, int lane) {
+  const int j = lane & 15, g = lane >> 4, key0 = b * QA_BLK;
+  uint32_t valid = 0;
+  f.kx = *(const u32x4_t*)(Kx + key0 + (j >> 2) * 16);
+  f.vx = *(const u32x4_t*)(Vx + key0 + g * 16);
+  const uint8_t* vb = V + (size_t)b * 64 * HD + lane * 16;
+#pragma unroll
+  for (int dt = 0; dt < HD / 16; ++dt) f.v[dt] = *(const u32x4_t*)(vb + dt * 1024);
+  // K: one slot a lane. Loads are unconditional (a key that is not attended reads its own block's first
+  // slot, which exists; its score is masked).
+#pragma unroll
+  for (int kt = 0; kt < 4; ++kt) {
+    const int pos = key0 + 16 * kt + j;
+    const int sl = pos < P ? pos : pos < L ? anc.slot[pos - P] : -1;
+    if (pos >= P) f.kx[kt] = pos < L ? anc.x[0][pos - P] * 0x01010101u : 0x7f7f7f7fu;
+#pragma unroll
+    for (int p = 0; p < HD / 64; ++p) f.k[kt][p] = *(const u32x4_t*)(K + q8_k_off(sl >= 0 ? sl : key0, 64 * p + 16 * g, HD));
+  }
+  // V and its exponents: the block's own slots, positions from P on cleared, then the ancestors' put in
+  u32x4_t own;
+#pragma unroll
+  for (int kt = 0; kt < 4; ++kt) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int pos = key0 + 16 * kt + 4 * g + e;
+      if (pos < P) m |= 0xffu << (8 * e), valid |= 1u << (4 * kt + e);
+    }
+    own[kt] = m;
+    f.vx[kt] = (f.vx[kt] & m) | (0x7f7f7f7fu & ~m);
+  }
+#pragma unroll
+  for (int dt = 0; dt < HD / 16; ++dt) f.v[dt] &= own;
+  const int a0 = max(P, key0) - P, a1 = min(L, key0 + QA_BLK) - P;
+  for (int an = a0; an < a1; ++an) {  // uniform
+    const int off = P + an - key0, kt = off >> 4, e = off & 3;
+    const bool mine = ((off >> 2) & 3) == g;
+    const uint32_t sel = mine ? 0xffu << (8 * e) : 0u, xv = anc.x[1][an] * 0x01010101u;
+    if (mine && anc.slot[an] >= 0) valid |= 1u << (4 * kt + e);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const uint32_t m = c == kt ? sel : 0u;
+      f.vx[c] = (f.vx[c] & ~m) | (xv & m);
+#pragma unroll
+      for (int dt = 0; dt < HD / 16; ++dt) f.v[dt][c] = (f.v[dt][c] & ~m) | ((anc.v[an][dt * 16 + j] * 0x01010101u) & m);
+    }
+  }
+  return valid;
+}
+
+// The row's keys: P cache slots, then L - P ancestors, staged by the whole workgroup.
+template <int HD, int NT>
+__device__ __forceinline__ void q8_stage_anc(const AttnQ8Args& a, int row, int D, const uint8_t* V, const uint8_t* Kx,
+                                             const uint8_t* Vx, Q8Anc<HD>& anc) {
+  if (D == 0) return;  // uniform
   if (threadIdx.x < QA_MAXD) {
     const int sl = threadIdx.x < D ? a.anc[(size_t)row * QA_MAXD + threadIdx.x] : -1;
     const bool ok = sl >= 0 && sl < a.max_len;
-    s_anc[threadIdx.x] = ok ? sl : -1;
-    s_x[0][threadIdx.x] = ok ? Kx[q8_x_off(sl)] : 127;
-    s_x[1][threadIdx.x] = ok ? Vx[q8_x_off(sl)] : 127;
+    anc.slot[threadIdx.x] = ok ? sl : -1;
+    anc.x[0][threadIdx.x] = ok ? Kx[q8_x_off(sl)] : 127;
+    anc.x[1][threadIdx.x] = ok ? Vx[q8_x_off(sl)] : 127;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < D * HD; i += 256) {
-    const int sl = s_anc[i / HD];
-    s_v[i / HD][i % HD] = sl >= 0 ? V[q8_v_off(sl, i % HD, HD)] : 0;
+  constexpr int IT = (QA_MAXD * HD + NT - 1) / NT;
+  uint8_t c[IT];
+#pragma unroll
+  for (int it = 0; it < IT; ++it) {
+    if (it * NT >= D * HD) break;  // uniform
+    const int i = min((int)threadIdx.x + it * NT, D * HD - 1), sl = anc.slot[i / HD];
+    c[it] = V[q8_v_off(sl >= 0 ? sl : 0, i % HD, HD)];
+  }
+#pragma unroll
+  for (int it = 0; it < IT; ++it) {
+    if (it * NT >= D * HD) break;
+    const int i = min((int)threadIdx.x + it * NT, D * HD - 1);
+    anc.v[i / HD][i % HD] = anc.slot[i / HD] >= 0 ? c[it] : 0;
   }
   __syncthreads();
-  const int cut = nb / a.span_blk;
-  for (int t0 = 0; t0 < a.rep; t0 += 16) {
-    const int hr = min(t0 + j, a.rep - 1), h = kvh * a.rep + hr;
-    const size_t rec0 = ((size_t)row * a.heads + h) * a.n_spans;
-    u32x4_t qf[HD / 32];
-    q8_load_q<HD>(qf, a.Q + (size_t)row * a.ldq + (size_t)h * HD, g);
-    for (int sp = cut + w; sp < n_sp; sp += 4) {  // spans are independent of each other: one wave each
-      const int b0 = max(nb, sp * a.span_blk), b1 = min(n_blk, (sp + 1) * a.span_blk);
-      if (b0 >= b1) continue;
-      Q8State<HD> st;
-      if (b0 > sp * a.span_blk) q8_load_state<HD>(a, rec0 + sp, st, g);
-      else q8_reset(st);
-      for (int b = b0; b < b1; ++b) {
-        const int key0 = b * QA_BLK;
-        Q8Frags<HD> f;
-        uint32_t valid = 0;
-        f.kx = *(const u32x4_t*)(Kx + key0 + g * 16);
-        f.vx = *(const u32x4_t*)(Vx + key0 + g * 16);
-        // K: one slot a lane. Loads are unconditional (a key that is not attended reads its own block's slot,
-        // which exists) and masked after.
+}
+
+// Wave w's span of group grp for the heads h0 .. h0 + nh of one row; false: no keys.
+template <int HD>
+__device__ __forceinline__ bool q8_own_span(const AttnQ8Args& a, size_t reg, int row, int h0, int nh, int span, int P, int L,
+                                            const Q8Anc<HD>& anc, int lane, Q8State<HD> (&st)[1]) {
+  const int b0 = span * a.span_blk, b1 = min((L + QA_BLK - 1) / QA_BLK, b0 + a.span_blk), j = lane & 15;
+  if (b0 >= b1) return false;
+  const uint8_t *K = a.K + reg * HD, *V = a.V + reg * HD, *Kx = a.Kx + reg, *Vx = a.Vx + reg;
+  u32x4_t qf[1][HD / 32];
+  q8_load_q<HD>(qf[0], a.Q + (size_t)row * a.ldq + (size_t)(h0 + min(j, nh - 1)) * HD, lane >> 4);
+  st[0].m = -INFINITY;
+  st[0].l = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int kt = 0; kt < 4; ++kt) {
-          const int pos = key0 + 16 * kt + j;
-          const int sl = pos < P ? pos : pos < L ? s_anc[pos - P] : -1;
-          const uint32_t keep = sl >= 0 ? 0xffffffffu : 0u;
-#pragma unroll
-          for (int p = 0; p < HD / 64; ++p)
-            f.k[kt][p] = *(const u32x4_t*)(K + q8_k_off(sl >= 0 ? sl : key0, 64 * p + 16 * g, HD)) & keep;
-        }
-        // V and the exponents: the block's own slots, positions from P on cleared, then the ancestors' put in
-        u32x4_t own;
-#pragma unroll
-        for (int kt = 0; kt < 4; ++kt) {
-          uint32_t m = 0;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int pos = key0 + 16 * kt + 4 * g + e;
-            if (pos < P) m |= 0xffu << (8 * e), valid |= 1u << (4 * kt + e);
-          }
-          own[kt] = m;
-          f.kx[kt] = (f.kx[kt] & m) | (0x7f7f7f7fu & ~m);
-          f.vx[kt] = (f.vx[kt] & m) | (0x7f7f7f7fu & ~m);
-        }
-        const uint8_t* vb = V + (size_t)b * 64 * HD + lane * 16;
-#pragma unroll
-        for (int dt = 0; dt < HD / 16; ++dt) f.v[dt] = *(const u32x4_t*)(vb + dt * 1024) & own;
-        const int a0 = max(P, key0) - P, a1 = min(L, key0 + QA_BLK) - P;
-        for (int an = a0; an < a1; ++an) {  // uniform
-          const int off = P + an - key0, kt = off >> 4, e = off & 3;
-          const bool mine = ((off >> 2) & 3) == g;
-          const uint32_t sel = mine ? 0xffu << (8 * e) : 0u;
-          const uint32_t xk = s_x[0][an] * 0x01010101u, xv = s_x[1][an] * 0x01010101u;
-          if (mine && s_anc[an] >= 0) valid |= 1u << (4 * kt + e);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const uint32_t m = c == kt ? sel : 0u;
-            f.kx[c] = (f.kx[c] & ~m) | (xk & m);
-            f.vx[c] = (f.vx[c] & ~m) | (xv & m);
-#pragma unroll
-            for (int dt = 0; dt < HD / 16; ++dt)
-              f.v[dt][c] = (f.v[dt][c] & ~m) | ((s_v[an][dt * 16 + j] * 0x01010101u) & m);
-          }
-        }
-        q8_fold<HD, true>(f, qf, valid, a.scale_log2, st);
-      }
-      q8_store_state<HD>(a, rec0 + sp, st, g);
-    }
+  for (int dt = 0; dt < HD / 16; ++dt) st[0].o[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  for (int b = b0; b < b1; ++b) {
+    Q8Frags<HD> f;
+    uint32_t valid = 0xffffu;
+    if ((b + 1) * QA_BLK <= P) q8_load_block<HD>(f, K, V, Kx, Vx, b, lane);
+    else valid = q8_load_own<HD>(f, K, V, Kx, Vx, b, P, L, anc, lane);
+    q8_fold<HD, 1, true, false>(f, qf, valid, a.scale_log2, j, st);
   }
-  __syncthreads();  // the records of this workgroup's waves
-  // fold the spans in order: maximum first, then the weighted sums
-  for (int i = threadIdx.x; i < a.rep * HD; i += 256) {
-    const int h = kvh * a.rep + i / HD, d = i % HD;
-    const size_t rec0 = ((size_t)row * a.heads + h) * a.n_spans;
-    float mx = -INFINITY;
-    for (int s = 0; s < n_sp; ++s) mx = fmaxf(mx, a.ws_ml[rec0 + s].x);
-    float l = 0.f, o = 0.f;
-    for (int s = 0; s < n_sp; ++s) {
-      const float2 ml = a.ws_ml[rec0 + s];
-      const float wgt = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - mx);
-      l = fmaf(ml.y, wgt, l);
-      o = fmaf(a.ws_o[(rec0 + s) * HD + d], wgt, o);
+  return true;
+}
+
+__device__ __forceinline__ void q8_row_keys(const AttnQ8Args& a, int row, int& P, int& L) {
+  P = min(max(a.prefix[row], 0), a.l_max);
+  L = min(P + min(max(a.depth[row], 0), QA_MAXD), a.l_max);
+}
+
+// A row's own groups: from the one its sequence's smallest prefix ends in to its last, one after the other, a wave a span.
+template <int HD>
+__device__ __forceinline__ void q8_own_groups(const AttnQ8Args& a, int id, int rows_max, Q8Spans<HD>& lds, Q8Anc<HD>& anc) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, j = lane & 15, g = lane >> 4;
+  const int kvh = id % a.kv, seq = id / a.kv / rows_max;
+  int r0, r1, P, L;
+  q8_rows(a, seq, r0, r1);
+  const int row = r0 + id / a.kv % rows_max;
+  if (row >= r1) return;
+  const int nb = q8_shared_blocks(a, r0, r1, lane), per = QA_GRP * a.span_blk;
+  q8_row_keys(a, row, P, L);
+  const size_t reg = ((size_t)seq * a.kv + kvh) * a.max_len;
+  const int n_grp = (L + per * QA_BLK - 1) / (per * QA_BLK);
+  if (nb / per >= n_grp) return;
+  q8_stage_anc<HD, 256>(a, row, L - P, a.V + reg * HD, a.Kx + reg, a.Vx + reg, anc);
+  for (int grp = nb / per; grp < n_grp; ++grp)
+    for (int t0 = 0; t0 < a.rep; t0 += 16) {
+      const int nh = min(16, a.rep - t0), h0 = kvh * a.rep + t0;
+      Q8State<HD> st[1];
+      const bool have = q8_own_span<HD>(a, reg, row, h0, nh, grp * QA_GRP + w, P, L, anc, lane, st);
+      __syncthreads();  // the tile before has been merged
+      q8_publish<HD>(lds, w, j, g, have, st[0]);
+      __syncthreads();
+      const int rr = threadIdx.x >> 4, dc = threadIdx.x & 15;
+      if (rr < nh) q8_store_record<HD>(a, ((size_t)row * a.heads + h0 + rr) * a.n_grps + grp, dc, q8_merge<HD>(lds, rr, dc));
     }
-    a.out[(size_t)row * a.ldo + (size_t)h * HD + d] = f2bf(l == 0.f ? 0.f : o / l);  // NaN stays NaN
+}
+
+template <int HD, int T>
+union alignas(16) Q8FoldLds {
+  Q8Spans<HD> shared[T];
+  struct {
+    Q8Spans<HD> spans;
+    Q8Anc<HD> anc;
+  } own;
+};
+
+// First launch: workgroups of rows (ids first: theirs is the longer chain of loads), then of shared groups.
+template <int HD, int T>
+__global__ __launch_bounds__(256, 2) void q8_fold_kernel(AttnQ8Args a, int rows_max, int own) {
+  __shared__ Q8FoldLds<HD, T> lds;
+  if ((int)blockIdx.x < own) {
+    if ((int)blockIdx.x < a.n_seq * rows_max * a.kv) q8_own_groups<HD>(a, blockIdx.x, rows_max, lds.own.spans, lds.own.anc);
+  } else {
+    q8_shared_group<HD, T>(a, blockIdx.x - own, lds.shared);
   }
 }
 
-static int q8_spans(int64_t l_max, int span) { return (int)((l_max + span - 1) / span); }
+// Second launch: one workgroup of four waves per (row, head). Weights from the groups' largest reference; wave r
+// adds groups r, r + 4, ... in order, then the four sums are added in order; l by a fixed exchange between
+// lanes, 64 groups at a time.
+template <int HD>
+__global__ __launch_bounds__(256) void q8_combine_kernel(AttnQ8Args a) {
+  constexpr int PER = HD / 64;  // dims a lane
+  const int lane = threadIdx.x & 63, r = threadIdx.x >> 6;
+  const int row = blockIdx.x / a.heads, h = blockIdx.x % a.heads;
+  const size_t rec0 = ((size_t)row * a.heads + h) * a.n_grps;
+  const float* O = a.ws_o + rec0 * HD + lane * PER;
+  __shared__ float part[4][HD];
+  // the first records before it is known how many there are (the workspace holds n_grps of them)
+  float x[4][PER];
+  auto load = [&](int g0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int d = 0; d < PER; ++d) x[i][d] = O[(size_t)min(g0 + 4 * i, a.n_grps - 1) * HD + d];
+  };
+  load(r);
+  float2 ml = a.ws_ml[rec0 + min(lane, a.n_grps - 1)];
+  if (row < a.row_begin[0] || row >= a.row_begin[a.n_seq]) return;  // uniform
+  int P, L;
+  q8_row_keys(a, row, P, L);
+  const int per = QA_GRP * a.span_blk * QA_BLK, n = (L + per - 1) / per;
+  if (lane >= n) ml = make_float2(-INFINITY, 0.f);
+  float top = ml.x;
+  for (int g = lane + 64; g < n; g += 64) top = fmaxf(top, a.ws_ml[rec0 + g].x);
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+  float l = 0.f, o[PER];
+#pragma unroll
+  for (int d = 0; d < PER; ++d) o[d] = 0.f;
+  for (int g0 = 0; g0 < n; g0 += 64) {
+    if (g0) ml = g0 + lane < n ? a.ws_ml[rec0 + g0 + lane] : make_float2(-INFINITY, 0.f);
+    const float wgt = q8_weight(ml.x, top);
+    float lw = ml.y * wgt;
+#pragma unroll
+    for (int s = 32; s >= 1; s >>= 1) lw += __shfl_xor(lw, s);
+    l += lw;
+    for (int g = g0 + r; g < min(n, g0 + 64); g += 16) {
+      if (g != r) load(g);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (g + 4 * i >= n) break;  // uniform
+        const float wi = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(wgt), g - g0 + 4 * i));
+#pragma unroll
+        for (int d = 0; d < PER; ++d) o[d] = fmaf(x[i][d], wi, o[d]);
+      }
+    }
+  }
+#pragma unroll
+  for (int d = 0; d < PER; ++d) part[r][lane * PER + d] = o[d];
+  __syncthreads();
+  if (threadIdx.x < HD / 2) {
+    const int d = threadIdx.x * 2;
+    float y[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float s = ((part[0][d + e] + part[1][d + e]) + part[2][d + e]) + part[3][d + e];
+      y[e] = l == 0.f ? 0.f : s / l;  // NaN stays NaN
+    }
+    *(uint32_t*)(a.out + (size_t)row * a.ldo + (size_t)h * HD + d) = pack_bf16x2(y[0], y[1]);
+  }
+}
+
+// Contexts of up to TEAMS <= 4 groups in one launch: a workgroup per (sequence, row, kv head), a team of four waves per
+// group. The records stay in LDS and are added as the second launch adds them.
+template <int HD, int TEAMS>
+struct alignas(16) Q8ShortLds {
+  Q8Spans<HD> spans[TEAMS];
+  Q8Anc<HD> anc;
+};
+
+template <int HD, int TEAMS>
+__global__ __launch_bounds__(256 * TEAMS) void q8_short_kernel(AttnQ8Args a, int rows_max) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6 & 3, team = threadIdx.x >> 8, j = lane & 15, g = lane >> 4;
+  const int kvh = blockIdx.x % a.kv, seq = blockIdx.x / a.kv / rows_max;
+  __shared__ Q8ShortLds<HD, TEAMS> lds;
+  __shared__ float rec_m[TEAMS][16], rec_l[TEAMS][16];
+  int r0, r1, P, L;
+  q8_rows(a, seq, r0, r1);
+  const int row = r0 + blockIdx.x / a.kv % rows_max;
+  if (row >= r1) return;
+  q8_row_keys(a, row, P, L);
+  const size_t reg = ((size_t)seq * a.kv + kvh) * a.max_len;
+  q8_stage_anc<HD, 256 * TEAMS>(a, row, L - P, a.V + reg * HD, a.Kx + reg, a.Vx + reg, lds.anc);
+  for (int t0 = 0; t0 < a.rep; t0 += 16) {
+    const int nh = min(16, a.rep - t0), h0 = kvh * a.rep + t0;
+    Q8State<HD> st[1];
+    const bool have = q8_own_span<HD>(a, reg, row, h0, nh, team * QA_GRP + w, P, L, lds.anc, lane, st);
+    if (t0) __syncthreads();  // the heads before have been written out
+    q8_publish<HD>(lds.spans[team], w, j, g, have, st[0]);
+    __syncthreads();
+    const int rr = threadIdx.x >> 4 & 15, dc = threadIdx.x & 15;
+    const Q8Record<HD> r = q8_merge<HD>(lds.spans[team], rr, dc);
+    float top = r.m;
+    if constexpr (TEAMS > 1) {
+      __syncthreads();
+      if (dc == 0) rec_m[team][rr] = r.m, rec_l[team][rr] = r.l;
+#pragma unroll
+      for (int i = 0; i < HD / 64; ++i) *(f32x4_t*)&lds.spans[team].o[0][rr][i * 64 + dc * 4] = r.o[i];
+      __syncthreads();
+      if (team) continue;
+#pragma unroll
+      for (int t = 1; t < TEAMS; ++t) top = fmaxf(top, rec_m[t][rr]);
+    }
+    if (rr >= nh) continue;
+    // sums of one group each, added in order; l in the order of the second launch's exchange
+    float wgt[4], lw[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const float m = t == 0 ? r.m : t < TEAMS ? rec_m[t < TEAMS ? t : 0][rr] : -INFINITY;
+      wgt[t] = q8_weight(m, top);
+      lw[t] = t == 0 ? r.l * wgt[0] : t < TEAMS ? rec_l[t < TEAMS ? t : 0][rr] * wgt[t] : 0.f;
+    }
+    const float l = (lw[0] + lw[2]) + (lw[1] + lw[3]);
+#pragma unroll
+    for (int i = 0; i < HD / 64; ++i) {
+      float y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float s = fmaf(r.o[i][e], wgt[0], 0.f);
+#pragma unroll
+        for (int t = 1; t < TEAMS; ++t) s += fmaf(lds.spans[t].o[0][rr][i * 64 + dc * 4 + e], wgt[t], 0.f);
+        y[e] = l == 0.f ? 0.f : s / l;
+      }
+      *(uint2*)(a.out + (size_t)row * a.ldo + (size_t)(h0 + rr) * HD + i * 64 + dc * 4) =
+          make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
+    }
+  }
+}
+
+static int q8_groups(int64_t l_max, int span) { return (int)((l_max + (int64_t)QA_GRP * span - 1) / ((int64_t)QA_GRP * span)); }
 
 template <int HD>
-static int launch_attn_q8(const AttnQ8Args& a, int rows_max, hipStream_t stream) {
-  const int64_t shared = (int64_t)a.n_seq * a.n_spans * a.kv * a.tiles, tail = (int64_t)a.n_seq * rows_max * a.kv;
-  if (shared > INT32_MAX || tail > INT32_MAX) return set_error(SSD_ERANGE, "attention_q8: too many workgroups");
-  if (a.l_max >= QA_BLK) {
-    SSD_LAUNCH((q8_shared_kernel<HD>), dim3((unsigned)shared), dim3(64), 0, stream, a);
-    if (int rc = check_launch("attn_q8_shared")) return rc;
-  }
-  SSD_LAUNCH((q8_tail_kernel<HD>), dim3((unsigned)tail), dim3(256), 0, stream, a, rows_max);
-  return check_launch("attn_q8_tail");
+static int launch_attn_q8(AttnQ8Args a, int rows_max, hipStream_t stream) {
+  using std::integral_constant;
+  const int64_t rows = (int64_t)a.n_seq * rows_max * a.kv;
+  const int tiles = (rows_max * a.rep + 15) / 16;
+  const bool single = tiles == 1;
+  a.sets = single ? 1 : (tiles + 1) / 2;
+  a.tiles_per_set = single ? 1 : (tiles + a.sets - 1) / a.sets;
+  const int64_t units = (int64_t)a.n_seq * a.n_grps * a.kv, shared = (units + 7) / 8 * 8 * a.sets, own = (rows + 7) / 8 * 8;
+  if (shared + own > INT32_MAX || (int64_t)a.M * a.heads > INT32_MAX)
+    return set_error(SSD_ERANGE, "attention_q8: too many workgroups");
+  a.units = (int)units;
+  auto one_launch = [&](auto t) {
+    SSD_LAUNCH((q8_short_kernel<HD, decltype(t)::value>), dim3((unsigned)rows), dim3(256 * decltype(t)::value), 0, stream, a, rows_max);
+    return check_launch("attn_q8_short");
+  };
+  if (a.n_grps == 1) return one_launch(integral_constant<int, 1>());
+  if (a.n_grps == 2 && rows <= 512) return one_launch(integral_constant<int, 2>());
+  if constexpr (HD == 64)
+    if (a.n_grps <= 4 && rows <= 256) return one_launch(integral_constant<int, 4>());
+  if (single) SSD_LAUNCH((q8_fold_kernel<HD, 1>), dim3((unsigned)(own + shared)), dim3(256), 0, stream, a, rows_max, (int)own);
+  else SSD_LAUNCH((q8_fold_kernel<HD, 2>), dim3((unsigned)(own + shared)), dim3(256), 0, stream, a, rows_max, (int)own);
+  if (int rc = check_launch("attn_q8_fold")) return rc;
+  SSD_LAUNCH((q8_combine_kernel<HD>), dim3((unsigned)(a.M * a.heads)), dim3(256), 0, stream, a);
+  return check_launch("attn_q8_combine");
 }
 
 }  // namespace ssd
@@ -357,8 +644,8 @@ static int launch_attn_q8(const AttnQ8Args& a, int rows_max, hipStream_t stream)
 using namespace ssd;
 
 SSD_API int64_t ssd_attn_q8_ws_floats(int M, int heads, int head_dim, int64_t l_max, int span) {
-  if (M < 0 || heads < 1 || head_dim < 1 || l_max < 1 || span < 64 || span % 64) return -1;
-  return (int64_t)M * heads * q8_spans(l_max, span) * (head_dim + 2);
+  if (M < 0 || heads < 1 || head_dim < 1 || l_max < 1 || span < 64 || span % 64 || span > 1 << 20) return -1;
+  return (int64_t)M * heads * q8_groups(l_max, span) * (head_dim + 2);
 }
 
 SSD_API int ssd_tree_attention_q8(const SsdKvQ8* cache, const uint16_t* q, int64_t ldq, int M, int heads,
@@ -373,7 +660,8 @@ SSD_API int ssd_tree_attention_q8(const SsdKvQ8* cache, const uint16_t* q, int64
     return set_error(SSD_ERANGE, "attention_q8: %d rows a sequence (1 to %d)", rows_max, QA_ROWS);
   if (l_max < 1 || l_max > cache->max_len)
     return set_error(SSD_EINVAL, "attention_q8: l_max %d outside [1, max_len %lld]", l_max, (long long)cache->max_len);
-  if (span < 64 || span % 64) return set_error(SSD_EINVAL, "attention_q8: span %d must be a multiple of 64", span);
+  if (!(scale > 0.f) || scale > 1e30f) return set_error(SSD_EINVAL, "attention_q8: scale must be positive, got %g", scale);
+  if (span < 64 || span % 64 || span > 1 << 20) return set_error(SSD_EINVAL, "attention_q8: span %d must be a multiple of 64 up to 2^20", span);
   const int64_t cols = (int64_t)heads * cache->head_dim;
   if (((uintptr_t)q & 15) || ldq % 8 || ldq < cols || ((uintptr_t)out & 15) || ldo % 8 || ldo < cols)
     return set_error(SSD_EINVAL, "attention_q8: q/out rows must be 16-byte aligned with strides >= heads * head_dim");
@@ -384,11 +672,10 @@ SSD_API int ssd_tree_attention_q8(const SsdKvQ8* cache, const uint16_t* q, int64
   a.Q = q, a.ldq = ldq, a.K = cache->k, a.V = cache->v, a.Kx = cache->k_exp, a.Vx = cache->v_exp;
   a.max_len = cache->max_len, a.n_seq = cache->n_seq, a.kv = cache->kv_heads, a.heads = heads, a.rep = heads / a.kv, a.M = M;
   a.row_begin = row_begin, a.prefix = prefix, a.depth = depth, a.anc = anc;
-  a.l_max = l_max, a.span_blk = span / 64, a.n_spans = q8_spans(l_max, span);
-  a.tiles = (rows_max * a.rep + 15) / 16;
+  a.l_max = l_max, a.span_blk = span / 64, a.n_grps = q8_groups(l_max, span);
   a.scale_log2 = scale * 1.4426950408889634f;
   a.ws_o = ws;
-  a.ws_ml = (float2*)(ws + (int64_t)M * heads * a.n_spans * cache->head_dim);
+  a.ws_ml = (float2*)(ws + (int64_t)M * heads * a.n_grps * cache->head_dim);
   a.out = out, a.ldo = ldo;
   return cache->head_dim == 64 ? launch_attn_q8<64>(a, rows_max, stream) : launch_attn_q8<128>(a, rows_max, stream);
 }

@@ -148,7 +148,10 @@ class KVCacheQ8:
 
     @staticmethod
     def default_span(sequences: int, kv_heads: int, capacity: int) -> int:
-        return 256
+        span = 64
+        while span < 1024 and sequences * kv_heads * (capacity // 64) >= 1024 * (2 * span // 64):
+            span *= 2
+        return span
 
     def layer(self, i: int) -> _lib.SsdKvQ8:
         """The descriptor of layer ``i`` for the ops that take a cache."""

@@ -228,6 +228,13 @@ def _table(rows):
     return (_i32(begin), _i32(prefix), _i32(depth), torch.tensor(anc, dtype=torch.int32, device=DEV).view(-1, 32)), begin, prefix, depth, anc
 
 
+def _tolerance(want, mag):
+    """A bf16 rounding is off by at most half a step, 2^-8 of the value (a step is 2^-7 of a power of two). Weights
+    p (1 + d) over the sum of the same: relative error at most 2 * 2^-8 each, so 2^-7 of mag = sum w |v|; the output's own
+    rounding 2^-8 of it; fp32 scores, exp2 and sums together below 2^-12 of mag."""
+    return mag * (2 ** -7 + 2 ** -12) + want.abs() * 2 ** -8
+
+
 def _check_attend(cache, rows, heads, seed, kv_vals, extra=0, ld_pad=0, scale=None, l_max=None):
     tab, begin, prefix, depth, anc = _table(rows)
     hd, M = cache.head_dim, begin[-1]
@@ -240,8 +247,7 @@ def _check_attend(cache, rows, heads, seed, kv_vals, extra=0, ld_pad=0, scale=No
     assert (out[M:] == 7).all() and (out[:, heads * hd:] == 7).all()
     got = out[:M, :heads * hd].cpu().view(M, heads, hd)
     want, mag = ref.tree_attention(q[:M, :heads * hd].view(M, heads, hd), *kv_vals, begin, prefix, depth, anc, scale)
-    # weights rounded to bf16 over their own sum: 2 * 2^-9 of sum w |v|; the output's rounding 2^-9; fp32 scores, exp2, sums: 2^-12
-    err, tol = (got.double() - want).abs(), mag * (2 ** -8 + 2 ** -12) + want.abs() * 2 ** -9
+    err, tol = (got.double() - want).abs(), _tolerance(want, mag)
     assert (err <= tol).all(), (float((err - tol).max()), (err > tol).nonzero()[:4].tolist())
     return got
 
@@ -288,7 +294,7 @@ def test_attend_ancestors_outside_the_cache_are_not_attended():
     q = torch.randn(2, heads * hd, generator=_gen(4)).to(BF16)
     got = cache.attend(0, q.to(DEV), *tab, 2, 128).cpu().view(2, heads, hd).double()
     want, mag = ref.tree_attention(q.view(2, heads, hd), *vals, [0, 2], [70, 0], [2, 0], [[80, 90], []])
-    assert ((got - want).abs() <= mag * (2 ** -8 + 2 ** -12) + want.abs() * 2 ** -9).all() and not got[1].any()
+    assert ((got - want).abs() <= _tolerance(want, mag)).all() and not got[1].any()
 
 
 def test_attend_masked_places_hold_anything():
@@ -329,7 +335,7 @@ def test_attend_nan_and_extreme_values():
     tab, begin, prefix, depth, anc = _table([[(40, [])]])
     got = cache.attend(0, q.to(DEV), *tab, 1, 40).cpu().view(1, heads, hd).double()
     want, mag = ref.tree_attention(q.view(1, heads, hd), *vals, begin, prefix, depth, anc)
-    assert ((got - want).abs() <= mag * (2 ** -8 + 2 ** -12) + want.abs() * 2 ** -9).all()
+    assert ((got - want).abs() <= _tolerance(want, mag)).all()
 
 
 @pytest.mark.parametrize("hd,heads,kv,span", [(128, 8, 2, 64), (128, 4, 1, 256), (64, 32, 8, 128)])
@@ -378,7 +384,7 @@ def test_attend_long_and_past_32_bits():
     for t, s, at in ((0, 0, list(range(5000))), (1, 0, list(range(4990)) + [4995]), (2, 8, [cap - 70 + i for i in range(32)]), (3, 8, [cap - 1])):
         k, v = (x.cpu().view(-1, kv, hd).transpose(0, 1)[None] for x in cache.read(0, _i32([s] * len(at)), _i32(at)))
         want, mag = ref.tree_attention(q[t:t + 1].view(1, heads, hd), k, v, [0, 1], [len(at)], [0], [[]])
-        assert ((got[t] - want[0]).abs() <= mag[0] * (2 ** -8 + 2 ** -12) + want[0].abs() * 2 ** -9).all(), t
+        assert ((got[t] - want[0]).abs() <= _tolerance(want[0], mag[0])).all(), t
 
 
 def test_attend_refuses_bad_tensors():
@@ -539,7 +545,7 @@ def test_a_round_of_them_against_the_definitions():
     tab, begin, prefix, depth, anc = _table(st["rows"])
     got = cache.attend(0, q, *tab, K + 1, st["l_max"]).cpu().view(-1, heads, hd).double()
     want, mag = ref.tree_attention(q.cpu().view(-1, heads, hd), kk, vv, begin, prefix, depth, anc)
-    assert ((got - want).abs() <= mag * (2 ** -8 + 2 ** -12) + want.abs() * 2 ** -9).all()
+    assert ((got - want).abs() <= _tolerance(want, mag)).all()
 
 
 def test_a_captured_round_replays_with_new_inputs():

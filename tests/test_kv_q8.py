@@ -201,7 +201,8 @@ def test_read_and_compact_refusals():
 
 @pytest.mark.parametrize("at,value,code,text", [
     (1, None, BAD, "null"), (13, None, BAD, "null"), (3, -1, BAD, "M=-1"), (4, 3, BAD, "heads"), (4, 0, BAD, "heads"), (9, 0, RANGE, "rows"),
-    (9, 65, RANGE, "rows"), (10, 0, BAD, "l_max"), (10, 129, BAD, "l_max"), (11, 32, BAD, "span"), (11, 96, BAD, "span"), (2, 508, BAD, "strides"),
+    (9, 65, RANGE, "rows"), (10, 0, BAD, "l_max"), (10, 129, BAD, "l_max"), (11, 32, BAD, "span"), (11, 96, BAD, "span"), (12, -1.0, BAD, "scale"), (12, 0.0, BAD, "scale"),
+    (12, float("nan"), BAD, "scale"), (12, float("inf"), BAD, "scale"), (2, 508, BAD, "strides"),
     (1, A + 8, BAD, "aligned"), (16, 504, BAD, "strides"), (14, 100, BAD, "workspace"), (13, A + 4, BAD, "workspace")])
 def test_attention_refusals(at, value, code, text):
     args = [C.byref(_cache()), A, 512, 5, 4, A, A, A, A, 5, 128, 64, 1.0, A, 5 * 4 * 2 * 130, A, 512, None]
@@ -223,9 +224,9 @@ def test_workspace_sizes():
     from ssd import _lib
 
     lib = _lib.load()
-    assert lib.ssd_attn_q8_ws_floats(3, 8, 128, 300, 128) == 3 * 8 * 3 * 130
+    assert lib.ssd_attn_q8_ws_floats(3, 8, 128, 600, 128) == 3 * 8 * 2 * 130
     assert lib.ssd_attn_q8_ws_floats(3, 8, 128, 300, 100) == -1 and lib.ssd_attn_q8_ws_floats(3, 8, 128, 0, 64) == -1
-    assert lib.ssd_attn_q8_ws_floats(64, 64, 128, 1 << 20, 64) == 64 * 64 * (1 << 14) * 130  # past 32 bits
+    assert lib.ssd_attn_q8_ws_floats(64, 64, 128, 1 << 20, 64) == 64 * 64 * (1 << 12) * 130  # past 32 bits
     assert lib.ssd_verify_chain_ws_bytes(3, 4097) == 3 * 2 * 16 and lib.ssd_verify_chain_ws_bytes(3, 0) == -1
 
 
