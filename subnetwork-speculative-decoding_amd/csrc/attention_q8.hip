@@ -84,9 +84,10 @@ __device__ __forceinline__ float q8_max32(float v) {
 // maximum only when that has grown by more than 2^8 (probabilities up to 2^8 are as exact as those up to 1):
 // after a span's first block the sums are hardly ever rescaled. Whether a row rescales is the row's own doing; that
 // a wave skips the products when none of its rows does changes nothing (they would be by 1).
-template <int HD, int T, bool MASKED, bool FIRST>
+// next_k / next_v: load the following block's operands into f, called as soon as this block's are used up.
+template <int HD, int T, bool MASKED, bool FIRST, typename NextK, typename NextV>
 __device__ __forceinline__ void q8_fold(const Q8Frags<HD>& f, const u32x4_t (&qf)[T][HD / 32], uint32_t valid, float scale_log2,
-                                        int j, Q8State<HD> (&st)[T]) {
+                                        int j, Q8State<HD> (&st)[T], NextK next_k, NextV next_v) {
   f32x4_t s[T][4];
 #pragma unroll
   for (int kt = 0; kt < 4; ++kt) {
@@ -102,6 +103,7 @@ __device__ __forceinline__ void q8_fold(const Q8Frags<HD>& f, const u32x4_t (&qf
         for (int t = 0; t < T; ++t) s[t][kt] = mfma16x16x32(ka, bits_bf16x8(qf[t][2 * p + hf]), s[t][kt]);
       }
   }
+  next_k();
   uint32_t pw[T][2][4];
 #pragma unroll
   for (int t = 0; t < T; ++t) {
@@ -159,6 +161,7 @@ __device__ __forceinline__ void q8_fold(const Q8Frags<HD>& f, const u32x4_t (&qf
       }
     }
   }
+  next_v();
 }
 
 // Query fragments: operand 2p + hf holds dims 64 p + 16 g + 8 hf .. + 8 of this lane's row.
@@ -171,17 +174,20 @@ __device__ __forceinline__ void q8_load_q(u32x4_t (&qf)[HD / 32], const bf16_t* 
 }
 
 template <int HD>
-__device__ __forceinline__ void q8_load_block(Q8Frags<HD>& f, const uint8_t* K, const uint8_t* V, const uint8_t* Kx,
-                                              const uint8_t* Vx, int blk, int lane) {
+__device__ __forceinline__ void q8_load_k(Q8Frags<HD>& f, const uint8_t* K, const uint8_t* Kx, int blk, int lane) {
   const uint8_t* kb = K + (size_t)blk * 64 * HD + lane * 16;
-  const uint8_t* vb = V + (size_t)blk * 64 * HD + lane * 16;
 #pragma unroll
   for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
     for (int p = 0; p < HD / 64; ++p) f.k[kt][p] = *(const u32x4_t*)(kb + (kt * (HD / 64) + p) * 1024);
+  f.kx = *(const u32x4_t*)(Kx + (size_t)blk * 64 + (lane >> 2 & 3) * 16);
+}
+
+template <int HD>
+__device__ __forceinline__ void q8_load_v(Q8Frags<HD>& f, const uint8_t* V, const uint8_t* Vx, int blk, int lane) {
+  const uint8_t* vb = V + (size_t)blk * 64 * HD + lane * 16;
 #pragma unroll
   for (int dt = 0; dt < HD / 16; ++dt) f.v[dt] = *(const u32x4_t*)(vb + dt * 1024);
-  f.kx = *(const u32x4_t*)(Kx + (size_t)blk * 64 + (lane >> 2 & 3) * 16);
   f.vx = *(const u32x4_t*)(Vx + (size_t)blk * 64 + (lane >> 4) * 16);
 }
 
@@ -289,13 +295,22 @@ __device__ __forceinline__ void q8_shared_group(const AttnQ8Args& a, int id, Q8S
     const int R = min((tile0 + min(t, a.tiles_per_set - 1)) * 16 + j, n_rows - 1);
     q8_load_q<HD>(qf[t], a.Q + (size_t)(r0 + R / a.rep) * a.ldq + (size_t)(kvh * a.rep + R % a.rep) * HD, g);
   }
-  const int b0 = (grp * QA_GRP + w) * a.span_blk;
+  const uint8_t *K = a.K + reg * HD, *V = a.V + reg * HD, *Kx = a.Kx + reg, *Vx = a.Vx + reg;
+  const int b0 = (grp * QA_GRP + w) * a.span_blk, b1 = b0 + a.span_blk;
   Q8Frags<HD> f;
-  q8_load_block<HD>(f, a.K + reg * HD, a.V + reg * HD, a.Kx + reg, a.Vx + reg, b0, lane);
-  q8_fold<HD, T, false, true>(f, qf, 0, a.scale_log2, j, st);
-  for (int b = b0 + 1; b < b0 + a.span_blk; ++b) {
-    q8_load_block<HD>(f, a.K + reg * HD, a.V + reg * HD, a.Kx + reg, a.Vx + reg, b, lane);
-    q8_fold<HD, T, false, false>(f, qf, 0, a.scale_log2, j, st);
+  q8_load_k<HD>(f, K, Kx, b0, lane);
+  q8_load_v<HD>(f, V, Vx, b0, lane);
+  int b = b0 + 1;
+  auto next_k = [&] {
+    if (b < b1) q8_load_k<HD>(f, K, Kx, b, lane);
+  };
+  auto next_v = [&] {
+    if (b < b1) q8_load_v<HD>(f, V, Vx, b, lane);
+  };
+  q8_fold<HD, T, false, true>(f, qf, 0, a.scale_log2, j, st, next_k, next_v);
+  while (b < b1) {
+    ++b;
+    q8_fold<HD, T, false, false>(f, qf, 0, a.scale_log2, j, st, next_k, next_v);
   }
 #pragma unroll
   for (int t = 0; t < T; ++t) q8_publish<HD>(lds[t], w, j, g, true, st[t]);
@@ -417,9 +432,13 @@ __device__ __forceinline__ bool q8_own_span(const AttnQ8Args& a, size_t reg, int
   for (int b = b0; b < b1; ++b) {
     Q8Frags<HD> f;
     uint32_t valid = 0xffffu;
-    if ((b + 1) * QA_BLK <= P) q8_load_block<HD>(f, K, V, Kx, Vx, b, lane);
-    else valid = q8_load_own<HD>(f, K, V, Kx, Vx, b, P, L, anc, lane);
-    q8_fold<HD, 1, true, false>(f, qf, valid, a.scale_log2, j, st);
+    if ((b + 1) * QA_BLK <= P) {
+      q8_load_k<HD>(f, K, Kx, b, lane);
+      q8_load_v<HD>(f, V, Vx, b, lane);
+    } else {
+      valid = q8_load_own<HD>(f, K, V, Kx, Vx, b, P, L, anc, lane);
+    }
+    q8_fold<HD, 1, true, false>(f, qf, valid, a.scale_log2, j, st, [] {}, [] {});
   }
   return true;
 }
