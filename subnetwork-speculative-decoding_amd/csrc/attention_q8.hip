@@ -88,21 +88,25 @@ __device__ __forceinline__ float q8_max32(float v) {
 template <int HD, int T, bool MASKED, bool FIRST, typename NextK, typename NextV>
 __device__ __forceinline__ void q8_fold(const Q8Frags<HD>& f, const u32x4_t (&qf)[T][HD / 32], uint32_t valid, float scale_log2,
                                         int j, Q8State<HD> (&st)[T], NextK next_k, NextV next_v) {
+  // key tiles innermost: consecutive MFMAs go to different accumulators
   f32x4_t s[T][4];
+  float ks[4];
 #pragma unroll
   for (int kt = 0; kt < 4; ++kt) {
-    const float ks = q8_scale(f.kx[kt] >> (8 * (j & 3)) & 0xffu);
+    ks[kt] = q8_scale(f.kx[kt] >> (8 * (j & 3)) & 0xffu);
 #pragma unroll
     for (int t = 0; t < T; ++t) s[t][kt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
 #pragma unroll
-    for (int p = 0; p < HD / 64; ++p)
+  for (int p = 0; p < HD / 64; ++p)
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const bf16x8_t ka = q8_bf16x8(f.k[kt][p][2 * hf], f.k[kt][p][2 * hf + 1], ks);
+    for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt) {
+        const bf16x8_t ka = q8_bf16x8(f.k[kt][p][2 * hf], f.k[kt][p][2 * hf + 1], ks[kt]);
 #pragma unroll
         for (int t = 0; t < T; ++t) s[t][kt] = mfma16x16x32(ka, bits_bf16x8(qf[t][2 * p + hf]), s[t][kt]);
       }
-  }
   next_k();
   uint32_t pw[T][2][4];
 #pragma unroll
@@ -282,12 +286,26 @@ __device__ __forceinline__ void q8_shared_group(const AttnQ8Args& a, int id, Q8S
   const int kvh = u % a.kv;
   u /= a.kv;
   const int grp = u % a.n_grps, seq = u / a.n_grps;
+  const size_t reg = ((size_t)seq * a.kv + kvh) * a.max_len;
+  const uint8_t *K = a.K + reg * HD, *V = a.V + reg * HD, *Kx = a.Kx + reg, *Vx = a.Vx + reg;
+  const int b0 = (grp * QA_GRP + w) * a.span_blk, b1 = b0 + a.span_blk;
+  Q8Frags<HD> f;
+  // One sequence: nearly all its groups are attended, so the first block is loaded before the rows and the
+  // prefixes are known (a chain of two loads). Of a batch whole sequences may be shorter than l_max.
+  const bool early = a.n_seq == 1 && b1 * QA_BLK <= a.l_max;
+  if (early) {
+    q8_load_k<HD>(f, K, Kx, b0, lane);
+    q8_load_v<HD>(f, V, Vx, b0, lane);
+  }
   int r0, r1;
   q8_rows(a, seq, r0, r1);
   const int n_rows = (r1 - r0) * a.rep, tile0 = set * a.tiles_per_set;
   if (r1 <= r0 || tile0 * 16 >= n_rows) return;
   if ((grp + 1) * QA_GRP * a.span_blk > q8_shared_blocks(a, r0, r1, lane)) return;  // the rows' own
-  const size_t reg = ((size_t)seq * a.kv + kvh) * a.max_len;
+  if (!early) {
+    q8_load_k<HD>(f, K, Kx, b0, lane);
+    q8_load_v<HD>(f, V, Vx, b0, lane);
+  }
   u32x4_t qf[T][HD / 32];
   Q8State<HD> st[T];
 #pragma unroll
@@ -295,11 +313,6 @@ __device__ __forceinline__ void q8_shared_group(const AttnQ8Args& a, int id, Q8S
     const int R = min((tile0 + min(t, a.tiles_per_set - 1)) * 16 + j, n_rows - 1);
     q8_load_q<HD>(qf[t], a.Q + (size_t)(r0 + R / a.rep) * a.ldq + (size_t)(kvh * a.rep + R % a.rep) * HD, g);
   }
-  const uint8_t *K = a.K + reg * HD, *V = a.V + reg * HD, *Kx = a.Kx + reg, *Vx = a.Vx + reg;
-  const int b0 = (grp * QA_GRP + w) * a.span_blk, b1 = b0 + a.span_blk;
-  Q8Frags<HD> f;
-  q8_load_k<HD>(f, K, Kx, b0, lane);
-  q8_load_v<HD>(f, V, Vx, b0, lane);
   int b = b0 + 1;
   auto next_k = [&] {
     if (b < b1) q8_load_k<HD>(f, K, Kx, b, lane);
