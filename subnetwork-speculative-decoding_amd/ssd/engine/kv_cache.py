@@ -15,6 +15,7 @@ accepted-path compaction) is one kernel launch over every layer. ``seq_len`` boo
 
 from __future__ import annotations
 
+import ctypes
 from typing import Optional
 
 import torch
@@ -144,7 +145,7 @@ class KVCacheQ8:
                                      self.v_exp[i].data_ptr(), sequences, kv_heads, head_dim, self.capacity)
                         for i in range(num_slots)]
         for d in self._layers:
-            d.device = self.device
+            d.ref, d.device_index = ctypes.byref(d), self.k.get_device()
 
     @staticmethod
     def default_span(capacity: int) -> int:

@@ -513,93 +513,111 @@ def add_rmsnorm(part, s, ld, h, m, w, eps, out, bias=None):
 
 
 # ------------------------------------------------------------------ 8-bit KV cache (SsdKvQ8)
-def _same_device(*tensors) -> int:
-    """The current stream, for tensors (or cache descriptors) that all live on the current device."""
-    cur = torch.cuda.current_device()
-    for t in tensors:
-        if t is not None and t.device.index != cur:
-            raise ValueError(f"tensors must be on the current device cuda:{cur}, got {t.device}")
-    return torch.cuda.current_stream().cuda_stream
+# These calls take a few microseconds on the device: their checks read each property once and nothing twice.
+I32, F32 = torch.int32, torch.float32
 
 
-def _rope_struct(rope, pos, interleaved, m, head_dim):
-    """SsdRope of (cos, sin) fp32 tables [rows, rot_dim / 2] for ``m`` rows at ``pos``; (None, None) without rope."""
+def _ptr(t, name: str, dtype, dev: int, least: int = 0) -> int:
+    """Address of a ``dtype`` tensor on device ``dev``; ``least`` > 0: contiguous with that many elements or more."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.get_device() != dev:
+        raise ValueError(f"{name} must be a {dtype} tensor on the current device cuda:{dev}, got "
+                         f"{(t.dtype, t.device) if isinstance(t, torch.Tensor) else type(t).__name__}")
+    if least and (t.numel() < least or not t.is_contiguous()):
+        raise ValueError(f"{name} must be contiguous with at least {least} elements, got {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+def _rows_ptr(t, name: str, dev: int, rows: int, cols: int) -> tuple:
+    """Address and row stride of bf16 rows [>= rows, >= cols] with unit column stride and 16-byte alignment."""
+    p = _ptr(t, name, BF16, dev)
+    if t.dim() != 2:
+        raise ValueError(f"{name} must be [>={rows}, >={cols}], got {tuple(t.shape)}")
+    (n, c), (ld, one) = t.shape, t.stride()
+    if n < rows or c < cols or one != 1 or p % 16 or ld % 8:
+        raise ValueError(f"{name} must be [>={rows}, >={cols}] with unit column stride and 16-byte aligned rows, got "
+                         f"{tuple(t.shape)}, strides {t.stride()}")
+    return p, ld
+
+
+def _stream(dev: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(dev)
+
+
+def _cache_dev(cache) -> int:
+    """The current device, which has to be the cache's."""
+    dev = torch.cuda.current_device()
+    if cache.device_index != dev:
+        raise ValueError(f"the cache is on cuda:{cache.device_index}, the current device is cuda:{dev}")
+    return dev
+
+
+def _rope_struct(rope, pos, interleaved, m, head_dim, dev):
+    """(SsdRope reference, positions' address) of (cos, sin) fp32 tables [rows, rot_dim / 2]; (None, None) without rope."""
     if rope is None:
         if pos is not None:
             raise ValueError("positions without rotary tables")
         return None, None
     cos, sin = rope
-    _check(cos, "cos", torch.float32); _check(sin, "sin", torch.float32)
-    if cos.dim() != 2 or cos.shape != sin.shape or not (cos.is_contiguous() and sin.is_contiguous()):
-        raise ValueError("rotary tables must be two contiguous [rows, rot_dim / 2] tensors")
-    if pos is None:
-        raise ValueError("rotary tables without positions")
-    _check(pos, "pos", torch.int32)
-    _vec(pos, "pos", m)
-    if 2 * cos.shape[1] > head_dim:
-        raise ValueError(f"rotary tables turn {2 * cos.shape[1]} dims of a head of {head_dim}")
-    return _lib.SsdRope(cos.data_ptr(), sin.data_ptr(), cos.shape[0], 2 * cos.shape[1], int(interleaved)), pos.data_ptr()
-
-
-def _vec(t: torch.Tensor, name: str, n: int) -> None:
-    if not t.is_contiguous() or t.numel() < n:
-        raise ValueError(f"{name} must be contiguous with at least {n} elements, got {tuple(t.shape)}")
+    if cos.dim() != 2 or cos.shape != sin.shape or 2 * cos.shape[1] > head_dim:
+        raise ValueError(f"rotary tables must be two [rows, rot_dim / 2] tensors, rot_dim <= {head_dim}, got "
+                         f"{tuple(cos.shape)}, {tuple(sin.shape)}")
+    n, half = cos.shape
+    st = _lib.SsdRope(_ptr(cos, "cos", F32, dev, n * half), _ptr(sin, "sin", F32, dev, n * half), n, 2 * half,
+                      1 if interleaved else 0)
+    return ctypes.byref(st), _ptr(pos, "pos", I32, dev, m)
 
 
 def rope(x, m, heads, head_dim, tables, pos, out, interleaved: bool = False):
     """out[:m] = x[:m] rotated to ``pos`` (int32): ``heads`` heads of ``head_dim`` a row, the first 2 * tables[0].shape[1]
     dims of each in pairs (i, i + rot / 2), or (2i, 2i + 1) when ``interleaved``. ``out`` may be ``x``."""
-    _check(x, "x"); _check(out, "out")
-    cols = heads * head_dim
-    st, pp = _rope_struct(tables, pos, interleaved, m, head_dim)
-    if st is None:
+    dev = torch.cuda.current_device()
+    if tables is None:
         raise ValueError("rope needs rotary tables")
-    if m == 0:
-        return out
-    _lib.call("ssd_rope_bf16", ctypes.byref(st), pp, x.data_ptr(), _rows(x, "x", cols, m), m, heads, head_dim,
-              out.data_ptr(), _rows(out, "out", cols, m), _same_device(x, out, pos, *tables))
+    px, ldx = _rows_ptr(x, "x", dev, m, heads * head_dim)
+    po, ldo = _rows_ptr(out, "out", dev, m, heads * head_dim)
+    st, pp = _rope_struct(tables, pos, interleaved, m, head_dim, dev)
+    if m:
+        _lib.call("ssd_rope_bf16", st, pp, px, ldx, m, heads, head_dim, po, ldo, _stream(dev))
     return out
 
 
 def kv_q8_write(cache, k, v, m, seq, slot, rope=None, pos=None, interleaved=False, q=None, heads=0, q_out=None):
     """Rows of K (rotated first when ``rope`` is given) and V quantised into ``cache`` (SsdKvQ8 of one layer) at
     (seq, slot); with ``q`` its rows are rotated into ``q_out`` in the same launch (ssd_kv_q8_write_bf16)."""
-    _check(k, "k"); _check(v, "v"); _check(seq, "seq", torch.int32); _check(slot, "slot", torch.int32)
-    _vec(seq, "seq", m); _vec(slot, "slot", m)
-    hd = cache.head_dim
-    cols, ldq, ldo = cache.kv_heads * hd, 0, 0
-    st, pp = _rope_struct(rope, pos, interleaved, m, hd)
-    if m == 0:
-        return
+    dev, hd = _cache_dev(cache), cache.head_dim
+    cols = cache.kv_heads * hd
+    pk, ldk = _rows_ptr(k, "k", dev, m, cols)
+    pv, ldv = _rows_ptr(v, "v", dev, m, cols)
+    ps, pl = _ptr(seq, "seq", I32, dev, m), _ptr(slot, "slot", I32, dev, m)
+    st, pp = _rope_struct(rope, pos, interleaved, m, hd, dev)
+    pq = po = None
+    ldq = ldo = 0
     if q is not None:
-        _check(q, "q"); _check(q_out, "q_out")
-        ldq, ldo = _rows(q, "q", heads * hd, m), _rows(q_out, "q_out", heads * hd, m)
-    _lib.call("ssd_kv_q8_write_bf16", ctypes.byref(cache), k.data_ptr(), _rows(k, "k", cols, m), v.data_ptr(),
-              _rows(v, "v", cols, m), m, seq.data_ptr(), slot.data_ptr(), st and ctypes.byref(st), pp, _p(q), ldq,
-              heads, _p(q_out), ldo, _same_device(cache, k, v, seq, slot, q, q_out, pos, *(rope or ())))
+        pq, ldq = _rows_ptr(q, "q", dev, m, heads * hd)
+        po, ldo = _rows_ptr(q_out, "q_out", dev, m, heads * hd)
+    if m:
+        _lib.call("ssd_kv_q8_write_bf16", cache.ref, pk, ldk, pv, ldv, m, ps, pl, st, pp, pq, ldq, heads, po, ldo,
+                  _stream(dev))
 
 
 def kv_q8_read(cache, m, seq, slot, k_out, v_out):
     """The cached values of (seq, slot) as bf16 rows (ssd_kv_q8_read_bf16); zeros for places outside the cache."""
-    _check(k_out, "k_out"); _check(v_out, "v_out"); _check(seq, "seq", torch.int32); _check(slot, "slot", torch.int32)
-    _vec(seq, "seq", m); _vec(slot, "slot", m)
+    dev = _cache_dev(cache)
     cols = cache.kv_heads * cache.head_dim
-    if m == 0:
-        return
-    _lib.call("ssd_kv_q8_read_bf16", ctypes.byref(cache), m, seq.data_ptr(), slot.data_ptr(), k_out.data_ptr(),
-              _rows(k_out, "k_out", cols, m), v_out.data_ptr(), _rows(v_out, "v_out", cols, m),
-              _same_device(cache, k_out, v_out, seq, slot))
+    ps, pl = _ptr(seq, "seq", I32, dev, m), _ptr(slot, "slot", I32, dev, m)
+    pk, ldk = _rows_ptr(k_out, "k_out", dev, m, cols)
+    pv, ldv = _rows_ptr(v_out, "v_out", dev, m, cols)
+    if m:
+        _lib.call("ssd_kv_q8_read_bf16", cache.ref, m, ps, pl, pk, ldk, pv, ldv, _stream(dev))
 
 
 def kv_q8_compact(cache, layers, start, src, n, n_max):
     """Per sequence, slots src[s, :n[s]] to [start[s], ...) in ``layers`` layers (ssd_kv_q8_compact)."""
-    for t, nm, k in ((start, "start", cache.n_seq), (src, "src", cache.n_seq * n_max), (n, "n", cache.n_seq)):
-        _check(t, nm, torch.int32)
-        _vec(t, nm, k)
-    if n_max == 0:
-        return
-    _lib.call("ssd_kv_q8_compact", ctypes.byref(cache), layers, start.data_ptr(), src.data_ptr(), n.data_ptr(), n_max,
-              _same_device(cache, start, src, n))
+    dev, seqs = _cache_dev(cache), cache.n_seq
+    pst, pn = _ptr(start, "start", I32, dev, seqs), _ptr(n, "n", I32, dev, seqs)
+    psr = _ptr(src, "src", I32, dev, seqs * n_max)
+    if n_max:
+        _lib.call("ssd_kv_q8_compact", cache.ref, layers, pst, psr, pn, n_max, _stream(dev))
 
 
 def attn_q8_ws_floats(m: int, heads: int, head_dim: int, l_max: int, span: int) -> int:
@@ -611,18 +629,15 @@ def attn_q8_ws_floats(m: int, heads: int, head_dim: int, l_max: int, span: int) 
 
 def tree_attention_q8(cache, q, m, heads, row_begin, prefix, depth, anc, rows_max, l_max, span, ws, out, scale=None):
     """Tree attention of a batch's rows over ``cache`` (SsdKvQ8 of one layer; ssd_tree_attention_q8)."""
-    hd = cache.head_dim
-    _check(q, "q"); _check(out, "out"); _check(ws, "ws", torch.float32)
-    for t, nm, n in ((row_begin, "row_begin", cache.n_seq + 1), (prefix, "prefix", m), (depth, "depth", m),
-                     (anc, "anc", m * 32)):
-        _check(t, nm, torch.int32)
-        _vec(t, nm, n)
-    if m == 0:
-        return out
-    _lib.call("ssd_tree_attention_q8", ctypes.byref(cache), q.data_ptr(), _rows(q, "q", heads * hd, m), m, heads,
-              row_begin.data_ptr(), prefix.data_ptr(), depth.data_ptr(), anc.data_ptr(), rows_max, l_max, span,
-              hd ** -0.5 if scale is None else float(scale), ws.data_ptr(), ws.numel(), out.data_ptr(),
-              _rows(out, "out", heads * hd, m), _same_device(cache, q, out, ws, row_begin, prefix, depth, anc))
+    dev, hd = _cache_dev(cache), cache.head_dim
+    pq, ldq = _rows_ptr(q, "q", dev, m, heads * hd)
+    po, ldo = _rows_ptr(out, "out", dev, m, heads * hd)
+    pb, pp = _ptr(row_begin, "row_begin", I32, dev, cache.n_seq + 1), _ptr(prefix, "prefix", I32, dev, m)
+    pd, pa = _ptr(depth, "depth", I32, dev, m), _ptr(anc, "anc", I32, dev, m * 32)
+    pw = _ptr(ws, "ws", F32, dev, 1)
+    if m:
+        _lib.call("ssd_tree_attention_q8", cache.ref, pq, ldq, m, heads, pb, pp, pd, pa, rows_max, l_max, span,
+                  hd ** -0.5 if scale is None else float(scale), pw, ws.numel(), po, ldo, _stream(dev))
     return out
 
 
@@ -745,28 +760,24 @@ def verify_chain_ws_bytes(n_seq: int, V: int) -> int:
 
 def verify_chain(P, Q, draft, u, u_next, n_draft, out_tok, out_n, ws):
     """ssd_verify_chain over P [n_seq, k + 1, V] and Q [n_seq, k, V] fp32 (unit column stride)."""
+    dev = torch.cuda.current_device()
     n_seq, rows, V = P.shape
     k = rows - 1
-    for t, nm, shape in ((P, "P", (n_seq, k + 1, V)), (Q, "Q", (n_seq, k, V)), (u, "u", (n_seq, k)),
-                         (u_next, "u_next", (n_seq,))):
-        _check(t, nm, torch.float32)
-        if tuple(t.shape) != shape:
-            raise ValueError(f"{nm} must be {shape}, got {tuple(t.shape)}")
-    for t, nm, shape in ((draft, "draft", (n_seq, k)), (n_draft, "n_draft", (n_seq,)), (out_tok, "out_tok", (n_seq, k + 1)),
-                         (out_n, "out_n", (n_seq,))):
-        if t is None and nm == "n_draft":
-            continue
-        _check(t, nm, torch.int32)
-        if tuple(t.shape) != shape:
-            raise ValueError(f"{nm} must be {shape}, got {tuple(t.shape)}")
-    for t, nm in ((u, "u"), (u_next, "u_next"), (draft, "draft"), (n_draft, "n_draft"), (out_tok, "out_tok"), (out_n, "out_n")):
-        if t is not None and not t.is_contiguous():
-            raise ValueError(f"{nm} must be contiguous")
-    if V > 1 and (P.stride(2) != 1 or (k and Q.stride(2) != 1)):
+    if Q.shape != (n_seq, k, V) or draft.shape != (n_seq, k) or u.shape != (n_seq, k) or u_next.shape != (n_seq,) or (
+            n_draft is not None and n_draft.shape != (n_seq,)) or out_tok.shape != (n_seq, rows) or out_n.shape != (n_seq,):
+        raise ValueError(f"verify_chain: for P {tuple(P.shape)} the others must be Q {(n_seq, k, V)}, draft and u {(n_seq, k)}, "
+                         f"u_next, n_draft and out_n {(n_seq,)}, out_tok {(n_seq, rows)}; got Q {tuple(Q.shape)}, draft "
+                         f"{tuple(draft.shape)}, u {tuple(u.shape)}, u_next {tuple(u_next.shape)}")
+    pp, pq = _ptr(P, "P", F32, dev), _ptr(Q, "Q", F32, dev)
+    pst, qst = P.stride(), Q.stride()
+    if V > 1 and (pst[2] != 1 or (k and qst[2] != 1)):
         raise ValueError("P and Q need unit column stride")
-    _check(ws, "ws", torch.uint8)
     if n_seq == 0:
         return
-    _lib.call("ssd_verify_chain", P.data_ptr(), P.stride(0), P.stride(1), Q.data_ptr(), Q.stride(0), Q.stride(1), V, n_seq, k,
-              draft.data_ptr(), _p(n_draft), u.data_ptr(), u_next.data_ptr(), ws.data_ptr(), ws.numel(), out_tok.data_ptr(),
-              out_n.data_ptr(), _same_device(P, Q, draft, n_draft, u, u_next, ws, out_tok, out_n))
+    # a dimension of one row has any stride
+    pd, pu = _ptr(draft, "draft", I32, dev, n_seq * k), _ptr(u, "u", F32, dev, n_seq * k)
+    pn, px = None if n_draft is None else _ptr(n_draft, "n_draft", I32, dev, n_seq), _ptr(u_next, "u_next", F32, dev, n_seq)
+    _lib.call("ssd_verify_chain", pp, pst[0], max(pst[1], V) if rows == 1 else pst[1], pq, qst[0],
+              max(qst[1], V) if k == 1 else qst[1], V, n_seq, k, pd, pn, pu, px, _ptr(ws, "ws", torch.uint8, dev, 1),
+              ws.numel(), _ptr(out_tok, "out_tok", I32, dev, n_seq * rows), _ptr(out_n, "out_n", I32, dev, n_seq),
+              _stream(dev))
