@@ -452,7 +452,7 @@ int ssd_accept_sample(const SsdTree* tree, const float* P, int64_t ldp, const fl
  * the next one is drawn from max(P_n - Q_n, 0) -- from P_n when every draft was accepted or that has no mass --
  * as the least y whose cumulative mass exceeds u_next[s] * total, all sums in 64 bits; a row without mass gives
  * -1. out_n[s] = n; out_tok[s][k_max + 1] = the accepted tokens, the next one, then -1.
- * ws: ssd_verify_chain_ws_bytes(n_seq, V) bytes, 8-byte aligned, no clearing needed; calls that overlap in time
+ * ws: ssd_verify_chain_ws_bytes(n_seq, V) bytes, 16-byte aligned, no clearing needed; calls that overlap in time
  * must not share it. k_max <= 64, V <= 2^24. */
 int64_t ssd_verify_chain_ws_bytes(int n_seq, int V);
 int ssd_verify_chain(const float* P, int64_t ldp_seq, int64_t ldp, const float* Q, int64_t ldq_seq, int64_t ldq, int V,

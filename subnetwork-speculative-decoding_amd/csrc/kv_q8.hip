@@ -57,30 +57,51 @@ __device__ __forceinline__ void store_chunk(bf16_t* p, const Chunk<E>& c) {
   else *(uint2*)p = make_uint2(w[0], w[1]);
 }
 
-// Dims d0 .. d0 + E of a head at x, rotated for one token. Products and sums are rounded one by one (no
-// multiply-add contraction), so the codes a rotated row is quantised to do not depend on the compiler.
+// cos and sin of dims d0 .. d0 + E for one token (their pairs' entries when interleaved), and whether they turn.
 template <int E>
-__device__ __forceinline__ Chunk<E> load_rotated(const bf16_t* x, int d0, const RopeArgs& r, int64_t pos) {
+struct Turn {
+  float c[E], s[E];
+  bool on;
+};
+
+template <int E>
+__device__ __forceinline__ Turn<E> load_turn(const RopeArgs& r, int d0, int64_t pos) {
+  Turn<E> t;
+  t.on = r.cos && d0 < r.rot;
+  if (!t.on) return t;
+  const int half = r.rot >> 1, e0 = r.interleaved ? d0 >> 1 : d0 < half ? d0 : d0 - half;
+  const float *ct = r.cos + pos * half + e0, *st = r.sin + pos * half + e0;
+  if (r.interleaved) {
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i) t.c[i] = ct[i], t.s[i] = st[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; ++i) t.c[i] = ct[i], t.s[i] = st[i];
+  }
+  return t;
+}
+
+// Dims d0 .. d0 + E of the head at x, rotated. Products and sums are rounded one by one (no multiply-add
+// contraction), so the codes a rotated row is quantised to do not depend on the compiler.
+template <int E>
+__device__ __forceinline__ Chunk<E> load_rotated(const bf16_t* x, int d0, const RopeArgs& r, const Turn<E>& t) {
 #pragma clang fp contract(off)
   Chunk<E> c = load_chunk<E>(x + d0);
-  if (!r.cos || d0 >= r.rot) return c;
-  const int half = r.rot >> 1;
-  const float *ct = r.cos + pos * half, *st = r.sin + pos * half;
+  if (!t.on) return c;
   if (r.interleaved) {
 #pragma unroll
     for (int i = 0; i < E; i += 2) {
-      const float cc = ct[(d0 + i) >> 1], ss = st[(d0 + i) >> 1], a = c.x[i], b = c.x[i + 1];
-      c.x[i] = a * cc - b * ss;
-      c.x[i + 1] = b * cc + a * ss;
+      const float a = c.x[i], b = c.x[i + 1];
+      c.x[i] = a * t.c[i / 2] - b * t.s[i / 2];
+      c.x[i + 1] = b * t.c[i / 2] + a * t.s[i / 2];
     }
   } else {
-    const bool low = d0 < half;  // half is a multiple of 8: a chunk lies in one half
+    const int half = r.rot >> 1;  // a multiple of 8: a chunk lies in one half
+    const bool low = d0 < half;
     const Chunk<E> o = load_chunk<E>(x + (low ? d0 + half : d0 - half));
-    const int t0 = low ? d0 : d0 - half;
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      const float cc = ct[t0 + i], ss = st[t0 + i];
-      const float xc = c.x[i] * cc, os = o.x[i] * ss;
+      const float xc = c.x[i] * t.c[i], os = o.x[i] * t.s[i];
       c.x[i] = low ? xc - os : xc + os;
     }
   }
@@ -93,8 +114,16 @@ __device__ __forceinline__ int64_t rope_row(const RopeArgs& r, int row) {
   return p < 0 ? 0 : p < r.rows ? p : r.rows - 1;
 }
 
+// Largest value over the 16 lanes of a row of the wave.
+__device__ __forceinline__ uint32_t max16(uint32_t v) {
+  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xb1, 0xf, 0xf, true));   // lane ^ 1
+  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4e, 0xf, 0xf, true));   // lane ^ 2
+  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xf, 0xf, true));  // the other half of 8
+  return max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x140, 0xf, 0xf, true));  // the other half of 16
+}
+
 // The row's exponent byte (the same on its 16 lanes) and the chunk's codes. Values that are not finite do
-// not count for the exponent and are stored as NaN.
+// not count for the exponent and are stored as NaN. All 16 lanes call it together.
 template <int E>
 __device__ __forceinline__ int quantise(const Chunk<E>& c, uint32_t (&w)[E / 4]) {
   uint32_t top = 0;
@@ -103,9 +132,7 @@ __device__ __forceinline__ int quantise(const Chunk<E>& c, uint32_t (&w)[E / 4])
     const uint32_t u = __float_as_uint(c.x[i]) & 0x7fffffffu;
     top = max(top, u < 0x7f800000u ? u : 0u);
   }
-#pragma unroll
-  for (int o = 1; o < 16; o <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
-  const int b = q8_exponent(__uint_as_float(top));
+  const int b = q8_exponent(__uint_as_float(max16(top)));
   const float inv = q8_inv_scale(b);
   float y[E];
 #pragma unroll
@@ -121,39 +148,113 @@ __device__ __forceinline__ int quantise(const Chunk<E>& c, uint32_t (&w)[E / 4])
   return b;
 }
 
-// Sixteen lanes per (token, head), E = head_dim / 16 dims a lane.
-template <int HD>
-__global__ __launch_bounds__(256) void kv_q8_write_kernel(WriteArgs a) {
+// Bytes i of four words become word i.
+__device__ __forceinline__ void transpose4(uint32_t (&w)[4]) {
+  const uint32_t l01 = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u), h01 = __builtin_amdgcn_perm(w[1], w[0], 0x07030602u);
+  const uint32_t l23 = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u), h23 = __builtin_amdgcn_perm(w[3], w[2], 0x07030602u);
+  w[0] = __builtin_amdgcn_perm(l23, l01, 0x05040100u), w[1] = __builtin_amdgcn_perm(l23, l01, 0x07060302u);
+  w[2] = __builtin_amdgcn_perm(h23, h01, 0x05040100u), w[3] = __builtin_amdgcn_perm(h23, h01, 0x07060302u);
+}
+
+// The R rows of a unit: where each goes, and whether they are four consecutive slots of one aligned quad (whose V
+// codes of one dim, and whose exponents, are one word).
+template <int R>
+struct Places {
+  int64_t reg[R];  // sequence * kv_heads, -1: outside the cache (or no such row)
+  int slot[R];
+  bool quad;
+};
+
+// Units of R = 4 rows start where row 0's slot quad does, so that a prompt's consecutive rows fall into whole quads.
+template <int R>
+__device__ __forceinline__ int unit_row(const int* slot, int unit) {
+  return R == 1 ? unit : unit * R - (slot[0] & (R - 1));
+}
+
+template <int R>
+__device__ __forceinline__ Places<R> load_places(const int* seq, const int* slot, int row0, int M, int n_seq, int64_t max_len, int kv) {
+  Places<R> p;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int row = row0 + i, r = min(max(row, 0), M - 1), sq = seq[r];
+    p.slot[i] = slot[r];
+    p.reg[i] = row == r && sq >= 0 && sq < n_seq && p.slot[i] >= 0 && p.slot[i] < max_len ? (int64_t)sq * kv : -1;
+  }
+  p.quad = R == 4 && p.reg[0] >= 0 && (p.slot[0] & 3) == 0;
+#pragma unroll
+  for (int i = 1; i < R; ++i) p.quad = p.quad && p.reg[i] == p.reg[0] && p.slot[i] == p.slot[0] + i;
+  return p;
+}
+
+// Workgroups [0, kv_wgs) write K and V: sixteen lanes per (R rows, kv head, K or V), E = head_dim / 16 dims a lane.
+// The others rotate q: sixteen lanes per (row, H heads), which share the row's cos and sin. R and H are 4 from
+// 256 rows on. Bound by the bytes of q (64 MiB of 96 for 4096 rows of 32 + 8 heads of 128).
+template <int HD, int R, int H>
+__global__ __launch_bounds__(256) void kv_q8_write_kernel(WriteArgs a, int kv_wgs, int kv_units, int q_units) {
   constexpr int E = HD / 16;
-  const int units = a.heads + 2 * a.kv;
-  const int64_t id = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-  if (id >= (int64_t)a.M * units) return;
-  const int row = (int)(id / units), u = (int)(id % units), ln = threadIdx.x & 15, d0 = ln * E;
-  if (u < a.heads) {
-    const Chunk<E> c = load_rotated<E>(a.q + (size_t)row * a.ldq + (size_t)u * HD, d0, a.rope, rope_row(a.rope, row));
-    store_chunk<E>(a.q_out + (size_t)row * a.ldo + (size_t)u * HD + d0, c);
+  const int ln = threadIdx.x & 15, d0 = ln * E;
+  if ((int)blockIdx.x >= kv_wgs) {
+    const int64_t id = (int64_t)(blockIdx.x - kv_wgs) * 16 + (threadIdx.x >> 4);
+    if (id >= (int64_t)a.M * q_units) return;
+    const int row = (int)(id / q_units), h0 = (int)(id % q_units) * H;
+    const Turn<E> t = load_turn<E>(a.rope, d0, rope_row(a.rope, row));
+    const bf16_t* x = a.q + (size_t)row * a.ldq;
+    bf16_t* y = a.q_out + (size_t)row * a.ldo;
+    Chunk<E> c[H];
+#pragma unroll
+    for (int i = 0; i < H; ++i) c[i] = load_rotated<E>(x + (size_t)min(h0 + i, a.heads - 1) * HD, d0, a.rope, t);
+#pragma unroll
+    for (int i = 0; i < H; ++i)
+      if (h0 + i < a.heads) store_chunk<E>(y + (size_t)(h0 + i) * HD + d0, c[i]);
     return;
   }
-  const int sq = a.seq[row], sl = a.slot[row];
-  if (sq < 0 || sq >= a.n_seq || sl < 0 || sl >= a.max_len) return;
-  const bool is_v = u >= a.heads + a.kv;
-  const int h = u - a.heads - (is_v ? a.kv : 0);
-  const size_t reg = (size_t)sq * a.kv + h;
-  uint32_t w[E / 4];
-  if (!is_v) {
-    const Chunk<E> c = load_rotated<E>(a.k + (size_t)row * a.ldk + (size_t)h * HD, d0, a.rope, rope_row(a.rope, row));
-    const int b = quantise<E>(c, w);
-    uint8_t* dst = a.ck + reg * a.max_len * HD + q8_k_off(sl, d0, HD);
-    if constexpr (E == 8) *(uint2*)dst = make_uint2(w[0], w[1]);
-    else *(uint32_t*)dst = w[0];
-    if (ln == 0) a.cxk[reg * a.max_len + q8_x_off(sl)] = (uint8_t)b;
-  } else {
-    const Chunk<E> c = load_chunk<E>(a.v + (size_t)row * a.ldv + (size_t)h * HD + d0);
-    const int b = quantise<E>(c, w);
-    uint8_t* dst = a.cv + reg * a.max_len * HD + q8_v_off(sl, d0, HD);
+  const int id = blockIdx.x * 16 + (threadIdx.x >> 4), unit = id / (2 * a.kv);
+  if (unit >= kv_units) return;
+  const int u = id % (2 * a.kv), h = u < a.kv ? u : u - a.kv;
+  const bool is_v = u >= a.kv;
+  const int row0 = unit_row<R>(a.slot, unit);
+  const Places<R> at = load_places<R>(a.seq, a.slot, row0, a.M, a.n_seq, a.max_len, a.kv);
+  uint32_t w[R][E / 4];
+  int b[R];
 #pragma unroll
-    for (int i = 0; i < E; ++i) dst[i * 16] = (uint8_t)(w[i / 4] >> (8 * (i & 3)));
-    if (ln == 0) a.cxv[reg * a.max_len + q8_x_off(sl)] = (uint8_t)b;
+  for (int i = 0; i < R; ++i) {
+    const int row = min(max(row0 + i, 0), a.M - 1);
+    Chunk<E> c;
+    if (is_v) c = load_chunk<E>(a.v + (size_t)row * a.ldv + (size_t)h * HD + d0);
+    else c = load_rotated<E>(a.k + (size_t)row * a.ldk + (size_t)h * HD, d0, a.rope, load_turn<E>(a.rope, d0, rope_row(a.rope, row)));
+    b[i] = quantise<E>(c, w[i]);
+  }
+  uint8_t *codes = is_v ? a.cv : a.ck, *exps = is_v ? a.cxv : a.cxk;
+  if constexpr (R == 4)
+    if (at.quad) {
+      const int64_t reg = at.reg[0] + h;
+      if (ln == 0) *(uint32_t*)(exps + reg * a.max_len + q8_x_off(at.slot[0])) = b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24;
+      if (is_v) {
+        uint8_t* dst = codes + reg * a.max_len * HD + q8_v_off(at.slot[0], d0, HD);
+#pragma unroll
+        for (int k = 0; k < E / 4; ++k) {
+          uint32_t t[4] = {w[0][k], w[1][k], w[2][k], w[3][k]};
+          transpose4(t);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) *(uint32_t*)(dst + (4 * k + i) * 16) = t[i];
+        }
+        return;
+      }
+    }
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    if (at.reg[i] < 0) continue;
+    const int64_t reg = at.reg[i] + h;
+    if (!is_v) {
+      uint8_t* dst = codes + reg * a.max_len * HD + q8_k_off(at.slot[i], d0, HD);
+      if constexpr (E == 8) *(uint2*)dst = make_uint2(w[i][0], w[i][1]);
+      else *(uint32_t*)dst = w[i][0];
+    } else {
+      uint8_t* dst = codes + reg * a.max_len * HD + q8_v_off(at.slot[i], d0, HD);
+#pragma unroll
+      for (int e = 0; e < E; ++e) dst[e * 16] = (uint8_t)(w[i][e / 4] >> (8 * (e & 3)));
+    }
+    if (ln == 0 && !(R == 4 && at.quad)) exps[reg * a.max_len + q8_x_off(at.slot[i])] = (uint8_t)b[i];
   }
 }
 
@@ -166,45 +267,77 @@ struct ReadArgs {
   int64_t ldk, ldv;
 };
 
-template <int HD>
-__global__ __launch_bounds__(256) void kv_q8_read_kernel(ReadArgs a) {
+// Sixteen lanes per (R rows, kv head, K or V), as they are written.
+template <int HD, int R>
+__global__ __launch_bounds__(256) void kv_q8_read_kernel(ReadArgs a, int units) {
   constexpr int E = HD / 16;
-  const int64_t id = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-  if (id >= (int64_t)a.M * 2 * a.kv) return;
-  const int row = (int)(id / (2 * a.kv)), u = (int)(id % (2 * a.kv)), ln = threadIdx.x & 15, d0 = ln * E;
-  const int sq = a.seq[row], sl = a.slot[row];
+  const int id = blockIdx.x * 16 + (threadIdx.x >> 4), unit = id / (2 * a.kv), ln = threadIdx.x & 15, d0 = ln * E;
+  if (unit >= units) return;
+  const int u = id % (2 * a.kv), h = u < a.kv ? u : u - a.kv;
   const bool is_v = u >= a.kv;
-  const int h = is_v ? u - a.kv : u;
-  bf16_t* dst = (is_v ? a.v + (size_t)row * a.ldv : a.k + (size_t)row * a.ldk) + (size_t)h * HD + d0;
-  if (sq < 0 || sq >= a.n_seq || sl < 0 || sl >= a.max_len) {
-    store_chunk<E>(dst, Chunk<E>{});
-    return;
-  }
-  const size_t reg = (size_t)sq * a.kv + h;
-  uint32_t w[E / 4];
-  if (!is_v) {
-    const uint8_t* src = a.ck + reg * a.max_len * HD + q8_k_off(sl, d0, HD);
-    if constexpr (E == 8) {
-      const uint2 t = *(const uint2*)src;
-      w[0] = t.x, w[1] = t.y;
-    } else {
-      w[0] = *(const uint32_t*)src;
+  const int row0 = unit_row<R>(a.slot, unit);
+  const Places<R> at = load_places<R>(a.seq, a.slot, row0, a.M, a.n_seq, a.max_len, a.kv);
+  const uint8_t *codes = is_v ? a.cv : a.ck, *exps = is_v ? a.cxv : a.cxk;
+  uint32_t w[R][E / 4], b[R];
+  bool done = false;
+  if constexpr (R == 4)
+    if (at.quad) {
+      const int64_t reg = at.reg[0] + h;
+      const uint32_t x = *(const uint32_t*)(exps + reg * a.max_len + q8_x_off(at.slot[0]));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) b[i] = x >> (8 * i) & 0xffu;
+      if (is_v) {
+        done = true;
+        const uint8_t* src = codes + reg * a.max_len * HD + q8_v_off(at.slot[0], d0, HD);
+#pragma unroll
+        for (int k = 0; k < E / 4; ++k) {
+          uint32_t t[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) t[i] = *(const uint32_t*)(src + (4 * k + i) * 16);
+          transpose4(t);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i][k] = t[i];
+        }
+      }
     }
-  } else {
-    const uint8_t* src = a.cv + reg * a.max_len * HD + q8_v_off(sl, d0, HD);
+  if (!done) {
 #pragma unroll
-    for (int i = 0; i < E; i += 4)
-      w[i / 4] = src[i * 16] | src[i * 16 + 16] << 8 | src[i * 16 + 32] << 16 | (uint32_t)src[i * 16 + 48] << 24;
-  }
-  const float sc = q8_scale((is_v ? a.cxv : a.cxk)[reg * a.max_len + q8_x_off(sl)]);
-  Chunk<E> c;
+    for (int i = 0; i < R; ++i) {  // places outside the cache read the first one's codes, and are cleared below
+      const int64_t reg = max(at.reg[i], (int64_t)0) + h;
+      const int sl = at.reg[i] < 0 ? 0 : at.slot[i];
+      b[i] = exps[reg * a.max_len + q8_x_off(sl)];
+      if (!is_v) {
+        const uint8_t* src = codes + reg * a.max_len * HD + q8_k_off(sl, d0, HD);
+        if constexpr (E == 8) {
+          const uint2 t = *(const uint2*)src;
+          w[i][0] = t.x, w[i][1] = t.y;
+        } else {
+          w[i][0] = *(const uint32_t*)src;
+        }
+      } else {
+        const uint8_t* src = codes + reg * a.max_len * HD + q8_v_off(sl, d0, HD);
 #pragma unroll
-  for (int i = 0; i < E; i += 4) {
-    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i / 4], false);
-    const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i / 4], true);
-    c.x[i] = lo[0] * sc, c.x[i + 1] = lo[1] * sc, c.x[i + 2] = hi[0] * sc, c.x[i + 3] = hi[1] * sc;
+        for (int e = 0; e < E; e += 4)
+          w[i][e / 4] = src[e * 16] | src[e * 16 + 16] << 8 | src[e * 16 + 32] << 16 | (uint32_t)src[e * 16 + 48] << 24;
+      }
+    }
   }
-  store_chunk<E>(dst, c);
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int row = row0 + i;
+    if (row < 0 || row >= a.M) continue;
+    const bool in = at.reg[i] >= 0;
+    const float sc = q8_scale(b[i]);
+    Chunk<E> c;
+#pragma unroll
+    for (int e = 0; e < E; e += 4) {
+      const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i][e / 4], false);
+      const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i][e / 4], true);
+      c.x[e] = in ? lo[0] * sc : 0.f, c.x[e + 1] = in ? lo[1] * sc : 0.f;
+      c.x[e + 2] = in ? hi[0] * sc : 0.f, c.x[e + 3] = in ? hi[1] * sc : 0.f;
+    }
+    store_chunk<E>((is_v ? a.v + (size_t)row * a.ldv : a.k + (size_t)row * a.ldk) + (size_t)h * HD + d0, c);
+  }
 }
 
 // One workgroup per (layer, sequence, kv head): every source row is read (K and V as 16-byte pieces of
@@ -234,36 +367,41 @@ __global__ __launch_bounds__(256) void kv_q8_compact_kernel(CompactArgs a) {
     s_src[threadIdx.x] = s >= 0 && s < a.max_len && d >= 0 && d < a.max_len ? s : -1;
   }
   __syncthreads();
-  constexpr int KC = HD / 16;                             // 16-byte pieces of a K row
+  // All loads are unconditional, from slots that exist (a skipped move reads slot 0 and is not stored): the
+  // number of them is uniform, and they are in flight together.
+  constexpr int KC = HD / 16;  // 16-byte pieces of a K row
   constexpr int KI = Q8_MAX_MOVE * KC / 256, VI = Q8_MAX_MOVE * HD / 256;
   uint4 kr[KI];
   uint8_t vr[VI];
-  uint8_t x = 0;
 #pragma unroll
   for (int it = 0; it < KI; ++it) {
-    const int j = (threadIdx.x + it * 256) / KC, d = (threadIdx.x + it * 256) % KC * 16;
-    if (j < n && s_src[j] >= 0) kr[it] = *(const uint4*)(ck + q8_k_off(s_src[j], d, HD));
+    if (it * 256 >= n * KC) break;  // uniform
+    const int i = min((int)threadIdx.x + it * 256, n * KC - 1);
+    kr[it] = *(const uint4*)(ck + q8_k_off(max(s_src[i / KC], 0), i % KC * 16, HD));
   }
 #pragma unroll
   for (int it = 0; it < VI; ++it) {
-    const int j = (threadIdx.x + it * 256) / HD, d = (threadIdx.x + it * 256) % HD;
-    if (j < n && s_src[j] >= 0) vr[it] = cv[q8_v_off(s_src[j], d, HD)];
+    if (it * 256 >= n * HD) break;
+    const int i = min((int)threadIdx.x + it * 256, n * HD - 1);
+    vr[it] = cv[q8_v_off(max(s_src[i / HD], 0), i % HD, HD)];
   }
-  const int xj = threadIdx.x >> 1;
+  const int xj = min((int)threadIdx.x >> 1, n - 1);
   uint8_t* xp = threadIdx.x & 1 ? xv : xk;
-  if (xj < n && s_src[xj] >= 0) x = xp[q8_x_off(s_src[xj])];
+  const uint8_t x = xp[q8_x_off(max(s_src[xj], 0))];
   __syncthreads();
 #pragma unroll
   for (int it = 0; it < KI; ++it) {
-    const int j = (threadIdx.x + it * 256) / KC, d = (threadIdx.x + it * 256) % KC * 16;
-    if (j < n && s_src[j] >= 0) *(uint4*)(ck + q8_k_off((int)start + j, d, HD)) = kr[it];
+    if (it * 256 >= n * KC) break;
+    const int i = threadIdx.x + it * 256, j = i / KC;
+    if (i < n * KC && s_src[j] >= 0) *(uint4*)(ck + q8_k_off((int)start + j, i % KC * 16, HD)) = kr[it];
   }
 #pragma unroll
   for (int it = 0; it < VI; ++it) {
-    const int j = (threadIdx.x + it * 256) / HD, d = (threadIdx.x + it * 256) % HD;
-    if (j < n && s_src[j] >= 0) cv[q8_v_off((int)start + j, d, HD)] = vr[it];
+    if (it * 256 >= n * HD) break;
+    const int i = threadIdx.x + it * 256, j = i / HD;
+    if (i < n * HD && s_src[j] >= 0) cv[q8_v_off((int)start + j, i % HD, HD)] = vr[it];
   }
-  if (xj < n && s_src[xj] >= 0) xp[q8_x_off((int)start + xj)] = x;
+  if ((int)threadIdx.x < 2 * n && s_src[xj] >= 0) xp[q8_x_off((int)start + xj)] = x;
 }
 
 // Checks shared by the entry points that take the cache.
@@ -298,13 +436,36 @@ static int by_head_dim(int hd, F f) {
   return 0;
 }
 
-static int launch_write(const WriteArgs& a, int hd, hipStream_t stream, const char* what) {
-  const int64_t wgs = ((int64_t)a.M * (a.heads + 2 * a.kv) + 15) / 16;
-  if (wgs > INT32_MAX) return set_error(SSD_ERANGE, "%s: too many rows", what);
-  by_head_dim(hd, [&](auto c) {
-    SSD_LAUNCH((kv_q8_write_kernel<decltype(c)::value>), dim3((unsigned)wgs), dim3(256), 0, stream, a);
-  });
+// Units of R rows that cover M rows: with R = 4 the first may begin up to three rows early.
+static int64_t row_units(int M, int r) { return r == 1 ? M : ((int64_t)M + 3) / 4 + 1; }
+// From this many rows on a unit takes four: below, more units are worth more than wider accesses (us for 32 and 4096 rows
+// of 8 kv heads and 32 q heads of 128, one row a unit / four: WRITE_FEW, WRITE_MANY).
+constexpr int Q8_QUAD_ROWS = 256;
+
+template <int HD>
+static int launch_write_hd(const WriteArgs& a, hipStream_t stream, const char* what) {
+  const bool many = a.M >= Q8_QUAD_ROWS;
+  const int64_t units = a.kv ? row_units(a.M, many ? 4 : 1) : 0, kv_wgs = (units * 2 * a.kv + 15) / 16;
+  const int q_units = (a.heads + (many ? 3 : 0)) / (many ? 4 : 1);
+  const int64_t wgs = kv_wgs + ((int64_t)a.M * q_units + 15) / 16;
+  if (wgs > INT32_MAX / 16) return set_error(SSD_ERANGE, "%s: too many rows", what);
+  if (many) SSD_LAUNCH((kv_q8_write_kernel<HD, 4, 4>), dim3((unsigned)wgs), dim3(256), 0, stream, a, (int)kv_wgs, (int)units, q_units);
+  else SSD_LAUNCH((kv_q8_write_kernel<HD, 1, 1>), dim3((unsigned)wgs), dim3(256), 0, stream, a, (int)kv_wgs, (int)units, q_units);
   return check_launch(what);
+}
+
+static int launch_write(const WriteArgs& a, int hd, hipStream_t stream, const char* what) {
+  return hd == 64 ? launch_write_hd<64>(a, stream, what) : launch_write_hd<128>(a, stream, what);
+}
+
+template <int HD>
+static int launch_read(const ReadArgs& a, hipStream_t stream) {
+  const bool many = a.M >= Q8_QUAD_ROWS;
+  const int64_t units = row_units(a.M, many ? 4 : 1), wgs = (units * 2 * a.kv + 15) / 16;
+  if (wgs > INT32_MAX / 16) return set_error(SSD_ERANGE, "kv_q8_read: too many rows");
+  if (many) SSD_LAUNCH((kv_q8_read_kernel<HD, 4>), dim3((unsigned)wgs), dim3(256), 0, stream, a, (int)units);
+  else SSD_LAUNCH((kv_q8_read_kernel<HD, 1>), dim3((unsigned)wgs), dim3(256), 0, stream, a, (int)units);
+  return check_launch("kv_q8_read");
 }
 
 }  // namespace ssd
@@ -358,15 +519,10 @@ SSD_API int ssd_kv_q8_read_bf16(const SsdKvQ8* cache, int M, const int32_t* row_
   if (M < 0) return set_error(SSD_EINVAL, "kv_q8_read: bad M=%d", M);
   if (bad_rows(k, ldk, cols) || bad_rows(v, ldv, cols))
     return set_error(SSD_EINVAL, "kv_q8_read: k/v rows must be 16-byte aligned with strides >= kv_heads * head_dim");
-  const int64_t wgs = ((int64_t)M * 2 * cache->kv_heads + 15) / 16;
-  if (wgs > INT32_MAX) return set_error(SSD_ERANGE, "kv_q8_read: too many rows");
   if (M == 0) return SSD_OK;
   const ReadArgs a{cache->k, cache->v, cache->k_exp, cache->v_exp, cache->n_seq, cache->kv_heads, M, cache->max_len,
                    row_seq, row_slot, k, v, ldk, ldv};
-  by_head_dim(cache->head_dim, [&](auto c) {
-    SSD_LAUNCH((kv_q8_read_kernel<decltype(c)::value>), dim3((unsigned)wgs), dim3(256), 0, stream, a);
-  });
-  return check_launch("kv_q8_read");
+  return cache->head_dim == 64 ? launch_read<64>(a, stream) : launch_read<128>(a, stream);
 }
 
 SSD_API int ssd_kv_q8_compact(const SsdKvQ8* cache, int layers, const int32_t* start, const int32_t* src, const int32_t* n,

@@ -1,23 +1,23 @@
 // Verification of drafted chains from given random numbers, a batch of sequences in two launches.
 //
-// chain_sum: workgroup (sequence, chunk of 4096 columns). Every workgroup of a sequence resolves the acceptance
-// tests itself (one wave, one gather per drafted token), which tells it the row to draw from, and adds up its
-// chunk's mass of max(P_n - Q_n, 0) and of P_n in 64 bits. chain_draw: one workgroup per sequence finds the
-// chunk that holds u_next * total, then the column in it.
-// What bounds it: two rows of V fp32 a sequence.
+// chain_sum: workgroup (sequence, chunk of columns; at most 64 chunks of whole 4096-column pieces a row). Each resolves
+// the sequence's acceptance tests itself (a gather per drafted token, one wave), which tells it the row to draw
+// from, and adds up its chunk's mass of max(P_n - Q_n, 0) and of P_n in 64 bits. chain_draw: one workgroup per sequence
+// finds the chunk that holds u_next * total (a lane a chunk), then the column in it.
+// What bounds it: two rows of V fp32 a sequence for a batch, the latency of two launches for a few sequences.
 #include "common.h"
 
 namespace ssd {
 
-constexpr int CHAIN_CHUNK = 4096, CHAIN_MAX = 64;
+constexpr int CHAIN_PIECE = 4096, CHAIN_MAX = 64, CHAIN_CHUNKS = 64;
 
 struct ChainArgs {
   const float *P, *Q;
   int64_t ldp_seq, ldp, ldq_seq, ldq;
-  int V, k_max, chunks;
+  int V, k_max, chunks, pieces;  // pieces of 4096 columns in a chunk
   const int *draft, *n_draft;
   const float *u, *u_next;
-  double* ws;  // [n_seq][chunks] pairs: residual mass, target mass
+  double2* ws;  // [n_seq][chunks + 1]: (residual mass, target mass) of each chunk, then (accepted, draws from the residual)
   int *out_tok, *out_n;
 };
 
@@ -59,6 +59,21 @@ __device__ __forceinline__ double residual(float p, float q) {
   return d > 0. ? d : 0.;
 }
 
+// Sixteen columns of a row pair from column c on: the residual's mass, or the target's where q is null.
+__device__ __forceinline__ void load_mass(const float* p, const float* q, int c, int V, double (&m)[16]) {
+  const bool wp = !((uintptr_t)p & 15), wq = !((uintptr_t)q & 15);
+  float4 x[4], y[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = load4(p, c + 4 * i, V, wp);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] = q ? load4(q, c + 4 * i, V, wq) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    m[4 * i] = residual(x[i].x, y[i].x), m[4 * i + 1] = residual(x[i].y, y[i].y);
+    m[4 * i + 2] = residual(x[i].z, y[i].z), m[4 * i + 3] = residual(x[i].w, y[i].w);
+  }
+}
+
 __global__ __launch_bounds__(256) void chain_sum_kernel(ChainArgs a) {
   const int s = blockIdx.x / a.chunks, ch = blockIdx.x % a.chunks, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   int todo;
@@ -67,121 +82,112 @@ __global__ __launch_bounds__(256) void chain_sum_kernel(ChainArgs a) {
   const float* q = n < todo ? a.Q + s * a.ldq_seq + n * a.ldq : nullptr;
   const bool wp = !((uintptr_t)p & 15), wq = !((uintptr_t)q & 15);
   double rs = 0., ps = 0.;
+  for (int pc = 0; pc < a.pieces; ++pc) {
 #pragma unroll
-  for (int it = 0; it < CHAIN_CHUNK / 1024; ++it) {
-    const int c = ch * CHAIN_CHUNK + it * 1024 + threadIdx.x * 4;
-    const float4 x = load4(p, c, a.V, wp);
-    const float4 y = q ? load4(q, c, a.V, wq) : make_float4(0.f, 0.f, 0.f, 0.f);
-    rs += residual(x.x, y.x) + residual(x.y, y.y) + residual(x.z, y.z) + residual(x.w, y.w);
-    ps += residual(x.x, 0.f) + residual(x.y, 0.f) + residual(x.z, 0.f) + residual(x.w, 0.f);
+    for (int it = 0; it < CHAIN_PIECE / 1024; ++it) {
+      const int c = (ch * a.pieces + pc) * CHAIN_PIECE + it * 1024 + threadIdx.x * 4;
+      const float4 x = load4(p, c, a.V, wp);
+      const float4 y = q ? load4(q, c, a.V, wq) : make_float4(0.f, 0.f, 0.f, 0.f);
+      rs += residual(x.x, y.x) + residual(x.y, y.y) + residual(x.z, y.z) + residual(x.w, y.w);
+      ps += residual(x.x, 0.f) + residual(x.y, 0.f) + residual(x.z, 0.f) + residual(x.w, 0.f);
+    }
   }
   __shared__ double part[4][2];
   rs = wave_sum(rs), ps = wave_sum(ps);
   if (lane == 0) part[w][0] = rs, part[w][1] = ps;
   __syncthreads();
-  if (threadIdx.x < 2)
-    a.ws[((size_t)s * a.chunks + ch) * 2 + threadIdx.x] =
-        part[0][threadIdx.x] + part[1][threadIdx.x] + part[2][threadIdx.x] + part[3][threadIdx.x];
+  double2* out = a.ws + (size_t)s * (a.chunks + 1);
+  if (threadIdx.x == 0)
+    out[ch] = make_double2(part[0][0] + part[1][0] + part[2][0] + part[3][0], part[0][1] + part[1][1] + part[2][1] + part[3][1]);
+  if (threadIdx.x == 64 && ch == 0) out[a.chunks] = make_double2(n, q ? 1. : 0.);
 }
 
-// Exclusive prefix of v over the workgroup's 256 threads, and the total.
-__device__ __forceinline__ double block_prefix(double v, double* s_w, double& total) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  double inc = v;
+__device__ __forceinline__ double wave_scan(double v, int lane) {  // inclusive
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const double t = __shfl_up(inc, o);
-    if (lane >= o) inc += t;
+    const double t = __shfl_up(v, o);
+    if (lane >= o) v += t;
   }
-  __syncthreads();  // s_w may still be read from an earlier call
-  if (lane == 63) s_w[w] = inc;
-  __syncthreads();
-  double base = 0.;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (i < w) base += s_w[i];
-  total = s_w[0] + s_w[1] + s_w[2] + s_w[3];
-  return base + inc - v;
+  return v;
+}
+
+// The least element whose cumulative mass exceeds `want`, else the last that has any; -1: none has.
+__device__ __forceinline__ int pick(uint64_t past, uint64_t any) {
+  return past ? __builtin_ctzll(past) : any ? 63 - __builtin_clzll(any) : -1;
 }
 
 __global__ __launch_bounds__(256) void chain_draw_kernel(ChainArgs a) {
-  const int s = blockIdx.x, lane = threadIdx.x & 63;
-  __shared__ double s_w[4];
-  __shared__ int s_best, s_last;
-  int todo;
-  const int n = chain_accepted(a, s, lane, todo);
-  const double* ws = a.ws + (size_t)s * a.chunks * 2;
-  // total residual mass; without any, draw from the target row
-  double rs = 0., ps = 0.;
-  for (int c = threadIdx.x; c < a.chunks; c += 256) rs += ws[2 * c], ps += ws[2 * c + 1];
-  double rt, pt;
-  block_prefix(rs, s_w, rt);
-  block_prefix(ps, s_w, pt);
-  const bool res = rt > 0.;
-  const double total = res ? rt : pt, want = (double)a.u_next[s] * total;
-  // the chunk: the first whose end passes `want`, else the last with mass
-  if (threadIdx.x == 0) s_best = INT32_MAX, s_last = -1;
-  double base = 0., before = 0.;  // mass before this window of 256 chunks; before the chosen chunk
-  int chunk = -1;
-  double chunk_before = 0.;
-  for (int c0 = 0; c0 < a.chunks; c0 += 256) {
-    const int c = c0 + threadIdx.x;
-    const double m = c < a.chunks ? ws[2 * c + (res ? 0 : 1)] : 0.;
-    double tot;
-    before = base + block_prefix(m, s_w, tot);
-    if (m > 0.) {
-      atomicMax(&s_last, c);
-      if (before + m > want) atomicMin(&s_best, c);
-    }
-    __syncthreads();
-    const int pick = s_best != INT32_MAX ? s_best : s_last;
-    if (c == pick) chunk_before = before, chunk = c;
-    base += tot;
-    __syncthreads();
-  }
-  __shared__ double s_before;
-  __shared__ int s_chunk;
-  const int pick = s_best != INT32_MAX ? s_best : s_last;
-  if (threadIdx.x == 0) s_chunk = pick;
-  if (chunk == pick && chunk >= 0) s_before = chunk_before;
-  __syncthreads();
+  const int s = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const double2* ws = a.ws + (size_t)s * (a.chunks + 1);
+  const double2 own = lane < a.chunks ? ws[lane] : make_double2(0., 0.), head = ws[a.chunks];
+  const float u = a.u_next[s];
+  const int n = (int)head.x;
+  // every wave finds the chunk: the residual's mass, or the target's without any
+  const double rc = wave_scan(own.x, lane), pc = wave_scan(own.y, lane);
+  const bool res = head.y != 0. && __shfl(rc, 63) > 0.;
+  const double m = res ? own.x : own.y, cum = res ? rc : pc, want = (double)u * __shfl(cum, 63);
+  const int ch = pick(__ballot(m > 0. && cum > want), __ballot(m > 0.));
+  const float* p = a.P + s * a.ldp_seq + n * a.ldp;
+  const float* q = res ? a.Q + s * a.ldq_seq + n * a.ldq : nullptr;
+  double base = __shfl(cum, max(ch - 1, 0));
+  if (ch <= 0) base = 0.;
+  __shared__ double sum[4];
+  __shared__ int first[4], last[4];
   int tok = -1;
-  if (s_chunk >= 0) {
-    const float* p = a.P + s * a.ldp_seq + n * a.ldp;
-    const float* q = res && n < todo ? a.Q + s * a.ldq_seq + n * a.ldq : nullptr;
-    const int c0 = s_chunk * CHAIN_CHUNK + threadIdx.x * 16;
-    double m[16], sum = 0.;
-    const bool wp = !((uintptr_t)p & 15), wq = !((uintptr_t)q & 15);
+  for (int pc2 = 0; ch >= 0 && pc2 < a.pieces; ++pc2) {  // uniform
+    const int c0 = (ch * a.pieces + pc2) * CHAIN_PIECE + threadIdx.x * 16;
+    double x[16], mine = 0.;
+    load_mass(p, q, c0, a.V, x);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) mine += x[i];
+    const double inc = wave_scan(mine, lane);
+    __syncthreads();  // the piece before has been read
+    if (lane == 63) sum[w] = inc;
+    __syncthreads();
+    double at = base;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float4 x = load4(p, c0 + 4 * i, a.V, wp);
-      const float4 y = q ? load4(q, c0 + 4 * i, a.V, wq) : make_float4(0.f, 0.f, 0.f, 0.f);
-      m[4 * i] = residual(x.x, y.x), m[4 * i + 1] = residual(x.y, y.y);
-      m[4 * i + 2] = residual(x.z, y.z), m[4 * i + 3] = residual(x.w, y.w);
+      if (i < w) at += sum[i];
+      base += sum[i];
     }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) sum += m[i];
-    double tot;
-    double cum = s_before + block_prefix(sum, s_w, tot);
-    if (threadIdx.x == 0) s_best = INT32_MAX, s_last = -1;
-    __syncthreads();
-    int first = INT32_MAX, last = -1;
+    const double below = __shfl_up(inc, 1);
+    at += lane ? below : 0.;
+    int f = -1, l = -1;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      cum += m[i];
-      if (m[i] > 0.) {
-        last = c0 + i;
-        if (cum > want && first == INT32_MAX) first = c0 + i;
+      at += x[i];
+      if (x[i] > 0.) {
+        l = c0 + i;
+        if (at > want && f < 0) f = c0 + i;
       }
     }
-    if (first != INT32_MAX) atomicMin(&s_best, first);
-    if (last >= 0) atomicMax(&s_last, last);
+    const uint64_t past = __ballot(f >= 0), any = __ballot(l >= 0);
+    const int fw = __shfl(f, past ? __builtin_ctzll(past) : 0), lw = __shfl(l, any ? 63 - __builtin_clzll(any) : 0);
+    if (lane == 0) first[w] = past ? fw : -1, last[w] = any ? lw : -1;
     __syncthreads();
-    tok = s_best != INT32_MAX ? s_best : s_last;
+    int found = -1;
+#pragma unroll
+    for (int i = 3; i >= 0; --i) found = first[i] >= 0 ? first[i] : found;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) tok = last[i] >= 0 ? last[i] : tok;
+    if (found >= 0) {
+      tok = found;
+      break;
+    }
   }
   int* out = a.out_tok + (size_t)s * (a.k_max + 1);
-  for (int i = threadIdx.x; i <= a.k_max; i += 256) out[i] = i < n ? a.draft[(size_t)s * a.k_max + i] : i == n ? tok : -1;
+  if ((int)threadIdx.x <= a.k_max) {
+    const int i = threadIdx.x;
+    out[i] = i < n ? a.draft[(size_t)s * a.k_max + i] : i == n ? tok : -1;
+  }
   if (threadIdx.x == 0) a.out_n[s] = n;
+}
+
+// Pieces a chunk so that a row has at most 64 chunks.
+static int chain_pieces(int V) { return (V + CHAIN_PIECE * CHAIN_CHUNKS - 1) / (CHAIN_PIECE * CHAIN_CHUNKS); }
+static int chain_chunks(int V) {
+  const int w = CHAIN_PIECE * chain_pieces(V);
+  return (V + w - 1) / w;
 }
 
 }  // namespace ssd
@@ -189,8 +195,8 @@ __global__ __launch_bounds__(256) void chain_draw_kernel(ChainArgs a) {
 using namespace ssd;
 
 SSD_API int64_t ssd_verify_chain_ws_bytes(int n_seq, int V) {
-  if (n_seq < 0 || V < 1) return -1;
-  return (int64_t)n_seq * ((V + CHAIN_CHUNK - 1) / CHAIN_CHUNK) * 2 * (int64_t)sizeof(double);
+  if (n_seq < 0 || V < 1 || V > 1 << 24) return -1;
+  return (int64_t)n_seq * (chain_chunks(V) + 1) * (int64_t)sizeof(double2);
 }
 
 SSD_API int ssd_verify_chain(const float* P, int64_t ldp_seq, int64_t ldp, const float* Q, int64_t ldq_seq, int64_t ldq, int V,
@@ -203,12 +209,13 @@ SSD_API int ssd_verify_chain(const float* P, int64_t ldp_seq, int64_t ldp, const
   if (!P || !u_next || !ws || !out_tok || !out_n || (k_max && (!Q || !draft || !u)))
     return set_error(SSD_EINVAL, "verify_chain: null pointer");
   if (ldp < V || (k_max && ldq < V)) return set_error(SSD_EINVAL, "verify_chain: row strides below V");
-  if ((uintptr_t)ws & 7) return set_error(SSD_EINVAL, "verify_chain: workspace must be 8-byte aligned");
+  if ((uintptr_t)ws & 15) return set_error(SSD_EINVAL, "verify_chain: workspace must be 16-byte aligned");
   if (ws_bytes < ssd_verify_chain_ws_bytes(n_seq, V)) return set_error(SSD_EINVAL, "verify_chain: workspace too small");
-  const int chunks = (V + CHAIN_CHUNK - 1) / CHAIN_CHUNK;
+  const int chunks = chain_chunks(V);
   if ((int64_t)n_seq * chunks > INT32_MAX) return set_error(SSD_ERANGE, "verify_chain: too many sequences");
   if (n_seq == 0) return SSD_OK;
-  const ChainArgs a{P, Q, ldp_seq, ldp, ldq_seq, ldq, V, k_max, chunks, draft, n_draft, u, u_next, (double*)ws, out_tok, out_n};
+  const ChainArgs a{P, Q, ldp_seq, ldp, ldq_seq, ldq, V, k_max, chunks, chain_pieces(V), draft, n_draft, u, u_next, (double2*)ws,
+                    out_tok, out_n};
   SSD_LAUNCH(chain_sum_kernel, dim3((unsigned)(n_seq * chunks)), dim3(256), 0, stream, a);
   if (int rc = check_launch("chain_sum")) return rc;
   SSD_LAUNCH(chain_draw_kernel, dim3((unsigned)n_seq), dim3(256), 0, stream, a);

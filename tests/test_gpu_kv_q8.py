@@ -432,7 +432,7 @@ def _same_chain(P, Q, draft, u, nxt, nd=None, ld=0):
 
 
 @pytest.mark.parametrize("B,K,V,ld", [(1, 4, 128256, 0), (7, 3, 32768, 0), (5, 1, 1000, 3), (33, 6, 517, 0), (2, 64, 300, 1), (3, 2, 1, 0),
-                                      (4, 5, 4096, 0), (4, 5, 4097, 0), (2, 0, 9000, 0)])
+                                      (4, 5, 4096, 0), (4, 5, 4097, 0), (2, 0, 9000, 0), (2, 2, 600001, 0)])
 def test_verify_chain(B, K, V, ld):
     P, Q, draft, u, nxt = _dists(B, K, V, B * 31 + K)
     _same_chain(P, Q, draft, u, nxt, None, ld)

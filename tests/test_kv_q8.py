@@ -213,9 +213,9 @@ def test_attention_refusals(at, value, code, text):
 @pytest.mark.parametrize("at,value,code,text", [
     (0, None, BAD, "null"), (3, None, BAD, "null"), (9, None, BAD, "null"), (11, None, BAD, "null"), (12, None, BAD, "null"), (15, None, BAD, "null"),
     (6, 0, BAD, "V=0"), (6, (1 << 24) + 1, RANGE, "columns"), (7, -1, BAD, "n_seq"), (8, -1, BAD, "k_max"), (8, 65, RANGE, "drafted"),
-    (2, 99, BAD, "strides"), (5, 99, BAD, "strides"), (13, A + 4, BAD, "aligned"), (14, 47, BAD, "workspace")])
+    (2, 99, BAD, "strides"), (5, 99, BAD, "strides"), (13, A + 4, BAD, "aligned"), (14, 95, BAD, "workspace")])
 def test_verify_chain_refusals(at, value, code, text):
-    args = [A, 400, 100, A, 300, 100, 100, 3, 3, A, None, A, A, A, 48, A, A, None]
+    args = [A, 400, 100, A, 300, 100, 100, 3, 3, A, None, A, A, A, 96, A, A, None]
     args[at] = value
     _refused("ssd_verify_chain", args, code, text)
 
@@ -227,7 +227,7 @@ def test_workspace_sizes():
     assert lib.ssd_attn_q8_ws_floats(3, 8, 128, 600, 128) == 3 * 8 * 2 * 130
     assert lib.ssd_attn_q8_ws_floats(3, 8, 128, 300, 100) == -1 and lib.ssd_attn_q8_ws_floats(3, 8, 128, 0, 64) == -1
     assert lib.ssd_attn_q8_ws_floats(64, 64, 128, 1 << 20, 64) == 64 * 64 * (1 << 12) * 130  # past 32 bits
-    assert lib.ssd_verify_chain_ws_bytes(3, 4097) == 3 * 2 * 16 and lib.ssd_verify_chain_ws_bytes(3, 0) == -1
+    assert lib.ssd_verify_chain_ws_bytes(3, 4097) == 3 * 3 * 16 and lib.ssd_verify_chain_ws_bytes(3, 0) == -1
 
 
 def test_python_refusals_without_a_gpu():
