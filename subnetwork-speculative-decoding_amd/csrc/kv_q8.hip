@@ -340,8 +340,8 @@ __global__ __launch_bounds__(256) void kv_q8_read_kernel(ReadArgs a, int units) 
   }
 }
 
-// One workgroup per (layer, sequence, kv head): every source row is read (K and V as 16-byte pieces of
-// dims, through registers) before the first destination is written.
+// One workgroup per (layer, sequence, kv head): every source row is read into LDS before the first destination is
+// written. Bound by its chain of loads: counts and places, then the rows (16 sequences of 5 rows, 2 layers: COMPACT_US).
 constexpr int Q8_MAX_MOVE = 64;
 
 struct CompactArgs {
@@ -367,40 +367,33 @@ __global__ __launch_bounds__(256) void kv_q8_compact_kernel(CompactArgs a) {
     s_src[threadIdx.x] = s >= 0 && s < a.max_len && d >= 0 && d < a.max_len ? s : -1;
   }
   __syncthreads();
-  // All loads are unconditional, from slots that exist (a skipped move reads slot 0 and is not stored): the
-  // number of them is uniform, and they are in flight together.
-  constexpr int KC = HD / 16;  // 16-byte pieces of a K row
-  constexpr int KI = Q8_MAX_MOVE * KC / 256, VI = Q8_MAX_MOVE * HD / 256;
-  uint4 kr[KI];
-  uint8_t vr[VI];
+  // K in 16-byte pieces, V and the exponents in bytes, four loads of a thread in flight. Loads are unconditional, from
+  // slots that exist (a skipped move reads slot 0 and is not stored).
+  constexpr int KC = HD / 16;
+  __shared__ uint4 s_k[Q8_MAX_MOVE * KC];
+  __shared__ uint8_t s_v[Q8_MAX_MOVE * HD];
+  auto fetch = [&](int count, auto load, auto keep) {
+    for (int i0 = threadIdx.x; i0 < count; i0 += 1024) {
+      decltype(load(0)) v[4];
 #pragma unroll
-  for (int it = 0; it < KI; ++it) {
-    if (it * 256 >= n * KC) break;  // uniform
-    const int i = min((int)threadIdx.x + it * 256, n * KC - 1);
-    kr[it] = *(const uint4*)(ck + q8_k_off(max(s_src[i / KC], 0), i % KC * 16, HD));
-  }
+      for (int u = 0; u < 4; ++u) v[u] = load(min(i0 + 256 * u, count - 1));
 #pragma unroll
-  for (int it = 0; it < VI; ++it) {
-    if (it * 256 >= n * HD) break;
-    const int i = min((int)threadIdx.x + it * 256, n * HD - 1);
-    vr[it] = cv[q8_v_off(max(s_src[i / HD], 0), i % HD, HD)];
-  }
+      for (int u = 0; u < 4; ++u)
+        if (i0 + 256 * u < count) keep(i0 + 256 * u, v[u]);
+    }
+  };
   const int xj = min((int)threadIdx.x >> 1, n - 1);
   uint8_t* xp = threadIdx.x & 1 ? xv : xk;
   const uint8_t x = xp[q8_x_off(max(s_src[xj], 0))];
+  fetch(n * KC, [&](int i) { return *(const uint4*)(ck + q8_k_off(max(s_src[i / KC], 0), i % KC * 16, HD)); },
+        [&](int i, uint4 v) { s_k[i] = v; });
+  fetch(n * HD, [&](int i) { return (uint32_t)cv[q8_v_off(max(s_src[i / HD], 0), i % HD, HD)]; },
+        [&](int i, uint32_t v) { s_v[i] = (uint8_t)v; });
   __syncthreads();
-#pragma unroll
-  for (int it = 0; it < KI; ++it) {
-    if (it * 256 >= n * KC) break;
-    const int i = threadIdx.x + it * 256, j = i / KC;
-    if (i < n * KC && s_src[j] >= 0) *(uint4*)(ck + q8_k_off((int)start + j, i % KC * 16, HD)) = kr[it];
-  }
-#pragma unroll
-  for (int it = 0; it < VI; ++it) {
-    if (it * 256 >= n * HD) break;
-    const int i = threadIdx.x + it * 256, j = i / HD;
-    if (i < n * HD && s_src[j] >= 0) cv[q8_v_off((int)start + j, i % HD, HD)] = vr[it];
-  }
+  for (int i = threadIdx.x; i < n * KC; i += 256)
+    if (s_src[i / KC] >= 0) *(uint4*)(ck + q8_k_off((int)start + i / KC, i % KC * 16, HD)) = s_k[i];
+  for (int i = threadIdx.x; i < n * HD; i += 256)
+    if (s_src[i / HD] >= 0) cv[q8_v_off((int)start + i / HD, i % HD, HD)] = s_v[i];
   if ((int)threadIdx.x < 2 * n && s_src[xj] >= 0) xp[q8_x_off((int)start + xj)] = x;
 }
 
