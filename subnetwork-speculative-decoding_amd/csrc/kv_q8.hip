@@ -57,45 +57,43 @@ __device__ __forceinline__ void store_chunk(bf16_t* p, const Chunk<E>& c) {
   else *(uint2*)p = make_uint2(w[0], w[1]);
 }
 
-// cos and sin of dims d0 .. d0 + E for one token (their pairs' entries when interleaved), and whether they turn.
-template <int E>
+enum { ROPE_NONE = 0, ROPE_HALF = 1, ROPE_PAIRS = 2 };  // no rotation; pairs (i, i + rot / 2); pairs (2i, 2i + 1)
+
+// cos and sin of dims d0 .. d0 + E for one token (their pairs' entries for ROPE_PAIRS), and whether they turn.
+template <int E, int MODE>
 struct Turn {
-  float c[E], s[E];
+  static constexpr int N = MODE == ROPE_PAIRS ? E / 2 : E;
+  float c[N], s[N];
   bool on;
 };
 
-template <int E>
-__device__ __forceinline__ Turn<E> load_turn(const RopeArgs& r, int d0, int64_t pos) {
-  Turn<E> t;
-  t.on = r.cos && d0 < r.rot;
+template <int E, int MODE>
+__device__ __forceinline__ Turn<E, MODE> load_turn(const RopeArgs& r, int d0, int64_t pos) {
+  Turn<E, MODE> t;
+  t.on = MODE != ROPE_NONE && d0 < r.rot;
   if (!t.on) return t;
-  const int half = r.rot >> 1, e0 = r.interleaved ? d0 >> 1 : d0 < half ? d0 : d0 - half;
+  const int half = r.rot >> 1, e0 = MODE == ROPE_PAIRS ? d0 >> 1 : d0 < half ? d0 : d0 - half;
   const float *ct = r.cos + pos * half + e0, *st = r.sin + pos * half + e0;
-  if (r.interleaved) {
 #pragma unroll
-    for (int i = 0; i < E / 2; ++i) t.c[i] = ct[i], t.s[i] = st[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < E; ++i) t.c[i] = ct[i], t.s[i] = st[i];
-  }
+  for (int i = 0; i < Turn<E, MODE>::N; ++i) t.c[i] = ct[i], t.s[i] = st[i];
   return t;
 }
 
 // Dims d0 .. d0 + E of the head at x, rotated. Products and sums are rounded one by one (no multiply-add
 // contraction), so the codes a rotated row is quantised to do not depend on the compiler.
-template <int E>
-__device__ __forceinline__ Chunk<E> load_rotated(const bf16_t* x, int d0, const RopeArgs& r, const Turn<E>& t) {
+template <int E, int MODE>
+__device__ __forceinline__ Chunk<E> load_rotated(const bf16_t* x, int d0, const RopeArgs& r, const Turn<E, MODE>& t) {
 #pragma clang fp contract(off)
   Chunk<E> c = load_chunk<E>(x + d0);
   if (!t.on) return c;
-  if (r.interleaved) {
+  if constexpr (MODE == ROPE_PAIRS) {
 #pragma unroll
     for (int i = 0; i < E; i += 2) {
       const float a = c.x[i], b = c.x[i + 1];
       c.x[i] = a * t.c[i / 2] - b * t.s[i / 2];
       c.x[i + 1] = b * t.c[i / 2] + a * t.s[i / 2];
     }
-  } else {
+  } else if constexpr (MODE == ROPE_HALF) {
     const int half = r.rot >> 1;  // a multiple of 8: a chunk lies in one half
     const bool low = d0 < half;
     const Chunk<E> o = load_chunk<E>(x + (low ? d0 + half : d0 - half));
@@ -108,8 +106,9 @@ __device__ __forceinline__ Chunk<E> load_rotated(const bf16_t* x, int d0, const 
   return c;
 }
 
+template <int MODE>
 __device__ __forceinline__ int64_t rope_row(const RopeArgs& r, int row) {
-  if (!r.cos) return 0;
+  if (MODE == ROPE_NONE) return 0;
   const int64_t p = r.pos[row];
   return p < 0 ? 0 : p < r.rows ? p : r.rows - 1;
 }
@@ -126,24 +125,30 @@ __device__ __forceinline__ uint32_t max16(uint32_t v) {
 // not count for the exponent and are stored as NaN. All 16 lanes call it together.
 template <int E>
 __device__ __forceinline__ int quantise(const Chunk<E>& c, uint32_t (&w)[E / 4]) {
-  uint32_t top = 0;
+  constexpr uint32_t INF = 0x7f800000u;
+  uint32_t u[E], top = 0;
 #pragma unroll
   for (int i = 0; i < E; ++i) {
-    const uint32_t u = __float_as_uint(c.x[i]) & 0x7fffffffu;
-    top = max(top, u < 0x7f800000u ? u : 0u);
+    u[i] = __float_as_uint(c.x[i]) & 0x7fffffffu;
+    top = max(top, u[i]);
+  }
+  float y[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) y[i] = c.x[i];
+  if (__any(top >= INF)) {  // rare: taken by the wave, changes only what is not finite
+    top = 0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      top = max(top, u[i] < INF ? u[i] : 0u);
+      y[i] = u[i] < INF ? y[i] : __uint_as_float(0x7fc00000u);
+    }
   }
   const int b = q8_exponent(__uint_as_float(max16(top)));
   const float inv = q8_inv_scale(b);
-  float y[E];
-#pragma unroll
-  for (int i = 0; i < E; ++i) {
-    const uint32_t u = __float_as_uint(c.x[i]) & 0x7fffffffu;
-    y[i] = u < 0x7f800000u ? c.x[i] * inv : __uint_as_float(0x7fc00000u);
-  }
 #pragma unroll
   for (int i = 0; i < E; i += 4) {
-    int p = __builtin_amdgcn_cvt_pk_fp8_f32(y[i], y[i + 1], 0, false);
-    w[i / 4] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[i + 2], y[i + 3], p, true);
+    int p = __builtin_amdgcn_cvt_pk_fp8_f32(y[i] * inv, y[i + 1] * inv, 0, false);
+    w[i / 4] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[i + 2] * inv, y[i + 3] * inv, p, true);
   }
   return b;
 }
@@ -160,7 +165,7 @@ __device__ __forceinline__ void transpose4(uint32_t (&w)[4]) {
 // codes of one dim, and whose exponents, are one word).
 template <int R>
 struct Places {
-  int64_t reg[R];  // sequence * kv_heads, -1: outside the cache (or no such row)
+  int reg[R];  // sequence * kv_heads, -1: outside the cache (or no such row)
   int slot[R];
   bool quad;
 };
@@ -172,13 +177,13 @@ __device__ __forceinline__ int unit_row(const int* slot, int unit) {
 }
 
 template <int R>
-__device__ __forceinline__ Places<R> load_places(const int* seq, const int* slot, int row0, int M, int n_seq, int64_t max_len, int kv) {
+__device__ __forceinline__ Places<R> load_places(const int* seq, const int* slot, int row0, int M, int n_seq, int max_len, int kv) {
   Places<R> p;
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const int row = row0 + i, r = min(max(row, 0), M - 1), sq = seq[r];
     p.slot[i] = slot[r];
-    p.reg[i] = row == r && sq >= 0 && sq < n_seq && p.slot[i] >= 0 && p.slot[i] < max_len ? (int64_t)sq * kv : -1;
+    p.reg[i] = row == r && (uint32_t)sq < (uint32_t)n_seq && (uint32_t)p.slot[i] < (uint32_t)max_len ? sq * kv : -1;
   }
   p.quad = R == 4 && p.reg[0] >= 0 && (p.slot[0] & 3) == 0;
 #pragma unroll
@@ -187,9 +192,9 @@ __device__ __forceinline__ Places<R> load_places(const int* seq, const int* slot
 }
 
 // Workgroups [0, kv_wgs) write K and V: sixteen lanes per (R rows, kv head, K or V), E = head_dim / 16 dims a lane.
-// The others rotate q: sixteen lanes per (row, H heads), which share the row's cos and sin. R and H are 4 from
-// 256 rows on. Bound by the bytes of q (64 MiB of 96 for 4096 rows of 32 + 8 heads of 128).
-template <int HD, int R, int H>
+// The others rotate q: sixteen lanes per (row, H heads), which share the row's cos and sin. R and H are 4 for
+// long calls. Bound by the bytes of q (64 MiB of 96 for 4096 rows of 32 + 8 heads of 128).
+template <int HD, int R, int H, int MODE>
 __global__ __launch_bounds__(256) void kv_q8_write_kernel(WriteArgs a, int kv_wgs, int kv_units, int q_units) {
   constexpr int E = HD / 16;
   const int ln = threadIdx.x & 15, d0 = ln * E;
@@ -197,12 +202,12 @@ __global__ __launch_bounds__(256) void kv_q8_write_kernel(WriteArgs a, int kv_wg
     const int64_t id = (int64_t)(blockIdx.x - kv_wgs) * 16 + (threadIdx.x >> 4);
     if (id >= (int64_t)a.M * q_units) return;
     const int row = (int)(id / q_units), h0 = (int)(id % q_units) * H;
-    const Turn<E> t = load_turn<E>(a.rope, d0, rope_row(a.rope, row));
+    const Turn<E, MODE> t = load_turn<E, MODE>(a.rope, d0, rope_row<MODE>(a.rope, row));
     const bf16_t* x = a.q + (size_t)row * a.ldq;
     bf16_t* y = a.q_out + (size_t)row * a.ldo;
     Chunk<E> c[H];
 #pragma unroll
-    for (int i = 0; i < H; ++i) c[i] = load_rotated<E>(x + (size_t)min(h0 + i, a.heads - 1) * HD, d0, a.rope, t);
+    for (int i = 0; i < H; ++i) c[i] = load_rotated<E, MODE>(x + (size_t)min(h0 + i, a.heads - 1) * HD, d0, a.rope, t);
 #pragma unroll
     for (int i = 0; i < H; ++i)
       if (h0 + i < a.heads) store_chunk<E>(y + (size_t)(h0 + i) * HD + d0, c[i]);
@@ -213,7 +218,7 @@ __global__ __launch_bounds__(256) void kv_q8_write_kernel(WriteArgs a, int kv_wg
   const int u = id % (2 * a.kv), h = u < a.kv ? u : u - a.kv;
   const bool is_v = u >= a.kv;
   const int row0 = unit_row<R>(a.slot, unit);
-  const Places<R> at = load_places<R>(a.seq, a.slot, row0, a.M, a.n_seq, a.max_len, a.kv);
+  const Places<R> at = load_places<R>(a.seq, a.slot, row0, a.M, a.n_seq, (int)a.max_len, a.kv);
   uint32_t w[R][E / 4];
   int b[R];
 #pragma unroll
@@ -221,7 +226,7 @@ __global__ __launch_bounds__(256) void kv_q8_write_kernel(WriteArgs a, int kv_wg
     const int row = min(max(row0 + i, 0), a.M - 1);
     Chunk<E> c;
     if (is_v) c = load_chunk<E>(a.v + (size_t)row * a.ldv + (size_t)h * HD + d0);
-    else c = load_rotated<E>(a.k + (size_t)row * a.ldk + (size_t)h * HD, d0, a.rope, load_turn<E>(a.rope, d0, rope_row(a.rope, row)));
+    else c = load_rotated<E, MODE>(a.k + (size_t)row * a.ldk + (size_t)h * HD, d0, a.rope, load_turn<E, MODE>(a.rope, d0, rope_row<MODE>(a.rope, row)));
     b[i] = quantise<E>(c, w[i]);
   }
   uint8_t *codes = is_v ? a.cv : a.ck, *exps = is_v ? a.cxv : a.cxk;
@@ -276,7 +281,7 @@ __global__ __launch_bounds__(256) void kv_q8_read_kernel(ReadArgs a, int units) 
   const int u = id % (2 * a.kv), h = u < a.kv ? u : u - a.kv;
   const bool is_v = u >= a.kv;
   const int row0 = unit_row<R>(a.slot, unit);
-  const Places<R> at = load_places<R>(a.seq, a.slot, row0, a.M, a.n_seq, a.max_len, a.kv);
+  const Places<R> at = load_places<R>(a.seq, a.slot, row0, a.M, a.n_seq, (int)a.max_len, a.kv);
   const uint8_t *codes = is_v ? a.cv : a.ck, *exps = is_v ? a.cxv : a.cxk;
   uint32_t w[R][E / 4], b[R];
   bool done = false;
@@ -303,7 +308,7 @@ __global__ __launch_bounds__(256) void kv_q8_read_kernel(ReadArgs a, int units) 
   if (!done) {
 #pragma unroll
     for (int i = 0; i < R; ++i) {  // places outside the cache read the first one's codes, and are cleared below
-      const int64_t reg = max(at.reg[i], (int64_t)0) + h;
+      const int64_t reg = max(at.reg[i], 0) + h;
       const int sl = at.reg[i] < 0 ? 0 : at.slot[i];
       b[i] = exps[reg * a.max_len + q8_x_off(sl)];
       if (!is_v) {
@@ -402,6 +407,7 @@ int q8_check(const SsdKvQ8* c, const char* what) {
   if (!c || !c->k || !c->v || !c->k_exp || !c->v_exp) return set_error(SSD_EINVAL, "%s: null cache", what);
   if (c->head_dim != 64 && c->head_dim != 128)
     return set_error(SSD_EINVAL, "%s: head_dim %d unsupported (64, 128)", what, c->head_dim);
+  if ((int64_t)c->n_seq * c->kv_heads > INT32_MAX) return set_error(SSD_ERANGE, "%s: too many sequences", what);
   if (c->n_seq < 1 || c->kv_heads < 1 || c->max_len < 64 || c->max_len % 64 || c->max_len > INT32_MAX - 63)
     return set_error(SSD_EINVAL, "%s: bad cache: %d sequences, %d kv heads, max_len %lld (a multiple of 64)", what,
                      c->n_seq, c->kv_heads, (long long)c->max_len);
@@ -431,20 +437,27 @@ static int by_head_dim(int hd, F f) {
 
 // Units of R rows that cover M rows: with R = 4 the first may begin up to three rows early.
 static int64_t row_units(int M, int r) { return r == 1 ? M : ((int64_t)M + 3) / 4 + 1; }
-// From this many rows on a unit takes four: below, more units are worth more than wider accesses (us for 32 and 4096 rows
-// of 8 kv heads and 32 q heads of 128, one row a unit / four: WRITE_FEW, WRITE_MANY).
-constexpr int Q8_QUAD_ROWS = 256;
+// From this many (row, kv head) pairs on a unit takes four rows: below, more units and less code are worth more than
+// wider accesses. us, one row a unit / four, 8 kv heads and 32 q heads of 128 rotated: WRITE_TABLE; read: READ_TABLE.
+constexpr int64_t Q8_WRITE_QUADS = 6144, Q8_READ_QUADS = 20480;
 
-template <int HD>
-static int launch_write_hd(const WriteArgs& a, hipStream_t stream, const char* what) {
-  const bool many = a.M >= Q8_QUAD_ROWS;
+template <int HD, int MODE>
+static int launch_write_as(const WriteArgs& a, hipStream_t stream, const char* what) {
+  const bool many = (int64_t)a.M * std::max(a.kv, 1) >= Q8_WRITE_QUADS;
   const int64_t units = a.kv ? row_units(a.M, many ? 4 : 1) : 0, kv_wgs = (units * 2 * a.kv + 15) / 16;
   const int q_units = (a.heads + (many ? 3 : 0)) / (many ? 4 : 1);
   const int64_t wgs = kv_wgs + ((int64_t)a.M * q_units + 15) / 16;
   if (wgs > INT32_MAX / 16) return set_error(SSD_ERANGE, "%s: too many rows", what);
-  if (many) SSD_LAUNCH((kv_q8_write_kernel<HD, 4, 4>), dim3((unsigned)wgs), dim3(256), 0, stream, a, (int)kv_wgs, (int)units, q_units);
-  else SSD_LAUNCH((kv_q8_write_kernel<HD, 1, 1>), dim3((unsigned)wgs), dim3(256), 0, stream, a, (int)kv_wgs, (int)units, q_units);
+  if (many) SSD_LAUNCH((kv_q8_write_kernel<HD, 4, 4, MODE>), dim3((unsigned)wgs), dim3(256), 0, stream, a, (int)kv_wgs, (int)units, q_units);
+  else SSD_LAUNCH((kv_q8_write_kernel<HD, 1, 1, MODE>), dim3((unsigned)wgs), dim3(256), 0, stream, a, (int)kv_wgs, (int)units, q_units);
   return check_launch(what);
+}
+
+template <int HD>
+static int launch_write_hd(const WriteArgs& a, hipStream_t stream, const char* what) {
+  return !a.rope.cos ? launch_write_as<HD, ROPE_NONE>(a, stream, what)
+         : a.rope.interleaved ? launch_write_as<HD, ROPE_PAIRS>(a, stream, what)
+                              : launch_write_as<HD, ROPE_HALF>(a, stream, what);
 }
 
 static int launch_write(const WriteArgs& a, int hd, hipStream_t stream, const char* what) {
@@ -453,7 +466,7 @@ static int launch_write(const WriteArgs& a, int hd, hipStream_t stream, const ch
 
 template <int HD>
 static int launch_read(const ReadArgs& a, hipStream_t stream) {
-  const bool many = a.M >= Q8_QUAD_ROWS;
+  const bool many = (int64_t)a.M * a.kv >= Q8_READ_QUADS;
   const int64_t units = row_units(a.M, many ? 4 : 1), wgs = (units * 2 * a.kv + 15) / 16;
   if (wgs > INT32_MAX / 16) return set_error(SSD_ERANGE, "kv_q8_read: too many rows");
   if (many) SSD_LAUNCH((kv_q8_read_kernel<HD, 4>), dim3((unsigned)wgs), dim3(256), 0, stream, a, (int)units);
