@@ -169,15 +169,14 @@ class KVCacheQ8:
         all places different; rows outside the cache are not written). ``rope``: (cos, sin) tables of
         ``models.llama.rope_tables_f32``, K rotated to ``pos`` before it is quantised; with ``q`` [M, heads * head_dim]
         its rows are rotated too and returned (in ``q_out`` if given, which may be ``q``)."""
-        heads = 0
-        if q is not None:
-            heads = q.shape[1] // self.head_dim
-            if q.shape[1] % self.head_dim:
-                raise ValueError(f"q has {q.shape[1]} columns, not a multiple of head_dim {self.head_dim}")
-            if q_out is None:
-                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        ops.kv_q8_write(self._layers[i], k, v, k.shape[0], seq, slot, rope, pos, interleaved, q, heads, q_out)
-        return q_out
+        heads = 0 if q is None else self._heads(q)
+        return ops.kv_q8_write(self._layers[i], k, v, k.shape[0], seq, slot, rope, pos, interleaved, q, heads, q_out)
+
+    def _heads(self, q: torch.Tensor) -> int:
+        heads, rest = divmod(q.shape[-1], self.head_dim)
+        if rest:
+            raise ValueError(f"q has {q.shape[-1]} columns, not a multiple of head_dim {self.head_dim}")
+        return heads
 
     def load(self, i: int, cache: KVCache, length: int, seq: int = 0, start: int = 0) -> None:
         """Slots [start, length) of a bf16 cache's layer ``i`` (a prompt's, after its prefill) into sequence ``seq``."""
@@ -189,10 +188,7 @@ class KVCacheQ8:
 
     def read(self, i: int, seq: torch.Tensor, slot: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """K, V [M, kv_heads * head_dim] bf16 of layer ``i`` at (seq[m], slot[m]); zeros for places outside the cache."""
-        m, cols = seq.numel(), self.kv_heads * self.head_dim
-        k, v = torch.empty(2, m, cols, dtype=torch.bfloat16, device=self.device)
-        ops.kv_q8_read(self._layers[i], m, seq, slot, k, v)
-        return k, v
+        return ops.kv_q8_read(self._layers[i], seq.numel(), seq, slot)
 
     def attend_floats(self, m: int, heads: int, l_max: int) -> int:
         """Workspace floats of ``attend`` for ``m`` rows."""
@@ -204,15 +200,7 @@ class KVCacheQ8:
         """Tree attention of q [M, heads * head_dim] over layer ``i``: sequence s owns rows row_begin[s] ..
         row_begin[s + 1] (at most rows_max <= 64), row t attends slots [0, prefix[t]) then anc[t, :depth[t]]; zeros for
         rows that attend nothing; rows of no sequence are left as ``out`` has them. l_max bounds prefix + depth. ``ws``: fp32, attend_floats(M, heads, l_max) (None: allocated here)."""
-        m, cols = q.shape
-        if cols % self.head_dim:
-            raise ValueError(f"q has {cols} columns, not a multiple of head_dim {self.head_dim}")
-        if out is None:
-            out = torch.empty(m, cols, dtype=q.dtype, device=q.device)
-        if ws is None:
-            ws = torch.empty(max(self.attend_floats(m, cols // self.head_dim, l_max), 4), dtype=torch.float32,
-                             device=q.device)
-        return ops.tree_attention_q8(self._layers[i], q, m, cols // self.head_dim, row_begin, prefix, depth, anc, rows_max,
+        return ops.tree_attention_q8(self._layers[i], q, q.shape[0], self._heads(q), row_begin, prefix, depth, anc, rows_max,
                                      l_max, self.span, ws, out, scale)
 
     def compact_device(self, start: torch.Tensor, src: torch.Tensor, n: torch.Tensor) -> None:

@@ -110,14 +110,4 @@ def verify_chain(P: torch.Tensor, Q: torch.Tensor, draft: torch.Tensor, u: torch
     (None: all); u [B, K] and u_next [B] uniforms in [0, 1). Returns (accepted counts [B], tokens [B, K + 1]:
     the accepted ones, the next one, then -1), int32. ``ws``: uint8 workspace of
     ops.verify_chain_ws_bytes(B, V) bytes (None: allocated here)."""
-    if P.dim() != 3:
-        raise ValueError(f"P must be [B, K + 1, V], got {tuple(P.shape)}")
-    B, rows, V = P.shape
-    if rows < 1 or V < 1:
-        raise ValueError(f"P must be [B, K + 1, V], got {tuple(P.shape)}")
-    i32 = dict(dtype=torch.int32, device=P.device)
-    tok, n = torch.empty(B, rows, **i32), torch.empty(B, **i32)
-    if ws is None:
-        ws = torch.empty(max(ops.verify_chain_ws_bytes(B, V), 16), dtype=torch.uint8, device=P.device)
-    ops.verify_chain(P, Q, draft, u, u_next, n_draft, tok, n, ws)
-    return n, tok
+    return ops.verify_chain(P, Q, draft, u, u_next, n_draft, ws=ws)

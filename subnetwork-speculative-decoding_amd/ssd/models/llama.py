@@ -138,7 +138,8 @@ def rope_inv_freq(hd: int, theta: float, scaling: Optional[tuple] = None) -> tor
     return torch.where(mid, blend, scaled)
 
 
-def rope_tables_f32(positions: int, rot_dim: int, theta: float, device, scaling: Optional[dict] = None) -> tuple:
+def rope_tables_f32(positions: int, rot_dim: int, theta: float, device,
+                    scaling: Optional[dict] = None) -> ops.RopeTables:
     """cos/sin [positions, rot_dim / 2] in fp32 for ``ops.rope`` and the 8-bit cache's write, from frequencies and angles
     in 64 bits (at position 10^6 an fp32 angle is off by 0.03). ``scaling`` (HF's keys, ``rope_type``): "linear"
     (factor), "llama3" (factor, low_freq_factor, high_freq_factor, original_max_position_embeddings) or "yarn"
@@ -171,7 +172,7 @@ def rope_tables_f32(positions: int, rot_dim: int, theta: float, device, scaling:
     elif kind != "default":
         raise ValueError(f"rope_type {kind!r} is not supported (default, linear, llama3, yarn)")
     ang = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * inv.to(device)
-    return (ang.cos() * gain).float(), (ang.sin() * gain).float()
+    return ops.RopeTables((ang.cos() * gain).float(), (ang.sin() * gain).float())
 
 
 def rope_tables(positions: int, hd: int, theta: float, device,

@@ -517,26 +517,26 @@ def add_rmsnorm(part, s, ld, h, m, w, eps, out, bias=None):
 I32, F32 = torch.int32, torch.float32
 
 
+def _refuse(t, name: str, dtype, dev: int, what: str):
+    got = f"{tuple(t.shape)}, strides {t.stride()}, {t.dtype} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
+    raise ValueError(f"{name} must be a {dtype} tensor on the current device cuda:{dev}{what}, got {got}")
+
+
 def _ptr(t, name: str, dtype, dev: int, least: int = 0) -> int:
     """Address of a ``dtype`` tensor on device ``dev``; ``least`` > 0: contiguous with that many elements or more."""
-    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.get_device() != dev:
-        raise ValueError(f"{name} must be a {dtype} tensor on the current device cuda:{dev}, got "
-                         f"{(t.dtype, t.device) if isinstance(t, torch.Tensor) else type(t).__name__}")
-    if least and (t.numel() < least or not t.is_contiguous()):
-        raise ValueError(f"{name} must be contiguous with at least {least} elements, got {tuple(t.shape)}")
-    return t.data_ptr()
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == dev and (
+            not least or t.numel() >= least and t.is_contiguous()):
+        return t.data_ptr()
+    _refuse(t, name, dtype, dev, f", contiguous with at least {least} elements" if least else "")
 
 
 def _rows_ptr(t, name: str, dev: int, rows: int, cols: int) -> tuple:
     """Address and row stride of bf16 rows [>= rows, >= cols] with unit column stride and 16-byte alignment."""
-    p = _ptr(t, name, BF16, dev)
-    if t.dim() != 2:
-        raise ValueError(f"{name} must be [>={rows}, >={cols}], got {tuple(t.shape)}")
-    (n, c), (ld, one) = t.shape, t.stride()
-    if n < rows or c < cols or one != 1 or p % 16 or ld % 8:
-        raise ValueError(f"{name} must be [>={rows}, >={cols}] with unit column stride and 16-byte aligned rows, got "
-                         f"{tuple(t.shape)}, strides {t.stride()}")
-    return p, ld
+    if isinstance(t, torch.Tensor) and t.dtype is BF16 and t.get_device() == dev and t.dim() == 2:
+        p, (ld, one), (n, c) = t.data_ptr(), t.stride(), t.shape
+        if one == 1 and n >= rows and c >= cols and not (p % 16 or ld % 8):
+            return p, ld
+    _refuse(t, name, BF16, dev, f", [>={rows}, >={cols}] with unit column stride and 16-byte aligned rows")
 
 
 def _stream(dev: int) -> int:
@@ -551,20 +551,33 @@ def _cache_dev(cache) -> int:
     return dev
 
 
-def _rope_struct(rope, pos, interleaved, m, head_dim, dev):
-    """(SsdRope reference, positions' address) of (cos, sin) fp32 tables [rows, rot_dim / 2]; (None, None) without rope."""
+class RopeTables(tuple):
+    """(cos, sin), contiguous fp32 [positions, rot_dim / 2], with their descriptors for the kernels."""
+
+    def __new__(cls, cos: torch.Tensor, sin: torch.Tensor):
+        if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype is not F32 or sin.dtype is not F32 or (
+                cos.device != sin.device or not (cos.is_contiguous() and sin.is_contiguous())):
+            raise ValueError(f"rotary tables must be two contiguous fp32 [positions, rot_dim / 2] tensors on one device, got "
+                             f"{tuple(cos.shape)} {cos.dtype}, {tuple(sin.shape)} {sin.dtype}")
+        self = super().__new__(cls, (cos, sin))
+        n, half = cos.shape
+        self.rot_dim, self.device_index = 2 * half, cos.get_device()
+        self._desc = [_lib.SsdRope(cos.data_ptr(), sin.data_ptr(), n, 2 * half, i) for i in (0, 1)]
+        self._refs = [ctypes.byref(d) for d in self._desc]
+        return self
+
+
+def _rope_args(rope, pos, interleaved, m, head_dim, dev):
+    """(descriptor reference, positions' address) for ``m`` rows; (None, None) without rope."""
     if rope is None:
         if pos is not None:
             raise ValueError("positions without rotary tables")
         return None, None
-    cos, sin = rope
-    if cos.dim() != 2 or cos.shape != sin.shape or 2 * cos.shape[1] > head_dim:
-        raise ValueError(f"rotary tables must be two [rows, rot_dim / 2] tensors, rot_dim <= {head_dim}, got "
-                         f"{tuple(cos.shape)}, {tuple(sin.shape)}")
-    n, half = cos.shape
-    st = _lib.SsdRope(_ptr(cos, "cos", F32, dev, n * half), _ptr(sin, "sin", F32, dev, n * half), n, 2 * half,
-                      1 if interleaved else 0)
-    return ctypes.byref(st), _ptr(pos, "pos", I32, dev, m)
+    if not isinstance(rope, RopeTables):
+        rope = RopeTables(*rope)
+    if rope.rot_dim > head_dim or rope.device_index != dev:
+        raise ValueError(f"rotary tables of {rope.rot_dim} dims on device {rope.device_index} for heads of {head_dim} on cuda:{dev}")
+    return rope._refs[1 if interleaved else 0], _ptr(pos, "pos", I32, dev, m)
 
 
 def rope(x, m, heads, head_dim, tables, pos, out, interleaved: bool = False):
@@ -575,7 +588,8 @@ def rope(x, m, heads, head_dim, tables, pos, out, interleaved: bool = False):
         raise ValueError("rope needs rotary tables")
     px, ldx = _rows_ptr(x, "x", dev, m, heads * head_dim)
     po, ldo = _rows_ptr(out, "out", dev, m, heads * head_dim)
-    st, pp = _rope_struct(tables, pos, interleaved, m, head_dim, dev)
+    tables = tables if isinstance(tables, RopeTables) else RopeTables(*tables)
+    st, pp = _rope_args(tables, pos, interleaved, m, head_dim, dev)
     if m:
         _lib.call("ssd_rope_bf16", st, pp, px, ldx, m, heads, head_dim, po, ldo, _stream(dev))
     return out
@@ -583,32 +597,47 @@ def rope(x, m, heads, head_dim, tables, pos, out, interleaved: bool = False):
 
 def kv_q8_write(cache, k, v, m, seq, slot, rope=None, pos=None, interleaved=False, q=None, heads=0, q_out=None):
     """Rows of K (rotated first when ``rope`` is given) and V quantised into ``cache`` (SsdKvQ8 of one layer) at
-    (seq, slot); with ``q`` its rows are rotated into ``q_out`` in the same launch (ssd_kv_q8_write_bf16)."""
+    (seq, slot); with ``q`` its rows are rotated into ``q_out`` (made here if None) in the same launch, and returned
+    (ssd_kv_q8_write_bf16)."""
     dev, hd = _cache_dev(cache), cache.head_dim
     cols = cache.kv_heads * hd
     pk, ldk = _rows_ptr(k, "k", dev, m, cols)
     pv, ldv = _rows_ptr(v, "v", dev, m, cols)
     ps, pl = _ptr(seq, "seq", I32, dev, m), _ptr(slot, "slot", I32, dev, m)
-    st, pp = _rope_struct(rope, pos, interleaved, m, hd, dev)
+    tables = rope if rope is None or isinstance(rope, RopeTables) else RopeTables(*rope)
+    st, pp = _rope_args(tables, pos, interleaved, m, hd, dev)
     pq = po = None
     ldq = ldo = 0
     if q is not None:
         pq, ldq = _rows_ptr(q, "q", dev, m, heads * hd)
-        po, ldo = _rows_ptr(q_out, "q_out", dev, m, heads * hd)
+        if q_out is None:
+            ldo = heads * hd
+            q_out = q.new_empty((q.shape[0], ldo))
+            po = q_out.data_ptr()
+        else:
+            po, ldo = _rows_ptr(q_out, "q_out", dev, m, heads * hd)
     if m:
         _lib.call("ssd_kv_q8_write_bf16", cache.ref, pk, ldk, pv, ldv, m, ps, pl, st, pp, pq, ldq, heads, po, ldo,
                   _stream(dev))
+    return q_out
 
 
-def kv_q8_read(cache, m, seq, slot, k_out, v_out):
-    """The cached values of (seq, slot) as bf16 rows (ssd_kv_q8_read_bf16); zeros for places outside the cache."""
+def kv_q8_read(cache, m, seq, slot, k_out=None, v_out=None):
+    """The cached values of (seq, slot) as bf16 rows k_out, v_out (made here if both are None; ssd_kv_q8_read_bf16); zeros for
+    places outside the cache."""
     dev = _cache_dev(cache)
     cols = cache.kv_heads * cache.head_dim
     ps, pl = _ptr(seq, "seq", I32, dev, m), _ptr(slot, "slot", I32, dev, m)
-    pk, ldk = _rows_ptr(k_out, "k_out", dev, m, cols)
-    pv, ldv = _rows_ptr(v_out, "v_out", dev, m, cols)
+    if k_out is None and v_out is None:
+        k_out = torch.empty((m, cols), dtype=BF16, device=seq.device)
+        v_out = torch.empty_like(k_out)
+        pk, pv, ldk, ldv = k_out.data_ptr(), v_out.data_ptr(), cols, cols
+    else:
+        pk, ldk = _rows_ptr(k_out, "k_out", dev, m, cols)
+        pv, ldv = _rows_ptr(v_out, "v_out", dev, m, cols)
     if m:
         _lib.call("ssd_kv_q8_read_bf16", cache.ref, m, ps, pl, pk, ldk, pv, ldv, _stream(dev))
+    return k_out, v_out
 
 
 def kv_q8_compact(cache, layers, start, src, n, n_max):
@@ -627,13 +656,21 @@ def attn_q8_ws_floats(m: int, heads: int, head_dim: int, l_max: int, span: int) 
     return n
 
 
-def tree_attention_q8(cache, q, m, heads, row_begin, prefix, depth, anc, rows_max, l_max, span, ws, out, scale=None):
-    """Tree attention of a batch's rows over ``cache`` (SsdKvQ8 of one layer; ssd_tree_attention_q8)."""
+def tree_attention_q8(cache, q, m, heads, row_begin, prefix, depth, anc, rows_max, l_max, span, ws=None, out=None, scale=None):
+    """Tree attention of a batch's rows over ``cache`` (SsdKvQ8 of one layer; ssd_tree_attention_q8). ``ws`` (fp32,
+    attn_q8_ws_floats(...)) and ``out`` are made here if None."""
     dev, hd = _cache_dev(cache), cache.head_dim
-    pq, ldq = _rows_ptr(q, "q", dev, m, heads * hd)
-    po, ldo = _rows_ptr(out, "out", dev, m, heads * hd)
+    cols = heads * hd
+    pq, ldq = _rows_ptr(q, "q", dev, m, cols)
+    if out is None:
+        out, ldo = q.new_empty((q.shape[0], cols)), cols
+        po = out.data_ptr()
+    else:
+        po, ldo = _rows_ptr(out, "out", dev, m, cols)
     pb, pp = _ptr(row_begin, "row_begin", I32, dev, cache.n_seq + 1), _ptr(prefix, "prefix", I32, dev, m)
     pd, pa = _ptr(depth, "depth", I32, dev, m), _ptr(anc, "anc", I32, dev, m * 32)
+    if ws is None:
+        ws = torch.empty(max(attn_q8_ws_floats(m, heads, hd, l_max, span), 4), dtype=F32, device=q.device)
     pw = _ptr(ws, "ws", F32, dev, 1)
     if m:
         _lib.call("ssd_tree_attention_q8", cache.ref, pq, ldq, m, heads, pb, pp, pd, pa, rows_max, l_max, span,
@@ -758,26 +795,35 @@ def verify_chain_ws_bytes(n_seq: int, V: int) -> int:
     return b
 
 
-def verify_chain(P, Q, draft, u, u_next, n_draft, out_tok, out_n, ws):
-    """ssd_verify_chain over P [n_seq, k + 1, V] and Q [n_seq, k, V] fp32 (unit column stride)."""
+def verify_chain(P, Q, draft, u, u_next, n_draft=None, out_tok=None, out_n=None, ws=None):
+    """ssd_verify_chain over P [n_seq, k + 1, V] and Q [n_seq, k, V] fp32 (unit column stride); draft, u [n_seq, k] and u_next,
+    n_draft [n_seq] contiguous. out_n [n_seq], out_tok [n_seq, k + 1] (int32) and ws (uint8,
+    verify_chain_ws_bytes(...)) are made here if None. Returns (out_n, out_tok)."""
     dev = torch.cuda.current_device()
-    n_seq, rows, V = P.shape
-    k = rows - 1
-    if Q.shape != (n_seq, k, V) or draft.shape != (n_seq, k) or u.shape != (n_seq, k) or u_next.shape != (n_seq,) or (
-            n_draft is not None and n_draft.shape != (n_seq,)) or out_tok.shape != (n_seq, rows) or out_n.shape != (n_seq,):
-        raise ValueError(f"verify_chain: for P {tuple(P.shape)} the others must be Q {(n_seq, k, V)}, draft and u {(n_seq, k)}, "
-                         f"u_next, n_draft and out_n {(n_seq,)}, out_tok {(n_seq, rows)}; got Q {tuple(Q.shape)}, draft "
-                         f"{tuple(draft.shape)}, u {tuple(u.shape)}, u_next {tuple(u_next.shape)}")
     pp, pq = _ptr(P, "P", F32, dev), _ptr(Q, "Q", F32, dev)
-    pst, qst = P.stride(), Q.stride()
-    if V > 1 and (pst[2] != 1 or (k and qst[2] != 1)):
-        raise ValueError("P and Q need unit column stride")
-    if n_seq == 0:
-        return
-    # a dimension of one row has any stride
+    if P.dim() != 3 or Q.dim() != 3:
+        raise ValueError(f"P and Q must be [n_seq, k + 1, V] and [n_seq, k, V], got {tuple(P.shape)}, {tuple(Q.shape)}")
+    (n_seq, rows, V), (ps, pr, pc), (qs, qr, qc) = P.shape, P.stride(), Q.stride()
+    k = rows - 1
+    if rows < 1 or V < 1 or Q.shape != (n_seq, k, V) or V > 1 and (pc != 1 or k and qc != 1):
+        raise ValueError(f"P and Q must be [n_seq, k + 1, V] and [n_seq, k, V] with unit column stride, got {tuple(P.shape)}, "
+                         f"strides {P.stride()}, and {tuple(Q.shape)}, strides {Q.stride()}")
     pd, pu = _ptr(draft, "draft", I32, dev, n_seq * k), _ptr(u, "u", F32, dev, n_seq * k)
     pn, px = None if n_draft is None else _ptr(n_draft, "n_draft", I32, dev, n_seq), _ptr(u_next, "u_next", F32, dev, n_seq)
-    _lib.call("ssd_verify_chain", pp, pst[0], max(pst[1], V) if rows == 1 else pst[1], pq, qst[0],
-              max(qst[1], V) if k == 1 else qst[1], V, n_seq, k, pd, pn, pu, px, _ptr(ws, "ws", torch.uint8, dev, 1),
-              ws.numel(), _ptr(out_tok, "out_tok", I32, dev, n_seq * rows), _ptr(out_n, "out_n", I32, dev, n_seq),
-              _stream(dev))
+    if draft.shape != (n_seq, k) or u.shape != (n_seq, k) or u_next.numel() != n_seq or n_draft is not None and (
+            n_draft.numel() != n_seq):
+        raise ValueError(f"for {n_seq} sequences of {k} drafted tokens: draft {tuple(draft.shape)}, u {tuple(u.shape)}, u_next "
+                         f"{tuple(u_next.shape)}, n_draft {None if n_draft is None else tuple(n_draft.shape)}")
+    if out_tok is None:
+        out_tok = draft.new_empty((n_seq, rows))
+    elif out_tok.shape != (n_seq, rows):
+        raise ValueError(f"out_tok must be {(n_seq, rows)}, got {tuple(out_tok.shape)}")
+    if out_n is None:
+        out_n = draft.new_empty(n_seq)
+    if ws is None:
+        ws = torch.empty(verify_chain_ws_bytes(n_seq, V) + 16, dtype=torch.uint8, device=P.device)
+    if n_seq:  # a dimension of one row may have any stride
+        _lib.call("ssd_verify_chain", pp, ps, pr if k else V, pq, qs, qr if k > 1 else V, V, n_seq, k, pd, pn, pu, px,
+                  _ptr(ws, "ws", torch.uint8, dev, 1), ws.numel(), _ptr(out_tok, "out_tok", I32, dev, n_seq),
+                  _ptr(out_n, "out_n", I32, dev, n_seq), _stream(dev))
+    return out_n, out_tok

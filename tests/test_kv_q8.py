@@ -232,7 +232,7 @@ def test_workspace_sizes():
 
 def test_python_refusals_without_a_gpu():
     from ssd.engine.kv_cache import KVCacheQ8
-    from ssd.engine.verify import verify_chain
+    from ssd import ops
 
     with pytest.raises(ValueError, match="head_dim"):
         KVCacheQ8(1, 64, 2, 96, "cpu")
@@ -240,5 +240,7 @@ def test_python_refusals_without_a_gpu():
         KVCacheQ8(1, 64, 2, 64, "cpu", span=100)
     with pytest.raises(ValueError, match="positive"):
         KVCacheQ8(1, 0, 2, 64, "cpu")
-    with pytest.raises(ValueError, match="B, K"):
-        verify_chain(torch.zeros(3, 5), None, None, None, None)
+    t = torch.zeros(4, 8)
+    for cos, sin in ((t, t[:, :4]), (t.double(), t.double()), (t[:, ::2], t[:, ::2]), (t[0], t[0])):
+        with pytest.raises(ValueError, match="rotary tables"):
+            ops.RopeTables(cos, sin)
