@@ -37,6 +37,7 @@ struct AttnQ8Args {
   const int *row_begin, *prefix, *depth, *anc;
   int l_max, span_blk, n_grps;
   int units, sets, tiles_per_set;  // launch geometry of the shared groups
+  int own_units, own_rows;         // and of the rows' own
   float scale_log2;
   float* ws_o;    // [row][head][group][HD]: O
   float2* ws_ml;  // [row][head][group]: (m, l)
@@ -230,13 +231,15 @@ struct alignas(16) Q8Spans {
   float m[QA_GRP][16], l[QA_GRP][16];
 };
 
-// Wave w leaves its span's state; one without keys leaves (-inf, 0, 0).
+// A wave leaves span s's state for tile rows r0 .. r0 + n, its lanes j < n; one without keys leaves (-inf, 0, 0).
 template <int HD>
-__device__ __forceinline__ void q8_publish(Q8Spans<HD>& lds, int w, int j, int g, bool have, const Q8State<HD>& st) {
-  lds.m[w][j] = have ? st.m : -INFINITY;  // the four lanes of row j write the same values
-  lds.l[w][j] = have ? st.l[0] : 0.f;
+__device__ __forceinline__ void q8_publish(Q8Spans<HD>& lds, int s, int r0, int n, int j, int g, bool have, const Q8State<HD>& st) {
+  if (j >= n) return;
+  lds.m[s][r0 + j] = have ? st.m : -INFINITY;  // the four lanes of row j write the same values
+  lds.l[s][r0 + j] = have ? st.l[0] : 0.f;
 #pragma unroll
-  for (int dt = 0; dt < HD / 16; ++dt) *(f32x4_t*)&lds.o[w][j][dt * 16 + 4 * g] = have ? st.o[dt] : f32x4_t{0.f, 0.f, 0.f, 0.f};
+  for (int dt = 0; dt < HD / 16; ++dt)
+    *(f32x4_t*)&lds.o[s][r0 + j][dt * 16 + 4 * g] = have ? st.o[dt] : f32x4_t{0.f, 0.f, 0.f, 0.f};
 }
 
 // Row rr's record, dims 4 dc .. + 4 of every 64: the largest reference first, then the weighted sums in order.
@@ -326,7 +329,7 @@ __device__ __forceinline__ void q8_shared_group(const AttnQ8Args& a, int id, Q8S
     q8_fold<HD, T, false, false>(f, qf, 0, a.scale_log2, j, st, next_k, next_v);
   }
 #pragma unroll
-  for (int t = 0; t < T; ++t) q8_publish<HD>(lds[t], w, j, g, true, st[t]);
+  for (int t = 0; t < T; ++t) q8_publish<HD>(lds[t], w, 0, 16, j, g, true, st[t]);
   __syncthreads();
   const int rr = threadIdx.x >> 4, dc = threadIdx.x & 15;
 #pragma unroll
@@ -399,45 +402,50 @@ __device__ __forceinline__ uint32_t q8_load_own(Q8Frags<HD>& f, const uint8_t* K
   return valid;
 }
 
-// The row's keys: P cache slots, then L - P ancestors, staged by the whole workgroup.
-template <int HD, int NT>
+// The row's D ancestors, staged by NT threads (tid < NT); sync makes their LDS writes visible to each other.
+template <int HD, int NT, typename Sync>
 __device__ __forceinline__ void q8_stage_anc(const AttnQ8Args& a, int row, int D, const uint8_t* V, const uint8_t* Kx,
-                                             const uint8_t* Vx, Q8Anc<HD>& anc) {
+                                             const uint8_t* Vx, Q8Anc<HD>& anc, int tid, Sync sync) {
   if (D == 0) return;  // uniform
-  if (threadIdx.x < QA_MAXD) {
-    const int sl = threadIdx.x < D ? a.anc[(size_t)row * QA_MAXD + threadIdx.x] : -1;
+  if (tid < QA_MAXD) {
+    const int sl = tid < D ? a.anc[(size_t)row * QA_MAXD + tid] : -1;
     const bool ok = sl >= 0 && sl < a.max_len;
-    anc.slot[threadIdx.x] = ok ? sl : -1;
-    anc.x[0][threadIdx.x] = ok ? Kx[q8_x_off(sl)] : 127;
-    anc.x[1][threadIdx.x] = ok ? Vx[q8_x_off(sl)] : 127;
+    anc.slot[tid] = ok ? sl : -1;
+    anc.x[0][tid] = ok ? Kx[q8_x_off(sl)] : 127;
+    anc.x[1][tid] = ok ? Vx[q8_x_off(sl)] : 127;
   }
-  __syncthreads();
-  constexpr int IT = (QA_MAXD * HD + NT - 1) / NT;
-  uint8_t c[IT];
+  sync();
+  // a thread takes the same dim of every NT / HD-th ancestor, sixteen loads in flight
+  constexpr int STEP = NT >= HD ? NT / HD : 1, DIMS = NT >= HD ? 1 : HD / NT, BATCH = 16 / DIMS;
+  const int d = tid % HD;
+  for (int n0 = NT >= HD ? tid / HD : 0; n0 < D; n0 += STEP * BATCH) {
+    uint8_t c[BATCH][DIMS];
 #pragma unroll
-  for (int it = 0; it < IT; ++it) {
-    if (it * NT >= D * HD) break;  // uniform
-    const int i = min((int)threadIdx.x + it * NT, D * HD - 1), sl = anc.slot[i / HD];
-    c[it] = V[q8_v_off(sl >= 0 ? sl : 0, i % HD, HD)];
-  }
+    for (int i = 0; i < BATCH; ++i) {
+      const int sl = anc.slot[min(n0 + i * STEP, D - 1)];
 #pragma unroll
-  for (int it = 0; it < IT; ++it) {
-    if (it * NT >= D * HD) break;
-    const int i = min((int)threadIdx.x + it * NT, D * HD - 1);
-    anc.v[i / HD][i % HD] = anc.slot[i / HD] >= 0 ? c[it] : 0;
+      for (int e = 0; e < DIMS; ++e) c[i][e] = V[q8_v_off(sl >= 0 ? sl : 0, d + e * NT, HD)];
+    }
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i)
+      if (n0 + i * STEP < D) {
+#pragma unroll
+        for (int e = 0; e < DIMS; ++e) anc.v[n0 + i * STEP][d + e * NT] = anc.slot[n0 + i * STEP] >= 0 ? c[i][e] : 0;
+      }
   }
-  __syncthreads();
+  sync();
 }
 
-// Wave w's span of group grp for the heads h0 .. h0 + nh of one row; false: no keys.
+// A span of keys (positions below P cache slots, those in [P, L) ancestors) for the query at q on each lane j; false:
+// no keys.
 template <int HD>
-__device__ __forceinline__ bool q8_own_span(const AttnQ8Args& a, size_t reg, int row, int h0, int nh, int span, int P, int L,
+__device__ __forceinline__ bool q8_own_span(const AttnQ8Args& a, size_t reg, const bf16_t* q, int span, int P, int L,
                                             const Q8Anc<HD>& anc, int lane, Q8State<HD> (&st)[1]) {
   const int b0 = span * a.span_blk, b1 = min((L + QA_BLK - 1) / QA_BLK, b0 + a.span_blk), j = lane & 15;
   if (b0 >= b1) return false;
   const uint8_t *K = a.K + reg * HD, *V = a.V + reg * HD, *Kx = a.Kx + reg, *Vx = a.Vx + reg;
   u32x4_t qf[1][HD / 32];
-  q8_load_q<HD>(qf[0], a.Q + (size_t)row * a.ldq + (size_t)(h0 + min(j, nh - 1)) * HD, lane >> 4);
+  q8_load_q<HD>(qf[0], q, lane >> 4);
   st[0].m = -INFINITY;
   st[0].l = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -461,31 +469,52 @@ __device__ __forceinline__ void q8_row_keys(const AttnQ8Args& a, int row, int& P
   L = min(P + min(max(a.depth[row], 0), QA_MAXD), a.l_max);
 }
 
-// A row's own groups: from the one its sequence's smallest prefix ends in to its last, one after the other, a wave a span.
+// The groups that rows of a sequence do not attend whole together: from the one the smallest prefix ends in to each
+// row's last. One workgroup per (sequence, kv head, up to four rows that fill a tile: 16 / rep); wave w has row w. Spans
+// all rows attend whole are folded for the tile (span s by wave 3 - s: with one row wave 0 is free for it), the
+// spans after by each row's wave; together they make the rows' records of the group.
 template <int HD>
-__device__ __forceinline__ void q8_own_groups(const AttnQ8Args& a, int id, int rows_max, Q8Spans<HD>& lds, Q8Anc<HD>& anc) {
+__device__ __forceinline__ void q8_own_groups(const AttnQ8Args& a, int id, Q8Spans<HD>& lds, Q8Anc<HD>& anc) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, j = lane & 15, g = lane >> 4;
-  const int kvh = id % a.kv, seq = id / a.kv / rows_max;
-  int r0, r1, P, L;
+  const int unit = id % a.own_units, kvh = unit % a.kv, seq = unit / a.kv;
+  if (seq >= a.n_seq) return;  // units are rounded up to 8: a unit's rows and its shared groups meet on one XCD
+  int r0, r1;
   q8_rows(a, seq, r0, r1);
-  const int row = r0 + id / a.kv % rows_max;
-  if (row >= r1) return;
-  const int nb = q8_shared_blocks(a, r0, r1, lane), per = QA_GRP * a.span_blk;
-  q8_row_keys(a, row, P, L);
+  const int base = r0 + id / a.own_units * a.own_rows, n_rows = min(a.own_rows, r1 - base);
+  if (n_rows <= 0) return;
+  const int cut = q8_shared_blocks(a, r0, r1, lane) / a.span_blk, per = QA_GRP * a.span_blk * QA_BLK;
   const size_t reg = ((size_t)seq * a.kv + kvh) * a.max_len;
-  const int n_grp = (L + per * QA_BLK - 1) / (per * QA_BLK);
-  if (nb / per >= n_grp) return;
-  q8_stage_anc<HD, 256>(a, row, L - P, a.V + reg * HD, a.Kx + reg, a.Vx + reg, anc);
-  for (int grp = nb / per; grp < n_grp; ++grp)
-    for (int t0 = 0; t0 < a.rep; t0 += 16) {
+  int p_of, l_of;  // of row base + lane (past the last: the last's)
+  q8_row_keys(a, base + min(lane, n_rows - 1), p_of, l_of);
+  const int n_grp = (-wave_min(-l_of) + per - 1) / per;
+  const int P = __builtin_amdgcn_readlane(p_of, w), L = __builtin_amdgcn_readlane(l_of, w);
+  if (cut / QA_GRP >= n_grp) return;
+  if (w < n_rows)
+    q8_stage_anc<HD, 64>(a, base + w, L - P, a.V + reg * HD, a.Kx + reg, a.Vx + reg, anc, lane, [] {
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");  // one wave's LDS accesses are in order: keep the compiler's so
+      __builtin_amdgcn_wave_barrier();
+    });
+  for (int grp = cut / QA_GRP; grp < n_grp; ++grp)
+    for (int t0 = 0; t0 < a.rep; t0 += 16) {  // more than one turn only with one row
       const int nh = min(16, a.rep - t0), h0 = kvh * a.rep + t0;
-      Q8State<HD> st[1];
-      const bool have = q8_own_span<HD>(a, reg, row, h0, nh, grp * QA_GRP + w, P, L, anc, lane, st);
       __syncthreads();  // the tile before has been merged
-      q8_publish<HD>(lds, w, j, g, have, st[0]);
+      for (int it = -1; it < QA_GRP; ++it) {
+        const bool all = it < 0;  // the span for all rows, then the row's own
+        const int s = all ? QA_GRP - 1 - w : it, span = grp * QA_GRP + s;
+        if (all ? span >= cut : w >= n_rows || span < cut) continue;
+        const int r = min(all ? j / nh : w, n_rows - 1), h = h0 + (all ? j % nh : min(j, nh - 1));
+        const int keys = all ? (span + 1) * a.span_blk * QA_BLK : 0;
+        Q8State<HD> st[1];
+        const bool have = q8_own_span<HD>(a, reg, a.Q + (size_t)(base + r) * a.ldq + (size_t)h * HD, span, all ? keys : P,
+                                          all ? keys : L, anc, lane, st);
+        q8_publish<HD>(lds, s, all ? 0 : w * nh, all ? 16 : nh, j, g, have, st[0]);
+      }
       __syncthreads();
       const int rr = threadIdx.x >> 4, dc = threadIdx.x & 15;
-      if (rr < nh) q8_store_record<HD>(a, ((size_t)row * a.heads + h0 + rr) * a.n_grps + grp, dc, q8_merge<HD>(lds, rr, dc));
+      if (rr < n_rows * nh) {
+        if (grp * per < __shfl(l_of, rr / nh))
+          q8_store_record<HD>(a, ((size_t)(base + rr / nh) * a.heads + h0 + rr % nh) * a.n_grps + grp, dc, q8_merge<HD>(lds, rr, dc));
+      }
     }
 }
 
@@ -494,19 +523,16 @@ union alignas(16) Q8FoldLds {
   Q8Spans<HD> shared[T];
   struct {
     Q8Spans<HD> spans;
-    Q8Anc<HD> anc;
+    Q8Anc<HD> anc[4];
   } own;
 };
 
 // First launch: workgroups of rows (ids first: theirs is the longer chain of loads), then of shared groups.
 template <int HD, int T>
-__global__ __launch_bounds__(256, 2) void q8_fold_kernel(AttnQ8Args a, int rows_max, int own) {
+__global__ __launch_bounds__(256, 2) void q8_fold_kernel(AttnQ8Args a, int own) {
   __shared__ Q8FoldLds<HD, T> lds;
-  if ((int)blockIdx.x < own) {
-    if ((int)blockIdx.x < a.n_seq * rows_max * a.kv) q8_own_groups<HD>(a, blockIdx.x, rows_max, lds.own.spans, lds.own.anc);
-  } else {
-    q8_shared_group<HD, T>(a, blockIdx.x - own, lds.shared);
-  }
+  if ((int)blockIdx.x < own) q8_own_groups<HD>(a, blockIdx.x, lds.own.spans, lds.own.anc[threadIdx.x >> 6]);
+  else q8_shared_group<HD, T>(a, blockIdx.x - own, lds.shared);
 }
 
 // Second launch: one workgroup of four waves per (row, head). Weights from the groups' largest reference; wave r
@@ -595,13 +621,14 @@ __global__ __launch_bounds__(256 * TEAMS) void q8_short_kernel(AttnQ8Args a, int
   if (row >= r1) return;
   q8_row_keys(a, row, P, L);
   const size_t reg = ((size_t)seq * a.kv + kvh) * a.max_len;
-  q8_stage_anc<HD, 256 * TEAMS>(a, row, L - P, a.V + reg * HD, a.Kx + reg, a.Vx + reg, lds.anc);
+  q8_stage_anc<HD, 256 * TEAMS>(a, row, L - P, a.V + reg * HD, a.Kx + reg, a.Vx + reg, lds.anc, threadIdx.x, [] { __syncthreads(); });
   for (int t0 = 0; t0 < a.rep; t0 += 16) {
     const int nh = min(16, a.rep - t0), h0 = kvh * a.rep + t0;
     Q8State<HD> st[1];
-    const bool have = q8_own_span<HD>(a, reg, row, h0, nh, team * QA_GRP + w, P, L, lds.anc, lane, st);
+    const bool have = q8_own_span<HD>(a, reg, a.Q + (size_t)row * a.ldq + (size_t)(h0 + min(j, nh - 1)) * HD, team * QA_GRP + w, P,
+                                      L, lds.anc, lane, st);
     if (t0) __syncthreads();  // the heads before have been written out
-    q8_publish<HD>(lds.spans[team], w, j, g, have, st[0]);
+    q8_publish<HD>(lds.spans[team], w, 0, 16, j, g, have, st[0]);
     __syncthreads();
     const int rr = threadIdx.x >> 4 & 15, dc = threadIdx.x & 15;
     const Q8Record<HD> r = q8_merge<HD>(lds.spans[team], rr, dc);
@@ -652,10 +679,12 @@ static int launch_attn_q8(AttnQ8Args a, int rows_max, hipStream_t stream) {
   const bool single = tiles == 1;
   a.sets = single ? 1 : (tiles + 1) / 2;
   a.tiles_per_set = single ? 1 : (tiles + a.sets - 1) / a.sets;
-  const int64_t units = (int64_t)a.n_seq * a.n_grps * a.kv, shared = (units + 7) / 8 * 8 * a.sets, own = (rows + 7) / 8 * 8;
+  const int64_t units = (int64_t)a.n_seq * a.n_grps * a.kv, shared = (units + 7) / 8 * 8 * a.sets;
+  a.own_rows = std::min(4, std::max(1, 16 / a.rep));
+  const int64_t own_units = ((int64_t)a.n_seq * a.kv + 7) / 8 * 8, own = own_units * ((rows_max + a.own_rows - 1) / a.own_rows);
   if (shared + own > INT32_MAX || (int64_t)a.M * a.heads > INT32_MAX)
     return set_error(SSD_ERANGE, "attention_q8: too many workgroups");
-  a.units = (int)units;
+  a.units = (int)units, a.own_units = (int)own_units;
   auto one_launch = [&](auto t) {
     SSD_LAUNCH((q8_short_kernel<HD, decltype(t)::value>), dim3((unsigned)rows), dim3(256 * decltype(t)::value), 0, stream, a, rows_max);
     return check_launch("attn_q8_short");
@@ -664,8 +693,8 @@ static int launch_attn_q8(AttnQ8Args a, int rows_max, hipStream_t stream) {
   if (a.n_grps == 2 && rows <= 512) return one_launch(integral_constant<int, 2>());
   if constexpr (HD == 64)
     if (a.n_grps <= 4 && rows <= 256) return one_launch(integral_constant<int, 4>());
-  if (single) SSD_LAUNCH((q8_fold_kernel<HD, 1>), dim3((unsigned)(own + shared)), dim3(256), 0, stream, a, rows_max, (int)own);
-  else SSD_LAUNCH((q8_fold_kernel<HD, 2>), dim3((unsigned)(own + shared)), dim3(256), 0, stream, a, rows_max, (int)own);
+  if (single) SSD_LAUNCH((q8_fold_kernel<HD, 1>), dim3((unsigned)(own + shared)), dim3(256), 0, stream, a, (int)own);
+  else SSD_LAUNCH((q8_fold_kernel<HD, 2>), dim3((unsigned)(own + shared)), dim3(256), 0, stream, a, (int)own);
   if (int rc = check_launch("attn_q8_fold")) return rc;
   SSD_LAUNCH((q8_combine_kernel<HD>), dim3((unsigned)(a.M * a.heads)), dim3(256), 0, stream, a);
   return check_launch("attn_q8_combine");
