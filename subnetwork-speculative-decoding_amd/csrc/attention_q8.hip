@@ -342,35 +342,83 @@ __device__ __forceinline__ void q8_shared_group(const AttnQ8Args& a, int id, Q8S
   }
 }
 
-// One block of a row's own keys: positions below P are cache slots, those in [P, L) the ancestors' slots.
+// A row's ancestors: lane n of each wave that works for the row holds ancestor n's slot (-1: not attended) and V
+// exponent, LDS their V codes. The codes are loaded by NT threads in two steps -- begin issues the loads, end
+// writes them down -- so that the row's own K and V are on their way at the same time.
 template <int HD>
-struct alignas(16) Q8Anc {
-  int slot[QA_MAXD];            // -1: not attended
-  uint8_t v[QA_MAXD][HD];       // V codes
-  uint8_t x[2][QA_MAXD];        // exponents (K, V)
+struct alignas(16) Q8Codes {
+  uint8_t v[QA_MAXD][HD];
 };
 
-template <int HD>
+template <int HD, int NT>
+struct Q8Anc {
+  // a thread takes one dim (two with 64 threads for 128 dims) of every STEP-th ancestor; which is the wave's choice
+  static constexpr int STEP = NT >= HD ? NT / HD : 1, DIMS = NT >= HD ? 1 : HD / NT;
+  static constexpr int BATCH = QA_MAXD / STEP < 8 ? (QA_MAXD + STEP - 1) / STEP : 8;
+  int slot, D;
+  uint32_t xv;
+  uint32_t c[BATCH][DIMS];
+
+  __device__ __forceinline__ uint32_t code(const uint8_t* V, int n, int d) const {
+    const int sl = __builtin_amdgcn_readlane(slot, n);
+    return sl >= 0 ? V[q8_v_off(sl, d, HD)] : 0;  // uniform
+  }
+  __device__ __forceinline__ void begin(const AttnQ8Args& a, int raw, int n_anc, const uint8_t* V, const uint8_t* Vx, int tid) {
+    const int lane = tid & 63;
+    D = n_anc;
+    slot = lane < D && raw >= 0 && raw < a.max_len ? raw : -1;
+    if (D == 0) return;  // uniform
+    const uint32_t x = Vx[q8_x_off(max(slot, 0))];
+    xv = slot >= 0 ? x : 127;
+    const int n0 = NT >= HD ? __builtin_amdgcn_readfirstlane(tid / HD) : 0, d = tid % HD;
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i)
+      if (n0 + i * STEP < D) {  // uniform
+#pragma unroll
+        for (int e = 0; e < DIMS; ++e) c[i][e] = code(V, n0 + i * STEP, d + e * NT);
+      }
+  }
+  template <typename Sync>
+  __device__ __forceinline__ void end(const uint8_t* V, Q8Codes<HD>& lds, int tid, Sync sync) const {
+    if (D == 0) return;
+    const int n0 = NT >= HD ? __builtin_amdgcn_readfirstlane(tid / HD) : 0, d = tid % HD;
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i)
+      if (n0 + i * STEP < D) {
+#pragma unroll
+        for (int e = 0; e < DIMS; ++e) lds.v[n0 + i * STEP][d + e * NT] = (uint8_t)c[i][e];
+      }
+    for (int n = n0 + BATCH * STEP; n < D; n += STEP)
+#pragma unroll
+      for (int e = 0; e < DIMS; ++e) lds.v[n][d + e * NT] = (uint8_t)code(V, n, d + e * NT);
+    sync();
+  }
+};
+
+// One block of a row's own keys: positions below P are cache slots, those in [P, L) the ancestors' slots. ready()
+// makes the ancestors' codes readable; called once the block's loads are on their way.
+template <int HD, int NT, typename Ready>
 __device__ __forceinline__ uint32_t q8_load_own(Q8Frags<HD>& f, const uint8_t* K, const uint8_t* V, const uint8_t* Kx,
-                                                const uint8_t* Vx, int b, int P, int L, const Q8Anc<HD>& anc, int lane) {
+                                                const uint8_t* Vx, int b, int P, int L, const Q8Anc<HD, NT>& anc,
+                                                const Q8Codes<HD>& codes, int lane, Ready ready) {
   const int j = lane & 15, g = lane >> 4, key0 = b * QA_BLK;
   uint32_t valid = 0;
-  f.kx = *(const u32x4_t*)(Kx + key0 + (j >> 2) * 16);
+  // K and its exponents: one slot a lane. Loads are unconditional (a key that is not attended reads its own
+  // block's first slot, which exists; its score is masked).
+#pragma unroll
+  for (int kt = 0; kt < 4; ++kt) {
+    const int pos = key0 + 16 * kt + j, from = __shfl(anc.slot, (pos - P) & 31);
+    const int sl = pos < P ? pos : pos < L && from >= 0 ? from : key0;
+    f.kx[kt] = Kx[q8_x_off(sl)] * 0x01010101u;
+#pragma unroll
+    for (int p = 0; p < HD / 64; ++p) f.k[kt][p] = *(const u32x4_t*)(K + q8_k_off(sl, 64 * p + 16 * g, HD));
+  }
+  // V and its exponents: the block's own slots, positions from P on cleared, then the ancestors' put in
   f.vx = *(const u32x4_t*)(Vx + key0 + g * 16);
   const uint8_t* vb = V + (size_t)b * 64 * HD + lane * 16;
 #pragma unroll
   for (int dt = 0; dt < HD / 16; ++dt) f.v[dt] = *(const u32x4_t*)(vb + dt * 1024);
-  // K: one slot a lane. Loads are unconditional (a key that is not attended reads its own block's first
-  // slot, which exists; its score is masked).
-#pragma unroll
-  for (int kt = 0; kt < 4; ++kt) {
-    const int pos = key0 + 16 * kt + j;
-    const int sl = pos < P ? pos : pos < L ? anc.slot[pos - P] : -1;
-    if (pos >= P) f.kx[kt] = pos < L ? anc.x[0][pos - P] * 0x01010101u : 0x7f7f7f7fu;
-#pragma unroll
-    for (int p = 0; p < HD / 64; ++p) f.k[kt][p] = *(const u32x4_t*)(K + q8_k_off(sl >= 0 ? sl : key0, 64 * p + 16 * g, HD));
-  }
-  // V and its exponents: the block's own slots, positions from P on cleared, then the ancestors' put in
+  ready();
   u32x4_t own;
 #pragma unroll
   for (int kt = 0; kt < 4; ++kt) {
@@ -389,58 +437,25 @@ __device__ __forceinline__ uint32_t q8_load_own(Q8Frags<HD>& f, const uint8_t* K
   for (int an = a0; an < a1; ++an) {  // uniform
     const int off = P + an - key0, kt = off >> 4, e = off & 3;
     const bool mine = ((off >> 2) & 3) == g;
-    const uint32_t sel = mine ? 0xffu << (8 * e) : 0u, xv = anc.x[1][an] * 0x01010101u;
-    if (mine && anc.slot[an] >= 0) valid |= 1u << (4 * kt + e);
+    const uint32_t sel = mine ? 0xffu << (8 * e) : 0u, xv = __builtin_amdgcn_readlane(anc.xv, an) * 0x01010101u;
+    if (mine && __builtin_amdgcn_readlane(anc.slot, an) >= 0) valid |= 1u << (4 * kt + e);
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       const uint32_t m = c == kt ? sel : 0u;
       f.vx[c] = (f.vx[c] & ~m) | (xv & m);
 #pragma unroll
-      for (int dt = 0; dt < HD / 16; ++dt) f.v[dt][c] = (f.v[dt][c] & ~m) | ((anc.v[an][dt * 16 + j] * 0x01010101u) & m);
+      for (int dt = 0; dt < HD / 16; ++dt) f.v[dt][c] = (f.v[dt][c] & ~m) | ((codes.v[an][dt * 16 + j] * 0x01010101u) & m);
     }
   }
   return valid;
 }
 
-// The row's D ancestors, staged by NT threads (tid < NT); sync makes their LDS writes visible to each other.
-template <int HD, int NT, typename Sync>
-__device__ __forceinline__ void q8_stage_anc(const AttnQ8Args& a, int row, int D, const uint8_t* V, const uint8_t* Kx,
-                                             const uint8_t* Vx, Q8Anc<HD>& anc, int tid, Sync sync) {
-  if (D == 0) return;  // uniform
-  if (tid < QA_MAXD) {
-    const int sl = tid < D ? a.anc[(size_t)row * QA_MAXD + tid] : -1;
-    const bool ok = sl >= 0 && sl < a.max_len;
-    anc.slot[tid] = ok ? sl : -1;
-    anc.x[0][tid] = ok ? Kx[q8_x_off(sl)] : 127;
-    anc.x[1][tid] = ok ? Vx[q8_x_off(sl)] : 127;
-  }
-  sync();
-  // a thread takes the same dim of every NT / HD-th ancestor, sixteen loads in flight
-  constexpr int STEP = NT >= HD ? NT / HD : 1, DIMS = NT >= HD ? 1 : HD / NT, BATCH = 16 / DIMS;
-  const int d = tid % HD;
-  for (int n0 = NT >= HD ? tid / HD : 0; n0 < D; n0 += STEP * BATCH) {
-    uint8_t c[BATCH][DIMS];
-#pragma unroll
-    for (int i = 0; i < BATCH; ++i) {
-      const int sl = anc.slot[min(n0 + i * STEP, D - 1)];
-#pragma unroll
-      for (int e = 0; e < DIMS; ++e) c[i][e] = V[q8_v_off(sl >= 0 ? sl : 0, d + e * NT, HD)];
-    }
-#pragma unroll
-    for (int i = 0; i < BATCH; ++i)
-      if (n0 + i * STEP < D) {
-#pragma unroll
-        for (int e = 0; e < DIMS; ++e) anc.v[n0 + i * STEP][d + e * NT] = anc.slot[n0 + i * STEP] >= 0 ? c[i][e] : 0;
-      }
-  }
-  sync();
-}
-
 // A span of keys (positions below P cache slots, those in [P, L) ancestors) for the query at q on each lane j; false:
 // no keys.
-template <int HD>
+template <int HD, int NT, typename Ready>
 __device__ __forceinline__ bool q8_own_span(const AttnQ8Args& a, size_t reg, const bf16_t* q, int span, int P, int L,
-                                            const Q8Anc<HD>& anc, int lane, Q8State<HD> (&st)[1]) {
+                                            const Q8Anc<HD, NT>& anc, const Q8Codes<HD>& codes, int lane, Q8State<HD> (&st)[1],
+                                            Ready ready) {
   const int b0 = span * a.span_blk, b1 = min((L + QA_BLK - 1) / QA_BLK, b0 + a.span_blk), j = lane & 15;
   if (b0 >= b1) return false;
   const uint8_t *K = a.K + reg * HD, *V = a.V + reg * HD, *Kx = a.Kx + reg, *Vx = a.Vx + reg;
@@ -457,7 +472,7 @@ __device__ __forceinline__ bool q8_own_span(const AttnQ8Args& a, size_t reg, con
       q8_load_k<HD>(f, K, Kx, b, lane);
       q8_load_v<HD>(f, V, Vx, b, lane);
     } else {
-      valid = q8_load_own<HD>(f, K, V, Kx, Vx, b, P, L, anc, lane);
+      valid = q8_load_own<HD>(f, K, V, Kx, Vx, b, P, L, anc, codes, lane, ready);
     }
     q8_fold<HD, 1, true, false>(f, qf, valid, a.scale_log2, j, st, [] {}, [] {});
   }
@@ -474,7 +489,7 @@ __device__ __forceinline__ void q8_row_keys(const AttnQ8Args& a, int row, int& P
 // all rows attend whole are folded for the tile (span s by wave 3 - s: with one row wave 0 is free for it), the
 // spans after by each row's wave; together they make the rows' records of the group.
 template <int HD>
-__device__ __forceinline__ void q8_own_groups(const AttnQ8Args& a, int id, Q8Spans<HD>& lds, Q8Anc<HD>& anc) {
+__device__ __forceinline__ void q8_own_groups(const AttnQ8Args& a, int id, Q8Spans<HD>& lds, Q8Codes<HD>& codes) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, j = lane & 15, g = lane >> 4;
   const int unit = id % a.own_units, kvh = unit % a.kv, seq = unit / a.kv;
   if (seq >= a.n_seq) return;  // units are rounded up to 8: a unit's rows and its shared groups meet on one XCD
@@ -484,16 +499,23 @@ __device__ __forceinline__ void q8_own_groups(const AttnQ8Args& a, int id, Q8Spa
   if (n_rows <= 0) return;
   const int cut = q8_shared_blocks(a, r0, r1, lane) / a.span_blk, per = QA_GRP * a.span_blk * QA_BLK;
   const size_t reg = ((size_t)seq * a.kv + kvh) * a.max_len;
+  const int raw = a.anc[(size_t)(base + min(w, n_rows - 1)) * QA_MAXD + (lane & (QA_MAXD - 1))];
   int p_of, l_of;  // of row base + lane (past the last: the last's)
   q8_row_keys(a, base + min(lane, n_rows - 1), p_of, l_of);
   const int n_grp = (-wave_min(-l_of) + per - 1) / per;
   const int P = __builtin_amdgcn_readlane(p_of, w), L = __builtin_amdgcn_readlane(l_of, w);
   if (cut / QA_GRP >= n_grp) return;
-  if (w < n_rows)
-    q8_stage_anc<HD, 64>(a, base + w, L - P, a.V + reg * HD, a.Kx + reg, a.Vx + reg, anc, lane, [] {
+  Q8Anc<HD, 64> anc;
+  anc.begin(a, raw, w < n_rows ? L - P : 0, a.V + reg * HD, a.Vx + reg, lane);
+  bool staged = false;
+  auto ready = [&] {
+    if (staged) return;  // uniform
+    staged = true;
+    anc.end(a.V + reg * HD, codes, lane, [] {
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");  // one wave's LDS accesses are in order: keep the compiler's so
       __builtin_amdgcn_wave_barrier();
     });
+  };
   for (int grp = cut / QA_GRP; grp < n_grp; ++grp)
     for (int t0 = 0; t0 < a.rep; t0 += 16) {  // more than one turn only with one row
       const int nh = min(16, a.rep - t0), h0 = kvh * a.rep + t0;
@@ -506,7 +528,7 @@ __device__ __forceinline__ void q8_own_groups(const AttnQ8Args& a, int id, Q8Spa
         const int keys = all ? (span + 1) * a.span_blk * QA_BLK : 0;
         Q8State<HD> st[1];
         const bool have = q8_own_span<HD>(a, reg, a.Q + (size_t)(base + r) * a.ldq + (size_t)h * HD, span, all ? keys : P,
-                                          all ? keys : L, anc, lane, st);
+                                          all ? keys : L, anc, codes, lane, st, ready);
         q8_publish<HD>(lds, s, all ? 0 : w * nh, all ? 16 : nh, j, g, have, st[0]);
       }
       __syncthreads();
@@ -523,7 +545,7 @@ union alignas(16) Q8FoldLds {
   Q8Spans<HD> shared[T];
   struct {
     Q8Spans<HD> spans;
-    Q8Anc<HD> anc[4];
+    Q8Codes<HD> codes[4];
   } own;
 };
 
@@ -531,7 +553,7 @@ union alignas(16) Q8FoldLds {
 template <int HD, int T>
 __global__ __launch_bounds__(256, 2) void q8_fold_kernel(AttnQ8Args a, int own) {
   __shared__ Q8FoldLds<HD, T> lds;
-  if ((int)blockIdx.x < own) q8_own_groups<HD>(a, blockIdx.x, lds.own.spans, lds.own.anc[threadIdx.x >> 6]);
+  if ((int)blockIdx.x < own) q8_own_groups<HD>(a, blockIdx.x, lds.own.spans, lds.own.codes[threadIdx.x >> 6]);
   else q8_shared_group<HD, T>(a, blockIdx.x - own, lds.shared);
 }
 
@@ -606,7 +628,7 @@ __global__ __launch_bounds__(256) void q8_combine_kernel(AttnQ8Args a) {
 template <int HD, int TEAMS>
 struct alignas(16) Q8ShortLds {
   Q8Spans<HD> spans[TEAMS];
-  Q8Anc<HD> anc;
+  Q8Codes<HD> codes;
 };
 
 template <int HD, int TEAMS>
@@ -619,14 +641,17 @@ __global__ __launch_bounds__(256 * TEAMS) void q8_short_kernel(AttnQ8Args a, int
   q8_rows(a, seq, r0, r1);
   const int row = r0 + blockIdx.x / a.kv % rows_max;
   if (row >= r1) return;
+  const int raw = a.anc[(size_t)row * QA_MAXD + (lane & (QA_MAXD - 1))];
   q8_row_keys(a, row, P, L);
   const size_t reg = ((size_t)seq * a.kv + kvh) * a.max_len;
-  q8_stage_anc<HD, 256 * TEAMS>(a, row, L - P, a.V + reg * HD, a.Kx + reg, a.Vx + reg, lds.anc, threadIdx.x, [] { __syncthreads(); });
+  Q8Anc<HD, 256 * TEAMS> anc;
+  anc.begin(a, raw, L - P, a.V + reg * HD, a.Vx + reg, threadIdx.x);
+  anc.end(a.V + reg * HD, lds.codes, threadIdx.x, [] { __syncthreads(); });
   for (int t0 = 0; t0 < a.rep; t0 += 16) {
     const int nh = min(16, a.rep - t0), h0 = kvh * a.rep + t0;
     Q8State<HD> st[1];
     const bool have = q8_own_span<HD>(a, reg, a.Q + (size_t)row * a.ldq + (size_t)(h0 + min(j, nh - 1)) * HD, team * QA_GRP + w, P,
-                                      L, lds.anc, lane, st);
+                                      L, anc, lds.codes, lane, st, [] {});
     if (t0) __syncthreads();  // the heads before have been written out
     q8_publish<HD>(lds.spans[team], w, 0, 16, j, g, have, st[0]);
     __syncthreads();
