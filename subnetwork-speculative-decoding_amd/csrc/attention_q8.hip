@@ -705,7 +705,10 @@ static int launch_attn_q8(AttnQ8Args a, int rows_max, hipStream_t stream) {
   a.sets = single ? 1 : (tiles + 1) / 2;
   a.tiles_per_set = single ? 1 : (tiles + a.sets - 1) / a.sets;
   const int64_t units = (int64_t)a.n_seq * a.n_grps * a.kv, shared = (units + 7) / 8 * 8 * a.sets;
-  a.own_rows = std::min(4, std::max(1, 16 / a.rep));
+  // A row a workgroup while all of those are resident at once, each on a CU of its own; then as many rows as fill a
+  // tile, since the spans they attend together are folded once. us, one / four rows: 25 rows of one sequence, prefixes
+  // 4097, 4060, 4000, 3900: 14.1 / 14.3, 14.9 / 16.4, 14.3 / 15.5, 14.1 / 15.4; 12 trees of up to 9 rows 30.4 / 26.2.
+  a.own_rows = rows <= 256 ? 1 : std::min(4, std::max(1, 16 / a.rep));
   const int64_t own_units = ((int64_t)a.n_seq * a.kv + 7) / 8 * 8, own = own_units * ((rows_max + a.own_rows - 1) / a.own_rows);
   if (shared + own > INT32_MAX || (int64_t)a.M * a.heads > INT32_MAX)
     return set_error(SSD_ERANGE, "attention_q8: too many workgroups");
