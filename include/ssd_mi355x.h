@@ -197,7 +197,7 @@ int ssd_tree_attention_bf16(const uint16_t* q, int64_t ldq, int M, int heads, in
  * keeps the row's largest finite magnitude within 448 (b >= 27), so a row rounds once, to four
  * significant bits, and its stored values are bf16 values. Values that are not finite are stored as NaN.
  * k, v: [n_seq][kv_heads] regions of max_len * head_dim bytes; k_exp, v_exp: regions of max_len bytes;
- * max_len a multiple of 64, head_dim 64 or 128, all arrays 16-byte aligned. A region is a sequence of
+ * max_len a multiple of 64 up to 2^30, head_dim 64 or 128, all arrays 16-byte aligned. A region is a sequence of
  * 64-slot blocks in the attention's operand order, offsets of slot s (within the region):
  *   K[s][d]: ((s/16)*(hd/64) + d/64)*1024 + (((d/16)%4)*16 + s%16)*16 + d%16;
  *   V[s][d]: ((s/64)*(hd/16) + d/16)*1024 + (((s/4)%4)*16 + d%16)*16 + ((s/32)%2)*8 + ((s/16)%2)*4 + s%4;
@@ -258,7 +258,7 @@ int ssd_kv_q8_compact(const SsdKvQ8* cache, int layers, const int32_t* start, co
  * span of `span` logical positions, a multiple of 64; four spans a group; the groups), so a row's result depends on
  * its query, its keys and span alone -- not on the other rows, the other sequences or the slots its ancestors
  * sit in: a verify row equals the autoregressive step at its position bit for bit.
- * heads / kv_heads any whole ratio; scale > 0. ws: ssd_attn_q8_ws_floats(...) floats, 16-byte aligned, no clearing needed; calls
+ * heads / kv_heads any whole ratio; scale > 0; V rows beyond 2^100 may overflow their sums. ws: ssd_attn_q8_ws_floats(...) floats, 16-byte aligned, no clearing needed; calls
  * that overlap in time must not share it. */
 int64_t ssd_attn_q8_ws_floats(int M, int heads, int head_dim, int64_t l_max, int span);
 int ssd_tree_attention_q8(const SsdKvQ8* cache, const uint16_t* q, int64_t ldq, int M, int heads, const int32_t* row_begin,

@@ -710,7 +710,7 @@ static int launch_attn_q8(AttnQ8Args a, int rows_max, hipStream_t stream) {
   // 4097, 4060, 4000, 3900: 14.1 / 14.3, 14.9 / 16.4, 14.3 / 15.5, 14.1 / 15.4; 12 trees of up to 9 rows 30.4 / 26.2.
   a.own_rows = rows <= 256 ? 1 : std::min(4, std::max(1, 16 / a.rep));
   const int64_t own_units = ((int64_t)a.n_seq * a.kv + 7) / 8 * 8, own = own_units * ((rows_max + a.own_rows - 1) / a.own_rows);
-  if (shared + own > INT32_MAX || (int64_t)a.M * a.heads > INT32_MAX)
+  if (grid_too_large(shared + own, 256) || grid_too_large(rows, 256) || grid_too_large((int64_t)a.M * a.heads, 256))
     return set_error(SSD_ERANGE, "attention_q8: too many workgroups");
   a.units = (int)units, a.own_units = (int)own_units;
   auto one_launch = [&](auto t) {

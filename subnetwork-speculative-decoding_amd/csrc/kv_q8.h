@@ -29,6 +29,9 @@ __device__ __forceinline__ int q8_x_off(int s) {
   return (s & ~63) + (((s >> 2) & 3) << 4) + (((s >> 4) & 3) << 2) + (s & 3);
 }
 
+// A launch holds at most 2^32 - 1 threads.
+__host__ inline bool grid_too_large(int64_t workgroups, int threads) { return workgroups * threads > (int64_t)UINT32_MAX; }
+
 constexpr int Q8_MIN_EXP = 27;  // exponent byte of 2^-100: codes, scales and their products stay normal numbers
 
 // Exponent byte for a row whose largest finite magnitude is amax: 448 = 0.875 * 2^9, so with amax = f * 2^n,

@@ -212,7 +212,7 @@ SSD_API int ssd_verify_chain(const float* P, int64_t ldp_seq, int64_t ldp, const
   if ((uintptr_t)ws & 15) return set_error(SSD_EINVAL, "verify_chain: workspace must be 16-byte aligned");
   if (ws_bytes < ssd_verify_chain_ws_bytes(n_seq, V)) return set_error(SSD_EINVAL, "verify_chain: workspace too small");
   const int chunks = chain_chunks(V);
-  if ((int64_t)n_seq * chunks > INT32_MAX) return set_error(SSD_ERANGE, "verify_chain: too many sequences");
+  if ((int64_t)n_seq * chunks * 256 > (int64_t)UINT32_MAX) return set_error(SSD_ERANGE, "verify_chain: too many sequences");
   if (n_seq == 0) return SSD_OK;
   const ChainArgs a{P, Q, ldp_seq, ldp, ldq_seq, ldq, V, k_max, chunks, chain_pieces(V), draft, n_draft, u, u_next, (double2*)ws,
                     out_tok, out_n};

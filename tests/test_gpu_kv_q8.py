@@ -368,6 +368,32 @@ def test_verify_rows_equal_autoregressive_steps_bit_for_bit(hd, heads, kv, span)
             assert torch.equal(one[0], tree[t]), (n, t, len(path))
 
 
+@pytest.mark.parametrize("hd,heads,kv,span", [(128, 32, 8, 64), (64, 24, 8, 128), (128, 40, 8, 64), (64, 16, 16, 192)])
+def test_a_batch_equals_each_sequence_alone_bit_for_bit(hd, heads, kv, span):
+    """Many rows (several of a sequence in one workgroup) against calls of one sequence and of one row: no bit differs."""
+    S = 14
+    cache = _cache(1, 900, kv, hd, S, span)
+    slots = torch.arange(900, dtype=torch.int32, device=DEV)
+    for s in range(S):
+        k, v = (torch.randn(900, kv * hd, generator=_gen(s * 2 + i)).to(BF16).to(DEV) for i in range(2))
+        cache.write(0, k, v, torch.full_like(slots, s), slots)
+    g = _gen(hd + heads)
+    rows = [_tree(60 * s + 3, 60 * s + 5, 1 + (5 * s) % 11, g) for s in range(S)]
+    rows[4] = [(p - 40 * (i % 2), a) for i, (p, a) in enumerate(rows[4])]  # a sequence of two prefixes
+    tab, begin, prefix, depth, anc = _table(rows)
+    q = torch.randn(begin[-1], heads * hd, generator=g).to(BF16).to(DEV)
+    top = max(p + d for p, d in zip(prefix, depth))
+    batch = cache.attend(0, q, *tab, 11, top)
+    for s in range(S):
+        only, *_ = _table([r if i == s else [] for i, r in enumerate(rows)])
+        a, b = begin[s], begin[s + 1]
+        l_max = max(p + d for p, d in zip(prefix[a:b], depth[a:b]))
+        assert torch.equal(cache.attend(0, q[a:b], *only, b - a, l_max), batch[a:b]), s
+        t = a + (b - a) // 2
+        one, *_ = _table([[rows[s][t - a]] if i == s else [] for i in range(S)])
+        assert torch.equal(cache.attend(0, q[t:t + 1], *one, 1, prefix[t] + depth[t])[0], batch[t]), (s, t)
+
+
 def test_attend_long_and_past_32_bits():
     """Regions past 4 GiB of codes, and a long context of many spans."""
     kv, hd, heads, cap = 8, 128, 8, 1 << 19

@@ -141,7 +141,7 @@ def _refused(name, args, code, text):
 
 BAD_CACHES = [(dict(k=None), "null"), (dict(v_exp=None), "null"), (dict(head_dim=96), "head_dim"), (dict(head_dim=32), "head_dim"),
               (dict(n_seq=0), "sequences"), (dict(kv_heads=0), "kv heads"), (dict(max_len=100), "max_len"), (dict(max_len=0), "max_len"),
-              (dict(max_len=2 ** 31), "max_len"), (dict(v=A + 8), "aligned")]
+              (dict(max_len=2 ** 30 + 64), "max_len"), (dict(v=A + 8), "aligned")]
 
 
 def _write(cache=None, **kw):
@@ -158,6 +158,19 @@ def test_bad_caches_are_refused(kw, text):
     _refused("ssd_kv_q8_read_bf16", [C.byref(c), 1, A, A, A, 256, A, 256, None], BAD, text)
     _refused("ssd_kv_q8_compact", [C.byref(c), 1, A, A, A, 4, None], BAD, text)
     _refused("ssd_tree_attention_q8", [C.byref(c), A, 256, 1, 2, A, A, A, A, 1, 64, 64, 1.0, A, 1 << 20, A, 256, None], BAD, text)
+
+
+def test_launches_beyond_the_grid_are_refused():
+    c = _cache(n_seq=1 << 22, kv_heads=8)
+    _refused("ssd_kv_q8_compact", [C.byref(c), 1, A, A, A, 4, None], RANGE, "too large")
+    _refused("ssd_kv_q8_write_bf16", _write(_cache(kv_heads=1024), k=A, ldk=1 << 17, ldv=1 << 17, M=1 << 20), RANGE, "too many rows")
+    c = _cache(kv_heads=1024)
+    _refused("ssd_kv_q8_read_bf16", [C.byref(c), 1 << 20, A, A, A, 1 << 17, A, 1 << 17, None], RANGE, "too many rows")
+    args = [C.byref(_cache(n_seq=1 << 20, kv_heads=1)), A, 1024, 1 << 24, 8, A, A, A, A, 64, 128, 64, 1.0, A, 1 << 40, A, 1024, None]
+    _refused("ssd_tree_attention_q8", args, RANGE, "workgroups")
+    _refused("ssd_kv_q8_compact", [C.byref(_cache(n_seq=1 << 20, kv_heads=1 << 12)), 1, A, A, A, 4, None], RANGE, "sequences")
+    args = [A, 1 << 20, 1 << 19, A, 1 << 20, 1 << 19, 1 << 19, 1 << 20, 1, A, None, A, A, A, 1 << 40, A, A, None]
+    _refused("ssd_verify_chain", args, RANGE, "sequences")
 
 
 def test_null_cache_is_refused():
