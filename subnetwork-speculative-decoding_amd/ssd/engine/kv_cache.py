@@ -149,14 +149,12 @@ class KVCacheQ8:
 
     @staticmethod
     def default_span(capacity: int) -> int:
-        """About 24 spans a full cache, 64 to 1024 keys each: a span is one wave's work in turn, four spans leave one
-        record. us at spans of 64 / 128 / 256 / 512 / 1024 keys: 25 rows, 32 heads, 4096 keys 18.9 / 14.6 / 15.8 / 18.7 /
-        25.9; 25 rows, 64 heads, 16384 keys 60.7 / 43.1 / 36.0 / 33.3 / 33.8; one row of 131000 keys 64.9 / 57.7 / 48.7 /
-        46.5 / 45.8; 32 rows of as many sequences at 8192 keys 88 / 82 / 82 / 81 / 84 (8 kv heads of 128)."""
-        span = 64
-        while span < 1024 and capacity >= 24 * span * 1.5:
-            span *= 2
-        return span
+        """Keys of a span (one wave's work in turn; four spans leave one record): short ones for latency, long ones for
+        fewer records. us at 64 / 128 / 256 / 512 / 1024 keys, 32 heads on 8 kv heads of 128, one row: 4096 keys 9.3 / 9.0 /
+        10.0 / 14.0 / 19.9, 8100 9.4 / 9.4 / 11.2 / 15.1 / 30.6, 16384 13.9 / 11.6 / 12.2 / 16.3 / 25.8, 33000 24.3 / 23.3 / 20.4 / 19.4 /
+        27.0; 25 rows: 18.8 / 14.8 / 15.8 / 18.7 / 22.2, 24.6 / 21.3 / 18.9 / 25.3 / 33.6, 38.7 / 30.4 / 26.3 / 23.4 / 32.1, 64.9 / 47.4 /
+        40.5 / 36.8 / 36.2."""
+        return 128 if capacity < 6144 else 256 if capacity < 16384 else 512
 
     def layer(self, i: int) -> _lib.SsdKvQ8:
         """The descriptor of layer ``i`` for the ops that take a cache."""
