@@ -487,8 +487,9 @@ __device__ __forceinline__ void q8_row_keys(const AttnQ8Args& a, int row, int& P
 // The groups that rows of a sequence do not attend whole together: from the one the smallest prefix ends in to each
 // row's last. One workgroup per (sequence, kv head, up to four rows that fill a tile: 16 / rep); wave w has row w. Spans
 // all rows attend whole are folded for the tile (span s by wave 3 - s: with one row wave 0 is free for it), the
-// spans after by each row's wave; together they make the rows' records of the group.
-template <int HD>
+// spans after by each row's wave; together they make the rows' records of the group. DIRECT: all keys lie in the first
+// group, and its sums are the rows' outputs.
+template <int HD, bool DIRECT>
 __device__ __forceinline__ void q8_own_groups(const AttnQ8Args& a, int id, Q8Spans<HD>& lds, Q8Codes<HD>& codes) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, j = lane & 15, g = lane >> 4;
   const int unit = id % a.own_units, kvh = unit % a.kv, seq = unit / a.kv;
@@ -502,9 +503,9 @@ __device__ __forceinline__ void q8_own_groups(const AttnQ8Args& a, int id, Q8Spa
   const int raw = a.anc[(size_t)(base + min(w, n_rows - 1)) * QA_MAXD + (lane & (QA_MAXD - 1))];
   int p_of, l_of;  // of row base + lane (past the last: the last's)
   q8_row_keys(a, base + min(lane, n_rows - 1), p_of, l_of);
-  const int n_grp = (-wave_min(-l_of) + per - 1) / per;
+  const int n_grp = DIRECT ? 1 : (-wave_min(-l_of) + per - 1) / per;
   const int P = __builtin_amdgcn_readlane(p_of, w), L = __builtin_amdgcn_readlane(l_of, w);
-  if (cut / QA_GRP >= n_grp) return;
+  if (!DIRECT && cut / QA_GRP >= n_grp) return;
   Q8Anc<HD, 64> anc;
   anc.begin(a, raw, w < n_rows ? L - P : 0, a.V + reg * HD, a.Vx + reg, lane);
   bool staged = false;
@@ -516,7 +517,7 @@ __device__ __forceinline__ void q8_own_groups(const AttnQ8Args& a, int id, Q8Spa
       __builtin_amdgcn_wave_barrier();
     });
   };
-  for (int grp = cut / QA_GRP; grp < n_grp; ++grp)
+  for (int grp = DIRECT ? 0 : cut / QA_GRP; grp < n_grp; ++grp)
     for (int t0 = 0; t0 < a.rep; t0 += 16) {  // more than one turn only with one row
       const int nh = min(16, a.rep - t0), h0 = kvh * a.rep + t0;
       __syncthreads();  // the tile before has been merged
@@ -534,10 +535,31 @@ __device__ __forceinline__ void q8_own_groups(const AttnQ8Args& a, int id, Q8Spa
       __syncthreads();
       const int rr = threadIdx.x >> 4, dc = threadIdx.x & 15;
       if (rr < n_rows * nh) {
-        if (grp * per < __shfl(l_of, rr / nh))
-          q8_store_record<HD>(a, ((size_t)(base + rr / nh) * a.heads + h0 + rr % nh) * a.n_grps + grp, dc, q8_merge<HD>(lds, rr, dc));
+        const int row = base + rr / nh, h = h0 + rr % nh;
+        if constexpr (DIRECT) {
+          const Q8Record<HD> r = q8_merge<HD>(lds, rr, dc);
+          const float wgt = q8_weight(r.m, r.m), l = r.l * wgt;  // the sum over one group, as the other kernels form it
+#pragma unroll
+          for (int i = 0; i < HD / 64; ++i) {
+            float y[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = l == 0.f ? 0.f : fmaf(r.o[i][e], wgt, 0.f) / l;
+            *(uint2*)(a.out + (size_t)row * a.ldo + (size_t)h * HD + i * 64 + dc * 4) =
+                make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
+          }
+        } else if (grp * per < __shfl(l_of, rr / nh)) {
+          q8_store_record<HD>(a, ((size_t)row * a.heads + h) * a.n_grps + grp, dc, q8_merge<HD>(lds, rr, dc));
+        }
       }
     }
+}
+
+// Contexts of one group, rows of a sequence that fill a tile a workgroup.
+template <int HD>
+__global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void q8_short_rows_kernel(AttnQ8Args a) {
+  __shared__ Q8Spans<HD> spans;
+  __shared__ Q8Codes<HD> codes[4];
+  q8_own_groups<HD, true>(a, blockIdx.x, spans, codes[threadIdx.x >> 6]);
 }
 
 template <int HD, int T>
@@ -553,7 +575,7 @@ union alignas(16) Q8FoldLds {
 template <int HD, int T>
 __global__ __launch_bounds__(256, 2) void q8_fold_kernel(AttnQ8Args a, int own) {
   __shared__ Q8FoldLds<HD, T> lds;
-  if ((int)blockIdx.x < own) q8_own_groups<HD>(a, blockIdx.x, lds.own.spans, lds.own.codes[threadIdx.x >> 6]);
+  if ((int)blockIdx.x < own) q8_own_groups<HD, false>(a, blockIdx.x, lds.own.spans, lds.own.codes[threadIdx.x >> 6]);
   else q8_shared_group<HD, T>(a, blockIdx.x - own, lds.shared);
 }
 
@@ -631,8 +653,11 @@ struct alignas(16) Q8ShortLds {
   Q8Codes<HD> codes;
 };
 
+// Heads of 64 with one team: 128 VGPRs and four workgroups a CU, 20 x 9 rows at 200 keys 13.7 -> 10.3 us, 40 x 8 at 400
+// 27 -> 19.6. Heads of 128 spill below 168 and are slower so.
 template <int HD, int TEAMS>
-__global__ __launch_bounds__(256 * TEAMS) void q8_short_kernel(AttnQ8Args a, int rows_max) {
+__global__ __launch_bounds__(256 * TEAMS, TEAMS == 4 || (TEAMS == 1 && HD == 64) ? 4 : 2) void q8_short_kernel(AttnQ8Args a,
+                                                                                                         int rows_max) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6 & 3, team = threadIdx.x >> 8, j = lane & 15, g = lane >> 4;
   const int kvh = blockIdx.x % a.kv, seq = blockIdx.x / a.kv / rows_max;
   __shared__ Q8ShortLds<HD, TEAMS> lds;
@@ -717,6 +742,14 @@ static int launch_attn_q8(AttnQ8Args a, int rows_max, hipStream_t stream) {
     SSD_LAUNCH((q8_short_kernel<HD, decltype(t)::value>), dim3((unsigned)rows), dim3(256 * decltype(t)::value), 0, stream, a, rows_max);
     return check_launch("attn_q8_short");
   };
+  // One group: four rows a workgroup once a row each would be more than are resident at once. us at 8 kv heads, a row /
+  // four: heads of 128, 6 x 9 rows at 98 keys 6.6 / 10.2, 40 x 2 at 60 8.6 / 8.0, 13 x 9 at 98 11.4 / 11.4, 20 x 8 at 60
+  // 14.7 / 10.4, 40 x 8 at 60 24.7 / 15.4, 12 x 25 at 450 27.4 / 20.1; heads of 64, 20 x 9 at 200 10.4 / 9.5, 40 x 25 at 200
+  // 33.6 / 24.2. With two rows (rep 8), 20 x 9 at 100, it is 16.7 / 18.0.
+  if (a.n_grps == 1 && rows > 512 && a.own_rows == 4 && rows_max > 1) {
+    SSD_LAUNCH((q8_short_rows_kernel<HD>), dim3((unsigned)own), dim3(256), 0, stream, a);
+    return check_launch("attn_q8_short_rows");
+  }
   if (a.n_grps == 1) return one_launch(integral_constant<int, 1>());
   if (a.n_grps == 2 && rows <= 512) return one_launch(integral_constant<int, 2>());
   if constexpr (HD == 64)

@@ -153,8 +153,8 @@ class KVCacheQ8:
         fewer records. us at 64 / 128 / 256 / 512 / 1024 keys, 32 heads on 8 kv heads of 128, one row: 4096 keys 9.3 / 9.0 /
         10.0 / 14.0 / 19.9, 8100 9.4 / 9.4 / 11.2 / 15.1 / 30.6, 16384 13.9 / 11.6 / 12.2 / 16.3 / 25.8, 33000 24.3 / 23.3 / 20.4 / 19.4 /
         27.0; 25 rows: 18.8 / 14.8 / 15.8 / 18.7 / 22.2, 24.6 / 21.3 / 18.9 / 25.3 / 33.6, 38.7 / 30.4 / 26.3 / 23.4 / 32.1, 64.9 / 47.4 /
-        40.5 / 36.8 / 36.2."""
-        return 128 if capacity < 6144 else 256 if capacity < 16384 else 512
+        40.5 / 36.8 / 36.2. Caches that end with a few blocks: 13 trees of 9 rows at 98 keys 11.7 / 14.0 at 64 / 128."""
+        return 64 if capacity <= 256 else 128 if capacity < 6144 else 256 if capacity < 16384 else 512
 
     def layer(self, i: int) -> _lib.SsdKvQ8:
         """The descriptor of layer ``i`` for the ops that take a cache."""

@@ -394,6 +394,24 @@ def test_a_batch_equals_each_sequence_alone_bit_for_bit(hd, heads, kv, span):
         assert torch.equal(cache.attend(0, q[t:t + 1], *one, 1, prefix[t] + depth[t])[0], batch[t]), (s, t)
 
 
+@pytest.mark.parametrize("hd,heads,kv,span", [(128, 32, 8, 64), (64, 24, 8, 64), (64, 12, 12, 128), (128, 40, 8, 64)])
+def test_many_short_trees(hd, heads, kv, span):
+    """More rows than are resident one a workgroup, all of few keys: the definition, and every row as it is alone."""
+    S = 22
+    cache = _cache(1, 256, kv, hd, S, span)
+    vals = _fill(cache, hd)
+    g = _gen(heads)
+    rows = [_tree(9 * s + 1, 9 * s + 3, 1 + s % 7, g) for s in range(S)]
+    rows[3], rows[8], rows[9] = [], [(0, [])] * 5, [(0, []), (77, [200, 201]), (0, [255]), (128, []), (63, [1, 0])]
+    batch = _check_attend(cache, rows, heads, kv, vals, extra=2, ld_pad=8).view(-1, heads * hd)
+    tab, begin, prefix, depth, anc = _table(rows)
+    q = torch.randn(begin[-1] + 2, heads * hd + 8, generator=_gen(kv)).to(BF16).to(DEV)[:begin[-1], :heads * hd]
+    for s in range(S):
+        for t in range(begin[s], begin[s + 1], 2):
+            one, *_ = _table([[rows[s][t - begin[s]]] if i == s else [] for i in range(S)])
+            assert torch.equal(cache.attend(0, q[t:t + 1], *one, 1, max(prefix[t] + depth[t], 1)).cpu()[0], batch[t]), (s, t)
+
+
 def test_attend_long_and_past_32_bits():
     """Regions past 4 GiB of codes, and a long context of many spans."""
     kv, hd, heads, cap = 8, 128, 8, 1 << 19
