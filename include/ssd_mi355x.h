@@ -195,7 +195,8 @@ int ssd_tree_attention_bf16(const uint16_t* q, int64_t ldq, int M, int heads, in
  * One layer of a batch of sequences' caches. Every row (sequence, slot, kv head) of K and of V is
  * head_dim e4m3 codes and one exponent byte b: value = code * 2^(b - 127), the least power of two that
  * keeps the row's largest finite magnitude within 448 (b >= 27), so a row rounds once, to four
- * significant bits, and its stored values are bf16 values. Values that are not finite are stored as NaN.
+ * significant bits, and its stored values are bf16 values (those from 1.9375 * 2^127 on round to infinity). Values that
+ * are not finite are stored as NaN.
  * k, v: [n_seq][kv_heads] regions of max_len * head_dim bytes; k_exp, v_exp: regions of max_len bytes;
  * max_len a multiple of 64 up to 2^30, head_dim 64 or 128, all arrays 16-byte aligned. A region is a sequence of
  * 64-slot blocks in the attention's operand order, offsets of slot s (within the region):
@@ -258,8 +259,8 @@ int ssd_kv_q8_compact(const SsdKvQ8* cache, int layers, const int32_t* start, co
  * span of `span` logical positions, a multiple of 64; four spans a group; the groups), so a row's result depends on
  * its query, its keys and span alone -- not on the other rows, the other sequences or the slots its ancestors
  * sit in: a verify row equals the autoregressive step at its position bit for bit.
- * heads / kv_heads any whole ratio; scale > 0; V rows beyond 2^100 may overflow their sums. ws: ssd_attn_q8_ws_floats(...) floats, 16-byte aligned, no clearing needed; calls
- * that overlap in time must not share it. */
+ * heads / kv_heads any whole ratio; scale > 0; V rows beyond 2^100 may overflow their sums. ws:
+ * ssd_attn_q8_ws_floats(...) floats, 16-byte aligned, no clearing needed; calls that overlap in time must not share it. */
 int64_t ssd_attn_q8_ws_floats(int M, int heads, int head_dim, int64_t l_max, int span);
 int ssd_tree_attention_q8(const SsdKvQ8* cache, const uint16_t* q, int64_t ldq, int M, int heads, const int32_t* row_begin,
                           const int32_t* prefix, const int32_t* depth, const int32_t* anc, int rows_max, int l_max,

@@ -3,7 +3,8 @@
 // A row (slot, kv head) of K or V is hd e4m3 codes and one exponent byte b: value = code * 2^(b - 127), with
 // the least power of two that keeps the row's largest magnitude at or below 448 (b >= 27). A power of two
 // costs a float code at most one of its 16 binades and makes every step exact: x * 2^-e before the one
-// rounding to four significant bits, and code * 2^e, which is a bf16 value, after it.
+// rounding to four significant bits, and code * 2^e, which is a bf16 value, after it (infinity where the row's
+// largest rounds to 2^128, from 1.9375 * 2^127 on).
 //
 // One (layer, sequence, kv head) holds max_len slots (a multiple of 64) of K and of V, hd bytes a slot, in
 // 64-slot blocks stored as the attention's MFMA operands, 16 bytes a lane and 1 KiB a load:

@@ -128,8 +128,8 @@ class KVCacheQ8:
             raise ValueError(f"KVCacheQ8: head_dim {head_dim} unsupported (64, 128)")
         if min(num_slots, max_length, kv_heads, sequences) < 1:
             raise ValueError("KVCacheQ8: layers, max_length, kv_heads and sequences must be positive")
-        if span is not None and (span < 64 or span % 64):
-            raise ValueError(f"KVCacheQ8: span {span} must be a multiple of 64")
+        if span is not None and (not 64 <= span <= 1 << 20 or span % 64):
+            raise ValueError(f"KVCacheQ8: span {span} must be a multiple of 64 up to 2^20")
         self.num_slots, self.max_length = num_slots, max_length
         self.kv_heads, self.head_dim, self.sequences = kv_heads, head_dim, sequences
         self.capacity = (max_length + 63) // 64 * 64
@@ -144,8 +144,9 @@ class KVCacheQ8:
         self._layers = [_lib.SsdKvQ8(self.k[i].data_ptr(), self.v[i].data_ptr(), self.k_exp[i].data_ptr(),
                                      self.v_exp[i].data_ptr(), sequences, kv_heads, head_dim, self.capacity)
                         for i in range(num_slots)]
-        for d in self._layers:
+        for i, d in enumerate(self._layers):  # a descriptor keeps its arrays, and knows how many layers they hold from its own on
             d.ref, d.device_index = ctypes.byref(d), self.k.get_device()
+            d.arrays, d.layers = (self.k, self.v, self.k_exp, self.v_exp), num_slots - i
 
     @staticmethod
     def default_span(capacity: int) -> int:
@@ -180,6 +181,9 @@ class KVCacheQ8:
         """Slots [start, length) of a bf16 cache's layer ``i`` (a prompt's, after its prefill) into sequence ``seq``."""
         if not 0 <= start <= length <= self.max_length or not 0 <= seq < self.sequences:
             raise ValueError(f"KVCacheQ8.load: slots [{start}, {length}) or sequence {seq} outside the cache")
+        if (cache.kv_heads, cache.head_dim) != (self.kv_heads, self.head_dim) or length > cache.max_length:
+            raise ValueError(f"KVCacheQ8.load: {length} slots of {self.kv_heads} heads of {self.head_dim} from a cache with "
+                             f"{cache.max_length} of {cache.kv_heads} of {cache.head_dim}")
         k, v = (x[:, start:].transpose(0, 1).flatten(1) for x in cache.read(i, length))
         slot = torch.arange(start, length, dtype=torch.int32, device=self.device)
         self.write(i, k, v, torch.full_like(slot, seq), slot)
@@ -197,7 +201,8 @@ class KVCacheQ8:
                ws: Optional[torch.Tensor] = None, scale: Optional[float] = None) -> torch.Tensor:
         """Tree attention of q [M, heads * head_dim] over layer ``i``: sequence s owns rows row_begin[s] ..
         row_begin[s + 1] (at most rows_max <= 64), row t attends slots [0, prefix[t]) then anc[t, :depth[t]]; zeros for
-        rows that attend nothing; rows of no sequence are left as ``out`` has them. l_max bounds prefix + depth. ``ws``: fp32, attend_floats(M, heads, l_max) (None: allocated here)."""
+        rows that attend nothing; rows of no sequence are left as ``out`` has them (unset without ``out``). l_max bounds
+        prefix + depth. ``ws``: fp32, attend_floats(M, heads, l_max) (None: allocated here)."""
         return ops.tree_attention_q8(self._layers[i], q, q.shape[0], self._heads(q), row_begin, prefix, depth, anc, rows_max,
                                      l_max, self.span, ws, out, scale)
 

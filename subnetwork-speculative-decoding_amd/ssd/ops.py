@@ -612,7 +612,7 @@ def kv_q8_write(cache, k, v, m, seq, slot, rope=None, pos=None, interleaved=Fals
         pq, ldq = _rows_ptr(q, "q", dev, m, heads * hd)
         if q_out is None:
             ldo = heads * hd
-            q_out = q.new_empty((q.shape[0], ldo))
+            q_out = q.new_empty((m, ldo))
             po = q_out.data_ptr()
         else:
             po, ldo = _rows_ptr(q_out, "q_out", dev, m, heads * hd)
@@ -641,8 +641,10 @@ def kv_q8_read(cache, m, seq, slot, k_out=None, v_out=None):
 
 
 def kv_q8_compact(cache, layers, start, src, n, n_max):
-    """Per sequence, slots src[s, :n[s]] to [start[s], ...) in ``layers`` layers (ssd_kv_q8_compact)."""
+    """Per sequence, slots src[s, :n[s]] to [start[s], ...) in ``layers`` layers from ``cache``'s on (ssd_kv_q8_compact)."""
     dev, seqs = _cache_dev(cache), cache.n_seq
+    if layers > cache.layers:
+        raise ValueError(f"kv_q8_compact: {layers} layers of a cache that holds {cache.layers} from this one on")
     pst, pn = _ptr(start, "start", I32, dev, seqs), _ptr(n, "n", I32, dev, seqs)
     psr = _ptr(src, "src", I32, dev, seqs * n_max)
     if n_max:
@@ -663,7 +665,7 @@ def tree_attention_q8(cache, q, m, heads, row_begin, prefix, depth, anc, rows_ma
     cols = heads * hd
     pq, ldq = _rows_ptr(q, "q", dev, m, cols)
     if out is None:
-        out, ldo = q.new_empty((q.shape[0], cols)), cols
+        out, ldo = q.new_empty((m, cols)), cols
         po = out.data_ptr()
     else:
         po, ldo = _rows_ptr(out, "out", dev, m, cols)

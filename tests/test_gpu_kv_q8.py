@@ -663,3 +663,15 @@ def test_prompt_from_the_bf16_cache():
         assert torch.equal(v2.cpu().double(), ref.stored((v - i)[0].transpose(0, 1).float().cpu()).flatten(1))
     with pytest.raises(ValueError, match="load"):
         cache.load(0, bf, n, seq=3)
+
+
+def test_values_that_round_past_the_largest_are_infinite():
+    cache = _cache(1, 64, 1, 64)
+    top = torch.tensor([1.9375, -1.9296875, 1.75]).double() * 2.0 ** 127
+    k = top.to(BF16)[:, None].repeat(1, 64)
+    assert torch.equal(k[:, 0].double(), top)
+    at = _i32([0, 1, 2])
+    cache.write(0, k.to(DEV), k.to(DEV), torch.zeros_like(at), at)
+    want = torch.tensor([float("inf"), -1.875 * 2.0 ** 127, 1.75 * 2.0 ** 127]).double()
+    for got in cache.read(0, torch.zeros_like(at), at):
+        assert torch.equal(got.cpu().double(), want[:, None].expand(3, 64))

@@ -257,3 +257,52 @@ def test_python_refusals_without_a_gpu():
     for cos, sin in ((t, t[:, :4]), (t.double(), t.double()), (t[:, ::2], t[:, ::2]), (t[0], t[0])):
         with pytest.raises(ValueError, match="rotary tables"):
             ops.RopeTables(cos, sin)
+
+
+def test_a_prompt_of_another_shape_is_not_loaded():
+    from ssd.engine.kv_cache import KVCache, KVCacheQ8
+
+    cache = KVCacheQ8(1, 256, 2, 64, "cpu")
+    for other in (KVCache(1, 256, 4, 64, "cpu"), KVCache(1, 256, 2, 128, "cpu"), KVCache(1, 100, 2, 64, "cpu")):
+        with pytest.raises(ValueError, match="slots of 2 heads of 64 from a cache"):
+            cache.load(0, other, 120)
+
+
+def test_a_span_beyond_the_kernels_is_refused():
+    from ssd.engine.kv_cache import KVCacheQ8
+
+    with pytest.raises(ValueError, match="span"):
+        KVCacheQ8(1, 64, 2, 64, "cpu", span=(1 << 20) + 64)
+
+
+def test_descriptors_keep_their_arrays_and_their_layers(monkeypatch):
+    import gc
+    import weakref
+
+    from ssd import ops
+    from ssd.engine.kv_cache import KVCacheQ8
+
+    cache = KVCacheQ8(3, 64, 2, 64, "cpu")
+    seen, first, second = weakref.ref(cache.k), cache.k.data_ptr(), cache.layer(1)
+    del cache
+    gc.collect()
+    assert seen() is not None and second.k == first + seen()[0].numel()
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: -1)
+    start = torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="3 layers of a cache that holds 2"):
+        ops.kv_q8_compact(second, 3, start, start[None], start, 1)
+
+
+def test_made_outputs_have_the_rows_that_are_written(monkeypatch):
+    from ssd import ops
+    from ssd.engine.kv_cache import KVCacheQ8
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: -1)
+    monkeypatch.setattr(ops, "_stream", lambda dev: 0)
+    monkeypatch.setattr(ops._lib, "call", lambda *a: 0)
+    cache = KVCacheQ8(1, 64, 2, 64, "cpu")
+    i = torch.zeros(8, dtype=torch.int32)
+    q, k = torch.zeros(5, 256, dtype=torch.bfloat16), torch.zeros(3, 128, dtype=torch.bfloat16)
+    assert cache.write(0, k, k, i, i, q=q).shape == (3, 256)
+    out = ops.tree_attention_q8(cache.layer(0), q, 3, 4, i, i, i, torch.zeros(8, 32, dtype=torch.int32), 1, 64, 64)
+    assert out.shape == (3, 256)
