@@ -579,6 +579,12 @@ __global__ __launch_bounds__(256, 2) void q8_fold_kernel(AttnQ8Args a, int own) 
   else q8_shared_group<HD, T>(a, blockIdx.x - own, lds.shared);
 }
 
+// Sums that stay sums: no multiply-add contraction with the products they are given.
+__device__ __forceinline__ float q8_add(float x, float y) {
+#pragma clang fp contract(off)
+  return x + y;
+}
+
 // Second launch: one workgroup of four waves per (row, head). Weights from the groups' largest reference; wave r
 // adds groups r, r + 4, ... in order, then the four sums are added in order; l by a fixed exchange between
 // lanes, 64 groups at a time.
@@ -617,7 +623,7 @@ __global__ __launch_bounds__(256) void q8_combine_kernel(AttnQ8Args a) {
     const float wgt = q8_weight(ml.x, top);
     float lw = ml.y * wgt;
 #pragma unroll
-    for (int s = 32; s >= 1; s >>= 1) lw += __shfl_xor(lw, s);
+    for (int s = 32; s >= 1; s >>= 1) lw = q8_add(lw, __shfl_xor(lw, s));
     l += lw;
     for (int g = g0 + r; g < min(n, g0 + 64); g += 16) {
       if (g != r) load(g);
@@ -643,6 +649,55 @@ __global__ __launch_bounds__(256) void q8_combine_kernel(AttnQ8Args a) {
     }
     *(uint32_t*)(a.out + (size_t)row * a.ldo + (size_t)h * HD + d) = pack_bf16x2(y[0], y[1]);
   }
+}
+
+// The same sums for up to G <= 8 groups, HD / 4 lanes a (row, head): every record of a pair is in flight at once.
+template <int HD, int G>
+__global__ __launch_bounds__(256) void q8_combine_few_kernel(AttnQ8Args a) {
+  constexpr int LANES = HD / 4, PAIRS = 256 / LANES;
+  const int64_t pair = (int64_t)blockIdx.x * PAIRS + threadIdx.x / LANES;
+  const int row = min((int)(pair / a.heads), a.M - 1), h = (int)(pair % a.heads), d = threadIdx.x % LANES * 4;
+  const size_t rec0 = ((size_t)row * a.heads + h) * a.n_grps;
+  f32x4_t x[G];
+  float2 ml[G];
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    const size_t rec = rec0 + min(g, a.n_grps - 1);
+    x[g] = *(const f32x4_t*)(a.ws_o + rec * HD + d);
+    ml[g] = a.ws_ml[rec];
+  }
+  if (pair >= (int64_t)a.M * a.heads || row < a.row_begin[0] || row >= a.row_begin[a.n_seq]) return;
+  int P, L;
+  q8_row_keys(a, row, P, L);
+  const int per = QA_GRP * a.span_blk * QA_BLK, n = (L + per - 1) / per;
+  float top = -INFINITY;
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    if (g >= n) ml[g] = make_float2(-INFINITY, 0.f);
+    top = fmaxf(top, ml[g].x);
+  }
+  float lw[G];
+  f32x4_t part[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) part[r] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    const float wgt = q8_weight(ml[g].x, top);
+    lw[g] = ml[g].y * wgt;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) part[g % 4][e] = g < n ? fmaf(x[g][e], wgt, part[g % 4][e]) : part[g % 4][e];
+  }
+#pragma unroll
+  for (int s = G / 2; s >= 1; s >>= 1)
+#pragma unroll
+    for (int g = 0; g < s; ++g) lw[g] = q8_add(lw[g], lw[g + s]);
+  float y[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float s = ((part[0][e] + part[1][e]) + part[2][e]) + part[3][e];
+    y[e] = lw[0] == 0.f ? 0.f : s / lw[0];  // NaN stays NaN
+  }
+  *(uint2*)(a.out + (size_t)row * a.ldo + (size_t)h * HD + d) = make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
 }
 
 // Contexts of up to TEAMS <= 4 groups in one launch: a workgroup per (sequence, row, kv head), a team of four waves per
@@ -702,7 +757,7 @@ __global__ __launch_bounds__(256 * TEAMS, TEAMS == 4 || (TEAMS == 1 && HD == 64)
       wgt[t] = q8_weight(m, top);
       lw[t] = t == 0 ? r.l * wgt[0] : t < TEAMS ? rec_l[t < TEAMS ? t : 0][rr] * wgt[t] : 0.f;
     }
-    const float l = (lw[0] + lw[2]) + (lw[1] + lw[3]);
+    const float l = q8_add(q8_add(lw[0], lw[2]), q8_add(lw[1], lw[3]));
 #pragma unroll
     for (int i = 0; i < HD / 64; ++i) {
       float y[4];
@@ -757,7 +812,13 @@ static int launch_attn_q8(AttnQ8Args a, int rows_max, hipStream_t stream) {
   if (single) SSD_LAUNCH((q8_fold_kernel<HD, 1>), dim3((unsigned)(own + shared)), dim3(256), 0, stream, a, (int)own);
   else SSD_LAUNCH((q8_fold_kernel<HD, 2>), dim3((unsigned)(own + shared)), dim3(256), 0, stream, a, (int)own);
   if (int rc = check_launch("attn_q8_fold")) return rc;
-  SSD_LAUNCH((q8_combine_kernel<HD>), dim3((unsigned)(a.M * a.heads)), dim3(256), 0, stream, a);
+  // Up to eight groups: lanes of several (row, head) pairs a workgroup. us of both launches, a workgroup a pair / lanes: 12 trees of
+  // up to 9 rows, 4 groups 25.7 / 23.7; 16 of 32 rows, 3 groups 50.3 / 41.6; one row, 8 groups 9.3 / 9.2; a tree of 25 rows,
+  // 6 groups 13.6 / 13.1. With 9 and 11 groups it would be 14.7 / 15.4 and 17.4 / 18.3.
+  const unsigned few = (unsigned)(((int64_t)a.M * a.heads + 1024 / HD - 1) / (1024 / HD));
+  if (a.n_grps <= 4) SSD_LAUNCH((q8_combine_few_kernel<HD, 4>), dim3(few), dim3(256), 0, stream, a);
+  else if (a.n_grps <= 8) SSD_LAUNCH((q8_combine_few_kernel<HD, 8>), dim3(few), dim3(256), 0, stream, a);
+  else SSD_LAUNCH((q8_combine_kernel<HD>), dim3((unsigned)(a.M * a.heads)), dim3(256), 0, stream, a);
   return check_launch("attn_q8_combine");
 }
 

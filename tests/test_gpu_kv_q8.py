@@ -675,3 +675,16 @@ def test_values_that_round_past_the_largest_are_infinite():
     want = torch.tensor([float("inf"), -1.875 * 2.0 ** 127, 1.75 * 2.0 ** 127]).double()
     for got in cache.read(0, torch.zeros_like(at), at):
         assert torch.equal(got.cpu().double(), want[:, None].expand(3, 64))
+
+
+@pytest.mark.parametrize("hd,heads,kv", [(128, 16, 4), (64, 32, 8)])
+@pytest.mark.parametrize("n", [1, 200, 500, 1000, 2000])
+def test_a_larger_bound_changes_no_bit(hd, heads, kv, n):
+    """l_max chooses the kernels (one launch, lanes or workgroups for the groups' sum), not the result."""
+    cache = _cache(1, 4096, kv, hd, 2, 64)
+    vals = _fill(cache, hd)
+    rows = [_tree(n, n + 2, 7, _gen(n)), [(n // 2, []), (0, [n + 1]), (0, [])]]
+    want = _check_attend(cache, rows, heads, n, vals)
+    for l_max in (256, 512, 1024, 2048, 2304, 4096):
+        if l_max >= n + 8:
+            assert torch.equal(_check_attend(cache, rows, heads, n, vals, l_max=l_max), want), l_max
