@@ -6,12 +6,19 @@
 // reference m, sum l and output O (fp32); the spans of a group, then the groups, are added with weights from
 // their largest m. First launch: groups that every row of a sequence attends whole are folded for all its rows at
 // once, a row's other groups by a workgroup of its own; each (row, head, group) leaves a record (m, l, O).
-// Second launch: the groups' sum. Contexts of few groups take one launch that does both.
+// Second launch: the groups' sum. Short contexts take one launch that does both.
 //
 // S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32_bf16: codes become bf16 exactly (v_cvt_scalef32_pk_bf16_fp8,
 // with K's exponents as its scale); V's exponents multiply the probabilities before those are rounded to bf16
 // (exact), so that rounding -- 2^-8 of a weight at most -- is the only one below fp32. l is summed by the MFMA too, from
 // the rounded probabilities (an A operand of 2^-(V exponent)), so the weights O is made of add up to l exactly.
+//
+// What bounds it, 8 kv heads of 128 (us, both launches): one row of 32 sequences at up to 8192 keys 82 for 410 MB, 5.0 TB/s, and
+// one row at 131000 keys 49 for 270 MB (43 the fold, 6.3 TB/s): bytes. 25 rows of 64 heads at 16384 keys 35 for 13.4
+// GFLOP: the VALU work of a score (conversion once per two tiles, maximum, exp2, packing) beside its MFMAs. 25 rows of 32
+// heads at 4096 keys 15 and 12 trees of up to 9 rows at 1900 24: the chains of a workgroup (rows, prefixes, ancestors,
+// keys, then one block after the other) at two waves a SIMD, which 248 VGPRs allow, and the second launch. One row at
+// 512 keys 5.5: a launch and that chain once.
 #include "kv_q8.h"
 
 #include <math.h>

