@@ -15,7 +15,6 @@ accepted-path compaction) is one kernel launch over every layer. ``seq_len`` boo
 
 from __future__ import annotations
 
-import ctypes
 from typing import Optional
 
 import torch
@@ -145,8 +144,8 @@ class KVCacheQ8:
                                      self.v_exp[i].data_ptr(), sequences, kv_heads, head_dim, self.capacity)
                         for i in range(num_slots)]
         for i, d in enumerate(self._layers):  # a descriptor keeps its arrays, and knows how many layers they hold from its own on
-            d.ref, d.device_index = ctypes.byref(d), self.k.get_device()
-            d.arrays, d.layers = (self.k, self.v, self.k_exp, self.v_exp), num_slots - i
+            # (no reference of ctypes to itself: such a cycle is never collected, nor are the arrays on it)
+            d.arrays, d.layers, d.device_index = (self.k, self.v, self.k_exp, self.v_exp), num_slots - i, self.k.get_device()
 
     @staticmethod
     def default_span(capacity: int) -> int:

@@ -617,7 +617,7 @@ def kv_q8_write(cache, k, v, m, seq, slot, rope=None, pos=None, interleaved=Fals
         else:
             po, ldo = _rows_ptr(q_out, "q_out", dev, m, heads * hd)
     if m:
-        _lib.call("ssd_kv_q8_write_bf16", cache.ref, pk, ldk, pv, ldv, m, ps, pl, st, pp, pq, ldq, heads, po, ldo,
+        _lib.call("ssd_kv_q8_write_bf16", cache, pk, ldk, pv, ldv, m, ps, pl, st, pp, pq, ldq, heads, po, ldo,
                   _stream(dev))
     return q_out
 
@@ -636,7 +636,7 @@ def kv_q8_read(cache, m, seq, slot, k_out=None, v_out=None):
         pk, ldk = _rows_ptr(k_out, "k_out", dev, m, cols)
         pv, ldv = _rows_ptr(v_out, "v_out", dev, m, cols)
     if m:
-        _lib.call("ssd_kv_q8_read_bf16", cache.ref, m, ps, pl, pk, ldk, pv, ldv, _stream(dev))
+        _lib.call("ssd_kv_q8_read_bf16", cache, m, ps, pl, pk, ldk, pv, ldv, _stream(dev))
     return k_out, v_out
 
 
@@ -648,7 +648,7 @@ def kv_q8_compact(cache, layers, start, src, n, n_max):
     pst, pn = _ptr(start, "start", I32, dev, seqs), _ptr(n, "n", I32, dev, seqs)
     psr = _ptr(src, "src", I32, dev, seqs * n_max)
     if n_max:
-        _lib.call("ssd_kv_q8_compact", cache.ref, layers, pst, psr, pn, n_max, _stream(dev))
+        _lib.call("ssd_kv_q8_compact", cache, layers, pst, psr, pn, n_max, _stream(dev))
 
 
 def attn_q8_ws_floats(m: int, heads: int, head_dim: int, l_max: int, span: int) -> int:
@@ -675,7 +675,7 @@ def tree_attention_q8(cache, q, m, heads, row_begin, prefix, depth, anc, rows_ma
         ws = torch.empty(max(attn_q8_ws_floats(m, heads, hd, l_max, span), 4), dtype=F32, device=q.device)
     pw = _ptr(ws, "ws", F32, dev, 1)
     if m:
-        _lib.call("ssd_tree_attention_q8", cache.ref, pq, ldq, m, heads, pb, pp, pd, pa, rows_max, l_max, span,
+        _lib.call("ssd_tree_attention_q8", cache, pq, ldq, m, heads, pb, pp, pd, pa, rows_max, l_max, span,
                   hd ** -0.5 if scale is None else float(scale), pw, ws.numel(), po, ldo, _stream(dev))
     return out
 

@@ -688,3 +688,26 @@ def test_a_larger_bound_changes_no_bit(hd, heads, kv, n):
     for l_max in (256, 512, 1024, 2048, 2304, 4096):
         if l_max >= n + 8:
             assert torch.equal(_check_attend(cache, rows, heads, n, vals, l_max=l_max), want), l_max
+
+
+def test_rebuilt_caches_keep_no_device_memory():
+    import gc
+
+    from ssd.models.llama import rope_tables_f32
+
+    def use():
+        cache = _cache(2, 4096, 8, 128, 4)
+        rope = rope_tables_f32(64, 128, 1e4, DEV)
+        k, at = torch.ones(3, 1024, dtype=BF16, device=DEV), _i32([0, 1, 2])
+        q = cache.write(1, k, k, at, at, rope=rope, pos=at, q=k)
+        cache.attend(1, q, _i32([0, 1, 2, 3, 3]), at + 1, at * 0, torch.zeros(3, 32, dtype=torch.int32, device=DEV), 1, 4)
+        cache.compact_device(_i32([0] * 4), _i32([[0]] * 4), _i32([1] * 4))
+        assert cache.read(1, at, at)[1].eq(1).all()
+
+    use()
+    gc.collect(), torch.cuda.synchronize()
+    held = torch.cuda.memory_allocated()
+    for _ in range(3):
+        use()
+    gc.collect(), torch.cuda.synchronize()
+    assert torch.cuda.memory_allocated() <= held

@@ -306,3 +306,52 @@ def test_made_outputs_have_the_rows_that_are_written(monkeypatch):
     assert cache.write(0, k, k, i, i, q=q).shape == (3, 256)
     out = ops.tree_attention_q8(cache.layer(0), q, 3, 4, i, i, i, torch.zeros(8, 32, dtype=torch.int32), 1, 64, 64)
     assert out.shape == (3, 256)
+
+
+def test_a_dropped_cache_frees_its_arrays():
+    """With no descriptor held, after a held one goes, and after the descriptors were used by calls."""
+    import gc
+    import weakref
+
+    from ssd.engine.kv_cache import KVCacheQ8
+
+    def arrays(cache):
+        return [weakref.ref(t) for t in (cache.k, cache.v, cache.k_exp, cache.v_exp)]
+
+    cache = KVCacheQ8(3, 64, 2, 64, "cpu")
+    seen = arrays(cache)
+    del cache
+    gc.collect()
+    assert not any(r() is not None for r in seen)
+
+    cache = KVCacheQ8(3, 64, 2, 64, "cpu")
+    seen, held = arrays(cache), cache.layer(1)
+    del cache
+    gc.collect()
+    assert all(r() is not None for r in seen)
+    del held
+    gc.collect()
+    assert not any(r() is not None for r in seen)
+
+
+def test_calls_keep_no_cache(monkeypatch):
+    import gc
+    import weakref
+
+    from ssd import ops
+    from ssd.engine.kv_cache import KVCacheQ8
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: -1)
+    monkeypatch.setattr(ops, "_stream", lambda dev: 0)
+    monkeypatch.setattr(ops._lib, "call", lambda name, *args: C.POINTER(ops._lib.SsdKvQ8).from_param(args[0]) and 0)
+    cache = KVCacheQ8(2, 64, 2, 64, "cpu")
+    seen = weakref.ref(cache.k)
+    i = torch.zeros(8, dtype=torch.int32)
+    k, q = torch.zeros(3, 128, dtype=torch.bfloat16), torch.zeros(3, 256, dtype=torch.bfloat16)
+    cache.write(0, k, k, i, i)
+    cache.read(1, i, i)
+    cache.attend(0, q, i, i, i, torch.zeros(8, 32, dtype=torch.int32), 3, 64)
+    cache.compact_device(i, i[None], i)
+    del cache
+    gc.collect()
+    assert seen() is None
