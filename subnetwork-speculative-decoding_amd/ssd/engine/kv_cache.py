@@ -199,9 +199,9 @@ class KVCacheQ8:
                anc: torch.Tensor, rows_max: int, l_max: int, out: Optional[torch.Tensor] = None,
                ws: Optional[torch.Tensor] = None, scale: Optional[float] = None) -> torch.Tensor:
         """Tree attention of q [M, heads * head_dim] over layer ``i``: sequence s owns rows row_begin[s] ..
-        row_begin[s + 1] (at most rows_max <= 64), row t attends slots [0, prefix[t]) then anc[t, :depth[t]]; zeros for
-        rows that attend nothing; rows of no sequence are left as ``out`` has them (unset without ``out``). l_max bounds
-        prefix + depth. ``ws``: fp32, attend_floats(M, heads, l_max) (None: allocated here)."""
+        row_begin[s + 1] (at most rows_max <= 64), row t attends slots [0, prefix[t]) then anc[t, :depth[t]] of anc [M, 32]
+        (a depth above 32 counts as 32); zeros for rows that attend nothing; rows of no sequence are left as ``out`` has
+        them (unset without ``out``). l_max bounds prefix + depth. ``ws``: fp32, attend_floats(M, heads, l_max) (None: allocated here)."""
         return ops.tree_attention_q8(self._layers[i], q, q.shape[0], self._heads(q), row_begin, prefix, depth, anc, rows_max,
                                      l_max, self.span, ws, out, scale)
 

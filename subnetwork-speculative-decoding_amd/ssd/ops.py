@@ -659,8 +659,8 @@ def attn_q8_ws_floats(m: int, heads: int, head_dim: int, l_max: int, span: int) 
 
 
 def tree_attention_q8(cache, q, m, heads, row_begin, prefix, depth, anc, rows_max, l_max, span, ws=None, out=None, scale=None):
-    """Tree attention of a batch's rows over ``cache`` (SsdKvQ8 of one layer; ssd_tree_attention_q8). ``ws`` (fp32,
-    attn_q8_ws_floats(...)) and ``out`` are made here if None."""
+    """Tree attention of a batch's rows over ``cache`` (SsdKvQ8 of one layer; ssd_tree_attention_q8). ``anc`` [m, 32]. ``ws``
+    (fp32, attn_q8_ws_floats(...)) and ``out`` are made here if None."""
     dev, hd = _cache_dev(cache), cache.head_dim
     cols = heads * hd
     pq, ldq = _rows_ptr(q, "q", dev, m, cols)
@@ -671,6 +671,8 @@ def tree_attention_q8(cache, q, m, heads, row_begin, prefix, depth, anc, rows_ma
         po, ldo = _rows_ptr(out, "out", dev, m, cols)
     pb, pp = _ptr(row_begin, "row_begin", I32, dev, cache.n_seq + 1), _ptr(prefix, "prefix", I32, dev, m)
     pd, pa = _ptr(depth, "depth", I32, dev, m), _ptr(anc, "anc", I32, dev, m * 32)
+    if m and anc.dim() > 1 and anc.shape[-1] != 32:  # rows of another width would be read as rows of 32
+        raise ValueError(f"anc must have rows of 32 slots, got {tuple(anc.shape)}")
     if ws is None:
         ws = torch.empty(max(attn_q8_ws_floats(m, heads, hd, l_max, span), 4), dtype=F32, device=q.device)
     pw = _ptr(ws, "ws", F32, dev, 1)

@@ -355,3 +355,33 @@ def test_calls_keep_no_cache(monkeypatch):
     del cache
     gc.collect()
     assert seen() is None
+
+
+def _calls_without_a_gpu(monkeypatch):
+    from ssd import ops
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: -1)
+    monkeypatch.setattr(ops, "_stream", lambda dev: 0)
+    monkeypatch.setattr(ops._lib, "call", lambda *a: 0)
+
+
+@pytest.mark.parametrize("shape", [(3, 64), (6, 16), (3, 33), (96, 1), (1, 96), (2, 32)])
+def test_ancestor_tables_of_another_width_are_refused(monkeypatch, shape):
+    """Rows of a table that is not 32 wide would be read as rows of 32."""
+    from ssd.engine.kv_cache import KVCacheQ8
+
+    _calls_without_a_gpu(monkeypatch)
+    cache = KVCacheQ8(1, 64, 2, 64, "cpu")
+    i, q = torch.zeros(8, dtype=torch.int32), torch.zeros(3, 256, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="anc"):
+        cache.attend(0, q, i, i, i, torch.zeros(shape, dtype=torch.int32), 3, 64)
+
+
+@pytest.mark.parametrize("shape", [(3, 32), (5, 32), (96,), (1, 3, 32)])
+def test_ancestor_tables_of_rows_of_32_are_taken(monkeypatch, shape):
+    from ssd.engine.kv_cache import KVCacheQ8
+
+    _calls_without_a_gpu(monkeypatch)
+    cache = KVCacheQ8(1, 64, 2, 64, "cpu")
+    i, q = torch.zeros(8, dtype=torch.int32), torch.zeros(3, 256, dtype=torch.bfloat16)
+    assert cache.attend(0, q, i, i, i, torch.zeros(shape, dtype=torch.int32), 3, 64).shape == (3, 256)
