@@ -385,3 +385,18 @@ def test_ancestor_tables_of_rows_of_32_are_taken(monkeypatch, shape):
     cache = KVCacheQ8(1, 64, 2, 64, "cpu")
     i, q = torch.zeros(8, dtype=torch.int32), torch.zeros(3, 256, dtype=torch.bfloat16)
     assert cache.attend(0, q, i, i, i, torch.zeros(shape, dtype=torch.int32), 3, 64).shape == (3, 256)
+
+
+def test_moves_of_another_width_are_refused(monkeypatch):
+    """Rows of `src` that are not n_max wide would be read as rows of n_max."""
+    from ssd import ops
+    from ssd.engine.kv_cache import KVCacheQ8
+
+    _calls_without_a_gpu(monkeypatch)
+    cache = KVCacheQ8(2, 64, 2, 64, "cpu", sequences=3)
+    i = torch.zeros(3, dtype=torch.int32)
+    for shape in ((3, 9), (4, 6), (3, 4), (15, 1), (1, 15)):
+        with pytest.raises(ValueError, match="src"):
+            ops.kv_q8_compact(cache.layer(0), 2, i, torch.zeros(shape, dtype=torch.int32), i, 5)
+    for shape in ((3, 5), (4, 5), (15,)):
+        ops.kv_q8_compact(cache.layer(0), 2, i, torch.zeros(shape, dtype=torch.int32), i, 5)
