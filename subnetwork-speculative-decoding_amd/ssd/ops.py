@@ -648,7 +648,7 @@ def kv_q8_compact(cache, layers, start, src, n, n_max):
         raise ValueError(f"kv_q8_compact: {layers} layers of a cache that holds {cache.layers} from this one on")
     pst, pn = _ptr(start, "start", I32, dev, seqs), _ptr(n, "n", I32, dev, seqs)
     psr = _ptr(src, "src", I32, dev, seqs * n_max)
-    if src.dim() > 1 and src.shape[-1] != n_max:  # rows of another width would be read as rows of n_max
+    if n_max and src.dim() > 1 and src.shape[-1] != n_max:  # rows of another width would be read as rows of n_max
         raise ValueError(f"src must have rows of n_max = {n_max} slots, got {tuple(src.shape)}")
     if n_max:
         _lib.call("ssd_kv_q8_compact", cache, layers, pst, psr, pn, n_max, _stream(dev))

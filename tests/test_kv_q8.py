@@ -400,3 +400,14 @@ def test_moves_of_another_width_are_refused(monkeypatch):
             ops.kv_q8_compact(cache.layer(0), 2, i, torch.zeros(shape, dtype=torch.int32), i, 5)
     for shape in ((3, 5), (4, 5), (15,)):
         ops.kv_q8_compact(cache.layer(0), 2, i, torch.zeros(shape, dtype=torch.int32), i, 5)
+
+
+def test_no_moves_take_any_table(monkeypatch):
+    from ssd import ops
+    from ssd.engine.kv_cache import KVCacheQ8
+
+    _calls_without_a_gpu(monkeypatch)
+    cache = KVCacheQ8(1, 64, 2, 64, "cpu", sequences=3)
+    i = torch.zeros(3, dtype=torch.int32)
+    ops.kv_q8_compact(cache.layer(0), 1, i, torch.zeros(3, 9, dtype=torch.int32), i, 0)
+    cache.compact_device(i, torch.zeros(3, 0, dtype=torch.int32), i)
