@@ -198,6 +198,8 @@ def tree_attention(q, m, heads, kv_heads, head_dim, k_cache, vt_cache, max_len, 
     for t, nm, n in ((prefix, "prefix", m), (depth, "depth", m), (anc, "anc", m * 32)):
         _check(t, nm, torch.int32)
         _len(t, nm, n)
+    if anc.dim() > 1 and (anc.shape[-1] != 32 or not anc.is_contiguous()):  # would be read as rows of 32
+        raise ValueError(f"anc must be contiguous rows of 32 slots, got {tuple(anc.shape)}, strides {anc.stride()}")
     if k_cache.numel() < kv_heads * max_len * head_dim or vt_cache.numel() < kv_heads * max_len * head_dim:
         raise ValueError("tree_attention: cache smaller than kv_heads * max_len * head_dim")
     scale = head_dim ** -0.5 if scale is None else scale

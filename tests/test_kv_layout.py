@@ -64,3 +64,25 @@ def test_tile_untile_round_trip_and_cache_update():
     kk, vv = cache.update(1, k2, k2)
     assert torch.equal(kk[0, :, :7], k[0].to(torch.bfloat16)) and torch.equal(kk[0, :, 7:], k2[0].to(torch.bfloat16))
     assert cache.k[0].abs().sum() == 0
+
+
+def test_tree_attention_refuses_ancestor_tables_that_are_not_rows_of_32(monkeypatch):
+    """The bf16 cache's attention: tables of another width, or with gaps between rows, would be read as rows of 32."""
+    ops = _ops()
+    monkeypatch.setattr(ops, "_check", lambda *a, **k: None)
+    monkeypatch.setattr(ops, "stream", lambda: 0)
+    monkeypatch.setattr(ops._lib, "call", lambda *a: 0)
+    q, kv = torch.zeros(3, 256, dtype=torch.bfloat16), torch.zeros(2 * 64 * 64, dtype=torch.bfloat16)
+    i, ws = torch.zeros(8, dtype=torch.int32), torch.zeros(8)
+
+    def call(anc):
+        ops.tree_attention(q, 3, 4, 2, 64, kv, kv, 64, i, i, anc, 0, 64, ws, torch.zeros_like(q))
+
+    def table(*shape):
+        return torch.zeros(*shape, dtype=torch.int32)
+
+    for anc in (table(3, 64), table(6, 16), table(96, 1), table(3, 40)[:, :32]):
+        with pytest.raises(ValueError, match="anc"):
+            call(anc)
+    for anc in (table(3, 32), table(8, 32)[2:], table(96)):
+        call(anc)
