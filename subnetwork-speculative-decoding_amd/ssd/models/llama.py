@@ -143,8 +143,10 @@ def rope_tables_f32(positions: int, rot_dim: int, theta: float, device,
     """cos/sin [positions, rot_dim / 2] in fp32 for ``ops.rope`` and the 8-bit cache's write, from frequencies and angles
     in 64 bits (at position 10^6 an fp32 angle is off by 0.03). ``scaling`` (HF's keys, ``rope_type``): "linear"
     (factor), "llama3" (factor, low_freq_factor, high_freq_factor, original_max_position_embeddings) or "yarn"
-    (factor, original_max_position_embeddings; optional beta_fast, beta_slow, attention_factor): YaRN's ramp between
-    the dims that turn beta_fast and beta_slow times in the original context, cos and sin times 0.1 ln(factor) + 1."""
+    (factor, original_max_position_embeddings; optional beta_fast, beta_slow, truncate, attention_factor, mscale,
+    mscale_all_dim): YaRN's ramp between the dims that turn beta_fast and beta_slow times in the original context (whole
+    dims unless truncate is False), cos and sin times attention_factor, or else g(mscale) / g(mscale_all_dim) where both
+    are given, or else g(1), with g(s) = 0.1 s ln(factor) + 1 for factors above 1 and 1 below."""
     if rot_dim < 2 or rot_dim % 2 or positions < 1:
         raise ValueError(f"rope_tables_f32: bad positions={positions} rot_dim={rot_dim}")
     i = torch.arange(rot_dim // 2, dtype=torch.float64)
@@ -163,12 +165,18 @@ def rope_tables_f32(positions: int, rot_dim: int, theta: float, device,
         def dim(turns):
             return rot_dim * math.log(ctx / (turns * 2 * math.pi)) / (2 * math.log(theta))
 
-        lo = max(math.floor(dim(float(scaling.get("beta_fast") or 32.0))), 0)
-        hi = min(math.ceil(dim(float(scaling.get("beta_slow") or 1.0))), rot_dim - 1)
+        lo, hi = dim(float(scaling.get("beta_fast") or 32.0)), dim(float(scaling.get("beta_slow") or 1.0))
+        if scaling.get("truncate", True):
+            lo, hi = math.floor(lo), math.ceil(hi)
+        lo, hi = max(lo, 0), min(hi, rot_dim - 1)
         slow = ((i - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
         inv = inv * (1 - slow) + inv / f * slow
-        given = scaling.get("attention_factor")
-        gain = 0.1 * math.log(f) + 1.0 if given is None and f > 1 else float(given or 1.0)
+
+        def g(s):
+            return 0.1 * s * math.log(f) + 1.0 if f > 1 else 1.0
+
+        given, one, both = (scaling.get(n) for n in ("attention_factor", "mscale", "mscale_all_dim"))
+        gain = float(given) if given is not None else g(float(one)) / g(float(both)) if one and both else g(1.0)
     elif kind != "default":
         raise ValueError(f"rope_type {kind!r} is not supported (default, linear, llama3, yarn)")
     ang = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * inv.to(device)

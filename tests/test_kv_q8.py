@@ -411,3 +411,48 @@ def test_no_moves_take_any_table(monkeypatch):
     i = torch.zeros(3, dtype=torch.int32)
     ops.kv_q8_compact(cache.layer(0), 1, i, torch.zeros(3, 9, dtype=torch.int32), i, 0)
     cache.compact_device(i, torch.zeros(3, 0, dtype=torch.int32), i)
+
+
+@pytest.mark.parametrize("extra,gain", [
+    ({}, 0.1 * math.log(40) + 1), (dict(mscale=1.0, mscale_all_dim=1.0), 1.0),
+    (dict(mscale=0.707, mscale_all_dim=1.0), (0.0707 * math.log(40) + 1) / (0.1 * math.log(40) + 1)),
+    (dict(mscale=1.5), 0.1 * math.log(40) + 1), (dict(mscale=1.0, mscale_all_dim=0), 0.1 * math.log(40) + 1),
+    (dict(attention_factor=0.75, mscale=0.707, mscale_all_dim=1.0), 0.75), (dict(factor=1.0), 1.0),
+    (dict(factor=0.5, mscale=2.0, mscale_all_dim=1.0), 1.0), (dict(attention_factor=None, mscale=None), 0.1 * math.log(40) + 1)])
+def test_rope_tables_yarn_factor_on_cos_and_sin(extra, gain):
+    """Position 0: cos is the factor. attention_factor as given; else the ratio of the two scales' 0.1 s ln(factor) + 1 where
+    both are given (and not 0); else 0.1 ln(factor) + 1; a factor of at most 1 scales by 1."""
+    from ssd.models.llama import rope_tables_f32
+
+    s = dict(rope_type="yarn", factor=40.0, original_max_position_embeddings=4096)
+    cos, _ = rope_tables_f32(2, 64, 10000.0, "cpu", {**s, **extra})
+    assert float((cos[0] - gain).abs().max()) <= gain * 2 ** -24  # one rounding to fp32
+
+
+@pytest.mark.parametrize("truncate", [None, True, False])
+@pytest.mark.parametrize("rot,theta,context,fast,slow", [(128, 500000.0, 8192, 32.0, 1.0), (64, 10000.0, 4096, 32.0, 1.0),
+                                                         (64, 150000.0, 4096, 32.0, 1.0), (32, 1e4, 16384, 8.0, 2.0)])
+def test_rope_tables_yarn_inside_the_ramp(rot, theta, context, fast, slow, truncate):
+    """Every dim's frequency against the definition, dim by dim: a dim that turns `fast` times or more in the original context
+    stays, one that turns `slow` times or less is divided by the factor, between them linear in the dim's number; the ends of the ramp are
+    whole dims (rounded outwards) unless truncate is False."""
+    from ssd.models.llama import rope_tables_f32
+
+    f = 4.0
+    s = dict(rope_type="yarn", factor=f, original_max_position_embeddings=context, beta_fast=fast, beta_slow=slow, attention_factor=1.0)
+    if truncate is not None:
+        s["truncate"] = truncate
+    _, sin = rope_tables_f32(2, rot, theta, "cpu", s)
+    # theta^(2 d / rot) = context / (2 pi turns) at dim d
+    first, last = (math.log(context / (2 * math.pi * turns), theta) * rot / 2 for turns in (fast, slow))
+    if truncate is not False:
+        first, last = math.floor(first), math.ceil(last)
+    first, last = max(first, 0), min(last, rot - 1)
+    inside = 0
+    for d in range(rot // 2):
+        t = min(max((d - first) / (last - first), 0.0), 1.0)
+        inside += 0 < t < 1
+        w = theta ** (-2 * d / rot)
+        want = math.sin(w * (1 - t) + w / f * t)  # position 1
+        assert abs(float(sin[1, d]) - want) <= abs(want) * (2 ** -24 + 2 ** -40), d  # one rounding; the doubles' own far below
+    assert inside >= 2  # the shortest ramp, 10.05 to 12.46, holds dims 11 and 12
