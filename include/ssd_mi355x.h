@@ -254,8 +254,9 @@ int ssd_kv_q8_compact(const SsdKvQ8* cache, int layers, const int32_t* start, co
 /* Tree attention over the 8-bit cache for a batch: sequence s owns rows [row_begin[s], row_begin[s + 1]) (device
  * int32 [n_seq + 1], increasing, at most rows_max <= 64 rows each), and row t attends slots [0, prefix[t]) then
  * anc[t][0 .. depth[t]) of its sequence (anc: rows of 32; a depth above 32 counts as 32), as
- * ssd_tree_attention_bf16 does. A row that attends nothing gets zeros; rows outside [row_begin[0], row_begin[n_seq]) are left as they were. l_max >= every prefix + depth (host bound;
- * keys at logical positions from l_max on are not attended). Keys are folded in a fixed order (blocks of 64 within a
+ * ssd_tree_attention_bf16 does. A row that attends nothing gets zeros; rows outside [row_begin[0], row_begin[n_seq])
+ * are left as they were. l_max >= every prefix + depth (host bound; keys at logical positions from l_max on are not
+ * attended). Keys are folded in a fixed order (blocks of 64 within a
  * span of `span` logical positions, a multiple of 64; four spans a group; the groups), so a row's result depends on
  * its query, its keys and span alone -- not on the other rows, the other sequences or the slots its ancestors
  * sit in: a verify row equals the autoregressive step at its position bit for bit.

@@ -113,8 +113,9 @@ class KVCache:
 class KVCacheQ8:
     """KV caches of ``sequences`` sequences in 8 bits: e4m3 codes and one power-of-two exponent per (slot, kv head) of
     K and of V, 2 * (head_dim + 1) bytes a slot and head against the bf16 cache's 4 * head_dim. Arrays
-    [layers, sequences, kv_heads, capacity * head_dim] (codes) and [..., capacity] (exponents), capacity the next
-    multiple of 64, in the operand order documented at SsdKvQ8 in the C header. head_dim 64 or 128.
+    [layers, sequences, kv_heads, capacity * head_dim] (codes) and [..., capacity] (exponents), in the operand order
+    documented at SsdKvQ8 in the C header. head_dim 64 or 128. ``capacity`` is max_length rounded up to a multiple of 64, and
+    the bound of every call: a sequence has slots [0, capacity), places outside them are outside the cache.
 
     Rows are quantised as they are written (``write``, K rotated in the same launch), every stored value is a bf16
     value, so ``read`` returns exactly what ``attend`` uses. Lengths are the caller's: rows name their sequence and slot.
@@ -164,9 +165,9 @@ class KVCacheQ8:
               interleaved: bool = False, q: Optional[torch.Tensor] = None,
               q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
         """Rows k, v [M, kv_heads * head_dim] (any row stride) into layer ``i`` at (seq[m], slot[m]) (int32 on the device,
-        all places different; rows outside the cache are not written). ``rope``: (cos, sin) tables of
-        ``models.llama.rope_tables_f32``, K rotated to ``pos`` before it is quantised; with ``q`` [M, heads * head_dim]
-        its rows are rotated too and returned (in ``q_out`` if given, which may be ``q``)."""
+        all places different; rows at slots outside [0, capacity) or of no sequence are not written). ``rope``: (cos, sin)
+        tables of ``models.llama.rope_tables_f32``, K rotated to ``pos`` before it is quantised; with ``q``
+        [M, heads * head_dim] its rows are rotated too and returned (in ``q_out`` if given, which may be ``q``)."""
         heads = 0 if q is None else self._heads(q)
         return ops.kv_q8_write(self._layers[i], k, v, k.shape[0], seq, slot, rope, pos, interleaved, q, heads, q_out)
 
@@ -178,7 +179,7 @@ class KVCacheQ8:
 
     def load(self, i: int, cache: KVCache, length: int, seq: int = 0, start: int = 0) -> None:
         """Slots [start, length) of a bf16 cache's layer ``i`` (a prompt's, after its prefill) into sequence ``seq``."""
-        if not 0 <= start <= length <= self.max_length or not 0 <= seq < self.sequences:
+        if not 0 <= start <= length <= self.capacity or not 0 <= seq < self.sequences:
             raise ValueError(f"KVCacheQ8.load: slots [{start}, {length}) or sequence {seq} outside the cache")
         if (cache.kv_heads, cache.head_dim) != (self.kv_heads, self.head_dim) or length > cache.max_length:
             raise ValueError(f"KVCacheQ8.load: {length} slots of {self.kv_heads} heads of {self.head_dim} from a cache with "
@@ -188,7 +189,8 @@ class KVCacheQ8:
         self.write(i, k, v, torch.full_like(slot, seq), slot)
 
     def read(self, i: int, seq: torch.Tensor, slot: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-        """K, V [M, kv_heads * head_dim] bf16 of layer ``i`` at (seq[m], slot[m]); zeros for places outside the cache."""
+        """K, V [M, kv_heads * head_dim] bf16 of layer ``i`` at (seq[m], slot[m]); zeros for slots outside [0, capacity) and
+        for no sequence."""
         return ops.kv_q8_read(self._layers[i], seq.numel(), seq, slot)
 
     def attend_floats(self, m: int, heads: int, l_max: int) -> int:
@@ -201,13 +203,15 @@ class KVCacheQ8:
         """Tree attention of q [M, heads * head_dim] over layer ``i``: sequence s owns rows row_begin[s] ..
         row_begin[s + 1] (at most rows_max <= 64), row t attends slots [0, prefix[t]) then anc[t, :depth[t]] of anc [M, 32]
         (a depth above 32 counts as 32); zeros for rows that attend nothing; rows of no sequence are left as ``out`` has
-        them (unset without ``out``). l_max bounds prefix + depth. ``ws``: fp32, attend_floats(M, heads, l_max) (None: allocated here)."""
+        them (unset without ``out``). l_max <= capacity bounds prefix + depth. ``ws``: fp32, attend_floats(M, heads, l_max)
+        (None: allocated here)."""
         return ops.tree_attention_q8(self._layers[i], q, q.shape[0], self._heads(q), row_begin, prefix, depth, anc, rows_max,
                                      l_max, self.span, ws, out, scale)
 
     def compact_device(self, start: torch.Tensor, src: torch.Tensor, n: torch.Tensor) -> None:
         """In every layer, sequence s's slots src[s, :n[s]] move to [start[s], start[s] + n[s]) (int32 on the device; src
-        [sequences, n_max <= 64]): the accepted paths of a verified batch, one launch."""
+        [sequences, n_max <= 64]): the accepted paths of a verified batch, one launch. Moves from or to slots outside
+        [0, capacity) are skipped."""
         if src.dim() != 2 or src.shape[0] != self.sequences:
             raise ValueError(f"src must be [{self.sequences}, n_max], got {tuple(src.shape)}")
         ops.kv_q8_compact(self._layers[0], self.num_slots, start, src, n, src.shape[1])

@@ -711,3 +711,27 @@ def test_rebuilt_caches_keep_no_device_memory():
         use()
     gc.collect(), torch.cuda.synchronize()
     assert torch.cuda.memory_allocated() <= held
+
+
+def test_slots_up_to_the_capacity_exist():
+    """max_length 200: 256 slots are written, read, loaded, attended and moved into; 256 and 257 are not there."""
+    from ssd.engine.kv_cache import KVCache
+
+    kv, hd, heads = 2, 64, 4
+    cache = _cache(1, 200, kv, hd, 2, 64)
+    x = torch.randn(5, kv * hd, generator=_gen(1)).to(BF16)
+    at = _i32([199, 200, 255, 256, 257])
+    cache.write(0, x.to(DEV), x.to(DEV), torch.ones_like(at), at)
+    for got in cache.read(0, torch.ones_like(at), at):
+        assert _same(got[:3].cpu(), ref.stored(x[:3].float().view(3, kv, hd)).flatten(1)) and not got[3:].any()
+    bf = KVCache(1, 256, kv, hd, DEV)
+    k, v = (torch.randn(1, kv, 256, hd, generator=_gen(2 + i)).to(BF16).to(DEV) for i in range(2))
+    bf.update(0, k, v)
+    cache.load(0, bf, 256)
+    every = torch.arange(256, dtype=torch.int32, device=DEV)
+    vals = [t.cpu().view(256, kv, hd).transpose(0, 1)[None].expand(2, -1, -1, -1) for t in cache.read(0, torch.zeros_like(every), every)]
+    assert _same(vals[0][0], ref.stored(k[0].float().cpu())) and _same(vals[1][0], ref.stored(v[0].float().cpu()))
+    _check_attend(cache, [[(256, []), (250, [255]), (0, [200])], []], heads, 5, vals)
+    cache.compact_device(_i32([254, 0]), _i32([[3, 4, 5], [0, 0, 0]]), _i32([3, 0]))
+    moved = cache.read(0, torch.zeros_like(every), every)[0].cpu().view(256, kv, hd).transpose(0, 1)
+    assert torch.equal(moved[:, 254:], vals[0][0][:, 3:5]) and torch.equal(moved[:, :254], vals[0][0][:, :254])

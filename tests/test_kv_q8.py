@@ -456,3 +456,19 @@ def test_rope_tables_yarn_inside_the_ramp(rot, theta, context, fast, slow, trunc
         want = math.sin(w * (1 - t) + w / f * t)  # position 1
         assert abs(float(sin[1, d]) - want) <= abs(want) * (2 ** -24 + 2 ** -40), d  # one rounding; the doubles' own far below
     assert inside >= 2  # the shortest ramp, 10.05 to 12.46, holds dims 11 and 12
+
+
+def test_a_prompt_may_fill_the_capacity(monkeypatch):
+    """Every slot of the capacity exists for write, read, attend and compaction, and for load alike."""
+    from ssd.engine.kv_cache import KVCache, KVCacheQ8
+
+    _calls_without_a_gpu(monkeypatch)
+    cache, full = KVCacheQ8(1, 200, 2, 64, "cpu"), KVCache(1, 300, 2, 64, "cpu")
+    assert cache.capacity == 256
+    written = []
+    monkeypatch.setattr(cache, "write", lambda i, k, v, seq, slot: written.append(slot.tolist()))
+    cache.load(0, full, 256, start=190)
+    assert written == [list(range(190, 256))]
+    for args in ((257,), (10, 0, 11), (10, 1), (10, 0, -1)):
+        with pytest.raises(ValueError, match="load"):
+            cache.load(0, full, *args)
