@@ -735,3 +735,105 @@ def test_slots_up_to_the_capacity_exist():
     cache.compact_device(_i32([254, 0]), _i32([[3, 4, 5], [0, 0, 0]]), _i32([3, 0]))
     moved = cache.read(0, torch.zeros_like(every), every)[0].cpu().view(256, kv, hd).transpose(0, 1)
     assert torch.equal(moved[:, 254:], vals[0][0][:, 3:5]) and torch.equal(moved[:, :254], vals[0][0][:, :254])
+
+
+@pytest.mark.parametrize("hd,kv,heads,interleaved,rot", [(128, 8, 32, False, 128), (128, 8, 1, True, 64), (64, 8, 6, False, 32),
+                                                         (64, 8, 32, True, 64), (128, 8, 6, False, 96)])
+@pytest.mark.parametrize("scattered", [False, True])
+def test_long_rotated_writes(hd, kv, heads, interleaved, rot, scattered):
+    """Calls of 6144 (row, kv head) pairs and more take four rows and four q heads a unit: a prompt's consecutive slots from an odd
+    one on, and rows at any place with some outside the cache; exactly the definition, and nothing else written."""
+    from ssd.models.llama import rope_tables_f32
+
+    rows, seqs, first = 803, 2, 37
+    g = _gen(hd + heads + scattered)
+    x = (torch.randn(rows, (heads + 2 * kv) * hd, generator=g) * torch.logspace(-2, 2, hd).repeat(heads + 2 * kv)).to(BF16)
+    q, k, v = x[:, :heads * hd], x[:, heads * hd:(heads + kv) * hd], x[:, (heads + kv) * hd:]
+    cache = _cache(1, 900, kv, hd, seqs)
+    cap = cache.capacity
+    if scattered:
+        places = torch.randperm(seqs * cap, generator=g)[:rows]
+        seq, slot = (places // cap).int(), (places % cap).int()
+        for i, (s, t) in enumerate(((-1, 3), (seqs, 4), (0, -1), (1, cap))):
+            seq[200 * i + i], slot[200 * i + i] = s, t
+    else:
+        seq, slot = torch.ones(rows, dtype=torch.int32), torch.arange(first, first + rows, dtype=torch.int32)
+    pos = torch.randint(-2, 4100, (rows,), generator=g, dtype=torch.int32)
+    cos, sin = rope_tables_f32(4096, rot, 500000.0, "cpu")
+    for t in (cache.k, cache.v, cache.k_exp, cache.v_exp):
+        t.fill_(93)
+    xd = x.to(DEV)
+    qd, kd, vd = xd[:, :heads * hd], xd[:, heads * hd:(heads + kv) * hd], xd[:, (heads + kv) * hd:]
+    got_q = cache.write(0, kd, vd, seq.to(DEV), slot.to(DEV), rope=(cos.to(DEV), sin.to(DEV)), pos=pos.to(DEV), interleaved=interleaved, q=qd)
+    assert _same(got_q.cpu(), _rot32(q, cos, sin, pos, interleaved, hd).to(BF16).flatten(1))
+    there = (seq >= 0) & (seq < seqs) & (slot >= 0) & (slot < cap)
+    assert int(there.sum()) == rows - 4 * scattered
+    k2, v2 = (t.cpu() for t in cache.read(0, seq.to(DEV), slot.to(DEV)))
+    assert _same(k2[there], ref.stored(_rot32(k, cos, sin, pos, interleaved, hd)).flatten(1)[there])
+    assert _same(v2[there], ref.stored(v.float().view(rows, kv, hd)).flatten(1)[there])
+    assert not k2[~there].any() and not v2[~there].any()
+    # the other slots' bytes are as they were, codes and exponents
+    every = torch.zeros(seqs, cap, dtype=torch.bool)
+    every[seq[there].long(), slot[there].long()] = True
+    at = torch.tensor([ref.x_offset(s) for s in range(cap)])
+    for t in (cache.k_exp, cache.v_exp):
+        assert (t[0].cpu()[:, :, at][~every[:, None].expand(-1, kv, -1)] == 93).all()
+    for t, off in ((cache.k, ref.k_offset), (cache.v, ref.v_offset)):
+        at_d = torch.tensor([[off(s, d, hd) for d in (0, 31, hd - 1)] for s in range(cap)])
+        assert (t[0].cpu()[:, :, at_d][~every[:, None, :, None].expand(-1, kv, -1, 3)] == 93).all()
+
+
+@pytest.mark.parametrize("hd,heads,interleaved,in_place", [(128, 1, False, False), (64, 6, True, True), (64, 3, False, True), (128, 5, True, False)])
+def test_rope_of_many_rows(hd, heads, interleaved, in_place):
+    """6144 rows and more: four heads of a row a unit, whatever the head count."""
+    from ssd import ops
+    from ssd.models.llama import rope_tables_f32
+
+    rows, g = 6147, _gen(heads)
+    x = torch.randn(rows, heads * hd + 8, generator=g).to(BF16)
+    pos = torch.randint(-5, 9000, (rows,), generator=g, dtype=torch.int32)
+    cos, sin = rope_tables_f32(8192, hd // 2, 1e4, "cpu")
+    xd = x.to(DEV)
+    out = xd if in_place else torch.zeros_like(xd)
+    ops.rope(xd, rows, heads, hd, (cos.to(DEV), sin.to(DEV)), pos.to(DEV), out, interleaved)
+    assert torch.equal(out[:, :heads * hd].cpu(), _rot32(x[:, :heads * hd], cos, sin, pos, interleaved, hd).to(BF16).flatten(1))
+    assert torch.equal(out[:, heads * hd:].cpu(), x[:, heads * hd:] if in_place else torch.zeros(rows, 8, dtype=BF16))
+
+
+@pytest.mark.parametrize("hd,heads,kv", [(128, 4, 1), (64, 4, 2)])
+@pytest.mark.parametrize("n", [16385, 16449, 33100])
+def test_attend_more_groups_than_lanes(hd, heads, kv, n):
+    """A group is 256 keys at a span of 64: past 64 of them the sum of the groups takes further turns (65, 65 and 130 here)."""
+    cache = _cache(1, 33280, kv, hd, 1, 64)
+    vals = _fill(cache, n)
+    rows = _tree(n, n + 2, 4, _gen(n)) + [(16384, []), (16380, [n + 1, n]), (0, [])]
+    got = _check_attend(cache, [rows], heads, n, vals)
+    assert torch.equal(_check_attend(cache, [rows], heads, n, vals, l_max=33280), got)
+
+
+def test_the_attention_inside_a_round():
+    """What a round's attention returns, against the definition over the cache as the round's write leaves it, and its bits
+    against the same call outside a round."""
+    heads, B, K, kv, hd, length = 8, 5, 4, 2, 64, 200
+    caches = [_cache(1, length + 32, kv, hd, B, 128) for _ in range(2)]
+    for c in caches:
+        _fill(c, 30)
+    st = _round_state(caches[0], 40, heads, B, K, length)
+    q, out, *_ = _round(caches[0], st)
+    other = caches[1]
+    assert torch.equal(other.write(0, st["k"], st["v"], st["seq"], st["slot"], rope=st["rope"], pos=st["slot"], q=st["q"]), q)
+    slots = torch.arange(other.capacity, dtype=torch.int32, device=DEV)
+    vals = [other.read(0, torch.full_like(slots, s), slots) for s in range(B)]
+    kk, vv = (torch.stack([x[i].cpu().view(-1, kv, hd).transpose(0, 1) for x in vals]) for i in range(2))
+    tab, begin, prefix, depth, anc = _table(st["rows"])
+    want, mag = ref.tree_attention(q.cpu().view(-1, heads, hd), kk, vv, begin, prefix, depth, anc)
+    assert ((out.cpu().view(-1, heads, hd).double() - want).abs() <= _tolerance(want, mag)).all()
+    assert torch.equal(other.attend(0, q, *tab, K + 1, st["l_max"]), out)
+
+
+def test_places_of_no_sequence_read_zeros():
+    cache = _cache(1, 64, 2, 64, 2)
+    _fill(cache, 6)
+    for s, t in ((-1, 5), (2, 5), (1 << 30, 0), (0, -1), (1, 64), (-(1 << 31), -(1 << 31))):
+        k, v = cache.read(0, _i32([s, 1]), _i32([t, 3]))
+        assert not k[0].any() and not v[0].any() and k[1].any() and v[1].any()
