@@ -260,7 +260,8 @@ int ssd_kv_q8_compact(const SsdKvQ8* cache, int layers, const int32_t* start, co
  * span of `span` logical positions, a multiple of 64; four spans a group; the groups), so a row's result depends on
  * its query, its keys and span alone -- not on the other rows, the other sequences or the slots its ancestors
  * sit in: a verify row equals the autoregressive step at its position bit for bit.
- * heads / kv_heads any whole ratio; scale > 0; V rows beyond 2^100 may overflow their sums. ws:
+ * heads / kv_heads any whole ratio; scale > 0; V rows beyond 2^100 may overflow their sums, and those at the least
+ * exponent (zeros, or below 2^-91) do not count where their weight is below 2^-26 of the largest of their span. ws:
  * ssd_attn_q8_ws_floats(...) floats, 16-byte aligned, no clearing needed; calls that overlap in time must not share it. */
 int64_t ssd_attn_q8_ws_floats(int M, int heads, int head_dim, int64_t l_max, int span);
 int ssd_tree_attention_q8(const SsdKvQ8* cache, const uint16_t* q, int64_t ldq, int M, int heads, const int32_t* row_begin,

@@ -12,11 +12,14 @@
 // with K's exponents as its scale); V's exponents multiply the probabilities before those are rounded to bf16
 // (exact), so that rounding -- 2^-8 of a weight at most -- is the only one below fp32. l is summed by the MFMA too, from
 // the rounded probabilities (an A operand of 2^-(V exponent)), so the weights O is made of add up to l exactly.
+// A product below 2^-126 is 0: at the least V exponent, 2^-100 (a row of zeros, or none above 2^-91), a key whose weight
+// is below 2^-26 of its span's reference does not count in l, at most span * 2^-26 of it (2^-17 at spans of up to 512).
 //
 // What bounds it, 8 kv heads of 128 (us, both launches): one row of 32 sequences at up to 8192 keys 82 for 410 MB, 5.0 TB/s, and
-// one row at 131000 keys 49 for 270 MB (43 the fold, 6.3 TB/s): bytes. 25 rows of 64 heads at 16384 keys 35 for 13.4
-// GFLOP: the VALU work of a score (conversion once per two tiles, maximum, exp2, packing) beside its MFMAs. 25 rows of 32
-// heads at 4096 keys 15 and 12 trees of up to 9 rows at 1900 24: the chains of a workgroup (rows, prefixes, ancestors,
+// one row at 131000 keys 47 for 270 MB (41 the fold, 6.5 TB/s): bytes. 25 rows of 64 heads at 16384 keys 32 for 13.4
+// GFLOP, 31 of them the fold: of the SIMDs' cycles VALU work (conversion once per two tiles, maximum, exp2, packing) takes 43 %
+// and MFMAs 21 %, and a CU has waves 73 % of the time, since 648 workgroups on 512 places take a second turn. 25 rows of 32
+// heads at 4096 keys 14 and 12 trees of up to 9 rows at 1900 24: the chains of a workgroup (rows, prefixes, ancestors,
 // keys, then one block after the other) at two waves a SIMD, which 248 VGPRs allow, and the second launch. One row at
 // 512 keys 5.5: a launch and that chain once.
 #include "kv_q8.h"
@@ -715,8 +718,8 @@ struct alignas(16) Q8ShortLds {
   Q8Codes<HD> codes;
 };
 
-// Heads of 64 with one team: 128 VGPRs and four workgroups a CU, 20 x 9 rows at 200 keys 13.7 -> 10.3 us, 40 x 8 at 400
-// 27 -> 19.6. Heads of 128 spill below 168 and are slower so.
+// Heads of 64 with one team: 128 VGPRs and four workgroups a CU, against two 20 x 9 rows at 200 keys 12.8 -> 11.2 us, 40 x 8
+// at 400 22.1 -> 20.4. Heads of 128 spill below 168 and are slower so.
 template <int HD, int TEAMS>
 __global__ __launch_bounds__(256 * TEAMS, TEAMS == 4 || (TEAMS == 1 && HD == 64) ? 4 : 2) void q8_short_kernel(AttnQ8Args a,
                                                                                                          int rows_max) {
@@ -794,7 +797,8 @@ static int launch_attn_q8(AttnQ8Args a, int rows_max, hipStream_t stream) {
   const int64_t units = (int64_t)a.n_seq * a.n_grps * a.kv, shared = (units + 7) / 8 * 8 * a.sets;
   // A row a workgroup while all of those are resident at once, each on a CU of its own; then as many rows as fill a
   // tile, since the spans they attend together are folded once. us, one / four rows: 25 rows of one sequence, prefixes
-  // 4097, 4060, 4000, 3900: 14.1 / 14.3, 14.9 / 16.4, 14.3 / 15.5, 14.1 / 15.4; 12 trees of up to 9 rows 30.4 / 26.2.
+  // 4097, 4060, 4000, 3900: 16.8 / 17.6, 15.8 / 18.0, 14.9 / 16.8, 15.9 / 18.6; 12 trees of 9 rows at 1900 keys 33 / 29, 4 of
+  // them 17.8 / 16.3.
   a.own_rows = rows <= 256 ? 1 : std::min(4, std::max(1, 16 / a.rep));
   const int64_t own_units = ((int64_t)a.n_seq * a.kv + 7) / 8 * 8, own = own_units * ((rows_max + a.own_rows - 1) / a.own_rows);
   if (grid_too_large(shared + own, 256) || grid_too_large(rows, 256) || grid_too_large((int64_t)a.M * a.heads, 256))
@@ -805,14 +809,17 @@ static int launch_attn_q8(AttnQ8Args a, int rows_max, hipStream_t stream) {
     return check_launch("attn_q8_short");
   };
   // One group: four rows a workgroup once a row each would be more than are resident at once. us at 8 kv heads, a row /
-  // four: heads of 128, 6 x 9 rows at 98 keys 6.6 / 10.2, 40 x 2 at 60 8.6 / 8.0, 13 x 9 at 98 11.4 / 11.4, 20 x 8 at 60
-  // 14.7 / 10.4, 40 x 8 at 60 24.7 / 15.4, 12 x 25 at 450 27.4 / 20.1; heads of 64, 20 x 9 at 200 10.4 / 9.5, 40 x 25 at 200
-  // 33.6 / 24.2. With two rows (rep 8), 20 x 9 at 100, it is 16.7 / 18.0.
+  // four: heads of 128, 6 x 9 rows at 98 keys 6.7 / 10.0, 40 x 2 at 60 9.0 / 8.5, 13 x 9 at 98 11.9 / 10.3, 20 x 8 at 60
+  // 15.3 / 10.6, 40 x 8 at 60 26 / 18, 12 x 25 at 450 41 / 26; heads of 64, 20 x 9 at 200 11.4 / 9.6, 40 x 25 at 200
+  // 49 / 32. With two rows (rep 8), 20 x 9 at 100, it is 17.0 / 17.0.
   if (a.n_grps == 1 && rows > 512 && a.own_rows == 4 && rows_max > 1) {
     SSD_LAUNCH((q8_short_rows_kernel<HD>), dim3((unsigned)own), dim3(256), 0, stream, a);
     return check_launch("attn_q8_short_rows");
   }
   if (a.n_grps == 1) return one_launch(integral_constant<int, 1>());
+  // Two to four groups, us in two launches / in one: a row of heads of 128 at 700 keys 9.2 / 7.5, 4 x 9 rows 13.9 / 17.4, 7 x 9
+  // 15.9 / 17.4, 8 x 9 17.3 / 25; of heads of 64 at 400 keys 8.1 / 4.9, 4 x 9 11.4 / 9.8, 7 x 9 12.1 / 10.6, 16 x 9 14.5 / 24, at
+  // 900 keys 8.2 / 6.9, 3 x 9 10.4 / 8.7, 6 x 9 12.2 / 15.6. (With heads of 128 the border lies below these 512 rows.)
   if (a.n_grps == 2 && rows <= 512) return one_launch(integral_constant<int, 2>());
   if constexpr (HD == 64)
     if (a.n_grps <= 4 && rows <= 256) return one_launch(integral_constant<int, 4>());
@@ -820,8 +827,8 @@ static int launch_attn_q8(AttnQ8Args a, int rows_max, hipStream_t stream) {
   else SSD_LAUNCH((q8_fold_kernel<HD, 2>), dim3((unsigned)(own + shared)), dim3(256), 0, stream, a, (int)own);
   if (int rc = check_launch("attn_q8_fold")) return rc;
   // Up to eight groups: lanes of several (row, head) pairs a workgroup. us of both launches, a workgroup a pair / lanes: 12 trees of
-  // up to 9 rows, 4 groups 25.7 / 23.7; 16 of 32 rows, 3 groups 50.3 / 41.6; one row, 8 groups 9.3 / 9.2; a tree of 25 rows,
-  // 6 groups 13.6 / 13.1. With 9 and 11 groups it would be 14.7 / 15.4 and 17.4 / 18.3.
+  // 9 rows, 4 groups 32 / 29; 16 of 32 rows, 3 groups 71 / 58; one row, 8 groups 10.0 / 10.0; a tree of 25 rows,
+  // 6 groups 15.1 / 14.5. With 9 and 11 groups it would be 16.2 / 16.9 and 18.2 / 19.3.
   const unsigned few = (unsigned)(((int64_t)a.M * a.heads + 1024 / HD - 1) / (1024 / HD));
   if (a.n_grps <= 4) SSD_LAUNCH((q8_combine_few_kernel<HD, 4>), dim3(few), dim3(256), 0, stream, a);
   else if (a.n_grps <= 8) SSD_LAUNCH((q8_combine_few_kernel<HD, 8>), dim3(few), dim3(256), 0, stream, a);

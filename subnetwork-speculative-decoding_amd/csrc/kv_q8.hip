@@ -440,8 +440,10 @@ static int by_head_dim(int hd, F f) {
 static int64_t row_units(int M, int r) { return r == 1 ? M : ((int64_t)M + 3) / 4 + 1; }
 // From this many (row, kv head) pairs on a unit takes four rows: below, more units and less code are worth more than
 // wider accesses. us, one row a unit / four, 8 kv heads and 32 q heads of 128: rotated and written, consecutive slots, 512
-// rows 7.0 / 6.8, 1024 11.9 / 9.1, 4096 36.5 / 22.0 (scattered slots, 1024 rows 12.7 / 12.7); read 1024 rows 5.1 / 6.6, 2048 7.9 /
-// 7.7, 4096 15.0 / 10.2.
+// rows 6.9 / 6.7, 768 9.2 / 7.7, 1024 11.9 / 8.6, 4096 37 / 22 (scattered slots, 768 rows 10.2 / 12.5, 1024 12.7 / 13.7, 4096 37 / 39:
+// a prompt's case decides); read 512 rows 3.7 / 4.2, 1024 4.9 / 5.0, 2048 7.7 / 6.0, 4096 14.6 / 8.5. Rotation alone has no kv
+// heads and counts its rows: 32 heads of 128, 1024 rows 5.0 / 4.9, 4096 14.8 / 13.0, 8192 25.0 / 23.0; 4096 rows of one
+// head 2.6 / 3.3.
 constexpr int64_t Q8_WRITE_QUADS = 6144, Q8_READ_QUADS = 20480;
 
 template <int HD, int MODE>

@@ -151,10 +151,10 @@ class KVCacheQ8:
     @staticmethod
     def default_span(capacity: int) -> int:
         """Keys of a span (one wave's work in turn; four spans leave one record): short ones for latency, long ones for
-        fewer records. us at 64 / 128 / 256 / 512 / 1024 keys, 32 heads on 8 kv heads of 128, one row: 4096 keys 9.3 / 9.0 /
-        10.0 / 14.0 / 19.9, 8100 9.4 / 9.4 / 11.2 / 15.1 / 30.6, 16384 13.9 / 11.6 / 12.2 / 16.3 / 25.8, 33000 24.3 / 23.3 / 20.4 / 19.4 /
-        27.0; 25 rows: 18.8 / 14.8 / 15.8 / 18.7 / 22.2, 24.6 / 21.3 / 18.9 / 25.3 / 33.6, 38.7 / 30.4 / 26.3 / 23.4 / 32.1, 64.9 / 47.4 /
-        40.5 / 36.8 / 36.2. Caches that end with a few blocks: 13 trees of 9 rows at 98 keys 11.7 / 14.0 at 64 / 128."""
+        fewer records. us at 64 / 128 / 256 / 512 / 1024 keys, 32 heads on 8 kv heads of 128, one row: 4096 keys 7.9 / 8.9 /
+        10.3 / 18.5 / 20.7, 8100 10.3 / 10.4 / 12.0 / 16.5 / 32, 16384 11.6 / 10.3 / 12.4 / 17.0 / 27, 33000 25 / 24 / 20.4 / 19.9 /
+        29; 25 rows: 19.6 / 15.6 / 16.1 / 19.0 / 24, 25 / 21.5 / 19.3 / 27 / 37, 38 / 30 / 27 / 24 / 33, 62 / 46 / 40 / 37 / 37. Caches that end
+        with a few blocks: 13 trees of 9 rows at 98 keys 10.3 / 12.3 at 64 / 128."""
         return 64 if capacity <= 256 else 128 if capacity < 6144 else 256 if capacity < 16384 else 512
 
     def layer(self, i: int) -> _lib.SsdKvQ8:
