@@ -269,6 +269,88 @@ int ssd_tree_attention_q8(const SsdKvQ8* cache, const uint16_t* q, int64_t ldq, 
                           int span, float scale, float* ws, int64_t ws_floats, uint16_t* out, int64_t ldo,
                           hipStream_t stream);
 
+/* ---- A batch served from a paged bf16 cache. The reference keeps one contiguous cache per generation
+ * (ssd/engine/kv_cache.py:21-73) and pads its batches (ssd/data/generate_selfdistill.py:60-108); here sequences of
+ * different lengths share a pool of pages.
+ *
+ * A page is 64 slots (SSD_PAGE_SLOTS) of every kv head of one layer; k and v are each [pages][kv_heads][64 * head_dim]
+ * bf16 (16-byte aligned), 64 slots of one head in the block layout of the other bf16 caches. head_dim 64 or 128. */
+#define SSD_PAGE_SLOTS 64
+typedef struct SsdPagedKv {  /* one layer */
+  uint16_t* k;
+  uint16_t* v;
+  int32_t pages, kv_heads, head_dim;
+} SsdPagedKv;
+
+/* The sequences of a call (device int32 arrays, read when the call runs). table[s * ld_table + p]: the page of
+ * slots 64 p .. 64 p + 63 of sequence s; slots whose page is outside [0, pages) or beyond table_cols do not exist: they are
+ * not written, read as zeros and not attended. lengths[s]: slots in use, new rows included. Sequence s owns the
+ * packed rows [row_begin[s], row_begin[s + 1]) of the call's operands (increasing, at most rows_max each; NULL with
+ * rows_max <= 1: row s); row i of its n sits at slot lengths[s] - n + i, rows before slot 0 nowhere. Rows of no sequence are
+ * left as they were. */
+typedef struct SsdPagedBatch {
+  const int32_t* table;
+  int64_t ld_table;
+  int32_t table_cols, n_seq;
+  const int32_t* row_begin;
+  int32_t* lengths;
+  int32_t rows_max;
+} SsdPagedBatch;
+
+/* Rows k, v [M][kv_heads * head_dim] into their slots, and back (zeros where there is none). Pages that rows of one call are
+ * written to belong to one sequence each. M = 0 does nothing. The paged counterpart of KVCache.update
+ * (ssd/engine/kv_cache.py:32-43). */
+int ssd_paged_write_bf16(const SsdPagedKv* cache, const SsdPagedBatch* batch, const uint16_t* k, int64_t ldk, const uint16_t* v,
+                         int64_t ldv, int M, hipStream_t stream);
+int ssd_paged_read_bf16(const SsdPagedKv* cache, const SsdPagedBatch* batch, int M, uint16_t* k, int64_t ldk, uint16_t* v,
+                        int64_t ldv, hipStream_t stream);
+
+/* Attention of the batch's rows q [M][heads * head_dim]: row i of a sequence attends slots [0, lengths - n + i], itself the
+ * last (the causal mask of ssd/models/subnetwork_draft.py:165-191 for a chunk behind a cache). Zeros for rows that attend
+ * nothing. l_max (1 .. 64 * table_cols): slots from there on are not attended. heads / kv_heads any whole ratio; scale > 0.
+ * A V value that is not finite reaches the rows that attend its slot and no other (where some rows attend only part of its
+ * 64-slot block it makes their outputs NaN).
+ *
+ * ssd_paged_attention_bf16 is for few rows a sequence: the length is cut into groups of 4 * span slots (span a multiple of 64 up
+ * to 4096), folded by a workgroup each and added up in a fixed order, so a row's result depends on its query, its keys
+ * and span alone. ws: ssd_paged_attn_ws_floats(...) floats, 16-byte aligned, no clearing needed; calls that overlap in
+ * time must not share it. With weights (may be NULL): for every slot t in use of sequence s and kv head h,
+ * weights[s * ldw_seq + h * ldw + t] becomes decay * itself + the sum over the sequence's rows and h's query heads of the
+ * softmax weight of t (decay in [0, 1]; 0: the old value is not read); the rest stays. Weights are summed in a
+ * fixed order.
+ * ssd_paged_prompt_bf16 is for many rows a sequence; its results depend on a row's query and keys and on how many
+ * rows the call has (which decides the tile), and differ from the other's by rounding. */
+int64_t ssd_paged_attn_ws_floats(int M, int heads, int head_dim, int64_t l_max, int span, int weights);
+int ssd_paged_attention_bf16(const SsdPagedKv* cache, const SsdPagedBatch* batch, const uint16_t* q, int64_t ldq, int M, int heads,
+                             int l_max, int span, float scale, float* ws, int64_t ws_floats, float* weights, int64_t ldw_seq,
+                             int64_t ldw, float decay, uint16_t* out, int64_t ldo, hipStream_t stream);
+int ssd_paged_prompt_bf16(const SsdPagedKv* cache, const SsdPagedBatch* batch, const uint16_t* q, int64_t ldq, int M, int heads,
+                          int l_max, float scale, uint16_t* out, int64_t ldo, hipStream_t stream);
+
+/* Eviction by received weight, in `layers` layers (cache: the first; layer_elems elements apart): of every (layer, sequence, kv head)
+ * with more than `keep` slots stay the first `first`, the last `recent`, and of those between as many as complete
+ * `keep`, those of the largest weight (equal ones: the lowest slots; NaN below every number); of shorter ones all. They move, in their
+ * order, to slots 0, 1, ... of the pages in after->table, which must be pages that `batch` does not use, and
+ * after->lengths becomes min(lengths, keep) (it may be batch->lengths itself). weights: [layers][n_seq][kv_heads] rows of cap
+ * floats, ldw apart, cap >= lengths (slots beyond it count as not there); out_weights, rows alike: the kept ones, then
+ * zeros. kept: [layers][n_seq][kv_heads][keep] int32, the slots they came from, then -1. The row_begin and rows_max of both
+ * batches are not used. No counterpart in the reference, whose caches only grow. */
+int ssd_paged_evict(const SsdPagedKv* cache, int layers, int64_t layer_elems, const SsdPagedBatch* batch, const SsdPagedBatch* after,
+                    const float* weights, int64_t ldw, int cap, int keep, int recent, int first, float* out_weights, int32_t* kept,
+                    hipStream_t stream);
+
+/* Of each row of logits (dtype 0 bf16, 1 fp16, 2 fp32; V columns, rows ld elements apart, aligned to their type): logprobs,
+ * the log softmax at tokens[m] (int32, or int64 with tokens64); entropy, in nats; rank, the number of columns that rank before the
+ * token (larger, or equal and lower); and the `top` <= 32 largest columns, best first (equal ones: the lowest first), with
+ * their log softmax: top_ids, top_logprobs [M][top]. A token outside [0, V) gives logprob 0 and rank -1. Columns of -inf have no mass;
+ * a row with a NaN or +inf, or without any mass, has NaN logprobs and entropy, and with a NaN rank -1. ws:
+ * ssd_token_logprobs_ws_bytes(...) bytes, 16-byte aligned, not cleared (0: NULL will do). M = 0 does nothing. The values
+ * of log_softmax at ssd/engine/tree_drafter.py:129-133 for tokens that are given. */
+int64_t ssd_token_logprobs_ws_bytes(int M, int V, int dtype, int top);
+int ssd_token_logprobs(const void* logits, int dtype, int64_t ld, int M, int V, const void* tokens, int tokens64, int top, void* ws,
+                       int64_t ws_bytes, float* logprobs, float* entropy, int32_t* rank, int32_t* top_ids, float* top_logprobs,
+                       hipStream_t stream);
+
 /* ---------------------------------------------------------------- rows */
 /* HF LlamaRMSNorm / bridge RMSNorm (ssd/models/bridges.py:33-37; subnetwork_draft.py:216,245,344). */
 int ssd_rmsnorm_bf16(const uint16_t* x, int64_t ldx, int M, int D, const uint16_t* w, float eps, uint16_t* y,

@@ -1,0 +1,422 @@
+// Attention of few new rows a sequence over the paged cache (paged.h), split over the length and joined; with it, on request,
+// the weight that each cached slot has received.
+//
+// The columns of S^T = K Q^T are the (row, q head) pairs of one sequence and kv head, rows outermost, sixteen a tile. A row's keys
+// are cut into groups of 4 * span slots: a workgroup folds one group for one tile, its wave w every fourth 64-key block from the
+// w-th on, with a running reference m, sum l and output O in fp32; the four waves' states are added in LDS. Several groups leave
+// records (m, l, O) that a second launch adds up with weights from their largest m; one group is written out at once.
+// So a row's result depends on its own keys, its query and the span, not on the other rows or sequences.
+// Probabilities are rounded to bf16 as the second product's operand; l sums them before that.
+//
+// With weights the first launch leaves the scores too (fp32, 16 bytes a key and four heads against 4 hd bytes of K and V), and
+// the second, knowing every (row, head)'s final m and l, adds up 2^(s - m) / l over the rows and heads of a kv head.
+#include "paged.h"
+
+#include <algorithm>
+
+namespace ssd {
+
+constexpr int PA_WAVES = 4;
+constexpr int PA_MAX_SPAN = 4096;  // a wave's pages are one table word a lane
+
+struct PagedAttnArgs {
+  PagedBatch b;
+  PagedCache c;
+  const bf16_t* Q;
+  int64_t ldq;
+  int M, heads, rep, l_cap;  // l_cap: slots from here on are not attended
+  int span_blk, n_grps, sets, units;
+  float scale_log2;
+  float* ws_o;    // [row][head][group][HD]
+  float2* ws_ml;  // [row][head][group]: (m, l)
+  float* ws_s;    // [row][head][ld_s]: products q k
+  int64_t ld_s;
+  bf16_t* out;
+  int64_t ldo;
+  float* weights;
+  int64_t ldw_seq, ldw;
+  float decay;
+  int join_wgs, chunks;  // second launch: workgroups that join, then key chunks of a (sequence, kv head)
+};
+
+template <int HD>
+struct PagedFrags {
+  u32x4_t k[4][HD / 32];
+  u32x4_t v[HD / 16][2];
+};
+
+template <int HD>
+struct PagedState {
+  float m, l;          // reference (log2 units; -inf: nothing yet), this lane's part of the sum
+  f32x4_t o[HD / 16];  // O[column j][16 dt + 4g + e]
+};
+
+template <int HD>
+__device__ __forceinline__ void paged_load_k(PagedFrags<HD>& f, const bf16_t* K, size_t at, int lane) {
+  const bf16_t* p = K + at + lane * 8;
+#pragma unroll
+  for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+    for (int ks = 0; ks < HD / 32; ++ks) f.k[kt][ks] = *(const u32x4_t*)(p + (kt * (HD / 32) + ks) * 512);
+}
+template <int HD>
+__device__ __forceinline__ void paged_load_v(PagedFrags<HD>& f, const bf16_t* V, size_t at, int lane) {
+  const bf16_t* p = V + at + lane * 8;
+#pragma unroll
+  for (int dt = 0; dt < HD / 16; ++dt)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) f.v[dt][c] = *(const u32x4_t*)(p + (dt * 2 + c) * 512);
+}
+
+// Folds one block into the state. left: the block's keys below it are attended by this lane's column (64 or more: all); masked
+// (uniform): some column does not attend the whole block. The reference follows the maximum only when that has grown by more
+// than 2^8: probabilities up to 2^8 are as exact as those up to 1, and after the first blocks nothing is rescaled.
+template <int HD, typename TakeOut, typename Scores, typename NextK, typename NextV>
+__device__ __forceinline__ void paged_fold(PagedFrags<HD>& f, const u32x4_t (&qf)[HD / 32], int left, bool masked, float scale_log2,
+                                           int g, PagedState<HD>& st, TakeOut take_out, Scores scores, NextK next_k, NextV next_v) {
+  f32x4_t s[4];
+#pragma unroll
+  for (int kt = 0; kt < 4; ++kt) s[kt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int ks = 0; ks < HD / 32; ++ks)
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt) s[kt] = mfma16x16x32(bits_bf16x8(f.k[kt][ks]), bits_bf16x8(qf[ks]), s[kt]);
+  next_k();
+  if (masked) {
+    take_out();
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[kt][e] = paged_key(kt, g, e) < left ? s[kt][e] : -INFINITY;
+  }
+  float mx = -INFINITY;
+#pragma unroll
+  for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) mx = fmaxf(mx, s[kt][e]);
+  mx = paged_max_lanes(mx) * scale_log2;
+  scores(s);
+  const float m = mx > st.m + 8.f || st.m == -INFINITY ? mx : st.m;
+  const float ms = m == -INFINITY ? 0.f : m;  // nothing attended so far: every p is 0
+  if (__any(m != st.m)) {
+    const float alpha = __builtin_amdgcn_exp2f(st.m - ms);
+    st.l *= alpha;
+#pragma unroll
+    for (int dt = 0; dt < HD / 16; ++dt) st.o[dt] *= alpha;
+  }
+  st.m = m;
+  u32x4_t pw[2];
+#pragma unroll
+  for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+    for (int e = 0; e < 4; e += 2) {
+      const float p0 = __builtin_amdgcn_exp2f(fmaf(s[kt][e], scale_log2, -ms));
+      const float p1 = __builtin_amdgcn_exp2f(fmaf(s[kt][e + 1], scale_log2, -ms));
+      st.l += p0 + p1;
+      pw[kt >> 1][(kt & 1) * 2 + e / 2] = pack_bf16x2(p0, p1);
+    }
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+#pragma unroll
+    for (int dt = 0; dt < HD / 16; ++dt) st.o[dt] = mfma16x16x32(bits_bf16x8(f.v[dt][c]), bits_bf16x8(pw[c]), st.o[dt]);
+  next_v();
+}
+
+__device__ __forceinline__ float paged_weight(float m, float top) {
+  return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+}
+
+// The waves' states meet here.
+template <int HD>
+struct alignas(16) PagedSpans {
+  float o[PA_WAVES][16][HD + 4];
+  float m[PA_WAVES][16], l[PA_WAVES][16];
+  int first_bad[HD];  // paged_take_out's
+};
+
+// Workgroup (sequence, group, kv head, tile). The tiles of one (sequence, group, kv head) are ids 8 apart: one XCD, whose L2 they share.
+template <int HD, bool WEIGHTS>
+__global__ __launch_bounds__(256, 2) void paged_fold_kernel(PagedAttnArgs a) {
+  __shared__ PagedSpans<HD> lds;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, g = lane >> 4;
+  const int rest = blockIdx.x >> 3, set = rest % a.sets;
+  int u = rest / a.sets * 8 + (blockIdx.x & 7);
+  if (u >= a.units) return;
+  const int kvh = u % a.c.kv;
+  u /= a.c.kv;
+  const int grp = u % a.n_grps, seq = u / a.n_grps;
+  const PagedRows r = paged_rows(a.b, seq, a.M);
+  const int n_cols = r.n * a.rep, c0 = set * 16;
+  if (c0 >= n_cols) return;
+  const int last = min(c0 + 15, n_cols - 1);
+  const int lim_lo = min(r.first + c0 / a.rep, a.l_cap - 1), lim_hi = min(r.first + last / a.rep, a.l_cap - 1);
+  const int b0 = grp * PA_WAVES * a.span_blk;
+  if (a.n_grps > 1 && b0 * PAGE > lim_hi) return;  // no record: the second launch counts them as this does
+  // lane i has the page of this wave's block i
+  const int nb = lim_hi < 0 ? 0 : min(max((lim_hi / PAGE - b0 - w) / PA_WAVES + (lim_hi / PAGE - b0 - w >= 0), 0), a.span_blk);
+  const int mine = lane < nb ? paged_page(a.b, seq, b0 + w + PA_WAVES * lane, a.c.pages) : -1;
+  const int col = min(c0 + j, n_cols - 1), row = r.r0 + col / a.rep, head = kvh * a.rep + col % a.rep;
+  const int lim = min(r.first + col / a.rep, a.l_cap - 1);
+  if (threadIdx.x < HD) lds.first_bad[threadIdx.x] = INT32_MAX;
+  __syncthreads();
+  PagedState<HD> st;
+  st.m = -INFINITY, st.l = 0.f;
+#pragma unroll
+  for (int dt = 0; dt < HD / 16; ++dt) st.o[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  if (nb > 0) {
+    u32x4_t qf[HD / 32];
+#pragma unroll
+    for (int ks = 0; ks < HD / 32; ++ks) qf[ks] = *(const u32x4_t*)(a.Q + row * a.ldq + head * HD + ks * 32 + g * 8);
+    auto at = [&](int i) { return ((size_t)max(__builtin_amdgcn_readlane(mine, i), 0) * a.c.kv + kvh) * PAGE * HD; };
+    PagedFrags<HD> f;
+    paged_load_k<HD>(f, a.c.k, at(0), lane);
+    paged_load_v<HD>(f, a.c.v, at(0), lane);
+    for (int i = 0; i < nb; ++i) {
+      const int key0 = (b0 + w + PA_WAVES * i) * PAGE;
+      const bool gone = __builtin_amdgcn_readlane(mine, i) < 0;  // no such page: none of its slots is attended
+      const bool masked = gone || key0 + PAGE - 1 > lim_lo;
+      const int note = gone ? INT32_MAX - PAGE : key0;
+      auto scores = [&](const f32x4_t (&s)[4]) {
+        if constexpr (WEIGHTS) {
+          if (c0 + j >= n_cols) return;
+          float* dst = a.ws_s + ((int64_t)row * a.heads + head) * a.ld_s + key0;
+#pragma unroll
+          for (int kt = 0; kt < 4; ++kt) *(f32x4_t*)(dst + paged_key(kt, g, 0)) = s[kt];
+        }
+      };
+      auto next_k = [&] {
+        if (i + 1 < nb) paged_load_k<HD>(f, a.c.k, at(i + 1), lane);
+      };
+      auto next_v = [&] {
+        if (i + 1 < nb) paged_load_v<HD>(f, a.c.v, at(i + 1), lane);
+      };
+      auto take_out = [&] {
+#pragma unroll
+        for (int dt = 0; dt < HD / 16; ++dt)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            __builtin_amdgcn_sched_barrier(0);  // one at a time: all at once would spill
+            u32x4_t x = f.v[dt][c];
+            asm volatile("" : "+v"(x));
+            if (__any(paged_not_finite(x[0]) || paged_not_finite(x[1]) || paged_not_finite(x[2]) || paged_not_finite(x[3])))
+              f.v[dt][c] = paged_take_out(x, note + c * 32 + g * 8, &lds.first_bad[dt * 16 + j]);
+          }
+      };
+      paged_fold<HD>(f, qf, gone ? 0 : lim - key0 + 1, masked, a.scale_log2, g, st, take_out, scores, next_k, next_v);
+    }
+  }
+  st.l = paged_sum_lanes(st.l);
+  lds.m[w][j] = st.m;  // the four lanes of column j write the same values
+  lds.l[w][j] = st.l;
+#pragma unroll
+  for (int dt = 0; dt < HD / 16; ++dt) *(f32x4_t*)&lds.o[w][j][dt * 16 + 4 * g] = st.o[dt];
+  __syncthreads();
+  // column rr, dims 4 dc .. + 4 of every 64
+  const int rr = threadIdx.x >> 4, dc = threadIdx.x & 15;
+  if (c0 + rr >= n_cols) return;
+  float top = -INFINITY, l = 0.f, wgt[PA_WAVES];
+#pragma unroll
+  for (int i = 0; i < PA_WAVES; ++i) top = fmaxf(top, lds.m[i][rr]);
+#pragma unroll
+  for (int i = 0; i < PA_WAVES; ++i) {
+    wgt[i] = paged_weight(lds.m[i][rr], top);
+    l = fmaf(lds.l[i][rr], wgt[i], l);
+  }
+  const int64_t orow = r.r0 + (c0 + rr) / a.rep;
+  const int ohead = kvh * a.rep + (c0 + rr) % a.rep;
+  const int olim = min(r.first + (c0 + rr) / a.rep, a.l_cap - 1);
+  const int64_t rec = (orow * a.heads + ohead) * a.n_grps + grp;
+  const bool direct = a.n_grps == 1;
+#pragma unroll
+  for (int i = 0; i < HD / 64; ++i) {
+    f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int v = 0; v < PA_WAVES; ++v) {
+      const f32x4_t x = *(const f32x4_t*)&lds.o[v][rr][i * 64 + dc * 4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], wgt[v], o[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (olim >= lds.first_bad[i * 64 + dc * 4 + e]) o[e] = __uint_as_float(0x7fc00000u);
+    if (direct) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = l == 0.f ? 0.f : o[e] / l;  // NaN stays NaN
+      *(uint2*)(a.out + orow * a.ldo + ohead * HD + i * 64 + dc * 4) = make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
+    } else {
+      *(f32x4_t*)(a.ws_o + rec * HD + i * 64 + dc * 4) = o;
+    }
+  }
+  if (dc == 0 && (!direct || WEIGHTS)) a.ws_ml[rec] = make_float2(top, l);
+}
+
+// Largest reference and the sum l of a (row, head)'s records, by the lanes of a power-of-two group of LG lanes.
+__device__ __forceinline__ float2 paged_total(const float2* ml, int ng, int part, int lg) {
+  float m = -INFINITY, l = 0.f;
+  for (int i = part; i < ng; i += lg) {
+    const float2 x = ml[i];
+    const float top = fmaxf(m, x.x);
+    l = l * paged_weight(m, top) + x.y * paged_weight(x.x, top);
+    m = top;
+  }
+  for (int o = 1; o < lg; o <<= 1) {
+    const float mo = __shfl_xor(m, o), lo = __shfl_xor(l, o), top = fmaxf(m, mo);
+    l = l * paged_weight(m, top) + lo * paged_weight(mo, top);
+    m = top;
+  }
+  return make_float2(m, l);
+}
+
+// Second launch. The first join_wgs workgroups add up the records: a wave per (sequence, row, head), which takes them in order.
+// The others add the received weights of 1024 slots of a (sequence, kv head), a thread four slots.
+template <int HD, bool WEIGHTS>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int grp_keys = PA_WAVES * a.span_blk * PAGE;
+  if ((int)blockIdx.x < a.join_wgs) {
+    constexpr int V = HD / 64;  // dims a lane
+    int u = blockIdx.x * 4 + w;
+    const int h = u % a.heads;
+    u /= a.heads;
+    const int i = u % a.b.rows_max, s = u / a.b.rows_max;
+    if (s >= a.b.n_seq) return;
+    const PagedRows r = paged_rows(a.b, s, a.M);
+    if (i >= r.n) return;
+    const int64_t row = r.r0 + i;
+    const int lim = min(r.first + i, a.l_cap - 1), ng = lim < 0 ? 0 : lim / grp_keys + 1;
+    const float2* ml = a.ws_ml + (row * a.heads + h) * a.n_grps;
+    const float* o = a.ws_o + (row * a.heads + h) * a.n_grps * HD + lane * V;
+    const float2 all = paged_total(ml, ng, lane, 64);
+    float acc[V] = {};
+    for (int g0 = 0; g0 < ng; g0 += 64) {
+      const float wg = g0 + lane < ng ? paged_weight(ml[g0 + lane].x, all.x) : 0.f;
+      const int n = min(64, ng - g0);
+      for (int q = 0; q < n; q += 8) {
+        float x[8][V];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+          for (int v = 0; v < V; ++v) x[e][v] = o[(int64_t)(g0 + min(q + e, n - 1)) * HD + v];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float t = __shfl(wg, min(q + e, 63));
+#pragma unroll
+          for (int v = 0; v < V; ++v) acc[v] = q + e < n ? fmaf(x[e][v], t, acc[v]) : acc[v];
+        }
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) acc[v] = all.y == 0.f ? 0.f : acc[v] / all.y;
+    bf16_t* dst = a.out + row * a.ldo + h * HD + lane * V;
+    if constexpr (V == 2) *(uint32_t*)dst = pack_bf16x2(acc[0], acc[1]);
+    else *dst = f2bf(acc[0]);
+    return;
+  }
+  if constexpr (WEIGHTS) {
+    __shared__ float2 total[256];  // (m, 1 / l) of up to 256 (row, head) pairs
+    int u = blockIdx.x - a.join_wgs;
+    const int ch = u % a.chunks;
+    u /= a.chunks;
+    const int kvh = u % a.c.kv, s = u / a.c.kv;
+    const PagedRows r = paged_rows(a.b, s, a.M);
+    const int end = min(r.first + r.n, a.l_cap);  // slots in use
+    if (r.n == 0 || ch * 1024 >= end) return;
+    const int key = ch * 1024 + threadIdx.x * 4, pairs = r.n * a.rep;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int p0 = 0; p0 < pairs; p0 += 256) {
+      const int np = min(256, pairs - p0);
+      int lg = 64;
+      while (lg > 1 && 256 / lg < np) lg >>= 1;
+      if (p0) __syncthreads();
+      for (int p = threadIdx.x / lg; p < (np + 256 / lg - 1) / (256 / lg) * (256 / lg); p += 256 / lg) {  // whole waves stay together
+        const int pc = min(p, np - 1) + p0;
+        const int lim = min(r.first + pc / a.rep, a.l_cap - 1);
+        const float2 t = paged_total(a.ws_ml + ((int64_t)(r.r0 + pc / a.rep) * a.heads + kvh * a.rep + pc % a.rep) * a.n_grps,
+                                     lim < 0 ? 0 : lim / grp_keys + 1, threadIdx.x % lg, lg);
+        if (p < np && threadIdx.x % lg == 0) total[p] = make_float2(t.x, t.y == 0.f ? 0.f : 1.f / t.y);
+      }
+      __syncthreads();
+      if (key < end)
+        for (int p = 0; p < np; ++p) {
+          const int pc = p0 + p, lim = min(r.first + pc / a.rep, a.l_cap - 1);
+          if (key > lim) continue;
+          const f32x4_t x = *(const f32x4_t*)(a.ws_s + ((int64_t)(r.r0 + pc / a.rep) * a.heads + kvh * a.rep + pc % a.rep) * a.ld_s + key);
+          const float2 t = total[p];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (key + e <= lim && x[e] != -INFINITY) sum[e] = fmaf(__builtin_amdgcn_exp2f(fmaf(x[e], a.scale_log2, -t.x)), t.y, sum[e]);
+        }
+    }
+    float* dst = a.weights + s * a.ldw_seq + kvh * a.ldw + key;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (key + e < end) dst[e] = a.decay == 0.f ? sum[e] : fmaf(a.decay, dst[e], sum[e]);
+  }
+}
+
+static int paged_groups(int64_t l_max, int span) { return (int)((l_max + (int64_t)PA_WAVES * span - 1) / ((int64_t)PA_WAVES * span)); }
+static int64_t paged_score_ld(int64_t l_max) { return (l_max + PAGE - 1) / PAGE * PAGE; }
+
+template <int HD, bool WEIGHTS>
+static int launch_paged_attn(PagedAttnArgs a, hipStream_t stream) {
+  const int tiles = (int)(((int64_t)a.b.rows_max * a.rep + 15) / 16);
+  a.sets = tiles;
+  const int64_t units = (int64_t)a.b.n_seq * a.n_grps * a.c.kv, grid = (units + 7) / 8 * 8 * tiles;
+  const int64_t pairs = (int64_t)a.b.n_seq * a.b.rows_max * a.heads, join = a.n_grps > 1 ? (pairs + 3) / 4 : 0;
+  a.chunks = WEIGHTS ? (a.l_cap + 1023) / 1024 : 0;
+  const int64_t extra = (int64_t)a.b.n_seq * a.c.kv * a.chunks;
+  if (units > INT32_MAX || paged_grid_too_large(grid, 256) || paged_grid_too_large(join + extra, 256))
+    return set_error(SSD_ERANGE, "paged_attention: too many workgroups");
+  a.units = (int)units, a.join_wgs = (int)join;
+  SSD_LAUNCH((paged_fold_kernel<HD, WEIGHTS>), dim3((unsigned)grid), dim3(256), 0, stream, a);
+  if (int rc = check_launch("paged_attention_fold")) return rc;
+  if (join + extra == 0) return SSD_OK;
+  SSD_LAUNCH((paged_join_kernel<HD, WEIGHTS>), dim3((unsigned)(join + extra)), dim3(256), 0, stream, a);
+  return check_launch("paged_attention_join");
+}
+
+}  // namespace ssd
+
+using namespace ssd;
+
+SSD_API int64_t ssd_paged_attn_ws_floats(int M, int heads, int head_dim, int64_t l_max, int span, int weights) {
+  if (M < 0 || heads < 1 || head_dim < 1 || l_max < 1 || l_max > 1 << 30 || span < 64 || span % 64 || span > PA_MAX_SPAN) return -1;
+  const int64_t pairs = (int64_t)M * heads, g = paged_groups(l_max, span);
+  return pairs * g * (head_dim + 2) + (pairs * g * 2) % 4 + (weights ? pairs * paged_score_ld(l_max) : 0);
+}
+
+SSD_API int ssd_paged_attention_bf16(const SsdPagedKv* cache, const SsdPagedBatch* batch, const uint16_t* q, int64_t ldq, int M,
+                                     int heads, int l_max, int span, float scale, float* ws, int64_t ws_floats, float* weights,
+                                     int64_t ldw_seq, int64_t ldw, float decay, uint16_t* out, int64_t ldo, hipStream_t stream) {
+  if (int rc = paged_check(cache, batch, "paged_attention")) return rc;
+  if (M < 0 || heads < 1 || heads % cache->kv_heads)
+    return set_error(SSD_EINVAL, "paged_attention: bad M=%d heads=%d kv_heads=%d", M, heads, cache->kv_heads);
+  if (l_max < 1 || (int64_t)l_max > (int64_t)batch->table_cols * PAGE)
+    return set_error(SSD_EINVAL, "paged_attention: l_max %d outside [1, %lld]", l_max, (long long)batch->table_cols * PAGE);
+  if (!(scale > 0.f) || scale > 1e30f) return set_error(SSD_EINVAL, "paged_attention: scale must be positive, got %g", scale);
+  if (span < 64 || span % 64 || span > PA_MAX_SPAN)
+    return set_error(SSD_EINVAL, "paged_attention: span %d must be a multiple of 64 up to %d", span, PA_MAX_SPAN);
+  if (M == 0 || batch->n_seq == 0 || batch->rows_max == 0) return SSD_OK;
+  if (!q || !ws || !out) return set_error(SSD_EINVAL, "paged_attention: null pointer");
+  const int64_t cols = (int64_t)heads * cache->head_dim;
+  if (((uintptr_t)q & 15) || ldq % 8 || ldq < cols || ((uintptr_t)out & 15) || ldo % 8 || ldo < cols)
+    return set_error(SSD_EINVAL, "paged_attention: q/out rows must be 16-byte aligned with strides >= heads * head_dim");
+  if (((uintptr_t)ws & 15) || ws_floats < ssd_paged_attn_ws_floats(M, heads, cache->head_dim, l_max, span, weights != nullptr))
+    return set_error(SSD_EINVAL, "paged_attention: workspace too small or not 16-byte aligned");
+  if (weights && (ldw < l_max || ldw_seq < (int64_t)cache->kv_heads * ldw))
+    return set_error(SSD_EINVAL, "paged_attention: weights rows of %lld for l_max %d, sequences %lld apart", (long long)ldw, l_max,
+                     (long long)ldw_seq);
+  if (weights && !(decay >= 0.f && decay <= 1.f)) return set_error(SSD_EINVAL, "paged_attention: decay must be in [0, 1], got %g", decay);
+  PagedAttnArgs a{};
+  a.b = paged_batch(batch);
+  a.b.rows_max = std::min(a.b.rows_max, M);
+  a.c = PagedCache{cache->k, cache->v, cache->pages, cache->kv_heads};
+  a.Q = q, a.ldq = ldq, a.M = M, a.heads = heads, a.rep = heads / cache->kv_heads, a.l_cap = l_max;
+  a.span_blk = span / PAGE, a.n_grps = paged_groups(l_max, span), a.scale_log2 = scale * 1.4426950408889634f;
+  const int64_t recs = (int64_t)M * heads * a.n_grps;
+  a.ws_o = ws, a.ws_ml = (float2*)(ws + recs * cache->head_dim);
+  a.ws_s = ws + recs * (cache->head_dim + 2) + (recs * 2) % 4, a.ld_s = paged_score_ld(l_max);
+  a.out = out, a.ldo = ldo, a.weights = weights, a.ldw_seq = ldw_seq, a.ldw = ldw, a.decay = decay;
+  if (cache->head_dim == 64) return weights ? launch_paged_attn<64, true>(a, stream) : launch_paged_attn<64, false>(a, stream);
+  return weights ? launch_paged_attn<128, true>(a, stream) : launch_paged_attn<128, false>(a, stream);
+}

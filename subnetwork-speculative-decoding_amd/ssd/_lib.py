@@ -95,6 +95,15 @@ class SsdRope(C.Structure):
     _fields_ = [("cos", P), ("sin", P), ("rows", I64), ("rot_dim", C.c_int32), ("interleaved", C.c_int32)]
 
 
+class SsdPagedKv(C.Structure):
+    _fields_ = [("k", P), ("v", P)] + [(n, C.c_int32) for n in ("pages", "kv_heads", "head_dim")]
+
+
+class SsdPagedBatch(C.Structure):
+    _fields_ = [("table", P), ("ld_table", I64), ("table_cols", C.c_int32), ("n_seq", C.c_int32), ("row_begin", P), ("lengths", P),
+                ("rows_max", C.c_int32)]
+
+
 _PROTOS = {
     "ssd_last_error": (C.c_char_p, []),
     "ssd_abi_version": (I32, []),
@@ -123,6 +132,16 @@ _PROTOS = {
     "ssd_attn_q8_ws_floats": (I64, [I32, I32, I32, I64, I32]),
     "ssd_tree_attention_q8": (I32, [C.POINTER(SsdKvQ8), P, I64, I32, I32, P, P, P, P, I32, I32, I32, F32, P, I64, P,
                                     I64, P]),
+    "ssd_paged_write_bf16": (I32, [C.POINTER(SsdPagedKv), C.POINTER(SsdPagedBatch), P, I64, P, I64, I32, P]),
+    "ssd_paged_read_bf16": (I32, [C.POINTER(SsdPagedKv), C.POINTER(SsdPagedBatch), I32, P, I64, P, I64, P]),
+    "ssd_paged_attn_ws_floats": (I64, [I32, I32, I32, I64, I32, I32]),
+    "ssd_paged_attention_bf16": (I32, [C.POINTER(SsdPagedKv), C.POINTER(SsdPagedBatch), P, I64, I32, I32, I32, I32, F32, P, I64, P,
+                                       I64, I64, F32, P, I64, P]),
+    "ssd_paged_prompt_bf16": (I32, [C.POINTER(SsdPagedKv), C.POINTER(SsdPagedBatch), P, I64, I32, I32, I32, F32, P, I64, P]),
+    "ssd_paged_evict": (I32, [C.POINTER(SsdPagedKv), I32, I64, C.POINTER(SsdPagedBatch), C.POINTER(SsdPagedBatch), P, I64, I32, I32,
+                              I32, I32, P, P, P]),
+    "ssd_token_logprobs_ws_bytes": (I64, [I32, I32, I32, I32]),
+    "ssd_token_logprobs": (I32, [P, I32, I64, I32, I32, P, I32, I32, P, I64, P, P, P, P, P, P]),
     "ssd_rmsnorm_bf16": (I32, [P, I64, I32, I32, P, F32, P, I64, P]),
     "ssd_embed_bf16": (I32, [P, I32, P, I64, I32, P, I64, P]),
     "ssd_kv_compact_bf16": (I32, [P, P, I32, I32, I32, I64, I32, P, P, I32, P, P]),

@@ -215,3 +215,150 @@ class KVCacheQ8:
         if src.dim() != 2 or src.shape[0] != self.sequences:
             raise ValueError(f"src must be [{self.sequences}, n_max], got {tuple(src.shape)}")
         ops.kv_q8_compact(self._layers[0], self.num_slots, start, src, n, src.shape[1])
+
+
+class PagedBatch:
+    """The sequences of a call on a paged cache, on its device (all int32): ``table`` [S, columns] (unit column stride), the page
+    of slots 64 p .. 64 p + 63 of sequence s at [s, p]; ``lengths`` [S], slots in use, new rows included; ``row_begin`` [S + 1],
+    sequence s's packed rows being row_begin[s] .. row_begin[s + 1] (increasing, at most ``rows_max`` each; None: one row a
+    sequence). Row i of a sequence's n sits at slot lengths[s] - n + i. The tensors are read when a call runs: they may be
+    updated in place between calls and between replays of a graph, and the object keeps them. ``capacity``: slots the table
+    can hold."""
+
+    def __init__(self, table: torch.Tensor, lengths: torch.Tensor, row_begin: Optional[torch.Tensor] = None, rows_max: int = 1):
+        for t, name in ((table, "table"), (lengths, "lengths"), (row_begin, "row_begin")):
+            if t is not None and (not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.device.type != "cuda"
+                                  or t.device != table.device):
+                got = f"{t.dtype} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
+                raise ValueError(f"PagedBatch: {name} must be an int32 tensor on the cache's device, got {got}")
+        if table.dim() != 2 or table.shape[1] < 1 or table.shape[1] > 1 and table.stride(1) != 1:
+            raise ValueError(f"PagedBatch: table must be [S, >= 1] with unit column stride, got {tuple(table.shape)}, strides "
+                             f"{table.stride()}")
+        n, cols = table.shape
+        if lengths.shape != (n,) or not lengths.is_contiguous():
+            raise ValueError(f"PagedBatch: lengths must be [{n}] and contiguous, got {tuple(lengths.shape)}")
+        if row_begin is not None and (row_begin.shape != (n + 1,) or not row_begin.is_contiguous()):
+            raise ValueError(f"PagedBatch: row_begin must be [{n + 1}] and contiguous, got {tuple(row_begin.shape)}")
+        if rows_max < 0 or row_begin is None and rows_max > 1:
+            raise ValueError(f"PagedBatch: rows_max {rows_max} " + ("needs row_begin" if rows_max > 1 else "must not be negative"))
+        ld = table.stride(0) if n > 1 else cols
+        if ld < cols:
+            raise ValueError(f"PagedBatch: the rows of table overlap (strides {table.stride()})")
+        self.table, self.lengths, self.row_begin, self.rows_max = table, lengths, row_begin, rows_max
+        self.n_seq, self.capacity, self.device_index = n, cols * PagedKVCache.PAGE, table.get_device()
+        self.desc = _lib.SsdPagedBatch(table.data_ptr(), ld, cols, n, None if row_begin is None else row_begin.data_ptr(),
+                                       lengths.data_ptr(), rows_max)
+
+
+class PagedKVCache:
+    """KV caches of a batch of sequences in pages of 64 slots, bf16: per layer a pool of ``pages`` pages, each with every kv head's K and
+    V of its slots. A page is the same number in every layer. Which page holds what is the caller's (``PagedBatch``);
+    ``alloc`` and ``free`` keep count of the unused ones. Arrays k, v [layers, pages, kv_heads, 64 * head_dim], 64 slots of a
+    head in the block layout of csrc/common.h; head_dim 64 or 128. Calls that write (``write``, ``evict``) need pages that
+    belong to one sequence; reads and attention may share pages (a common prefix).
+
+    ``span``: slots of a wave's share of a group in ``attend`` (four a group; a multiple of 64 up to 4096), part of its arithmetic: rows agree bit
+    for bit between calls of the same span, whatever their batch. None: by the table's width (``default_span``)."""
+
+    PAGE = 64
+
+    def __init__(self, num_slots: int, pages: int, kv_heads: int, head_dim: int, device, span: Optional[int] = None):
+        if head_dim not in (64, 128):
+            raise ValueError(f"PagedKVCache: head_dim {head_dim} unsupported (64, 128)")
+        if min(num_slots, pages, kv_heads) < 1:
+            raise ValueError("PagedKVCache: layers, pages and kv_heads must be positive")
+        if span is not None and (not 64 <= span <= 4096 or span % 64):
+            raise ValueError(f"PagedKVCache: span {span} must be a multiple of 64 up to 4096")
+        self.num_slots, self.pages, self.kv_heads, self.head_dim, self.span = num_slots, pages, kv_heads, head_dim, span
+        shape = (num_slots, pages, kv_heads, self.PAGE * head_dim)
+        self.k = torch.zeros(shape, dtype=torch.bfloat16, device=device)
+        self.v = torch.zeros_like(self.k)
+        self.device = self.k.device
+        self._free = list(range(pages - 1, -1, -1))
+        self._layers = [_lib.SsdPagedKv(self.k[i].data_ptr(), self.v[i].data_ptr(), pages, kv_heads, head_dim)
+                        for i in range(num_slots)]
+        for i, d in enumerate(self._layers):  # as KVCacheQ8's
+            d.arrays, d.layers, d.device_index = (self.k, self.v), num_slots - i, self.k.get_device()
+
+    @staticmethod
+    def default_span(capacity: int) -> int:
+        """Slots of a wave's share for tables of ``capacity`` slots: short ones for latency, long ones for fewer records."""
+        return 64 if capacity <= 256 else 128 if capacity < 6144 else 256 if capacity < 16384 else 512
+
+    # ------------------------------------------------------------------ pages
+    @classmethod
+    def pages_for(cls, length: int) -> int:
+        """Pages that ``length`` slots take."""
+        return (length + cls.PAGE - 1) // cls.PAGE
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def alloc(self, n: int) -> list:
+        """``n`` unused pages; RuntimeError if there are not as many."""
+        if n < 0:
+            raise ValueError(f"PagedKVCache: cannot allocate {n} pages")
+        if n > len(self._free):
+            raise RuntimeError(f"PagedKVCache overflow: {n} pages wanted, {len(self._free)} of {self.pages} unused")
+        return [self._free.pop() for _ in range(n)]
+
+    def free(self, pages) -> None:
+        """Takes pages back; work already enqueued on them on this stream runs before what reuses them."""
+        pages = [int(p) for p in pages]
+        if any(not 0 <= p < self.pages for p in pages) or len(set(pages)) != len(pages) or not set(pages).isdisjoint(self._free):
+            raise ValueError(f"PagedKVCache: pages {pages} are not all in use")
+        self._free.extend(reversed(pages))
+
+    # ------------------------------------------------------------------ operators
+    def layer(self, i: int) -> _lib.SsdPagedKv:
+        """The descriptor of layer ``i`` for the ops that take a cache."""
+        return self._layers[i]
+
+    def _heads(self, q: torch.Tensor) -> int:
+        heads, rest = divmod(q.shape[-1], self.head_dim)
+        if rest or heads % self.kv_heads or not heads:
+            raise ValueError(f"q has {q.shape[-1]} columns, not heads of {self.head_dim} in a multiple of {self.kv_heads}")
+        return heads
+
+    def _span(self, batch: PagedBatch) -> int:
+        return self.default_span(batch.capacity) if self.span is None else self.span
+
+    def write(self, i: int, k: torch.Tensor, v: torch.Tensor, batch: PagedBatch) -> None:
+        """Rows k, v [M, kv_heads * head_dim] (any row stride) into layer ``i`` at their sequences' slots; K as it is to be attended
+        (rotated: ``ops.rope``). Rows without a slot are not written."""
+        ops.paged_write(self._layers[i], batch, k, v)
+
+    def read(self, i: int, batch: PagedBatch, m: int, k_out: Optional[torch.Tensor] = None,
+             v_out: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
+        """K, V [m, kv_heads * head_dim] of layer ``i``: the rows that ``write`` would write; zeros for rows without a slot."""
+        return ops.paged_read(self._layers[i], batch, m, k_out, v_out)
+
+    def attend_floats(self, m: int, heads: int, batch: PagedBatch, l_max: Optional[int] = None, weights: bool = False) -> int:
+        """Workspace floats of ``attend`` for ``m`` rows."""
+        return ops.paged_attn_ws_floats(m, heads, self.head_dim, batch.capacity if l_max is None else l_max, self._span(batch), weights)
+
+    def attend(self, i: int, q: torch.Tensor, batch: PagedBatch, l_max: Optional[int] = None, out: Optional[torch.Tensor] = None,
+               ws: Optional[torch.Tensor] = None, scale: Optional[float] = None, weights: Optional[torch.Tensor] = None,
+               decay: float = 1.0) -> torch.Tensor:
+        """Attention of q [M, heads * head_dim], few rows a sequence (a decode step, a drafted chain, the last rows of a prompt), over
+        layer ``i``: every row attends its sequence's slots up to its own. Zeros for rows that attend nothing. ``l_max`` (None: the
+        table's capacity) bounds the lengths: slots from there on are not attended, and a close bound saves empty
+        workgroups. ``weights`` fp32 [S, kv_heads, >= l_max]: decay * weights + the softmax weights each slot in use received from the
+        call's rows, summed over rows and a kv head's query heads (decay 0: set). ``ws``: fp32, attend_floats(...)."""
+        return ops.paged_attention(self._layers[i], batch, q, self._heads(q), l_max, self._span(batch), ws, out, scale, weights, decay)
+
+    def attend_prompt(self, i: int, q: torch.Tensor, batch: PagedBatch, l_max: Optional[int] = None,
+                      out: Optional[torch.Tensor] = None, scale: Optional[float] = None) -> torch.Tensor:
+        """The same for many rows a sequence: whole prompts or further pieces of them, packed, whose K and V have been written."""
+        return ops.paged_prompt(self._layers[i], batch, q, self._heads(q), l_max, out, scale)
+
+    def evict(self, batch: PagedBatch, after: PagedBatch, weights: torch.Tensor, keep: int, recent: int = 0, first: int = 0,
+              out_weights: Optional[torch.Tensor] = None, kept: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
+        """Cuts every sequence of ``batch`` to ``keep`` slots, in all layers, each layer and kv head by its own ``weights`` fp32
+        [layers, S, kv_heads, >= lengths]: the ``first`` and the ``recent`` last slots stay, and those of the largest weight between
+        (equal ones: the lowest). What stays moves to the pages of ``after``, which must not be pages of ``batch``, and
+        after.lengths becomes min(lengths, keep). Returns (kept [layers, S, kv_heads, keep] int32: the slots it came from, then -1;
+        the weights that moved along, then zeros)."""
+        return ops.paged_evict(self._layers[0], self.num_slots, self.k.stride(0), batch, after, weights, keep, recent, first, out_weights,
+                               kept)

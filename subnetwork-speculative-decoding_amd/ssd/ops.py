@@ -687,6 +687,167 @@ def tree_attention_q8(cache, q, m, heads, row_begin, prefix, depth, anc, rows_ma
     return out
 
 
+# ------------------------------------------------------------------ paged bf16 cache (SsdPagedKv, SsdPagedBatch)
+def _batch_dev(cache, batch) -> int:
+    """The current device, which has to be the cache's and the batch's."""
+    dev = _cache_dev(cache)
+    if batch.device_index != dev:
+        raise ValueError(f"the batch is on cuda:{batch.device_index}, the current device is cuda:{dev}")
+    return dev
+
+
+def _l_max(batch, l_max) -> int:
+    return batch.capacity if l_max is None else l_max
+
+
+def paged_write(cache, batch, k, v):
+    """Rows k, v [M, kv_heads * head_dim] into their sequences' slots (ssd_paged_write_bf16)."""
+    dev, cols, m = _batch_dev(cache, batch), cache.kv_heads * cache.head_dim, k.shape[0]
+    pk, ldk = _rows_ptr(k, "k", dev, m, cols)
+    pv, ldv = _rows_ptr(v, "v", dev, m, cols)
+    if m:
+        _lib.call("ssd_paged_write_bf16", cache, batch.desc, pk, ldk, pv, ldv, m, _stream(dev))
+
+
+def paged_read(cache, batch, m, k_out=None, v_out=None):
+    """The rows that ``batch`` names (``m`` in all), as bf16 k_out, v_out (zeros where there is no slot; rows of no
+    sequence are left as they are, unset if both are None and so made here; ssd_paged_read_bf16)."""
+    dev, cols = _batch_dev(cache, batch), cache.kv_heads * cache.head_dim
+    if k_out is None and v_out is None:
+        k_out = torch.empty((m, cols), dtype=BF16, device=batch.lengths.device)
+        v_out = torch.empty_like(k_out)
+    pk, ldk = _rows_ptr(k_out, "k_out", dev, m, cols)
+    pv, ldv = _rows_ptr(v_out, "v_out", dev, m, cols)
+    if m:
+        _lib.call("ssd_paged_read_bf16", cache, batch.desc, m, pk, ldk, pv, ldv, _stream(dev))
+    return k_out, v_out
+
+
+def paged_attn_ws_floats(m: int, heads: int, head_dim: int, l_max: int, span: int, weights: bool = False) -> int:
+    n = int(_lib.load().ssd_paged_attn_ws_floats(m, heads, head_dim, l_max, span, int(weights)))
+    if n < 0:
+        raise ValueError(f"paged_attn_ws_floats: bad m={m} heads={heads} l_max={l_max} span={span}")
+    return n
+
+
+def paged_attention(cache, batch, q, heads, l_max, span, ws=None, out=None, scale=None, weights=None, decay=1.0):
+    """Attention of few rows a sequence over the pages (ssd_paged_attention_bf16). ``weights``: fp32 [n_seq, kv_heads, >= l_max],
+    updated in place. ``ws`` (fp32, paged_attn_ws_floats(...)) and ``out`` are made here if None."""
+    dev, hd, m = _batch_dev(cache, batch), cache.head_dim, q.shape[0]
+    cols = heads * hd
+    pq, ldq = _rows_ptr(q, "q", dev, m, cols)
+    l_max = _l_max(batch, l_max)
+    if out is None:
+        out, ldo = q.new_empty((m, cols)), cols
+        po = out.data_ptr()
+    else:
+        po, ldo = _rows_ptr(out, "out", dev, m, cols)
+    pw, lds, ldw = None, 0, 0
+    if weights is not None:
+        pw = _ptr(weights, "weights", F32, dev)
+        shape = (batch.n_seq, cache.kv_heads)
+        if weights.dim() != 3 or weights.shape[:2] != shape or weights.stride(2) != 1 or weights.shape[2] < l_max:
+            raise ValueError(f"weights must be {shape} rows of at least {l_max}, contiguous each, got {tuple(weights.shape)}, strides "
+                             f"{weights.stride()}")
+        lds, ldw = weights.stride(0), weights.stride(1)
+        # the stride of a dimension of one is nobody's
+        ldw = max(ldw, weights.shape[2]) if shape[1] == 1 else ldw
+        lds = max(lds, shape[1] * ldw) if shape[0] == 1 else lds
+    if ws is None:
+        ws = torch.empty(max(paged_attn_ws_floats(m, heads, hd, l_max, span, weights is not None), 4), dtype=F32, device=q.device)
+    px = _ptr(ws, "ws", F32, dev, 1)
+    if m:
+        _lib.call("ssd_paged_attention_bf16", cache, batch.desc, pq, ldq, m, heads, l_max, span,
+                  hd ** -0.5 if scale is None else float(scale), px, ws.numel(), pw, lds, ldw, float(decay), po, ldo, _stream(dev))
+    return out
+
+
+def paged_prompt(cache, batch, q, heads, l_max, out=None, scale=None):
+    """Causal attention of many rows a sequence over the pages (ssd_paged_prompt_bf16); ``out`` is made here if None."""
+    dev, hd, m = _batch_dev(cache, batch), cache.head_dim, q.shape[0]
+    cols = heads * hd
+    pq, ldq = _rows_ptr(q, "q", dev, m, cols)
+    if out is None:
+        out, ldo = q.new_empty((m, cols)), cols
+        po = out.data_ptr()
+    else:
+        po, ldo = _rows_ptr(out, "out", dev, m, cols)
+    if m:
+        _lib.call("ssd_paged_prompt_bf16", cache, batch.desc, pq, ldq, m, heads, _l_max(batch, l_max),
+                  hd ** -0.5 if scale is None else float(scale), po, ldo, _stream(dev))
+    return out
+
+
+def paged_evict(cache, layers, layer_elems, batch, after, weights, keep, recent=0, first=0, out_weights=None, kept=None):
+    """Eviction by received weight into after's pages (ssd_paged_evict). weights: fp32 [layers, n_seq, kv_heads, cap], contiguous; kept
+    (int32 [layers, n_seq, kv_heads, keep]) and out_weights (like weights) are made here if None. Returns (kept, out_weights)."""
+    dev = _batch_dev(cache, batch)
+    _batch_dev(cache, after)
+    if layers > cache.layers:
+        raise ValueError(f"paged_evict: {layers} layers of a cache that holds {cache.layers} from this one on")
+    lead = (layers, batch.n_seq, cache.kv_heads)
+    pw = _ptr(weights, "weights", F32, dev)
+    if weights.dim() != 4 or weights.shape[:3] != lead or not weights.is_contiguous():
+        raise ValueError(f"weights must be {lead} rows, contiguous, got {tuple(weights.shape)}, strides {weights.stride()}")
+    if out_weights is None:
+        out_weights = torch.empty_like(weights)
+    if kept is None:
+        kept = torch.empty((*lead, max(keep, 0)), dtype=I32, device=weights.device)
+    cap = weights.shape[3]
+    po, pk = _ptr(out_weights, "out_weights", F32, dev), _ptr(kept, "kept", I32, dev)
+    if out_weights.shape != weights.shape or kept.shape != (*lead, keep) or not (out_weights.is_contiguous() and kept.is_contiguous()):
+        raise ValueError(f"out_weights must be like weights {tuple(weights.shape)} and kept {(*lead, keep)}, contiguous, got "
+                         f"{tuple(out_weights.shape)}, strides {out_weights.stride()}, and {tuple(kept.shape)}, strides {kept.stride()}")
+    lo, hi = weights.data_ptr(), weights.data_ptr() + 4 * weights.numel()
+    if batch.n_seq and po < hi and lo < po + 4 * out_weights.numel():
+        raise ValueError("paged_evict: out_weights must not overlap weights")
+    if batch.n_seq:
+        _lib.call("ssd_paged_evict", cache, layers, layer_elems, batch.desc, after.desc, pw, cap, cap, keep, recent, first, po, pk,
+                  _stream(dev))
+    return kept, out_weights
+
+
+# ------------------------------------------------------------------ log probabilities of given tokens
+_LOGIT_TYPES = {BF16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def token_logprobs(logits, tokens, top=0, ws=None):
+    """ssd_token_logprobs over logits [M, V] (bf16, fp16 or fp32, unit column stride, any row stride) and tokens [M] (int32 or int64,
+    contiguous). Returns (logprobs, entropy, rank, top_ids, top_logprobs), the last two [M, top]. ``ws``: uint8,
+    token_logprobs_ws_bytes(...) (None: made here)."""
+    dev = torch.cuda.current_device()
+    if not isinstance(logits, torch.Tensor) or logits.dtype not in _LOGIT_TYPES or logits.get_device() != dev or logits.dim() != 2 or (
+            logits.shape[1] > 1 and logits.stride(1) != 1):
+        _refuse(logits, "logits", "bfloat16, float16 or float32", dev, ", [M, V] with unit column stride")
+    m, V = logits.shape
+    if not isinstance(tokens, torch.Tensor) or tokens.dtype not in (I32, torch.int64) or tokens.get_device() != dev or (
+            tokens.shape != (m,) or not tokens.is_contiguous()):
+        _refuse(tokens, "tokens", "int32 or int64", dev, f", [{m}] and contiguous")
+    kind = _LOGIT_TYPES[logits.dtype]
+    need = token_logprobs_ws_bytes(m, V, logits.dtype, top)
+    if need and ws is None:
+        ws = torch.empty(need, dtype=torch.uint8, device=logits.device)
+    f32 = torch.empty((2, m), dtype=F32, device=logits.device)
+    rank = torch.empty(m, dtype=I32, device=logits.device)
+    ids = torch.empty((m, top), dtype=I32, device=logits.device)
+    lps = torch.empty((m, top), dtype=F32, device=logits.device)
+    if m:
+        _lib.call("ssd_token_logprobs", logits.data_ptr(), kind, logits.stride(0) if m > 1 else V, m, V, tokens.data_ptr(),
+                  int(tokens.dtype == torch.int64), top, None if ws is None else _ptr(ws, "ws", torch.uint8, dev, need),
+                  0 if ws is None else ws.numel(), f32[0].data_ptr(), f32[1].data_ptr(), rank.data_ptr(), ids.data_ptr(),
+                  lps.data_ptr(), _stream(dev))
+    return f32[0], f32[1], rank, ids, lps
+
+
+def token_logprobs_ws_bytes(m: int, V: int, dtype, top: int = 0) -> int:
+    if dtype not in _LOGIT_TYPES:
+        raise ValueError(f"token_logprobs: logits of {dtype} (bfloat16, float16, float32)")
+    b = int(_lib.load().ssd_token_logprobs_ws_bytes(m, V, _LOGIT_TYPES[dtype], top))
+    if b < 0:
+        raise ValueError(f"token_logprobs: bad m={m} V={V} top={top}")
+    return b
+
+
 # ------------------------------------------------------------------------ sampling
 def sample_ws_bytes(rows: int, n: int) -> int:
     b = int(_lib.load().ssd_sample_ws_bytes(rows, n))
