@@ -318,14 +318,16 @@ int ssd_paged_read_bf16(const SsdPagedKv* cache, const SsdPagedBatch* batch, int
  * weights[s * ldw_seq + h * ldw + t] becomes decay * itself + the sum over the sequence's rows and h's query heads of the
  * softmax weight of t (decay in [0, 1]; 0: the old value is not read); the rest stays. Weights are summed in a
  * fixed order.
- * ssd_paged_prompt_bf16 is for many rows a sequence; its results depend on a row's query and keys and on how many
- * rows the call has (which decides the tile), and differ from the other's by rounding. */
+ * ssd_paged_prompt_bf16 is for many rows a sequence; where they are too few to fill the chip it cuts the length into parts
+ * too (ws: ssd_paged_prompt_ws_floats(...) floats, as above; 0: NULL will do). The parts follow from M, the heads, n_seq and
+ * l_max, and the results differ by rounding between numbers of parts and from the other's. */
 int64_t ssd_paged_attn_ws_floats(int M, int heads, int head_dim, int64_t l_max, int span, int weights);
 int ssd_paged_attention_bf16(const SsdPagedKv* cache, const SsdPagedBatch* batch, const uint16_t* q, int64_t ldq, int M, int heads,
                              int l_max, int span, float scale, float* ws, int64_t ws_floats, float* weights, int64_t ldw_seq,
                              int64_t ldw, float decay, uint16_t* out, int64_t ldo, hipStream_t stream);
+int64_t ssd_paged_prompt_ws_floats(int M, int heads, int kv_heads, int head_dim, int n_seq, int64_t l_max);
 int ssd_paged_prompt_bf16(const SsdPagedKv* cache, const SsdPagedBatch* batch, const uint16_t* q, int64_t ldq, int M, int heads,
-                          int l_max, float scale, uint16_t* out, int64_t ldo, hipStream_t stream);
+                          int l_max, float scale, float* ws, int64_t ws_floats, uint16_t* out, int64_t ldo, hipStream_t stream);
 
 /* Eviction by received weight, in `layers` layers (cache: the first; layer_elems elements apart): of every (layer, sequence, kv head)
  * with more than `keep` slots stay the first `first`, the last `recent`, and of those between as many as complete

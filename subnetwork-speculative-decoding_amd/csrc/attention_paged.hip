@@ -25,7 +25,7 @@ struct PagedAttnArgs {
   const bf16_t* Q;
   int64_t ldq;
   int M, heads, rep, l_cap;  // l_cap: slots from here on are not attended
-  int span_blk, n_grps, sets, units;
+  int span_blk, n_grps, grp_keys, sets, units;  // grp_keys: keys of a group
   float scale_log2;
   float* ws_o;    // [row][head][group][HD]
   float2* ws_ml;  // [row][head][group]: (m, l)
@@ -272,7 +272,7 @@ __device__ __forceinline__ float2 paged_total(const float2* ml, int ng, int part
 template <int HD, bool WEIGHTS>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int grp_keys = PA_WAVES * a.span_blk * PAGE;
+  const int grp_keys = a.grp_keys;
   if ((int)blockIdx.x < a.join_wgs) {
     constexpr int V = HD / 64;  // dims a lane
     int u = blockIdx.x * 4 + w;
@@ -375,6 +375,20 @@ static int launch_paged_attn(PagedAttnArgs a, hipStream_t stream) {
   return check_launch("paged_attention_join");
 }
 
+int paged_join(const PagedBatch& b, int M, int heads, int head_dim, int l_cap, int grp_keys, int n_grps, float* ws_o, float2* ws_ml,
+               bf16_t* out, int64_t ldo, hipStream_t stream) {
+  PagedAttnArgs a{};
+  a.b = b, a.M = M, a.heads = heads, a.l_cap = l_cap, a.grp_keys = grp_keys, a.n_grps = n_grps;
+  a.b.rows_max = std::min(b.rows_max, M);
+  a.ws_o = ws_o, a.ws_ml = ws_ml, a.out = out, a.ldo = ldo;
+  const int64_t join = ((int64_t)b.n_seq * a.b.rows_max * heads + 3) / 4;
+  if (paged_grid_too_large(join, 256)) return set_error(SSD_ERANGE, "paged_attention_join: too many workgroups");
+  a.join_wgs = (int)join;
+  if (head_dim == 64) SSD_LAUNCH((paged_join_kernel<64, false>), dim3((unsigned)join), dim3(256), 0, stream, a);
+  else SSD_LAUNCH((paged_join_kernel<128, false>), dim3((unsigned)join), dim3(256), 0, stream, a);
+  return check_launch("paged_attention_join");
+}
+
 }  // namespace ssd
 
 using namespace ssd;
@@ -412,7 +426,7 @@ SSD_API int ssd_paged_attention_bf16(const SsdPagedKv* cache, const SsdPagedBatc
   a.b.rows_max = std::min(a.b.rows_max, M);
   a.c = PagedCache{cache->k, cache->v, cache->pages, cache->kv_heads};
   a.Q = q, a.ldq = ldq, a.M = M, a.heads = heads, a.rep = heads / cache->kv_heads, a.l_cap = l_max;
-  a.span_blk = span / PAGE, a.n_grps = paged_groups(l_max, span), a.scale_log2 = scale * 1.4426950408889634f;
+  a.span_blk = span / PAGE, a.n_grps = paged_groups(l_max, span), a.grp_keys = PA_WAVES * span, a.scale_log2 = scale * 1.4426950408889634f;
   const int64_t recs = (int64_t)M * heads * a.n_grps;
   a.ws_o = ws, a.ws_ml = (float2*)(ws + recs * cache->head_dim);
   a.ws_s = ws + recs * (cache->head_dim + 2) + (recs * 2) % 4, a.ld_s = paged_score_ld(l_max);

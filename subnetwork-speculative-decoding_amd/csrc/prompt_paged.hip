@@ -2,16 +2,29 @@
 // lengths in one launch.
 //
 // The columns of S^T = K Q^T are the (row, q head) pairs of one sequence and kv head, rows outermost: whatever the number of
-// heads that share a kv head, a workgroup of four waves has 64 NT columns of one kv head, and a block's K and V are copied into
-// LDS once for all of them (global to LDS, 16 bytes a lane, one block ahead of their use, in two buffers). Blocks are folded with a
-// running reference m, sum l and output O in fp32; the reference follows a column's maximum only when that has grown by more than
+// heads that share a kv head, a workgroup of four waves has 128 columns of one kv head, 32 a wave, and a block's K and V are copied
+// into LDS once for all of them (global to LDS, 16 bytes a lane, into two buffers each). Blocks are folded with a running
+// reference m, sum l and output O in fp32; the reference follows a column's maximum only when that has grown by more than
 // 2^8. Probabilities are rounded to bf16 as the second product's operand; l sums them before that.
+//
+// v_mfma_f32_32x32x16_bf16 rather than 16x16x32: the vector pipe stands still for about 8 cycles with every matrix instruction that another
+// wave issues, whatever its size, so half as many of twice the work leave it more (a wave of products beside one of multiply-adds:
+// 406 ns against 345 for the same work). While a block's scores become probabilities and meet V, the next block's scores are
+// under way; the blocks that some columns attend only part of, one or two a tile, follow without that.
+// What bounds it, 32 heads on 8 kv heads of 128 (8b shapes): a prompt of 16384 rows 1.95 ms, 1130 TFLOP/s, where a large library product reaches
+// 1300: matrix pipe, vector pipe and LDS reads, each about half of a block's 1.9 us for two workgroups a CU. Shorter
+// prompts: a tile's beginning and end, about 8 us (rows, pages, first copies; the partly attended blocks; the output), of which a
+// second workgroup on the CU hides half: 4096 rows 157 us, 16 prompts of 232 to 1500 rows 180.
+// Tried: eight waves a workgroup (a prompt of 4096 147 us, 16 prompts 193, 100 rows after 8000 keys 180 against 136 with the length
+// in one part), 64 columns a wave with twice the registers (269), two groups of waves taking turns at the matrix pipe (155).
 #include "paged.h"
 
 #include <algorithm>
 #include <type_traits>
 
 namespace ssd {
+
+constexpr int PP_WAVES = 4;
 
 typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(3))) u32x4_t lds_u32x4;
@@ -25,213 +38,369 @@ struct PagedPromptArgs {
   float scale_log2;
   bf16_t* out;
   int64_t ldo;
+  int splits, per;  // the length in `splits` parts of `per` blocks
+  float* ws_o;      // [row][head][part][HD]: O, for more than one part
+  float2* ws_ml;    // [row][head][part]: (m, l)
 };
 
-template <int HD, int NT>
-struct PromptState {
-  u32x4_t qf[NT][HD / 32];
-  float m[NT], l[NT];  // reference (log2 units), this lane's part of the sum
-  f32x4_t o[NT][HD / 16];
-  int lim[NT];         // the last slot that this lane's column attends
-};
+typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16_t;
 
-// Copies the 64-key block at element offset `at` of both arenas into LDS: wave w, load i takes pieces 256 i + 64 w + lane.
+// A wave's 32 columns. v_mfma_f32_32x32x16_bf16 leaves lane (g, n) = 32 g + n column n's rows 8 (r / 4) + 4 g + r % 4 in register r. The
+// keys of a half block are assigned to the rows so that registers 8 u .. 8 u + 7 are slots 16 u + 8 g .. + 8 of the half: the second product's
+// operand without a move between lanes, against eight consecutive slots of V.
 template <int HD>
-__device__ __forceinline__ void prompt_copy(const PagedCache& c, size_t at, int w, int lane, lds_u32x4* k, lds_u32x4* v) {
-  const char *ks = (const char*)(c.k + at) + w * 1024, *vs = (const char*)(c.v + at) + w * 1024;
-  const uint32_t l16 = lane * 16;
-#pragma unroll
-  for (int i = 0; i < HD / 32; ++i) {
-    __builtin_amdgcn_global_load_lds((const void*)(ks + 4096 * i + l16), (lds_void*)(k + 256 * i + 64 * w), 16, 0, 0);
-    __builtin_amdgcn_global_load_lds((const void*)(vs + 4096 * i + l16), (lds_void*)(v + 256 * i + 64 * w), 16, 0, 0);
-  }
+struct PromptState {
+  u32x4_t qf[HD / 16];  // dims 16 q + 8 g .. + 8 of the lane's column
+  float m, l;           // reference (log2 units), this lane's part of the sum
+  f32x16_t o[HD / 32];  // dims 32 d + 8 (r / 4) + 4 g + r % 4
+  int lim;              // the last slot that the column attends
+};
+
+__device__ __forceinline__ f32x16_t mfma32x32x16(u32x4_t a, u32x4_t b, f32x16_t c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(bits_bf16x8(a), bits_bf16x8(b), c, 0, 0, 0);
 }
 
-// One block from LDS into the wave's columns. MASKED: some column may not attend all of it.
-template <int HD, int NT, bool MASKED>
-__device__ __forceinline__ void prompt_block(PromptState<HD, NT>& st, int key0, float scale_log2, int lane,
-                                             const lds_u32x4* __restrict__ ck, const lds_u32x4* __restrict__ cv) {
-  constexpr int KS = HD / 32, DT = HD / 16;
-  const int g = lane >> 4;
-  f32x4_t s[NT][4];
+__device__ __forceinline__ int prompt_key(int c, int r, int g) { return 32 * c + 16 * (r >> 3) + 8 * g + (r & 7); }
+
+// Where this lane reads its operands of K and of V in LDS (16-byte pieces; a block lies there as in the page).
+struct PromptLanes {
+  int k, v;
+};
+template <int HD>
+__device__ __forceinline__ PromptLanes prompt_lanes(int lane) {
+  const int g = lane >> 5, h = lane >> 3 & 1, i = (lane >> 4 & 1) * 8 + (lane & 7);
+  return PromptLanes{h * (HD / 32) * 64 + g * 16 + i, (lane >> 4 & 1) * 128 + g * 16 + (lane & 15)};
+}
+
+// Copies one arena's 64-key block into LDS: wave w, load i takes tile W i + w.
+template <int HD>
+__device__ __forceinline__ void prompt_copy(const bf16_t* from, int w, int lane, lds_u32x4* to) {
+  constexpr int W = PP_WAVES;
+  const char* p = (const char*)from + w * 1024;
 #pragma unroll
-  for (int rt = 0; rt < NT; ++rt)
+  for (int i = 0; i < HD / 8 / W; ++i)
+    __builtin_amdgcn_global_load_lds((const void*)(p + 1024 * W * i + (uint32_t)lane * 16), (lds_void*)(to + 64 * (W * i + w)), 16, 0, 0);
+}
+
+template <int HD>
+__device__ __forceinline__ void prompt_qk(const PromptState<HD>& st, const PromptLanes& at, const lds_u32x4* __restrict__ ck, f32x16_t (&s)[2]) {
+  s[0] = f32x16_t{}, s[1] = f32x16_t{};
 #pragma unroll
-    for (int kt = 0; kt < 4; ++kt) s[rt][kt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-    for (int kt = 0; kt < 4; ++kt) {
-      const u32x4_t kf = ck[(kt * KS + ks) * 64 + lane];
-#pragma unroll
-      for (int rt = 0; rt < NT; ++rt) s[rt][kt] = mfma16x16x32(bits_bf16x8(kf), bits_bf16x8(st.qf[rt][ks]), s[rt][kt]);
-    }
-  u32x4_t vf[DT][2];
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-    for (int c = 0; c < 2; ++c) vf[dt][c] = cv[(dt * 2 + c) * 64 + lane];
-#pragma unroll
-  for (int rt = 0; rt < NT; ++rt) {
-    const int left = st.lim[rt] - key0 + 1;
-    u32x4_t pw[2];
-    float mx = -INFINITY;
-#pragma unroll
-    for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (MASKED) s[rt][kt][e] = paged_key(kt, g, e) < left ? s[rt][kt][e] : -INFINITY;
-        mx = fmaxf(mx, s[rt][kt][e]);
-      }
-    mx = paged_max_lanes(mx) * scale_log2;
-    const bool grow = mx > st.m[rt] + 8.f || (st.m[rt] == -INFINITY && mx != st.m[rt]);
-    const float m = grow ? mx : st.m[rt], ms = m == -INFINITY ? 0.f : m;
-    if (__any(grow)) {  // multiplying by 1 changes nothing
-      const float alpha = grow ? __builtin_amdgcn_exp2f(st.m[rt] - ms) : 1.f;
-      st.l[rt] *= alpha;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) st.o[rt][dt] *= alpha;
-    }
-    st.m[rt] = m;
-#pragma unroll
-    for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-      for (int e = 0; e < 4; e += 2) {
-        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[rt][kt][e], scale_log2, -ms));
-        const float p1 = __builtin_amdgcn_exp2f(fmaf(s[rt][kt][e + 1], scale_log2, -ms));
-        st.l[rt] += p0 + p1;
-        pw[kt >> 1][(kt & 1) * 2 + e / 2] = pack_bf16x2(p0, p1);
-      }
+  for (int q = 0; q < HD / 16; ++q)
 #pragma unroll
     for (int c = 0; c < 2; ++c)
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) st.o[rt][dt] = mfma16x16x32(bits_bf16x8(vf[dt][c]), bits_bf16x8(pw[c]), st.o[rt][dt]);
-  }
+      s[c] = mfma32x32x16(ck[at.k + (2 * c * (HD / 32) + q / 2) * 64 + q % 2 * 32], st.qf[q], s[c]);
 }
 
-// Workgroup (tile of 64 NT columns of some sequence, kv head); the tiles of all sequences are numbered one behind the other, each
-// sequence's last rows, which attend the most, first. The kv head varies fastest: with eight of them an XCD serves one, whose
-// blocks its L2 keeps.
-template <int HD, int NT>
-__global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedPromptArgs a) {
-  constexpr int KS = HD / 32, DT = HD / 16, CW = 64 * NT, PIECES = 64 * HD / 8;
-  __shared__ int first_bad[HD];
-  __shared__ __align__(16) u32x4_t kA[PIECES], vA[PIECES], kB[PIECES], vB[PIECES];
-  typedef __attribute__((address_space(3))) u32x4_t* lp;
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, g = lane >> 4;
-  const int kvh = blockIdx.x % a.c.kv;
-  // every wave finds the tile's sequence for itself
-  int t = blockIdx.x / a.c.kv, seq = -1, tile = 0;
-  for (int s0 = 0; s0 < a.b.n_seq; s0 += 64) {
-    const int cnt = s0 + lane < a.b.n_seq ? (paged_rows(a.b, s0 + lane, a.M).n * a.rep + CW - 1) / CW : 0;
-    int inc = cnt;
+// Takes the reference to the block's maximum where that has outgrown it.
+template <int HD>
+__device__ __forceinline__ void prompt_reference(PromptState<HD>& st, const f32x16_t (&s)[2], float scale_log2) {
+  float mx = -INFINITY;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
+  for (int c = 0; c < 2; ++c)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[c][r]);
+  const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+  mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * scale_log2;
+  const bool grow = mx > st.m + 8.f || (st.m == -INFINITY && mx != st.m);
+  if (!__any(grow)) return;
+  asm volatile("" ::: "memory");  // a branch that is taken now and then, not products with 1 in every block
+  const float alpha = grow ? __builtin_amdgcn_exp2f(st.m - mx) : 1.f;
+  st.l *= alpha;
+#pragma unroll
+  for (int d = 0; d < HD / 32; ++d) st.o[d] *= alpha;
+  st.m = grow ? mx : st.m;
+}
+
+template <int HD>
+__device__ __forceinline__ void prompt_exp(PromptState<HD>& st, const f32x16_t (&s)[2], float scale_log2, u32x4_t (&p)[4]) {
+  const float ms = st.m == -INFINITY ? 0.f : st.m;  // nothing attended so far: every p is 0
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+#pragma unroll
+    for (int r = 0; r < 16; r += 2) {
+      const float p0 = __builtin_amdgcn_exp2f(fmaf(s[c][r], scale_log2, -ms));
+      const float p1 = __builtin_amdgcn_exp2f(fmaf(s[c][r + 1], scale_log2, -ms));
+      st.l += p0 + p1;
+      p[2 * c + r / 8][r % 8 / 2] = pack_bf16x2(p0, p1);
+    }
+}
+
+template <int HD>
+__device__ __forceinline__ void prompt_pv(PromptState<HD>& st, const PromptLanes& at, const lds_u32x4* __restrict__ cv, const u32x4_t (&p)[4]) {
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int d = 0; d < HD / 32; ++d) st.o[d] = mfma32x32x16(cv[at.v + (4 * d + t / 2) * 64 + t % 2 * 32], p[t], st.o[d]);
+}
+
+// The t-th tile of CW columns: the tiles of all sequences are numbered one behind the other, each sequence's last first. Every wave
+// finds it for itself.
+struct PromptTile {
+  int seq, tile;
+  PagedRows rows;
+};
+template <int CW>
+__device__ __forceinline__ PromptTile prompt_tile(const PagedPromptArgs& a, int t, int lane) {
+  for (int s0 = 0; s0 < a.b.n_seq; s0 += 64) {
+    const PagedRows r = paged_rows(a.b, min(s0 + lane, a.b.n_seq - 1), a.M);
+    int inc = s0 + lane < a.b.n_seq ? (r.n * a.rep + CW - 1) / CW : 0;
+    for (int o = 1; o < min(a.b.n_seq - s0, 64); o <<= 1) {  // as many steps as there are sequences to add up
       const int x = __shfl_up(inc, o);
       if (lane >= o) inc += x;
     }
     const uint64_t past = __ballot(inc > t);
     if (past) {
       const int l = __builtin_ctzll(past);
-      seq = s0 + l;
-      tile = __builtin_amdgcn_readlane(inc, l) - 1 - t;  // the last one first
-      break;
+      return PromptTile{s0 + l, __builtin_amdgcn_readlane(inc, l) - 1 - t,
+                        PagedRows{__builtin_amdgcn_readlane(r.r0, l), __builtin_amdgcn_readlane(r.n, l), __builtin_amdgcn_readlane(r.first, l)}};
     }
     t -= __builtin_amdgcn_readlane(inc, 63);
   }
-  if (seq < 0) return;
-  seq = __builtin_amdgcn_readfirstlane(seq);
-  const PagedRows r = paged_rows(a.b, seq, a.M);
-  const int n_cols = r.n * a.rep, c0 = tile * CW, w0 = c0 + w * 16 * NT;
-  PromptState<HD, NT> st;
-#pragma unroll
-  for (int rt = 0; rt < NT; ++rt) {
-    const int col = min(w0 + rt * 16 + j, n_cols - 1), i = col / a.rep;
-    st.lim[rt] = min(r.first + i, a.l_cap - 1);
+  return PromptTile{-1, 0, {}};
+}
+
+// Workgroup (tile of 32 W columns of some sequence, kv head). The kv head varies fastest: with eight of them an XCD serves one, whose
+// blocks its L2 keeps.
+template <int HD>
+__global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedPromptArgs a) {
+  constexpr int W = PP_WAVES, CW = 32 * W, PIECES = 64 * HD / 8;
+  __shared__ int first_bad[HD], any_bad;
+  __shared__ __align__(16) u32x4_t kA[PIECES], vA[PIECES], kB[PIECES], vB[PIECES];
+  typedef __attribute__((address_space(3))) u32x4_t* lp;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, g = lane >> 5;
+  int u = blockIdx.x;
+  const int kvh = u % a.c.kv;
+  u /= a.c.kv;
+  const int part = u % a.splits;
+  const PromptTile pt = prompt_tile<CW>(a, u / a.splits, lane);
+  if (pt.seq < 0) return;
+  const int seq = pt.seq, c0 = pt.tile * CW, w0 = c0 + w * 32;
+  const PagedRows r = pt.rows;
+  const int n_cols = r.n * a.rep;
+  auto lim_of = [&](int col) { return min(r.first + min(col, n_cols - 1) / a.rep, a.l_cap - 1); };
+  const int last = lim_of(c0 + CW - 1), n_blk = min(last < 0 ? 0 : last / PAGE + 1, (part + 1) * a.per);
+  const int full = min((lim_of(c0) + 1) / PAGE, n_blk);  // blocks that every column attends whole
+  const int hi = w0 < n_cols ? lim_of(w0 + 31) : -1;     // this wave's last key
+  int base = part * a.per;
+  if (part && base >= n_blk) return;  // no record: the join counts the parts as this does
+  int pages = base + lane < n_blk ? paged_page(a.b, seq, base + lane, a.c.pages) : -1;
+  const PromptLanes at = prompt_lanes<HD>(lane);
+  PromptState<HD> st;
+  {
+    const int col = min(w0 + n, n_cols - 1), i = col / a.rep;
+    st.lim = min(r.first + i, a.l_cap - 1);
     const bf16_t* q = a.Q + (int64_t)(r.r0 + i) * a.ldq + (kvh * a.rep + col % a.rep) * HD;
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) st.qf[rt][ks] = *(const u32x4_t*)(q + ks * 32 + g * 8);
-    st.m[rt] = -INFINITY, st.l[rt] = 0.f;
+    for (int k = 0; k < HD / 16; ++k) st.qf[k] = *(const u32x4_t*)(q + k * 16 + g * 8);
+    st.m = -INFINITY, st.l = 0.f;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) st.o[rt][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int d = 0; d < HD / 32; ++d) st.o[d] = f32x16_t{};
   }
-  auto lim_of = [&](int col) { return min(r.first + min(col, n_cols - 1) / a.rep, a.l_cap - 1); };
-  const int last = lim_of(c0 + CW - 1), n_blk = last < 0 ? 0 : last / PAGE + 1;
-  const int full = min((lim_of(c0) + 1) / PAGE, n_blk);           // blocks that every column attends whole
-  const int hi = w0 < n_cols ? lim_of(w0 + 16 * NT - 1) : -1;  // this wave's last key
-  // lane i has the page of block i of the present 64
-  int pages = lane < n_blk ? paged_page(a.b, seq, lane, a.c.pages) : -1;
-  auto page = [&](int b) { return __builtin_amdgcn_readlane(pages, b & 63); };
-  auto place = [&](int pg) { return ((size_t)max(pg, 0) * a.c.kv + kvh) * PAGE * HD; };
-  if (threadIdx.x < HD) first_bad[threadIdx.x] = INT32_MAX;  // read behind the first block's barrier
-  if (n_blk > 0) prompt_copy<HD>(a.c, place(page(0)), w, lane, (lp)kA, (lp)vA);
-  auto step = [&](auto masked, int b, lds_u32x4* ck, lds_u32x4* cv, lds_u32x4* nk, lds_u32x4* nv) {
-    // this block's copy has landed (a barrier does not wait for it), and every wave is done with the other buffer
+  // the blocks that exist, in order: lane i has the page of block base + i, live those not yet handed out
+  struct Block {
+    int b;
+    size_t at;
+  };
+  uint64_t live = __ballot(pages >= 0);
+  auto next = [&] {
+    while (!live && (base += 64) < n_blk) {
+      pages = base + lane < n_blk ? paged_page(a.b, seq, base + lane, a.c.pages) : -1;
+      live = __ballot(pages >= 0);
+    }
+    if (!live) return Block{INT32_MAX, 0};
+    const int i = __builtin_ctzll(live);
+    live &= live - 1;
+    return Block{base + i, ((size_t)__builtin_amdgcn_readlane(pages, i) * a.c.kv + kvh) * PAGE * HD};
+  };
+  auto copy_k = [&](const Block& x, lds_u32x4* to) {
+    if (x.b < n_blk) prompt_copy<HD>(a.c.k + x.at, w, lane, to);
+  };
+  auto copy_v = [&](const Block& x, lds_u32x4* to) {
+    if (x.b < n_blk) prompt_copy<HD>(a.c.v + x.at, w, lane, to);
+  };
+  // What was copied has landed (a barrier does not wait for it), and every wave is done with the other buffers.
+  auto landed = [&] {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    const bool gone = page(b) < 0;  // nobody attends it
-    if (b + 1 < n_blk) {
-      if (((b + 1) & 63) == 0) pages = b + 1 + lane < n_blk ? paged_page(a.b, seq, b + 1 + lane, a.c.pages) : -1;
-      prompt_copy<HD>(a.c, place(page(b + 1)), w, lane, nk, nv);
-    }
-    if (gone) return;
-    if constexpr (decltype(masked)::value) {
-#pragma unroll
-      for (int i = 0; i < HD / 32; ++i) {
-        const int n = 256 * i + (int)threadIdx.x;  // piece n: tile n / 64, lane n % 64
-        const u32x4_t x = cv[n];
-        if (paged_not_finite(x[0]) || paged_not_finite(x[1]) || paged_not_finite(x[2]) || paged_not_finite(x[3]))
-          cv[n] = paged_take_out(x, b * PAGE + (n >> 6 & 1) * 32 + (n >> 4 & 3) * 8, &first_bad[(n >> 7) * 16 + (n & 15)]);
-      }
-      __syncthreads();
-    }
-    if (b * PAGE > hi) return;
-    prompt_block<HD, NT, decltype(masked)::value>(st, b * PAGE, a.scale_log2, lane, ck, cv);
   };
-  using yes_t = std::integral_constant<bool, true>;
-  using no_t = std::integral_constant<bool, false>;
-  int b = 0;
-  for (; b + 1 < full; b += 2) {
-    step(no_t{}, b, (lp)kA, (lp)vA, (lp)kB, (lp)vB);
-    step(no_t{}, b + 1, (lp)kB, (lp)vB, (lp)kA, (lp)vA);
-  }
-  for (; b < n_blk; b += 2) {  // at most one block more that every column attends whole, then the others
-    step(yes_t{}, b, (lp)kA, (lp)vA, (lp)kB, (lp)vB);
-    if (b + 1 < n_blk) step(yes_t{}, b + 1, (lp)kB, (lp)vB, (lp)kA, (lp)vA);
-  }
-  __syncthreads();  // no block's notes are under way
+  for (int i = threadIdx.x; i < HD; i += 64 * W) first_bad[i] = INT32_MAX;
+  if (threadIdx.x == 0) any_bad = 0;
+  Block cur = next(), nxt = next();  // K and V of the i-th existing block go to buffers A for even i, B for odd
+  copy_k(cur, (lp)kA);
+  copy_v(cur, (lp)vA);
+  copy_k(nxt, (lp)kB);
+  landed();
+  bool odd = false;
+  if (cur.b < full) {
+    f32x16_t s0[2], s1[2];
+    u32x4_t p[4];
+    prompt_qk<HD>(st, at, (lp)kA, s0);
+    prompt_reference<HD>(st, s0, a.scale_log2);
+    // scores s of the present block; V in cv; the next block's K in nk, its scores into sn; free: ck, nv
+    auto step = [&](f32x16_t (&s)[2], f32x16_t (&sn)[2], lds_u32x4* ck, lds_u32x4* cv, lds_u32x4* nk, lds_u32x4* nv) {
+      landed();
+      const Block then = next();
+      copy_k(then, ck);
+      copy_v(nxt, nv);
+      __builtin_amdgcn_sched_barrier(0);
+      prompt_qk<HD>(st, at, nk, sn);
+      prompt_exp<HD>(st, s, a.scale_log2, p);
+      prompt_pv<HD>(st, at, cv, p);
+#ifdef SGB
+      __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
 #pragma unroll
-  for (int rt = 0; rt < NT; ++rt) {
-    const float l = paged_sum_lanes(st.l[rt]);
-    const int col = w0 + rt * 16 + j;
-    if (col >= n_cols) continue;
-    const float inv = l == 0.f ? 0.f : 1.f / l;  // NaN stays NaN
-    bf16_t* dst = a.out + (int64_t)(r.r0 + col / a.rep) * a.ldo + (kvh * a.rep + col % a.rep) * HD;
+      for (int i = 0; i < 16; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x2, 7, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      float y[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = st.lim[rt] >= first_bad[dt * 16 + 4 * g + e] ? __uint_as_float(0x7fc00000u) : st.o[rt][dt][e] * inv;
-      *(uint2*)(dst + dt * 16 + 4 * g) = make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
+      for (int i = 0; i < 12; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x8, 4, 0);
+#endif
+      prompt_reference<HD>(st, sn, a.scale_log2);
+      cur = nxt, nxt = then;
+    };
+    while (nxt.b < full) {
+      step(s0, s1, (lp)kA, (lp)vA, (lp)kB, (lp)vB);
+      odd = true;
+      if (!(nxt.b < full)) break;
+      step(s1, s0, (lp)kB, (lp)vB, (lp)kA, (lp)vA);
+      odd = false;
     }
+    // the last of them
+    landed();
+    const Block then = next();
+    copy_k(then, odd ? (lp)kB : (lp)kA);
+    copy_v(nxt, odd ? (lp)vA : (lp)vB);
+    if (odd) {
+      prompt_exp<HD>(st, s1, a.scale_log2, p);
+      prompt_pv<HD>(st, at, (lp)vB, p);
+    } else {
+      prompt_exp<HD>(st, s0, a.scale_log2, p);
+      prompt_pv<HD>(st, at, (lp)vA, p);
+    }
+    cur = nxt, nxt = then;
+    odd = !odd;
+    landed();
+  }
+  // blocks that some columns attend only part of: K and V of the present one and K of the next one have landed
+  for (; cur.b < n_blk; odd = !odd) {
+    const lds_u32x4* ck = odd ? (lp)kB : (lp)kA;
+    lds_u32x4 *cv = odd ? (lp)vB : (lp)vA, *nv = odd ? (lp)vA : (lp)vB;
+    copy_v(nxt, nv);
+    // V values that are not finite are taken out
+#pragma unroll
+    for (int i = 0; i < HD / 8 / W; ++i) {
+      const int x = 64 * W * i + (int)threadIdx.x;  // piece x: tile x / 64, lane x % 64
+      const u32x4_t y = cv[x];
+      if (paged_not_finite(y[0]) || paged_not_finite(y[1]) || paged_not_finite(y[2]) || paged_not_finite(y[3]))
+        cv[x] = paged_take_out(y, cur.b * PAGE + (x >> 6 & 1) * 32 + (x >> 4 & 3) * 8, &first_bad[(x >> 7) * 16 + (x & 15)]), any_bad = 1;
+    }
+    __syncthreads();
+    if (cur.b * PAGE <= hi) {
+      f32x16_t s[2];
+      u32x4_t p[4];
+      prompt_qk<HD>(st, at, ck, s);
+      const int left = st.lim - cur.b * PAGE + 1;
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[c][e] = prompt_key(c, e, g) < left ? s[c][e] : -INFINITY;
+      prompt_reference<HD>(st, s, a.scale_log2);
+      prompt_exp<HD>(st, s, a.scale_log2, p);
+      prompt_pv<HD>(st, at, cv, p);
+    }
+    __syncthreads();  // this block's K buffer is free
+    const Block then = next();
+    copy_k(then, odd ? (lp)kB : (lp)kA);
+    cur = nxt, nxt = then;
+    landed();
+  }
+  const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(st.l), __float_as_uint(st.l), false, false);
+  const float l = __uint_as_float(sw[0]) + __uint_as_float(sw[1]), inv = a.splits > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;  // NaN stays NaN
+#pragma unroll
+  for (int d = 0; d < HD / 32; ++d) st.o[d] *= inv;
+  if (any_bad) {
+#pragma unroll
+    for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (st.lim >= first_bad[32 * d + e / 4 * 8 + 4 * g + e % 4]) st.o[d][e] = __uint_as_float(0x7fc00000u);
+  }
+  if (a.splits > 1) {
+    const int col = w0 + n;
+    if (col >= n_cols) return;
+    const int64_t rec = ((int64_t)(r.r0 + col / a.rep) * a.heads + kvh * a.rep + col % a.rep) * a.splits + part;
+#pragma unroll
+    for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *(f32x4_t*)(a.ws_o + rec * HD + 32 * d + 8 * i + 4 * g) =
+            f32x4_t{st.o[d][4 * i], st.o[d][4 * i + 1], st.o[d][4 * i + 2], st.o[d][4 * i + 3]};
+    if (g == 0) a.ws_ml[rec] = make_float2(st.m, l);
+    return;
+  }
+  // The wave's columns leave through LDS as whole rows: 16-byte pieces, piece i of column c at i ^ (c & 7) of its row.
+  constexpr int PC = HD / 8;
+  lds_u32x4* mine = w & 1 ? (w & 2 ? (lp)vB : (lp)vA) : (w & 2 ? (lp)kB : (lp)kA);
+#pragma unroll
+  for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      typedef unsigned int u32x2_t __attribute__((ext_vector_type(2)));
+      const u32x2_t x = {pack_bf16x2(st.o[d][4 * i], st.o[d][4 * i + 1]), pack_bf16x2(st.o[d][4 * i + 2], st.o[d][4 * i + 3])};
+      ((__attribute__((address_space(3))) u32x2_t*)(mine + n * PC + ((4 * d + i) ^ (n & 7))))[g] = x;
+    }
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < PC / 2; ++i) {
+    const int x = 64 * i + lane, c = x / PC, col = w0 + c;
+    if (col < n_cols) *(u32x4_t*)(a.out + (int64_t)(r.r0 + col / a.rep) * a.ldo + (kvh * a.rep + col % a.rep) * HD + x % PC * 8) =
+        mine[c * PC + (x % PC ^ (c & 7))];
   }
 }
 
-template <int HD, int NT>
+// Workgroups of a call with the length in one part: every sequence's tiles are at most a whole-tile share of the rows and one more.
+static int64_t prompt_tiles(int64_t M, int rep, int n_seq, int kv) { return (M * rep / (32 * PP_WAVES) + n_seq) * kv; }
+
+// Parts of the length: one while the tiles fill the chip's 256 CUs, else as many as bring two workgroups a CU, of eight blocks or more
+// (one / several parts, us: 100 rows of 32 heads after 8000 keys 136 / 37, 500 149 / 87, 40 rows of 15 heads 134 / 22). Two parts
+// pay for their records only over a long length: 4 times 100 rows of 64 heads after 4000 keys 77 / 83.
+static int prompt_splits(int64_t M, int rep, int n_seq, int kv, int64_t l_max) {
+  const int64_t wgs = prompt_tiles(M, rep, n_seq, kv), blocks = (l_max + PAGE - 1) / PAGE;
+  if (wgs >= 256) return 1;
+  const int64_t n = std::max<int64_t>(1, std::min(512 / std::max<int64_t>(wgs, 1), blocks / 8));
+  return n == 2 && blocks < 96 ? 1 : (int)n;
+}
+
+template <int HD>
 static int launch_paged_prompt(const PagedPromptArgs& a, hipStream_t stream) {
-  // every sequence's tiles: at most a whole-tile share of the rows and one more each
-  const int64_t wgs = ((int64_t)a.M * a.rep / (64 * NT) + a.b.n_seq) * a.c.kv;
+  const int64_t wgs = prompt_tiles(a.M, a.rep, a.b.n_seq, a.c.kv) * a.splits;
   if (paged_grid_too_large(wgs, 256)) return set_error(SSD_ERANGE, "paged_prompt: too many workgroups");
-  SSD_LAUNCH((paged_prompt_kernel<HD, NT>), dim3((unsigned)wgs), dim3(256), 0, stream, a);
-  return check_launch("paged_prompt");
+  SSD_LAUNCH((paged_prompt_kernel<HD>), dim3((unsigned)wgs), dim3(256), 0, stream, a);
+  if (int rc = check_launch("paged_prompt")) return rc;
+  if (a.splits == 1) return SSD_OK;
+  return paged_join(a.b, a.M, a.heads, HD, a.l_cap, a.per * PAGE, a.splits, a.ws_o, a.ws_ml, a.out, a.ldo, stream);
 }
 
 }  // namespace ssd
 
 using namespace ssd;
 
+SSD_API int64_t ssd_paged_prompt_ws_floats(int M, int heads, int kv_heads, int head_dim, int n_seq, int64_t l_max) {
+  if (M < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads || head_dim < 1 || n_seq < 0 || l_max < 1 || l_max > 1 << 30) return -1;
+  const int splits = prompt_splits(M, heads / kv_heads, n_seq, kv_heads, l_max);
+  return splits == 1 ? 0 : (int64_t)M * heads * splits * (head_dim + 2);
+}
+
 SSD_API int ssd_paged_prompt_bf16(const SsdPagedKv* cache, const SsdPagedBatch* batch, const uint16_t* q, int64_t ldq, int M, int heads,
-                                  int l_max, float scale, uint16_t* out, int64_t ldo, hipStream_t stream) {
+                                  int l_max, float scale, float* ws, int64_t ws_floats, uint16_t* out, int64_t ldo,
+                                  hipStream_t stream) {
   if (int rc = paged_check(cache, batch, "paged_prompt")) return rc;
   if (M < 0 || heads < 1 || heads % cache->kv_heads)
     return set_error(SSD_EINVAL, "paged_prompt: bad M=%d heads=%d kv_heads=%d", M, heads, cache->kv_heads);
@@ -250,7 +419,11 @@ SSD_API int ssd_paged_prompt_bf16(const SsdPagedKv* cache, const SsdPagedBatch* 
   a.Q = q, a.ldq = ldq, a.M = M, a.heads = heads, a.rep = heads / cache->kv_heads, a.l_cap = l_max;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.out = out, a.ldo = ldo;
-  const bool small = ((int64_t)M * a.rep / 128 + a.b.n_seq) * a.c.kv <= 256;
-  if (cache->head_dim == 64) return small ? launch_paged_prompt<64, 1>(a, stream) : launch_paged_prompt<64, 2>(a, stream);
-  return small ? launch_paged_prompt<128, 1>(a, stream) : launch_paged_prompt<128, 2>(a, stream);
+  const int64_t need = ssd_paged_prompt_ws_floats(M, heads, cache->kv_heads, cache->head_dim, batch->n_seq, l_max);
+  if (need && (!ws || ((uintptr_t)ws & 15) || ws_floats < need))
+    return set_error(SSD_EINVAL, "paged_prompt: workspace too small or not 16-byte aligned");
+  a.splits = prompt_splits(M, a.rep, batch->n_seq, a.c.kv, l_max);
+  a.per = ((l_max + PAGE - 1) / PAGE + a.splits - 1) / a.splits;
+  a.ws_o = ws, a.ws_ml = (float2*)(ws + (int64_t)M * heads * a.splits * cache->head_dim);
+  return cache->head_dim == 64 ? launch_paged_prompt<64>(a, stream) : launch_paged_prompt<128>(a, stream);
 }

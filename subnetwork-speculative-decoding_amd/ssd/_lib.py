@@ -137,7 +137,8 @@ _PROTOS = {
     "ssd_paged_attn_ws_floats": (I64, [I32, I32, I32, I64, I32, I32]),
     "ssd_paged_attention_bf16": (I32, [C.POINTER(SsdPagedKv), C.POINTER(SsdPagedBatch), P, I64, I32, I32, I32, I32, F32, P, I64, P,
                                        I64, I64, F32, P, I64, P]),
-    "ssd_paged_prompt_bf16": (I32, [C.POINTER(SsdPagedKv), C.POINTER(SsdPagedBatch), P, I64, I32, I32, I32, F32, P, I64, P]),
+    "ssd_paged_prompt_ws_floats": (I64, [I32, I32, I32, I32, I32, I64]),
+    "ssd_paged_prompt_bf16": (I32, [C.POINTER(SsdPagedKv), C.POINTER(SsdPagedBatch), P, I64, I32, I32, I32, F32, P, I64, P, I64, P]),
     "ssd_paged_evict": (I32, [C.POINTER(SsdPagedKv), I32, I64, C.POINTER(SsdPagedBatch), C.POINTER(SsdPagedBatch), P, I64, I32, I32,
                               I32, I32, P, P, P]),
     "ssd_token_logprobs_ws_bytes": (I64, [I32, I32, I32, I32]),

@@ -348,10 +348,15 @@ class PagedKVCache:
         call's rows, summed over rows and a kv head's query heads (decay 0: set). ``ws``: fp32, attend_floats(...)."""
         return ops.paged_attention(self._layers[i], batch, q, self._heads(q), l_max, self._span(batch), ws, out, scale, weights, decay)
 
+    def prompt_floats(self, m: int, heads: int, batch: PagedBatch, l_max: Optional[int] = None) -> int:
+        """Workspace floats of ``attend_prompt`` for ``m`` rows."""
+        return ops.paged_prompt_ws_floats(m, heads, self.kv_heads, self.head_dim, batch.n_seq, batch.capacity if l_max is None else l_max)
+
     def attend_prompt(self, i: int, q: torch.Tensor, batch: PagedBatch, l_max: Optional[int] = None,
-                      out: Optional[torch.Tensor] = None, scale: Optional[float] = None) -> torch.Tensor:
-        """The same for many rows a sequence: whole prompts or further pieces of them, packed, whose K and V have been written."""
-        return ops.paged_prompt(self._layers[i], batch, q, self._heads(q), l_max, out, scale)
+                      out: Optional[torch.Tensor] = None, ws: Optional[torch.Tensor] = None, scale: Optional[float] = None) -> torch.Tensor:
+        """The same for many rows a sequence: whole prompts or further pieces of them, packed, whose K and V have been written. ``ws``:
+        fp32, prompt_floats(...)."""
+        return ops.paged_prompt(self._layers[i], batch, q, self._heads(q), l_max, ws, out, scale)
 
     def evict(self, batch: PagedBatch, after: PagedBatch, weights: torch.Tensor, keep: int, recent: int = 0, first: int = 0,
               out_weights: Optional[torch.Tensor] = None, kept: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:

@@ -762,19 +762,32 @@ def paged_attention(cache, batch, q, heads, l_max, span, ws=None, out=None, scal
     return out
 
 
-def paged_prompt(cache, batch, q, heads, l_max, out=None, scale=None):
-    """Causal attention of many rows a sequence over the pages (ssd_paged_prompt_bf16); ``out`` is made here if None."""
+def paged_prompt_ws_floats(m: int, heads: int, kv_heads: int, head_dim: int, n_seq: int, l_max: int) -> int:
+    n = int(_lib.load().ssd_paged_prompt_ws_floats(m, heads, kv_heads, head_dim, n_seq, l_max))
+    if n < 0:
+        raise ValueError(f"paged_prompt_ws_floats: bad m={m} heads={heads} kv_heads={kv_heads} n_seq={n_seq} l_max={l_max}")
+    return n
+
+
+def paged_prompt(cache, batch, q, heads, l_max, ws=None, out=None, scale=None):
+    """Causal attention of many rows a sequence over the pages (ssd_paged_prompt_bf16). ``ws`` (fp32, paged_prompt_ws_floats(...)) and
+    ``out`` are made here if None."""
     dev, hd, m = _batch_dev(cache, batch), cache.head_dim, q.shape[0]
     cols = heads * hd
     pq, ldq = _rows_ptr(q, "q", dev, m, cols)
+    l_max = _l_max(batch, l_max)
     if out is None:
         out, ldo = q.new_empty((m, cols)), cols
         po = out.data_ptr()
     else:
         po, ldo = _rows_ptr(out, "out", dev, m, cols)
+    need = paged_prompt_ws_floats(m, heads, cache.kv_heads, hd, batch.n_seq, l_max)
+    if need and ws is None:
+        ws = torch.empty(need, dtype=F32, device=q.device)
+    pw, n = (None, 0) if ws is None else (_ptr(ws, "ws", F32, dev, 1), ws.numel())
     if m:
-        _lib.call("ssd_paged_prompt_bf16", cache, batch.desc, pq, ldq, m, heads, _l_max(batch, l_max),
-                  hd ** -0.5 if scale is None else float(scale), po, ldo, _stream(dev))
+        _lib.call("ssd_paged_prompt_bf16", cache, batch.desc, pq, ldq, m, heads, l_max, hd ** -0.5 if scale is None else float(scale), pw, n,
+                  po, ldo, _stream(dev))
     return out
 
 

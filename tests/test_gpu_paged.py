@@ -177,6 +177,21 @@ def test_attend_prompt_more_than_64_pages():
     s.check(s.cache.attend_prompt(0, s.q.cuda(), s.batch))
 
 
+@pytest.mark.parametrize("heads,kv,hd", [(32, 8, 128), (15, 5, 128), (16, 16, 64)])
+def test_attend_prompt_of_few_rows_behind_a_long_past(heads, kv, hd):
+    """The length in parts, which some sequences do not reach."""
+    lens, rows = [4400, 900, 64, 3000, 0, 1], [20, 33, 5, 1, 2, 1]
+    s = Setup(lens, rows, heads, kv, hd, seed=30).fill()
+    ws = torch.full((s.cache.prompt_floats(sum(rows), heads, s.batch),), NAN, device="cuda")
+    assert ws.numel()
+    s.check(s.cache.attend_prompt(0, s.q.cuda(), s.batch, ws=ws))
+    s.table[0, 1:40] = -1  # whole parts without a page
+    out = s.cache.attend_prompt(0, s.q.cuda(), s.batch)[:20].double().cpu().view(20, heads, hd)
+    keep = [t for t in range(4400) if not 64 <= t < 40 * 64]
+    want, mag, _, _ = ref.attention(s.q[:20].view(20, heads, hd), s.k[0][keep], s.v[0][keep], [len(keep) - 20 + i for i in range(20)])
+    assert ((out - want).abs() <= 2 ** -8 * want.abs() + 2 ** -7.9 * mag).all()
+
+
 @pytest.mark.parametrize("span", [64, 192, 1024, 4096])
 def test_spans_and_rows_alone_or_in_a_batch(span):
     lens, rows = [1500, 64, 900, 3], [3, 1, 5, 2]

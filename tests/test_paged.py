@@ -84,7 +84,7 @@ def test_bad_descriptors_are_refused_everywhere(kv, batch, code, text):
     c, b = _kv(**kv), _batch(**batch)
     for name, args in (("ssd_paged_write_bf16", (c, b, A, 128, A, 128, 4, None)), ("ssd_paged_read_bf16", (c, b, 4, A, 128, A, 128, None)),
                        ("ssd_paged_attention_bf16", (c, b, A, 256, 4, 4, 64, 64, 0.1, A, 1 << 20, None, 0, 0, 1.0, A, 256, None)),
-                       ("ssd_paged_prompt_bf16", (c, b, A, 256, 4, 4, 64, 0.1, A, 256, None)),
+                       ("ssd_paged_prompt_bf16", (c, b, A, 256, 4, 4, 64, 0.1, A, 1 << 20, A, 256, None)),
                        ("ssd_paged_evict", (c, 1, 1 << 20, b, _batch(), A, 192, 192, 8, 1, 1, A + 4096, A, None))):
         _refused(name, args, code, text)
 
@@ -116,7 +116,7 @@ def test_bad_attention_is_refused(kw, code, text):
              out=A, ldo=256) | kw
     _refused("ssd_paged_attention_bf16", (_kv(), _batch(), *d.values(), None), code, text)
     if not {"ws", "ws_floats", "span", "weights"} & set(kw):
-        args = [d[n] for n in ("q", "ldq", "M", "heads", "l_max", "scale", "out", "ldo")]
+        args = [d[n] for n in ("q", "ldq", "M", "heads", "l_max", "scale", "ws", "ws_floats", "out", "ldo")]
         _refused("ssd_paged_prompt_bf16", (_kv(), _batch(), *args, None), code, text)
 
 
@@ -124,8 +124,8 @@ def test_grids_beyond_a_launch_are_refused():
     big = _batch(n_seq=1 << 24, rows_max=1000)
     _refused("ssd_paged_write_bf16", (_kv(), big, A, 128, A, 128, 1 << 20, None), RANGE, "workgroups")
     _refused("ssd_paged_attention_bf16", (_kv(), big, A, 256, 1 << 20, 4, 64, 64, 0.1, A, 1 << 60, None, 0, 0, 1.0, A, 256, None), RANGE, "workgroups")
-    _refused("ssd_paged_prompt_bf16", (_kv(), big, A, 256, 1 << 20, 4, 64, 0.1, A, 256, None), RANGE, "workgroups")
-    _refused("ssd_paged_prompt_bf16", (_kv(), _batch(), A, 256, 1 << 29, 4, 64, 0.1, A, 256, None), RANGE, "rows")
+    _refused("ssd_paged_prompt_bf16", (_kv(), big, A, 256, 1 << 20, 4, 64, 0.1, A, 1 << 60, A, 256, None), RANGE, "workgroups")
+    _refused("ssd_paged_prompt_bf16", (_kv(), _batch(), A, 256, 1 << 29, 4, 64, 0.1, A, 1 << 60, A, 256, None), RANGE, "rows")
     _refused("ssd_paged_evict", (_kv(), 64, 1 << 20, big, _batch(n_seq=1 << 24), A, 192, 192, 8, 1, 1, A + 4096, A, None), RANGE, "workgroups")
 
 
@@ -159,6 +159,17 @@ def test_bad_logprobs_are_refused(kw, code, text):
     d = dict(logits=A, dtype=0, ld=128256, M=3, V=128256, tokens=A, tokens64=0, top=5, ws=A, ws_bytes=1 << 20, logprobs=A, entropy=A, rank=A,
              top_ids=A, top_logprobs=A) | kw
     _refused("ssd_token_logprobs", (*d.values(), None), code, text)
+
+
+def test_a_prompt_call_that_cuts_the_length_needs_its_workspace():
+    from ssd import ops
+
+    b = _batch(table_cols=128, ld_table=128)
+    assert ops.paged_prompt_ws_floats(4, 4, 2, 64, 2, 8192) > 0 and ops.paged_prompt_ws_floats(4, 4, 2, 64, 2, 400) == 0
+    assert ops.paged_prompt_ws_floats(8192, 32, 8, 128, 1, 8192) == 0
+    call = lambda ws, n: (_kv(), b, A, 256, 4, 4, 8192, 0.1, ws, n, A, 256, None)  # noqa: E731
+    for ws, n in ((None, 1 << 20), (A, 100), (A + 4, 1 << 20)):
+        _refused("ssd_paged_prompt_bf16", call(ws, n), BAD, "workspace")
 
 
 def test_workspace_sizes():
