@@ -4,8 +4,12 @@
 // (m, z, t) of the columns it has seen and rescales them when its maximum grows; threads, then chunks of a row, are added with
 // weights from their largest m.
 // The k alternatives: the maxima of 64 groups of threads are values of the row, so its k-th largest value is at least the k-th
-// largest of them; only the few threads whose maximum reaches that bound look at their columns again (a wave together), what
-// reaches it is collected, and a value's place is the number of those above it. Equal values rank by column, lowest first.
+// largest of them; only the few threads whose maximum reaches that bound look at their columns again (from registers, or a wave
+// together), what reaches it is collected, and a value's place is the number of those above it. Equal values rank by column, lowest
+// first. More candidates than the list holds (rows of equal logits) take a pass over the chunk for each place.
+// What bounds it: bytes and the vector pipe (about 13 operations a column): 1800 rows of 50257 fp32 columns 66 us, 5.4 TB/s; 1400
+// of 128256 bf16 columns 80 without alternatives, 4.5 TB/s, and 83 with 5. For few rows the latency of two launches and their
+// steps: 25 rows of 128256 bf16 columns 6.9 us without alternatives, 13.5 with 5.
 #include "topk.h"
 
 #include <algorithm>
@@ -57,6 +61,31 @@ __device__ __forceinline__ LpSum lp_add(const LpSum& a, const LpSum& b) {
   return LpSum{m, x.z + y.z, x.t + y.t};
 }
 
+// f over a wave's lanes, the same on all: DPP exchanges within 16 lanes, then the swaps across them.
+template <typename F>
+__device__ __forceinline__ uint32_t lp_wave(uint32_t v, F f) {
+  v = f(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xb1, 0xf, 0xf, true));   // lane ^ 1
+  v = f(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4e, 0xf, 0xf, true));   // lane ^ 2
+  v = f(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xf, 0xf, true));  // the other half of 8
+  v = f(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x140, 0xf, 0xf, true));  // the other half of 16
+  auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = f(r[0], r[1]);
+  r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return f(r[0], r[1]);
+}
+__device__ __forceinline__ float lp_wave_sum(float v) {
+  return __uint_as_float(lp_wave(__float_as_uint(v), [](uint32_t a, uint32_t b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); }));
+}
+__device__ __forceinline__ int lp_wave_sum(int v) {
+  return (int)lp_wave((uint32_t)v, [](uint32_t a, uint32_t b) { return a + b; });
+}
+__device__ __forceinline__ LpSum lp_wave_add(const LpSum& s) {
+  const float m = __uint_as_float(
+      lp_wave(__float_as_uint(s.m), [](uint32_t a, uint32_t b) { return __float_as_uint(lp_max(__uint_as_float(a), __uint_as_float(b))); }));
+  const LpSum x = lp_rescale(s, m);
+  return LpSum{m, lp_wave_sum(x.z), lp_wave_sum(x.t)};
+}
+
 template <typename T, int E>
 __device__ __forceinline__ void lp_unpack(const uint4& u, float (&x)[E]) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
@@ -101,6 +130,7 @@ __device__ __forceinline__ void lp_places(const uint64_t* list, int n, int k, ui
   for (int i = threadIdx.x; i < n; i += 256) {
     const uint64_t mine = list[i];
     int above = 0;
+#pragma unroll 4
     for (int q = 0; q < n; ++q) above += list[q] > mine;
     if (above < k) best[above] = mine;
   }
@@ -125,7 +155,7 @@ __device__ __forceinline__ void lp_write(const LogprobArgs& a, int row, const Lp
 struct LpShared {
   LpSum part[4];
   int ahead[4];
-  float group[64];
+  alignas(16) float group[64];
   uint64_t best[LP_TOP], wave[4];
   int n;
   uint64_t list[LP_LIST];
@@ -138,41 +168,43 @@ __global__ __launch_bounds__(256) void lp_chunk_kernel(LogprobArgs a) {
   const int row = blockIdx.x / a.chunks, ch = blockIdx.x % a.chunks, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const LpRow<T> r(a, row);
   const int v0 = ch * a.vecs, v1 = min(v0 + a.vecs, r.vecs);
+  // a batch's absent vectors are all -inf; the first batch is on its way before the token's chain of two loads
+  constexpr uint32_t NONE = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, _Float16>::value ? 0xfc00fc00u : 0xff80ff80u;
+  uint4 u[U];
+  auto load = [&](int v) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) u[i] = v + 256 * i < v1 ? r.load(v + 256 * i) : make_uint4(NONE, NONE, NONE, NONE);
+  };
+  load(v0 + tid);
   const int tok = lp_token(a, row);
   const float xt = tok >= 0 ? lp_one(r.p + tok) : 0.f;
   LpSum s{-INFINITY, 0.f, 0.f};
   int ahead = 0;
-  auto fold = [&](const float (&x)[32], int n) {  // n: of them there, whole vectors
-    float top = -INFINITY;
+  auto fold = [&](const float (&x)[32]) {
+    float top = x[0];
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (i < n) top = lp_max(top, x[i]);
+    for (int i = 1; i < 32; ++i) top = lp_max(top, x[i]);
     const float m = lp_max(s.m, top);
     if (__any(m != s.m)) s = lp_rescale(s, m);
     const float ref = m == -INFINITY ? 0.f : m * LP_LOG2E;
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (i < n) {
-        const float y = fmaxf(fmaf(x[i], LP_LOG2E, -ref), -1e4f);  // -inf: a weight of 0, and 0 times it
-        const float e = __builtin_amdgcn_exp2f(y);
-        s.z += e;
-        s.t = fmaf(e, y, s.t);
-      }
-  };
-  auto count = [&](const float* x, int col) {  // a vector
-    if (col + E <= tok) {
-#pragma unroll
-      for (int i = 0; i < E; ++i) ahead += x[i] >= xt;
-    } else {
-#pragma unroll
-      for (int i = 0; i < E; ++i) ahead += x[i] > xt || (x[i] == xt && col + i < tok);
+    for (int i = 0; i < 32; ++i) {
+      const float y = fmaxf(fmaf(x[i], LP_LOG2E, -ref), -1e4f);  // -inf: a weight of 0, and 0 times it
+      const float e = __builtin_amdgcn_exp2f(y);
+      s.z += e;
+      s.t = fmaf(e, y, s.t);
     }
   };
-  int v = v0 + tid;
-  for (; v + 256 * (U - 1) < v1; v += 256 * U) {
-    uint4 u[U];
-#pragma unroll
-    for (int i = 0; i < U; ++i) u[i] = r.load(v + 256 * i);
+  // Columns before the token rank before it from its value on, those behind it above its value: not (x <= the next smaller float) and
+  // not (x <= it). The token's own vector counts as behind; its columns before the token are looked at one by one.
+  const uint32_t xb = __float_as_uint(xt + 0.f);
+  const float under = xt == -INFINITY ? __uint_as_float(0x7fc00000u) : __uint_as_float(xb == 0 ? 0x80000001u : (xb >> 31) ? xb + 1 : xb - 1);
+  {
+    const int tv = tok >= r.head ? (tok - r.head) / E : -1, c = r.column(tv) + tid;
+    if (tv >= v0 && tv < v1 && c < tok) ahead += lp_one(r.p + c) == xt;
+  }
+  for (int v = v0 + tid; v < v1; v += 256 * U) {
+    if (v != v0 + tid) load(v);
     float x[32];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
@@ -181,17 +213,14 @@ __global__ __launch_bounds__(256) void lp_chunk_kernel(LogprobArgs a) {
 #pragma unroll
       for (int e = 0; e < E; ++e) x[i * E + e] = y[e];
     }
-    fold(x, 32);
+    fold(x);
 #pragma unroll
-    for (int i = 0; i < U; ++i) count(x + i * E, r.column(v + 256 * i));
-  }
-  for (; v < v1; v += 256) {
-    float y[E], x[32];
-    lp_unpack<T, E>(r.load(v), y);
+    for (int i = 0; i < U; ++i) {
+      const int vi = v + 256 * i;
+      const float over = vi >= v1 ? INFINITY : r.column(vi) + E <= tok ? under : xt;
 #pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = y[e];
-    fold(x, E);
-    count(x, r.column(v));
+      for (int e = 0; e < E; ++e) ahead += !(x[i * E + e] <= over);
+    }
   }
   const bool has = ch == 0 && tid < r.extra;  // one column of head or tail
   const int xcol = has ? r.extra_column(tid) : 0;
@@ -202,12 +231,8 @@ __global__ __launch_bounds__(256) void lp_chunk_kernel(LogprobArgs a) {
     ahead += xone > xt || (xone == xt && xcol < tok);
   }
   const float own = s.m;  // the largest of this thread's columns
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const LpSum q{__shfl_xor(s.m, o), __shfl_xor(s.z, o), __shfl_xor(s.t, o)};
-    s = lp_add(s, q);
-    ahead += __shfl_xor(ahead, o);
-  }
+  s = lp_wave_add(s);
+  ahead = lp_wave_sum(ahead);
   if (lane == 0) sh.part[w] = s, sh.ahead[w] = ahead;
   if (TOP) {
     float gm = lp_max(own, __shfl_xor(own, 1));
@@ -224,7 +249,12 @@ __global__ __launch_bounds__(256) void lp_chunk_kernel(LogprobArgs a) {
     if (!slow) {
       const float mine = sh.group[lane];
       int above = 0;
-      for (int i = 0; i < 64; ++i) above += sh.group[i] > mine || (sh.group[i] == mine && i < lane);
+#pragma unroll
+      for (int i = 0; i < 64; i += 4) {
+        const f32x4_t x = *(const f32x4_t*)&sh.group[i];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) above += x[e] > mine || (x[e] == mine && i + e < lane);
+      }
       const float bound = __shfl(mine, __builtin_ctzll(__ballot(above == a.top - 1)));
       auto collect = [&](float y, int col) {
         if (y >= bound) {
@@ -232,13 +262,26 @@ __global__ __launch_bounds__(256) void lp_chunk_kernel(LogprobArgs a) {
           if (at < LP_LIST) sh.list[at] = rank_key(y + 0.f, col);  // -0 ranks as 0
         }
       };
-      for (uint64_t who = __ballot(own >= bound); who; who &= who - 1) {
-        const int l = __builtin_ctzll(who);
-        for (int q = v0 + 64 * w + l + 256 * lane; q < v1; q += 256 * 64) {
-          float y[E];
-          lp_unpack<T, E>(r.load(q), y);
+      // the columns of a vector that reach the bound, one after the other
+      auto pick = [&](const uint4& w4, int col) {
+        float y[E];
+        lp_unpack<T, E>(w4, y);
+        uint32_t hit = 0;
 #pragma unroll
-          for (int e = 0; e < E; ++e) collect(y[e], r.column(q) + e);
+        for (int e = 0; e < E; ++e) hit |= (y[e] >= bound ? 1u : 0u) << e;
+        for (; hit; hit &= hit - 1) {
+          const int c = col + __builtin_ctz(hit);
+          collect(lp_one(r.p + c), c);
+        }
+      };
+      if (v1 - v0 <= 256 * U) {  // one batch, still in registers
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+          if (v0 + tid + 256 * i < v1) pick(u[i], r.column(v0 + tid + 256 * i));
+      } else {
+        for (uint64_t who = __ballot(own >= bound); who; who &= who - 1) {
+          const int l = __builtin_ctzll(who);
+          for (int q = v0 + 64 * w + l + 256 * lane; q < v1; q += 256 * 64) pick(r.load(q), r.column(q));
         }
       }
       if (has) collect(xone, xcol);
@@ -254,12 +297,7 @@ __global__ __launch_bounds__(256) void lp_chunk_kernel(LogprobArgs a) {
           const uint64_t key = rank_key(y + 0.f, col);
           if (key < below && key > most) most = key;
         };
-        for (int q = v0 + tid; q < v1; q += 256) {
-          float y[E];
-          lp_unpack<T, E>(r.load(q), y);
-#pragma unroll
-          for (int e = 0; e < E; ++e) look(y[e], r.column(q) + e);
-        }
+        for (int c = r.column(v0) + tid; c < r.column(v1); c += 256) look(lp_one(r.p + c), c);
         if (has) look(xone, xcol);
         most = wave_max_u64(most);
         __syncthreads();
@@ -281,57 +319,51 @@ __global__ __launch_bounds__(256) void lp_chunk_kernel(LogprobArgs a) {
   if (TOP && tid < a.top) ((uint64_t*)(rec + sizeof(LpRecord)))[tid] = sh.best[tid];
 }
 
-// Adds up a row's chunks, in order of the lanes; their keys' places are found among those that reach the k-th best first key.
+// Adds up a row's chunks; their keys' places are found among those that reach the k-th best of the chunks' first ones.
 __global__ __launch_bounds__(256) void lp_merge_kernel(LogprobArgs a) {
-  __shared__ uint64_t list[LP_CHUNKS * LP_TOP], first[LP_CHUNKS], best[LP_TOP];
+  __shared__ uint64_t all[LP_CHUNKS * LP_TOP], list[LP_CHUNKS * LP_TOP], best[LP_TOP];
   __shared__ int n;
-  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, keys = a.chunks * a.top;
   const int64_t size = lp_record_bytes(a.top);
   const char* rec = a.ws + (int64_t)row * a.chunks * size;
   const int tok = lp_token(a, row);
-  LpSum s{-INFINITY, 0.f, 0.f};
-  int ahead = 0;
-  if (lane < a.chunks) {
-    const LpRecord x = *(const LpRecord*)(rec + lane * size);
-    s = x.sum, ahead = x.ahead;
-  }
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const LpSum q{__shfl_xor(s.m, o), __shfl_xor(s.z, o), __shfl_xor(s.t, o)};
-    s = lp_add(s, q);
-    ahead += __shfl_xor(ahead, o);
-  }
+  for (int i = tid; i < keys; i += 256) all[i] = ((const uint64_t*)(rec + i / a.top * size + sizeof(LpRecord)))[i % a.top];
+  const LpRecord x = *(const LpRecord*)(rec + min(lane, a.chunks - 1) * size);
+  const LpSum s = lp_wave_add(lane < a.chunks ? x.sum : LpSum{-INFINITY, 0.f, 0.f});
+  const int ahead = lp_wave_sum(lane < a.chunks ? x.ahead : 0);
   if (a.top) {
-    auto key = [&](int c, int k) { return ((const uint64_t*)(rec + c * size + sizeof(LpRecord)))[k]; };
-    if (tid < a.chunks) first[tid] = key(tid, 0);
     if (tid == 0) n = 0;
     if (tid < LP_TOP) best[tid] = 0;
     __syncthreads();
-    uint64_t bound = 1;
-    if (a.chunks >= a.top) {
-      const uint64_t mine = lane < a.chunks ? first[lane] : 0;
-      int above = 0;
-      for (int i = 0; i < a.chunks; ++i) above += first[i] > mine || (first[i] == mine && i < lane);
-      const int l = __builtin_ctzll(__ballot(above == a.top - 1));
-      bound = max(bound, (uint64_t)__shfl((uint32_t)(mine >> 32), l) << 32 | __shfl((uint32_t)mine, l));
+    // the chunks' first keys, as many of each as make `top` or more; 0 for no column
+    const int firsts = a.chunks * ((a.top + a.chunks - 1) / a.chunks);  // fewer than 64, or a.chunks
+    const uint64_t mine = lane < firsts ? all[lane % a.chunks * a.top + lane / a.chunks] : 0;
+    int above = 0;
+    for (int i = 0; i < firsts; ++i) {
+      const uint64_t y = (uint64_t)__builtin_amdgcn_readlane((uint32_t)(mine >> 32), i) << 32 | (uint32_t)__builtin_amdgcn_readlane((uint32_t)mine, i);
+      above += y > mine || (y == mine && i < lane);
     }
-    for (int i = tid; i < a.chunks * a.top; i += 256) {
-      const uint64_t x = key(i / a.top, i % a.top);
-      if (x >= bound) list[atomicAdd(&n, 1)] = x;
-    }
+    const int l = __builtin_ctzll(__ballot(above == a.top - 1));
+    const uint64_t bound = max((uint64_t)1, (uint64_t)__builtin_amdgcn_readlane((uint32_t)(mine >> 32), l) << 32 |
+                                                (uint32_t)__builtin_amdgcn_readlane((uint32_t)mine, l));
+    for (int i = tid; i < keys; i += 256)
+      if (all[i] >= bound) list[atomicAdd(&n, 1)] = all[i];
     __syncthreads();
     lp_places(list, n, a.top, best);
     __syncthreads();
   }
-  lp_write(a, row, s, ahead, ((const LpRecord*)rec)->xt, tok, best);
+  lp_write(a, row, s, ahead, x.xt, tok, best);
 }
 
-// Chunks of a row: one where the rows fill the chip (four workgroups a CU and more), else as many as bring 1024 workgroups, of 1024
-// vectors at least.
+// Chunks of a row. A workgroup takes about 6 us and 0.7 for each batch of 1024 vectors, the second launch 4 to 6, so short rows, and those of
+// many rows, are one chunk; else as many as bring 1024 workgroups, or of one batch each where those are at most twice as many.
+// us at 128256 bf16 columns and 5 alternatives, 1 / 4 / 16 chunks: 1 row 22 / 15 / 12, 64 23 / 17 / 16, 300 35 / 31 / 49, 500
+// 38 / 41 / 74; 300 rows of 32000 columns 16 / 20 / 42.
 static int lp_chunks(int M, int V, int elem) {
-  const int64_t vecs = ((int64_t)V * elem + 15) / 16;
-  const int64_t want = (1024 + M - 1) / std::max(M, 1), most = (vecs + 1023) / 1024;
-  return (int)std::max<int64_t>(1, std::min<int64_t>({want, most, LP_CHUNKS}));
+  const int64_t batches = (((int64_t)V * elem + 15) / 16 + 1023) / 1024;
+  if (M >= 400 || batches < 8) return 1;
+  const int64_t want = (1024 + M - 1) / std::max(M, 1);
+  return (int)std::min<int64_t>(2 * want >= batches ? batches : want, LP_CHUNKS);
 }
 
 }  // namespace ssd

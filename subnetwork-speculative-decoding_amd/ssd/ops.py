@@ -8,6 +8,7 @@ device, alignment, shapes) before a launch, so a bad call raises instead of faul
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional
 
 import torch
@@ -840,18 +841,18 @@ def token_logprobs(logits, tokens, top=0, ws=None):
     need = token_logprobs_ws_bytes(m, V, logits.dtype, top)
     if need and ws is None:
         ws = torch.empty(need, dtype=torch.uint8, device=logits.device)
-    f32 = torch.empty((2, m), dtype=F32, device=logits.device)
-    rank = torch.empty(m, dtype=I32, device=logits.device)
+    pw, size = (None, 0) if ws is None else (_ptr(ws, "ws", torch.uint8, dev), ws.numel())
     ids = torch.empty((m, top), dtype=I32, device=logits.device)
     lps = torch.empty((m, top), dtype=F32, device=logits.device)
+    rank, logprobs, entropy = ids.new_empty(m), lps.new_empty(m), lps.new_empty(m)
     if m:
         _lib.call("ssd_token_logprobs", logits.data_ptr(), kind, logits.stride(0) if m > 1 else V, m, V, tokens.data_ptr(),
-                  int(tokens.dtype == torch.int64), top, None if ws is None else _ptr(ws, "ws", torch.uint8, dev, need),
-                  0 if ws is None else ws.numel(), f32[0].data_ptr(), f32[1].data_ptr(), rank.data_ptr(), ids.data_ptr(),
-                  lps.data_ptr(), _stream(dev))
-    return f32[0], f32[1], rank, ids, lps
+                  1 if tokens.dtype is torch.int64 else 0, top, pw, size, logprobs.data_ptr(), entropy.data_ptr(), rank.data_ptr(),
+                  ids.data_ptr(), lps.data_ptr(), _stream(dev))
+    return logprobs, entropy, rank, ids, lps
 
 
+@functools.lru_cache(maxsize=256)
 def token_logprobs_ws_bytes(m: int, V: int, dtype, top: int = 0) -> int:
     if dtype not in _LOGIT_TYPES:
         raise ValueError(f"token_logprobs: logits of {dtype} (bfloat16, float16, float32)")
