@@ -145,16 +145,16 @@ __global__ __launch_bounds__(256, 2) void paged_fold_kernel(PagedAttnArgs a) {
   const int kvh = u % a.c.kv;
   u /= a.c.kv;
   const int grp = u % a.n_grps, seq = u / a.n_grps;
+  const int b0 = grp * PA_WAVES * a.span_blk, blk = b0 + w + PA_WAVES * lane;
+  // lane i has the page of this wave's block i; the table is read before the lengths are known, a chain of loads less
+  int mine = lane < a.span_blk && blk * PAGE < a.l_cap ? paged_page(a.b, seq, blk, a.c.pages) : -1;
   const PagedRows r = paged_rows(a.b, seq, a.M);
   const int n_cols = r.n * a.rep, c0 = set * 16;
   if (c0 >= n_cols) return;
   const int last = min(c0 + 15, n_cols - 1);
   const int lim_lo = min(r.first + c0 / a.rep, a.l_cap - 1), lim_hi = min(r.first + last / a.rep, a.l_cap - 1);
-  const int b0 = grp * PA_WAVES * a.span_blk;
   if (a.n_grps > 1 && b0 * PAGE > lim_hi) return;  // no record: the second launch counts them as this does
-  // lane i has the page of this wave's block i
   const int nb = lim_hi < 0 ? 0 : min(max((lim_hi / PAGE - b0 - w) / PA_WAVES + (lim_hi / PAGE - b0 - w >= 0), 0), a.span_blk);
-  const int mine = lane < nb ? paged_page(a.b, seq, b0 + w + PA_WAVES * lane, a.c.pages) : -1;
   const int col = min(c0 + j, n_cols - 1), row = r.r0 + col / a.rep, head = kvh * a.rep + col % a.rep;
   const int lim = min(r.first + col / a.rep, a.l_cap - 1);
   if (threadIdx.x < HD) lds.first_bad[threadIdx.x] = INT32_MAX;
@@ -164,13 +164,13 @@ __global__ __launch_bounds__(256, 2) void paged_fold_kernel(PagedAttnArgs a) {
 #pragma unroll
   for (int dt = 0; dt < HD / 16; ++dt) st.o[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   if (nb > 0) {
-    u32x4_t qf[HD / 32];
-#pragma unroll
-    for (int ks = 0; ks < HD / 32; ++ks) qf[ks] = *(const u32x4_t*)(a.Q + row * a.ldq + head * HD + ks * 32 + g * 8);
     auto at = [&](int i) { return ((size_t)max(__builtin_amdgcn_readlane(mine, i), 0) * a.c.kv + kvh) * PAGE * HD; };
     PagedFrags<HD> f;
     paged_load_k<HD>(f, a.c.k, at(0), lane);
     paged_load_v<HD>(f, a.c.v, at(0), lane);
+    u32x4_t qf[HD / 32];
+#pragma unroll
+    for (int ks = 0; ks < HD / 32; ++ks) qf[ks] = *(const u32x4_t*)(a.Q + row * a.ldq + head * HD + ks * 32 + g * 8);
     for (int i = 0; i < nb; ++i) {
       const int key0 = (b0 + w + PA_WAVES * i) * PAGE;
       const bool gone = __builtin_amdgcn_readlane(mine, i) < 0;  // no such page: none of its slots is attended
@@ -267,15 +267,17 @@ __device__ __forceinline__ float2 paged_total(const float2* ml, int ng, int part
   return make_float2(m, l);
 }
 
-// Second launch. The first join_wgs workgroups add up the records: a wave per (sequence, row, head), which takes them in order.
-// The others add the received weights of 1024 slots of a (sequence, kv head), a thread four slots.
-template <int HD, bool WEIGHTS>
+// Second launch. The first join_wgs workgroups add up the records: WPP waves a (sequence, row, head), each a run of groups in order, the
+// waves' sums then in order. The others (WK > 0) add the received weights of 1024 / WK slots of a (sequence, kv head): a lane four slots; WK
+// waves share its (row, head) pairs, a run each, and their sums are added in order.
+template <int HD, int WK, int WPP>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int grp_keys = a.grp_keys;
   if ((int)blockIdx.x < a.join_wgs) {
     constexpr int V = HD / 64;  // dims a lane
-    int u = blockIdx.x * 4 + w;
+    __shared__ float part[4][HD];
+    int u = WPP == 4 ? blockIdx.x : blockIdx.x * 4 + w;
     const int h = u % a.heads;
     u /= a.heads;
     const int i = u % a.b.rows_max, s = u / a.b.rows_max;
@@ -288,9 +290,10 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
     const float* o = a.ws_o + (row * a.heads + h) * a.n_grps * HD + lane * V;
     const float2 all = paged_total(ml, ng, lane, 64);
     float acc[V] = {};
-    for (int g0 = 0; g0 < ng; g0 += 64) {
-      const float wg = g0 + lane < ng ? paged_weight(ml[g0 + lane].x, all.x) : 0.f;
-      const int n = min(64, ng - g0);
+    const int run = WPP == 4 ? (ng + 3) / 4 : ng, from = WPP == 4 ? w * run : 0, to = min(from + run, ng);
+    for (int g0 = from; g0 < to; g0 += 64) {
+      const float wg = g0 + lane < to ? paged_weight(ml[g0 + lane].x, all.x) : 0.f;
+      const int n = min(64, to - g0);
       for (int q = 0; q < n; q += 8) {
         float x[8][V];
 #pragma unroll
@@ -305,6 +308,14 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
         }
       }
     }
+    if constexpr (WPP == 4) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) part[w][lane * V + v] = acc[v];
+      __syncthreads();
+      if (w) return;
+#pragma unroll
+      for (int v = 0; v < V; ++v) acc[v] = ((acc[v] + part[1][lane * V + v]) + part[2][lane * V + v]) + part[3][lane * V + v];
+    }
 #pragma unroll
     for (int v = 0; v < V; ++v) acc[v] = all.y == 0.f ? 0.f : acc[v] / all.y;
     bf16_t* dst = a.out + row * a.ldo + h * HD + lane * V;
@@ -312,17 +323,19 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
     else *dst = f2bf(acc[0]);
     return;
   }
-  if constexpr (WEIGHTS) {
+  if constexpr (WK > 0) {
+    constexpr int CHUNK = 1024 / WK;
     __shared__ float2 total[256];  // (m, 1 / l) of up to 256 (row, head) pairs
+    __shared__ __align__(16) float sums[WK][CHUNK];
     int u = blockIdx.x - a.join_wgs;
     const int ch = u % a.chunks;
     u /= a.chunks;
     const int kvh = u % a.c.kv, s = u / a.c.kv;
     const PagedRows r = paged_rows(a.b, s, a.M);
     const int end = min(r.first + r.n, a.l_cap);  // slots in use
-    if (r.n == 0 || ch * 1024 >= end) return;
-    const int key = ch * 1024 + threadIdx.x * 4, pairs = r.n * a.rep;
-    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    if (r.n == 0 || ch * CHUNK >= end) return;
+    const int key = ch * CHUNK + (WK == 4 ? lane : threadIdx.x) * 4, pairs = r.n * a.rep;
+    f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
     for (int p0 = 0; p0 < pairs; p0 += 256) {
       const int np = min(256, pairs - p0);
       int lg = 64;
@@ -336,22 +349,57 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
         if (p < np && threadIdx.x % lg == 0) total[p] = make_float2(t.x, t.y == 0.f ? 0.f : 1.f / t.y);
       }
       __syncthreads();
-      if (key < end)
-        for (int p = 0; p < np; ++p) {
-          const int pc = p0 + p, lim = min(r.first + pc / a.rep, a.l_cap - 1);
-          if (key > lim) continue;
-          const f32x4_t x = *(const f32x4_t*)(a.ws_s + ((int64_t)(r.r0 + pc / a.rep) * a.heads + kvh * a.rep + pc % a.rep) * a.ld_s + key);
-          const float2 t = total[p];
+      const int run = (np + WK - 1) / WK, from = WK == 4 ? w * run : 0, to = min(from + run, np);
+      for (int p = from; p < to; p += 4) {  // four pairs' scores on their way at once; a pair past the last one repeats it and does not count
+        f32x4_t x[4];
+        int lim[4];
+        float2 t[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (key + e <= lim && x[e] != -INFINITY) sum[e] = fmaf(__builtin_amdgcn_exp2f(fmaf(x[e], a.scale_log2, -t.x)), t.y, sum[e]);
+        for (int e = 0; e < 4; ++e) {
+          const int pc = p0 + min(p + e, to - 1), i = pc / a.rep;
+          lim[e] = p + e < to ? min(r.first + i, a.l_cap - 1) : -1;
+          t[e] = total[pc - p0];
+          // slots that no block holds (behind the bound's last one) read the row's first
+          x[e] = *(const f32x4_t*)(a.ws_s + ((int64_t)(r.r0 + i) * a.heads + kvh * a.rep + pc % a.rep) * a.ld_s + (key < a.ld_s ? key : 0));
         }
-    }
-    float* dst = a.weights + s * a.ldw_seq + kvh * a.ldw + key;
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (key + e < end) dst[e] = a.decay == 0.f ? sum[e] : fmaf(a.decay, dst[e], sum[e]);
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {  // scores of slots that are not attended may be anything
+            const float wgt = __builtin_amdgcn_exp2f(fmaf(x[e][q], a.scale_log2, -t[e].x)) * t[e].y;
+            sum[q] += key + q <= lim[e] && x[e][q] != -INFINITY ? wgt : 0.f;
+          }
+      }
+    }
+    float* dst = a.weights + s * a.ldw_seq + kvh * a.ldw;
+    if constexpr (WK == 4) {
+      *(f32x4_t*)&sums[w][lane * 4] = sum;
+      __syncthreads();
+      const int x = threadIdx.x, at = ch * CHUNK + x;
+      if (at >= end) return;
+      const float y = ((sums[0][x] + sums[1][x]) + sums[2][x]) + sums[3][x];
+      dst[at] = a.decay == 0.f ? y : fmaf(a.decay, dst[at], y);
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (key + q < end) dst[key + q] = a.decay == 0.f ? sum[q] : fmaf(a.decay, dst[key + q], sum[q]);
+    }
   }
+}
+
+// Second launch of WK waves a set of slots (0: no weights). Waves a (row, head): four where few pairs have many records (us of one row of 32
+// heads with 64 records, one wave / four: 8.9 / 5.5).
+template <int HD, int WK>
+static int launch_paged_join(PagedAttnArgs& a, hipStream_t stream) {
+  const int64_t pairs = a.n_grps > 1 ? (int64_t)a.b.n_seq * a.b.rows_max * a.heads : 0;
+  a.chunks = WK ? (int)(((int64_t)a.l_cap * WK + 1023) / 1024) : 0;
+  const bool four = a.n_grps > 8 && pairs <= 2048;
+  const int64_t join = four ? pairs : (pairs + 3) / 4, all = join + (int64_t)a.b.n_seq * a.c.kv * a.chunks;
+  if (paged_grid_too_large(all, 256)) return set_error(SSD_ERANGE, "paged_attention: too many workgroups");
+  a.join_wgs = (int)join;
+  if (four) SSD_LAUNCH((paged_join_kernel<HD, WK, 4>), dim3((unsigned)all), dim3(256), 0, stream, a);
+  else SSD_LAUNCH((paged_join_kernel<HD, WK, 1>), dim3((unsigned)all), dim3(256), 0, stream, a);
+  return check_launch("paged_attention_join");
 }
 
 static int paged_groups(int64_t l_max, int span) { return (int)((l_max + (int64_t)PA_WAVES * span - 1) / ((int64_t)PA_WAVES * span)); }
@@ -362,17 +410,17 @@ static int launch_paged_attn(PagedAttnArgs a, hipStream_t stream) {
   const int tiles = (int)(((int64_t)a.b.rows_max * a.rep + 15) / 16);
   a.sets = tiles;
   const int64_t units = (int64_t)a.b.n_seq * a.n_grps * a.c.kv, grid = (units + 7) / 8 * 8 * tiles;
-  const int64_t pairs = (int64_t)a.b.n_seq * a.b.rows_max * a.heads, join = a.n_grps > 1 ? (pairs + 3) / 4 : 0;
-  a.chunks = WEIGHTS ? (a.l_cap + 1023) / 1024 : 0;
-  const int64_t extra = (int64_t)a.b.n_seq * a.c.kv * a.chunks;
-  if (units > INT32_MAX || paged_grid_too_large(grid, 256) || paged_grid_too_large(join + extra, 256))
+  if (units > INT32_MAX || paged_grid_too_large(grid, 256)) return set_error(SSD_ERANGE, "paged_attention: too many workgroups");
+  a.units = (int)units;
+  // the second launch's size is checked before the first is enqueued
+  if (paged_grid_too_large((int64_t)a.b.n_seq * (a.b.rows_max * (int64_t)a.heads + (WEIGHTS ? a.c.kv * (int64_t)(a.l_cap / 256 + 1) : 0)), 256))
     return set_error(SSD_ERANGE, "paged_attention: too many workgroups");
-  a.units = (int)units, a.join_wgs = (int)join;
   SSD_LAUNCH((paged_fold_kernel<HD, WEIGHTS>), dim3((unsigned)grid), dim3(256), 0, stream, a);
   if (int rc = check_launch("paged_attention_fold")) return rc;
-  if (join + extra == 0) return SSD_OK;
-  SSD_LAUNCH((paged_join_kernel<HD, WEIGHTS>), dim3((unsigned)(join + extra)), dim3(256), 0, stream, a);
-  return check_launch("paged_attention_join");
+  // Received weights: the waves of a workgroup share the (row, head) pairs of a set of slots where there are many (us of the second launch, a
+  // wave / four: 6 x 16 rows, 4 heads a kv head, 4000 keys 39 / 12; 24 sequences of one row, 3 heads, 4000 keys 6.1 / 9.7).
+  if constexpr (WEIGHTS) return a.b.rows_max * a.rep > 16 ? launch_paged_join<HD, 4>(a, stream) : launch_paged_join<HD, 1>(a, stream);
+  return a.n_grps > 1 ? launch_paged_join<HD, 0>(a, stream) : SSD_OK;
 }
 
 int paged_join(const PagedBatch& b, int M, int heads, int head_dim, int l_cap, int grp_keys, int n_grps, float* ws_o, float2* ws_ml,
@@ -381,12 +429,7 @@ int paged_join(const PagedBatch& b, int M, int heads, int head_dim, int l_cap, i
   a.b = b, a.M = M, a.heads = heads, a.l_cap = l_cap, a.grp_keys = grp_keys, a.n_grps = n_grps;
   a.b.rows_max = std::min(b.rows_max, M);
   a.ws_o = ws_o, a.ws_ml = ws_ml, a.out = out, a.ldo = ldo;
-  const int64_t join = ((int64_t)b.n_seq * a.b.rows_max * heads + 3) / 4;
-  if (paged_grid_too_large(join, 256)) return set_error(SSD_ERANGE, "paged_attention_join: too many workgroups");
-  a.join_wgs = (int)join;
-  if (head_dim == 64) SSD_LAUNCH((paged_join_kernel<64, false>), dim3((unsigned)join), dim3(256), 0, stream, a);
-  else SSD_LAUNCH((paged_join_kernel<128, false>), dim3((unsigned)join), dim3(256), 0, stream, a);
-  return check_launch("paged_attention_join");
+  return head_dim == 64 ? launch_paged_join<64, 0>(a, stream) : launch_paged_join<128, 0>(a, stream);
 }
 
 }  // namespace ssd

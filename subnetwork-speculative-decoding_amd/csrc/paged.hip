@@ -261,7 +261,7 @@ __global__ __launch_bounds__(EV_T) void evict_select_kernel(EvictArgs a) {
 }
 
 // A workgroup per (layer, sequence, destination page, kv head) gathers the page's rows. Every 16-byte piece of V holds 8 slots of a
-// dim, which come from 8 places.
+// dim, which come from up to 8 places.
 template <int HD>
 __global__ __launch_bounds__(256) void evict_gather_kernel(EvictArgs a) {
   constexpr int PC = HD / 8;
@@ -295,21 +295,37 @@ __global__ __launch_bounds__(256) void evict_gather_kernel(EvictArgs a) {
   const bf16_t *K = a.c.k + layer * a.layer_elems, *V = a.c.v + layer * a.layer_elems;
   const size_t at = layer * a.layer_elems + ((size_t)page * a.c.kv + kvh) * PAGE * HD;
   auto from = [&](int o) { return ((size_t)max(src_page[o], 0) * a.c.kv + kvh) * PAGE * HD; };
-  for (int i = tid; i < PAGE * PC; i += 256) {
-    const int o = i % PAGE, d = i / PAGE * 8;
-    if (src_slot[o] < 0) continue;
-    uint4 x = make_uint4(0, 0, 0, 0);
-    if (src_page[o] >= 0) x = *(const uint4*)(K + from(o) + k_off(src_slot[o] & 63, d, HD));
-    *(uint4*)(a.c.k + at + k_off(o, d, HD)) = x;
+  // All loads of a thread's pieces are under way before the first is used; places without a source read slot 0 of page 0 and give zeros.
+  constexpr int KN = PAGE * PC / 256;
+  uint4 kx[KN];
+#pragma unroll
+  for (int i = 0; i < KN; ++i) {
+    const int o = tid % PAGE, d = (tid / PAGE + 4 * i) * 8;
+    kx[i] = *(const uint4*)(K + from(o) + k_off(max(src_slot[o], 0) & 63, d, HD));
   }
-  for (int i = tid; i < PAGE / 8 * HD; i += 256) {
-    const int d = i % HD, o = i / HD * 8;
+#pragma unroll
+  for (int i = 0; i < KN; ++i) {
+    const int o = tid % PAGE, d = (tid / PAGE + 4 * i) * 8;
+    if (src_page[o] < 0) kx[i] = make_uint4(0, 0, 0, 0);
+    if (src_slot[o] >= 0) *(uint4*)(a.c.k + at + k_off(o, d, HD)) = kx[i];
+  }
+  // A wave takes 64 dims of eight slots, whose places are the same for all its lanes: whole pieces of V, of which each gives one slot.
+#pragma unroll
+  for (int i = 0; i < PAGE / 8 * HD / 256; ++i) {
+    const int x = 256 * i + tid, d = x % HD, o = __builtin_amdgcn_readfirstlane(x / HD * 8);
     if (src_slot[o] < 0) continue;
+    uint4 y[8];
+    int t[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      t[e] = __builtin_amdgcn_readfirstlane(src_page[o + e] < 0 ? -1 : src_slot[o + e]);  // -1: zeros (behind the last kept slot, or no page)
+      y[e] = *(const uint4*)(V + from(o + e) + v_off(max(t[e], 0) & 56, d, HD));
+    }
     uint32_t w[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {  // slots past the last kept one get zeros
-      const int t = src_slot[o + e], pg = src_page[o + e];
-      w[e] = pg >= 0 ? V[from(o + e) + v_off(max(t, 0) & 63, d, HD)] : 0;
+    for (int e = 0; e < 8; ++e) {
+      const uint64_t half = t[e] & 4 ? (uint64_t)y[e].w << 32 | y[e].z : (uint64_t)y[e].y << 32 | y[e].x;
+      w[e] = t[e] < 0 ? 0u : (uint32_t)(half >> (16 * (t[e] & 3))) & 0xffffu;
     }
     *(uint4*)(a.c.v + at + v_off(o, d, HD)) = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
   }
