@@ -8,8 +8,17 @@
 // So a row's result depends on its own keys, its query and the span, not on the other rows or sequences.
 // Probabilities are rounded to bf16 as the second product's operand; l sums them before that.
 //
-// With weights the first launch leaves the scores too (fp32, 16 bytes a key and four heads against 4 hd bytes of K and V), and
-// the second, knowing every (row, head)'s final m and l, adds up 2^(s - m) / l over the rows and heads of a kv head.
+// With weights the second launch, knowing every (row, head)'s final m and l, also adds up 2^(s - m) / l over the rows and heads of
+// a kv head. For up to sixteen pairs the first launch leaves it the scores (fp32: 8 bytes a pair and key, written and read, against
+// 4 hd bytes of K and V); for more it reads K again and makes them anew, in the same order and so the same.
+//
+// What bounds it: bytes of K and V, each read once where a kv head's pairs are one tile. A wave has one block's K and V in
+// registers and loads the next block's as soon as a product has used the present one's, 32 KB in flight; with 245 registers that
+// is two workgroups a CU. 32 heads on 8 kv heads of 128, us: 32 sequences of one row and up to 8192 keys 139 (5.3 TB/s), one
+// row after 131000 keys 97 (5.5), 24 sequences with weights 38; 6 sequences of 16 rows and 1200 to 4001 keys, four tiles that share
+// K and V through L2, 25 and 17 for the join and the weights. One row after 500 keys of the smallest shape 4.8: latency.
+// Tried: two tiles a workgroup, whose registers leave one workgroup a CU (6 sequences of 16 rows 29 us against 25, 2 of 60 rows and
+// 8000 keys 87 against 76).
 #include "paged.h"
 
 #include <algorithm>
@@ -17,6 +26,10 @@
 namespace ssd {
 
 constexpr int PA_WAVES = 4;
+// Most (row, head) pairs of a kv head whose scores are kept for the weights (us of both launches, hd 128, 4 heads a kv head, kept / made
+// anew: 24 sequences of one row and 4000 keys 138 / 166, 6 of 4 rows 52 / 54, of 8 rows 58 / 58, of 16 rows and 1200 to 4001 keys
+// 63 / 58, 2 of 60 rows and 8000 keys 138 / 107).
+constexpr int PA_SCORES = 16;
 constexpr int PA_MAX_SPAN = 4096;  // a wave's pages are one table word a lane
 
 struct PagedAttnArgs {
@@ -30,13 +43,14 @@ struct PagedAttnArgs {
   float* ws_o;    // [row][head][group][HD]
   float2* ws_ml;  // [row][head][group]: (m, l)
   float* ws_s;    // [row][head][ld_s]: products q k
+  float2* ws_t;   // [kv head][group][row][q head of it]: (m, l) again, where there are no products
   int64_t ld_s;
   bf16_t* out;
   int64_t ldo;
   float* weights;
   int64_t ldw_seq, ldw;
   float decay;
-  int join_wgs, chunks;  // second launch: workgroups that join, then key chunks of a (sequence, kv head)
+  int weight_wgs, chunks;  // second launch: workgroups that add up weights (the others join), key chunks of a (sequence, kv head)
 };
 
 template <int HD>
@@ -135,7 +149,7 @@ struct alignas(16) PagedSpans {
 };
 
 // Workgroup (sequence, group, kv head, tile). The tiles of one (sequence, group, kv head) are ids 8 apart: one XCD, whose L2 they share.
-template <int HD, bool WEIGHTS>
+template <int HD, bool SCORES>
 __global__ __launch_bounds__(256, 2) void paged_fold_kernel(PagedAttnArgs a) {
   __shared__ PagedSpans<HD> lds;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, g = lane >> 4;
@@ -177,7 +191,7 @@ __global__ __launch_bounds__(256, 2) void paged_fold_kernel(PagedAttnArgs a) {
       const bool masked = gone || key0 + PAGE - 1 > lim_lo;
       const int note = gone ? INT32_MAX - PAGE : key0;
       auto scores = [&](const f32x4_t (&s)[4]) {
-        if constexpr (WEIGHTS) {
+        if constexpr (SCORES) {
           if (c0 + j >= n_cols) return;
           float* dst = a.ws_s + ((int64_t)row * a.heads + head) * a.ld_s + key0;
 #pragma unroll
@@ -247,17 +261,26 @@ __global__ __launch_bounds__(256, 2) void paged_fold_kernel(PagedAttnArgs a) {
       *(f32x4_t*)(a.ws_o + rec * HD + i * 64 + dc * 4) = o;
     }
   }
-  if (dc == 0 && (!direct || WEIGHTS)) a.ws_ml[rec] = make_float2(top, l);
+  if (dc == 0) {
+    if (!direct || SCORES) a.ws_ml[rec] = make_float2(top, l);
+    if (!SCORES && a.weights) a.ws_t[(((int64_t)kvh * a.n_grps + grp) * a.M + r.r0) * a.rep + c0 + rr] = make_float2(top, l);
+  }
 }
 
-// Largest reference and the sum l of a (row, head)'s records, by the lanes of a power-of-two group of LG lanes.
-__device__ __forceinline__ float2 paged_total(const float2* ml, int ng, int part, int lg) {
+// Largest reference and the sum l of a (row, head)'s records, `step` apart, by the lanes of a power-of-two group of lg lanes.
+__device__ __forceinline__ float2 paged_total(const float2* ml, int64_t step, int ng, int part, int lg) {
   float m = -INFINITY, l = 0.f;
-  for (int i = part; i < ng; i += lg) {
-    const float2 x = ml[i];
-    const float top = fmaxf(m, x.x);
-    l = l * paged_weight(m, top) + x.y * paged_weight(x.x, top);
-    m = top;
+  for (int i = part; i < ng; i += 4 * lg) {  // four records on their way at once
+    float2 x[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = ml[min(i + e * lg, ng - 1) * step];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (i + e * lg >= ng) break;
+      const float top = fmaxf(m, x[e].x);
+      l = l * paged_weight(m, top) + x[e].y * paged_weight(x[e].x, top);
+      m = top;
+    }
   }
   for (int o = 1; o < lg; o <<= 1) {
     const float mo = __shfl_xor(m, o), lo = __shfl_xor(l, o), top = fmaxf(m, mo);
@@ -267,17 +290,19 @@ __device__ __forceinline__ float2 paged_total(const float2* ml, int ng, int part
   return make_float2(m, l);
 }
 
-// Second launch. The first join_wgs workgroups add up the records: WPP waves a (sequence, row, head), each a run of groups in order, the
-// waves' sums then in order. The others (WK > 0) add the received weights of 1024 / WK slots of a (sequence, kv head): a lane four slots; WK
-// waves share its (row, head) pairs, a run each, and their sums are added in order.
+// Second launch. Workgroups that add up the records: WPP waves a (sequence, row, head), each a run of groups in order, the
+// waves' sums then in order. Workgroups that add up received weights, of a set of slots of a (sequence, kv head), in a fixed order too: WK = 1
+// from the kept scores, a lane four slots; WK = 2 from K, a wave a block, sixteen pairs at a time, the lanes' sums last.
 template <int HD, int WK, int WPP>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int grp_keys = a.grp_keys;
-  if ((int)blockIdx.x < a.join_wgs) {
+  // the workgroups that add up weights, which take longer, come first
+  if (WK == 0 || (int)blockIdx.x >= a.weight_wgs) {
     constexpr int V = HD / 64;  // dims a lane
     __shared__ float part[4][HD];
-    int u = WPP == 4 ? blockIdx.x : blockIdx.x * 4 + w;
+    int u = blockIdx.x - (WK ? a.weight_wgs : 0);
+    if (WPP == 1) u = u * 4 + w;
     const int h = u % a.heads;
     u /= a.heads;
     const int i = u % a.b.rows_max, s = u / a.b.rows_max;
@@ -288,7 +313,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
     const int lim = min(r.first + i, a.l_cap - 1), ng = lim < 0 ? 0 : lim / grp_keys + 1;
     const float2* ml = a.ws_ml + (row * a.heads + h) * a.n_grps;
     const float* o = a.ws_o + (row * a.heads + h) * a.n_grps * HD + lane * V;
-    const float2 all = paged_total(ml, ng, lane, 64);
+    const float2 all = paged_total(ml, 1, ng, lane, 64);
     float acc[V] = {};
     const int run = WPP == 4 ? (ng + 3) / 4 : ng, from = WPP == 4 ? w * run : 0, to = min(from + run, ng);
     for (int g0 = from; g0 < to; g0 += 64) {
@@ -324,41 +349,40 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
     return;
   }
   if constexpr (WK > 0) {
-    constexpr int CHUNK = 1024 / WK;
-    __shared__ float2 total[256];  // (m, 1 / l) of up to 256 (row, head) pairs
-    __shared__ __align__(16) float sums[WK][CHUNK];
-    int u = blockIdx.x - a.join_wgs;
+    int u = blockIdx.x;
     const int ch = u % a.chunks;
     u /= a.chunks;
     const int kvh = u % a.c.kv, s = u / a.c.kv;
+    int page = -1;  // of the wave's block, read before the lengths are known, as in the first launch
+    if (WK == 2 && (ch * 4 + w) * PAGE < a.l_cap) page = paged_page(a.b, s, ch * 4 + w, a.c.pages);
     const PagedRows r = paged_rows(a.b, s, a.M);
     const int end = min(r.first + r.n, a.l_cap);  // slots in use
-    if (r.n == 0 || ch * CHUNK >= end) return;
-    const int key = ch * CHUNK + (WK == 4 ? lane : threadIdx.x) * 4, pairs = r.n * a.rep;
-    f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
-    for (int p0 = 0; p0 < pairs; p0 += 256) {
-      const int np = min(256, pairs - p0);
-      int lg = 64;
-      while (lg > 1 && 256 / lg < np) lg >>= 1;
-      if (p0) __syncthreads();
-      for (int p = threadIdx.x / lg; p < (np + 256 / lg - 1) / (256 / lg) * (256 / lg); p += 256 / lg) {  // whole waves stay together
-        const int pc = min(p, np - 1) + p0;
-        const int lim = min(r.first + pc / a.rep, a.l_cap - 1);
-        const float2 t = paged_total(a.ws_ml + ((int64_t)(r.r0 + pc / a.rep) * a.heads + kvh * a.rep + pc % a.rep) * a.n_grps,
-                                     lim < 0 ? 0 : lim / grp_keys + 1, threadIdx.x % lg, lg);
-        if (p < np && threadIdx.x % lg == 0) total[p] = make_float2(t.x, t.y == 0.f ? 0.f : 1.f / t.y);
-      }
+    if (r.n == 0 || ch * (WK == 1 ? 1024 : 256) >= end) return;
+    const int pairs = r.n * a.rep;
+    float* dst = a.weights + s * a.ldw_seq + kvh * a.ldw;
+    __shared__ float2 total[256];  // (m, 1 / l) of (row, head) pairs p0 ..
+    // a pair whose scores are all -inf gives weights of 0
+    auto ready = [](float2 t) { return make_float2(t.x == -INFINITY ? 0.f : t.x, t.y == 0.f ? 0.f : 1.f / t.y); };
+    auto limit = [&](int p) { return min(r.first + p / a.rep, a.l_cap - 1); };  // the last slot that pair p attends
+    auto records = [&](int p) { return limit(p) < 0 ? 0 : limit(p) / grp_keys + 1; };
+    auto share = [&](float x, float2 t) { return __builtin_amdgcn_exp2f(fmaf(x, a.scale_log2, -t.x)); };
+    if constexpr (WK == 1) {
+      const int key = ch * 1024 + threadIdx.x * 4;
+      f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+      const int mine = min((int)threadIdx.x >> 4, pairs - 1);
+      const float2 all = paged_total(a.ws_ml + ((int64_t)(r.r0 + mine / a.rep) * a.heads + kvh * a.rep + mine % a.rep) * a.n_grps, 1,
+                                     records(mine), threadIdx.x & 15, 16);
+      if ((threadIdx.x & 15) == 0 && (int)threadIdx.x >> 4 < pairs) total[mine] = ready(all);
       __syncthreads();
-      const int run = (np + WK - 1) / WK, from = WK == 4 ? w * run : 0, to = min(from + run, np);
-      for (int p = from; p < to; p += 4) {  // four pairs' scores on their way at once; a pair past the last one repeats it and does not count
+      for (int p = 0; p < pairs; p += 4) {  // four pairs' scores on their way at once; a pair past the last one repeats it and does not count
         f32x4_t x[4];
         int lim[4];
         float2 t[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int pc = p0 + min(p + e, to - 1), i = pc / a.rep;
-          lim[e] = p + e < to ? min(r.first + i, a.l_cap - 1) : -1;
-          t[e] = total[pc - p0];
+          const int pc = min(p + e, pairs - 1), i = pc / a.rep;
+          lim[e] = p + e < pairs ? limit(pc) : -1;
+          t[e] = total[pc];
           // slots that no block holds (behind the bound's last one) read the row's first
           x[e] = *(const f32x4_t*)(a.ws_s + ((int64_t)(r.r0 + i) * a.heads + kvh * a.rep + pc % a.rep) * a.ld_s + (key < a.ld_s ? key : 0));
         }
@@ -366,37 +390,88 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
         for (int e = 0; e < 4; ++e)
 #pragma unroll
           for (int q = 0; q < 4; ++q) {  // scores of slots that are not attended may be anything
-            const float wgt = __builtin_amdgcn_exp2f(fmaf(x[e][q], a.scale_log2, -t[e].x)) * t[e].y;
-            sum[q] += key + q <= lim[e] && x[e][q] != -INFINITY ? wgt : 0.f;
+            const float wgt = share(x[e][q], t[e]) * t[e].y;
+            sum[q] += key + q <= lim[e] ? wgt : 0.f;
           }
       }
-    }
-    float* dst = a.weights + s * a.ldw_seq + kvh * a.ldw;
-    if constexpr (WK == 4) {
-      *(f32x4_t*)&sums[w][lane * 4] = sum;
-      __syncthreads();
-      const int x = threadIdx.x, at = ch * CHUNK + x;
-      if (at >= end) return;
-      const float y = ((sums[0][x] + sums[1][x]) + sums[2][x]) + sums[3][x];
-      dst[at] = a.decay == 0.f ? y : fmaf(a.decay, dst[at], y);
-    } else {
 #pragma unroll
       for (int q = 0; q < 4; ++q)
         if (key + q < end) dst[key + q] = a.decay == 0.f ? sum[q] : fmaf(a.decay, dst[key + q], sum[q]);
+    } else {
+      const int j = lane & 15, g = lane >> 4, blk = ch * 4 + w, key0 = blk * PAGE;
+      page = key0 < end ? __builtin_amdgcn_readfirstlane(page) : -1;
+      PagedFrags<HD> f;
+      paged_load_k<HD>(f, a.c.k, ((size_t)max(page, 0) * a.c.kv + kvh) * PAGE * HD, lane);
+      auto load_q = [&](int col, u32x4_t (&q)[HD / 32]) {
+        const int pc = min(col, pairs - 1);
+#pragma unroll
+        for (int ks = 0; ks < HD / 32; ++ks)
+          q[ks] = *(const u32x4_t*)(a.Q + (r.r0 + pc / a.rep) * a.ldq + (kvh * a.rep + pc % a.rep) * HD + ks * 32 + g * 8);
+      };
+      u32x4_t qn[HD / 32];
+      load_q(j, qn);
+      float sum[16] = {};
+      for (int p0 = 0; p0 < pairs; p0 += 256) {
+        const int np = min(256, pairs - p0);
+        if (p0) __syncthreads();
+        int lg = 16;  // lanes a pair
+        while (lg > 1 && 256 / lg < np) lg >>= 1;
+        const int mine = min((int)threadIdx.x / lg, np - 1);
+        const float2 all = paged_total(a.ws_t + ((int64_t)kvh * a.n_grps * a.M + r.r0) * a.rep + p0 + mine, (int64_t)a.M * a.rep,
+                                       records(p0 + mine), threadIdx.x % lg, lg);
+        if (threadIdx.x % lg == 0 && (int)threadIdx.x / lg < np) total[mine] = ready(all);
+        __syncthreads();
+        if (page < 0) continue;
+        for (int c0 = 0; c0 < np; c0 += 16) {
+          u32x4_t qf[HD / 32];
+#pragma unroll
+          for (int ks = 0; ks < HD / 32; ++ks) qf[ks] = qn[ks];
+          load_q(p0 + c0 + 16 + j, qn);
+          f32x4_t x[4] = {};
+#pragma unroll
+          for (int ks = 0; ks < HD / 32; ++ks)
+#pragma unroll
+            for (int kt = 0; kt < 4; ++kt) x[kt] = mfma16x16x32(bits_bf16x8(f.k[kt][ks]), bits_bf16x8(qf[ks]), x[kt]);
+          float2 t = total[min(c0 + j, np - 1)];
+          if (c0 + j >= np) t.y = 0.f;  // the last pair again
+          if (limit(p0 + c0) >= key0 + PAGE - 1) {  // every column attends the whole block
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sum[i] = fmaf(share(x[i / 4][i % 4], t), t.y, sum[i]);
+          } else {  // scores of slots that are not attended may be anything
+            const int left = limit(p0 + min(c0 + j, np - 1)) - key0;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float wgt = share(x[i / 4][i % 4], t) * t.y;
+              sum[i] += paged_key(i / 4, g, i % 4) <= left ? wgt : 0.f;
+            }
+          }
+        }
+      }
+      float mine = 0.f;  // lane j: the sum over the columns of value j
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float v = sum[i];
+        v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0xb1, 0xf, 0xf, true));   // lane ^ 1
+        v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x4e, 0xf, 0xf, true));   // lane ^ 2
+        v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x141, 0xf, 0xf, true));  // the other half of 8
+        v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x140, 0xf, 0xf, true));  // the other half of 16
+        mine = i == j ? v : mine;
+      }
+      const int at = key0 + paged_key(j >> 2, g, j & 3);
+      if (at < end) dst[at] = a.decay == 0.f ? mine : fmaf(a.decay, dst[at], mine);
     }
   }
 }
 
-// Second launch of WK waves a set of slots (0: no weights). Waves a (row, head): four where few pairs have many records (us of one row of 32
-// heads with 64 records, one wave / four: 8.9 / 5.5).
+// Waves a (row, head): four where few pairs have many records (us of one row of 32 heads with 64 records, one wave / four: 8.9 / 5.5).
 template <int HD, int WK>
 static int launch_paged_join(PagedAttnArgs& a, hipStream_t stream) {
   const int64_t pairs = a.n_grps > 1 ? (int64_t)a.b.n_seq * a.b.rows_max * a.heads : 0;
-  a.chunks = WK ? (int)(((int64_t)a.l_cap * WK + 1023) / 1024) : 0;
+  a.chunks = WK == 0 ? 0 : WK == 1 ? (a.l_cap + 1023) / 1024 : (a.l_cap + 255) / 256;
   const bool four = a.n_grps > 8 && pairs <= 2048;
-  const int64_t join = four ? pairs : (pairs + 3) / 4, all = join + (int64_t)a.b.n_seq * a.c.kv * a.chunks;
+  const int64_t sums = (int64_t)a.b.n_seq * a.c.kv * a.chunks, all = sums + (four ? pairs : (pairs + 3) / 4);
   if (paged_grid_too_large(all, 256)) return set_error(SSD_ERANGE, "paged_attention: too many workgroups");
-  a.join_wgs = (int)join;
+  a.weight_wgs = (int)sums;
   if (four) SSD_LAUNCH((paged_join_kernel<HD, WK, 4>), dim3((unsigned)all), dim3(256), 0, stream, a);
   else SSD_LAUNCH((paged_join_kernel<HD, WK, 1>), dim3((unsigned)all), dim3(256), 0, stream, a);
   return check_launch("paged_attention_join");
@@ -405,7 +480,7 @@ static int launch_paged_join(PagedAttnArgs& a, hipStream_t stream) {
 static int paged_groups(int64_t l_max, int span) { return (int)((l_max + (int64_t)PA_WAVES * span - 1) / ((int64_t)PA_WAVES * span)); }
 static int64_t paged_score_ld(int64_t l_max) { return (l_max + PAGE - 1) / PAGE * PAGE; }
 
-template <int HD, bool WEIGHTS>
+template <int HD, bool SCORES>
 static int launch_paged_attn(PagedAttnArgs a, hipStream_t stream) {
   const int tiles = (int)(((int64_t)a.b.rows_max * a.rep + 15) / 16);
   a.sets = tiles;
@@ -413,13 +488,12 @@ static int launch_paged_attn(PagedAttnArgs a, hipStream_t stream) {
   if (units > INT32_MAX || paged_grid_too_large(grid, 256)) return set_error(SSD_ERANGE, "paged_attention: too many workgroups");
   a.units = (int)units;
   // the second launch's size is checked before the first is enqueued
-  if (paged_grid_too_large((int64_t)a.b.n_seq * (a.b.rows_max * (int64_t)a.heads + (WEIGHTS ? a.c.kv * (int64_t)(a.l_cap / 256 + 1) : 0)), 256))
+  if (paged_grid_too_large((int64_t)a.b.n_seq * (a.b.rows_max * (int64_t)a.heads + (a.weights ? a.c.kv * (int64_t)(a.l_cap / 256 + 1) : 0)), 256))
     return set_error(SSD_ERANGE, "paged_attention: too many workgroups");
-  SSD_LAUNCH((paged_fold_kernel<HD, WEIGHTS>), dim3((unsigned)grid), dim3(256), 0, stream, a);
+  SSD_LAUNCH((paged_fold_kernel<HD, SCORES>), dim3((unsigned)grid), dim3(256), 0, stream, a);
   if (int rc = check_launch("paged_attention_fold")) return rc;
-  // Received weights: the waves of a workgroup share the (row, head) pairs of a set of slots where there are many (us of the second launch, a
-  // wave / four: 6 x 16 rows, 4 heads a kv head, 4000 keys 39 / 12; 24 sequences of one row, 3 heads, 4000 keys 6.1 / 9.7).
-  if constexpr (WEIGHTS) return a.b.rows_max * a.rep > 16 ? launch_paged_join<HD, 4>(a, stream) : launch_paged_join<HD, 1>(a, stream);
+  if constexpr (SCORES) return launch_paged_join<HD, 1>(a, stream);
+  if (a.weights) return launch_paged_join<HD, 2>(a, stream);
   return a.n_grps > 1 ? launch_paged_join<HD, 0>(a, stream) : SSD_OK;
 }
 
@@ -472,8 +546,9 @@ SSD_API int ssd_paged_attention_bf16(const SsdPagedKv* cache, const SsdPagedBatc
   a.span_blk = span / PAGE, a.n_grps = paged_groups(l_max, span), a.grp_keys = PA_WAVES * span, a.scale_log2 = scale * 1.4426950408889634f;
   const int64_t recs = (int64_t)M * heads * a.n_grps;
   a.ws_o = ws, a.ws_ml = (float2*)(ws + recs * cache->head_dim);
-  a.ws_s = ws + recs * (cache->head_dim + 2) + (recs * 2) % 4, a.ld_s = paged_score_ld(l_max);
+  a.ws_s = ws + recs * (cache->head_dim + 2) + (recs * 2) % 4, a.ld_s = paged_score_ld(l_max), a.ws_t = (float2*)a.ws_s;
   a.out = out, a.ldo = ldo, a.weights = weights, a.ldw_seq = ldw_seq, a.ldw = ldw, a.decay = decay;
-  if (cache->head_dim == 64) return weights ? launch_paged_attn<64, true>(a, stream) : launch_paged_attn<64, false>(a, stream);
-  return weights ? launch_paged_attn<128, true>(a, stream) : launch_paged_attn<128, false>(a, stream);
+  const bool scores = weights && (int64_t)a.b.rows_max * a.rep <= PA_SCORES;
+  if (cache->head_dim == 64) return scores ? launch_paged_attn<64, true>(a, stream) : launch_paged_attn<64, false>(a, stream);
+  return scores ? launch_paged_attn<128, true>(a, stream) : launch_paged_attn<128, false>(a, stream);
 }

@@ -247,21 +247,6 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedPromptArgs a)
       prompt_qk<HD>(st, at, nk, sn);
       prompt_exp<HD>(st, s, a.scale_log2, p);
       prompt_pv<HD>(st, at, cv, p);
-#ifdef SGB
-      __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x2, 7, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      }
-#pragma unroll
-      for (int i = 0; i < 12; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      }
-      __builtin_amdgcn_sched_group_barrier(0x8, 4, 0);
-#endif
       prompt_reference<HD>(st, sn, a.scale_log2);
       cur = nxt, nxt = then;
     };
