@@ -316,8 +316,8 @@ int ssd_paged_read_bf16(const SsdPagedKv* cache, const SsdPagedBatch* batch, int
  * and span alone. ws: ssd_paged_attn_ws_floats(...) floats, 16-byte aligned, no clearing needed; calls that overlap in
  * time must not share it. With weights (may be NULL): for every slot t in use of sequence s and kv head h,
  * weights[s * ldw_seq + h * ldw + t] becomes decay * itself + the sum over the sequence's rows and h's query heads of the
- * softmax weight of t (decay in [0, 1]; 0: the old value is not read); the rest stays. Weights are summed in a
- * fixed order.
+ * softmax weight of t (decay in [0, 1]; 0: the old value is not read); the rest stays, and so do the weights of sequences
+ * without rows in the call. Weights are summed in a fixed order.
  * ssd_paged_prompt_bf16 is for many rows a sequence; where they are too few to fill the chip it cuts the length into parts
  * too (ws: ssd_paged_prompt_ws_floats(...) floats, as above; 0: NULL will do). The parts follow from M, the heads, n_seq and
  * l_max, and the results differ by rounding between numbers of parts and from the other's. */
@@ -334,8 +334,8 @@ int ssd_paged_prompt_bf16(const SsdPagedKv* cache, const SsdPagedBatch* batch, c
  * `keep`, those of the largest weight (equal ones: the lowest slots; NaN below every number); of shorter ones all. They move, in their
  * order, to slots 0, 1, ... of the pages in after->table, which must be pages that `batch` does not use, and
  * after->lengths becomes min(lengths, keep) (it may be batch->lengths itself). weights: [layers][n_seq][kv_heads] rows of cap
- * floats, ldw apart, cap >= lengths (slots beyond it count as not there); out_weights, rows alike: the kept ones, then
- * zeros. kept: [layers][n_seq][kv_heads][keep] int32, the slots they came from, then -1. The row_begin and rows_max of both
+ * floats, ldw apart, cap >= lengths (slots beyond it count as not there); out_weights, rows alike and elsewhere: the kept
+ * ones, then zeros. kept: [layers][n_seq][kv_heads][keep] int32, the slots they came from, then -1. The row_begin and rows_max of both
  * batches are not used. No counterpart in the reference, whose caches only grow. */
 int ssd_paged_evict(const SsdPagedKv* cache, int layers, int64_t layer_elems, const SsdPagedBatch* batch, const SsdPagedBatch* after,
                     const float* weights, int64_t ldw, int cap, int keep, int recent, int first, float* out_weights, int32_t* kept,

@@ -352,7 +352,7 @@ class PagedKVCache:
         layer ``i``: every row attends its sequence's slots up to its own. Zeros for rows that attend nothing. ``l_max`` (None: the
         table's capacity) bounds the lengths: slots from there on are not attended, and a close bound saves empty
         workgroups. ``weights`` fp32 [S, kv_heads, >= l_max]: decay * weights + the softmax weights each slot in use received from the
-        call's rows, summed over rows and a kv head's query heads (decay 0: set). ``ws``: fp32, attend_floats(...)."""
+        call's rows, summed over rows and a kv head's query heads (decay 0: set); sequences without rows keep theirs. ``ws``: fp32, attend_floats(...)."""
         return ops.paged_attention(self._layers[i], batch, q, self._heads(q), l_max, self._span(batch), ws, out, scale, weights, decay)
 
     def prompt_floats(self, m: int, heads: int, batch: PagedBatch, l_max: Optional[int] = None) -> int:
