@@ -11,12 +11,15 @@
 // wave issues, whatever its size, so half as many of twice the work leave it more (a wave of products beside one of multiply-adds:
 // 406 ns against 345 for the same work). While a block's scores become probabilities and meet V, the next block's scores are
 // under way; the blocks that some columns attend only part of, one or two a tile, follow without that.
-// What bounds it, 32 heads on 8 kv heads of 128 (8b shapes): a prompt of 16384 rows 1.95 ms, 1130 TFLOP/s, where a large library product reaches
-// 1300: matrix pipe, vector pipe and LDS reads, each about half of a block's 1.9 us for two workgroups a CU. Shorter
-// prompts: a tile's beginning and end, about 8 us (rows, pages, first copies; the partly attended blocks; the output), of which a
-// second workgroup on the CU hides half: 4096 rows 157 us, 16 prompts of 232 to 1500 rows 180.
-// Tried: eight waves a workgroup (a prompt of 4096 147 us, 16 prompts 193, 100 rows after 8000 keys 180 against 136 with the length
-// in one part), 64 columns a wave with twice the registers (269), two groups of waves taking turns at the matrix pipe (155).
+// What bounds it, 32 heads on 8 kv heads of 128 (8b shapes): a prompt of 16384 rows 1.89 ms, 1160 TFLOP/s, where a large library product reaches
+// 1300: matrix pipe and vector pipe, each about half of a block's 1.9 us for two workgroups a CU, at the clock that the power leaves.
+// Shorter prompts: a tile's beginning and end, about 8 us (rows, pages, first copies; the partly attended blocks; the output), of
+// which a second workgroup on the CU hides half, and the last tiles' end: 4096 rows 145 to 155 us (by box), 16 prompts of 232 to 1500
+// rows 183 to 191.
+// Tried (us of 16 prompts, 191 on that box): tiles dealt to resident workgroups, the next one's first blocks copied before the output 202;
+// the longest tiles of all sequences first 192. Eight waves a workgroup: a prompt of 4096 rows 138 against 147, of 2048 60 against 50,
+// 16 prompts 170 against 160. 64 columns a wave with twice the registers 269 for 157, two groups of waves taking turns at the
+// matrix pipe 155, sums of l by dot products no change.
 #include "paged.h"
 
 #include <algorithm>
@@ -161,14 +164,15 @@ __device__ __forceinline__ PromptTile prompt_tile(const PagedPromptArgs& a, int 
 }
 
 // Workgroup (tile of 32 W columns of some sequence, kv head). The kv head varies fastest: with eight of them an XCD serves one, whose
-// blocks its L2 keeps.
-template <int HD>
+// blocks its L2 keeps. TURNS: the workgroups of a CU take turns at going first (prompt_turns).
+template <int HD, bool TURNS>
 __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedPromptArgs a) {
   constexpr int W = PP_WAVES, CW = 32 * W, PIECES = 64 * HD / 8;
   __shared__ int first_bad[HD], any_bad;
   __shared__ __align__(16) u32x4_t kA[PIECES], vA[PIECES], kB[PIECES], vB[PIECES];
   typedef __attribute__((address_space(3))) u32x4_t* lp;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, g = lane >> 5;
+  if (TURNS) __builtin_amdgcn_s_setprio(1);
   int u = blockIdx.x;
   const int kvh = u % a.c.kv;
   u /= a.c.kv;
@@ -251,12 +255,15 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedPromptArgs a)
       cur = nxt, nxt = then;
     };
     while (nxt.b < full) {
+      if (TURNS) __builtin_amdgcn_s_setprio(2);
       step(s0, s1, (lp)kA, (lp)vA, (lp)kB, (lp)vB);
       odd = true;
       if (!(nxt.b < full)) break;
+      if (TURNS) __builtin_amdgcn_s_setprio(0);
       step(s1, s0, (lp)kB, (lp)vB, (lp)kA, (lp)vA);
       odd = false;
     }
+    if (TURNS) __builtin_amdgcn_s_setprio(1);
     // the last of them
     landed();
     const Block then = next();
@@ -363,11 +370,26 @@ static int prompt_splits(int64_t M, int rep, int n_seq, int kv, int64_t l_max) {
   return n == 2 && blocks < 96 ? 1 : (int)n;
 }
 
+// Of two workgroups on a CU the older one's waves go first, and its tile ends long before the other's (1.7 us a block against 2.4). That is
+// as it should be where a last, part round of tiles follows or the longest tiles begin first and all at once. Where all tiles make two
+// rounds, or one of tiles of like lengths (behind a long past), they had better end together: a wave's priority then goes up and
+// down from block to block. us without / with, heads of 128, by workgroups for the 512 places: prompts of 2048 rows (520) 51 / 54, 2600 (656)
+// 66 / 69, 3400 (856) 103 / 98, 4096 (1032) 141 / 131, 5000 (1256) 196 / 203, 8192 (2056) 486 / 487; 8 pieces of 256 rows after 2000 keys
+// (576) 76 / 74, (1088) 141 / 139; 3 of 500 rows after 6000 (768) 290 / 323, 3 of 256 to 511 (528) 195 / 187. Heads of 64: 2048 rows 35 / 39.
+static bool prompt_turns(int64_t wgs, int rows_max, int l_max) {
+  return (wgs >= 820 && wgs <= 1126) || (wgs > 512 && wgs <= 614 && rows_max <= l_max / 2);  // 1.6 to 2.2 rounds, 1 to 1.2
+}
+
 template <int HD>
 static int launch_paged_prompt(const PagedPromptArgs& a, hipStream_t stream) {
   const int64_t wgs = prompt_tiles(a.M, a.rep, a.b.n_seq, a.c.kv) * a.splits;
   if (paged_grid_too_large(wgs, 256)) return set_error(SSD_ERANGE, "paged_prompt: too many workgroups");
-  SSD_LAUNCH((paged_prompt_kernel<HD>), dim3((unsigned)wgs), dim3(256), 0, stream, a);
+  if constexpr (HD == 128) {
+    if (prompt_turns(wgs, a.b.rows_max, a.l_cap)) SSD_LAUNCH((paged_prompt_kernel<HD, true>), dim3((unsigned)wgs), dim3(256), 0, stream, a);
+    else SSD_LAUNCH((paged_prompt_kernel<HD, false>), dim3((unsigned)wgs), dim3(256), 0, stream, a);
+  } else {
+    SSD_LAUNCH((paged_prompt_kernel<HD, false>), dim3((unsigned)wgs), dim3(256), 0, stream, a);
+  }
   if (int rc = check_launch("paged_prompt")) return rc;
   if (a.splits == 1) return SSD_OK;
   return paged_join(a.b, a.M, a.heads, HD, a.l_cap, a.per * PAGE, a.splits, a.ws_o, a.ws_ml, a.out, a.ldo, stream);
