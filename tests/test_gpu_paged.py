@@ -320,6 +320,50 @@ def test_more_pairs_than_the_weights_kernel_holds_at_once():
     s.check(s.cache.attend(0, s.q.cuda(), s.batch, 330, weights=weights), weights, torch.zeros_like(weights))
 
 
+@pytest.mark.parametrize("heads,kv,hd", [(32, 8, 128), (15, 5, 128), (16, 16, 64), (64, 8, 64)])
+@pytest.mark.parametrize("rows", [1, 2, 16, 17])
+def test_received_weights_of_a_step_and_of_a_window(heads, kv, hd, rows):
+    """Both sides of the number of pairs up to which scores are kept, several groups, and a sequence that takes no part."""
+    lens, rows = [600, 333, 70, 2400], [rows, 0, rows, 1]
+    s = Setup(lens, rows, heads, kv, hd, seed=31, span=64).fill()
+    weights = torch.rand(4, kv, 2500, generator=torch.Generator().manual_seed(2)).cuda()
+    start = weights.clone()
+    out = s.cache.attend(0, s.q.cuda(), s.batch, 2432, weights=weights, decay=0.75)
+    assert torch.equal(weights[1], start[1])  # without rows: as they were
+    start[1, :, :333] /= 0.75  # what check expects to have been decayed
+    s.check(out, weights, start, 0.75)
+
+
+def test_weights_where_a_pair_attends_scores_of_minus_infinity_alone():
+    s = Setup([40, 100], [1, 20], 4, 1, 64, seed=32).fill()
+    s.q[:] = 0
+    s.q[:, ::64] = 1.0
+    s.k[0][..., 0], s.k[1][..., 0] = float("-inf"), float("-inf")
+    s.fill()
+    weights = torch.zeros(2, 1, 128, device="cuda")
+    for b, q, w in ((s.batch, s.q, weights), (s.PB(s.table[:1], s.lengths[:1]), s.q[:1], weights[:1])):  # from K again, and kept
+        out = s.cache.attend(0, q.cuda(), b, weights=w, decay=0.0)
+        assert not out.any() and not w.any()
+
+
+def test_sequences_that_share_pages():
+    """A common prefix of two whole pages in one place, and as many copies."""
+    s = Setup([200, 170], [9, 3], 32, 8, 128, seed=33).fill()
+    s.k[1][:128], s.v[1][:128] = s.k[0][:128], s.v[0][:128]
+    s.table[1, :2] = s.table[0, :2]
+    weights = torch.zeros(2, 8, 256, device="cuda")
+    s.check(s.cache.attend(0, s.q.cuda(), s.batch, weights=weights), weights, torch.zeros_like(weights))
+    s.check(s.cache.attend_prompt(0, s.q.cuda(), s.batch))
+
+
+@pytest.mark.parametrize("rows", [4, 7])
+def test_attend_prompt_of_a_round_of_pieces_behind_a_past(rows):
+    """As many workgroups as one round and a little more, whose waves take turns, and a bound that ends it."""
+    lens = [150 + 37 * i % 400 for i in range(17)]
+    s = Setup(lens, [rows] * 17, 32, 32, 128, seed=34).fill()
+    s.check(s.cache.attend_prompt(0, s.q.cuda(), s.batch))
+
+
 # ------------------------------------------------------------------------------------------------- eviction
 @pytest.mark.parametrize("hd,kv", [(128, 2), (64, 3)])
 @pytest.mark.parametrize("keep,recent,first", [(64, 8, 4), (100, 0, 0), (1, 0, 0), (1, 1, 0), (130, 100, 30), (600, 5, 1), (63, 0, 63)])

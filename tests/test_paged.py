@@ -141,6 +141,13 @@ def test_bad_eviction_is_refused(kw, text):
     _refused("ssd_paged_evict", (_kv(), d["layers"], d["layer_elems"], _batch(), _batch(), *list(d.values())[:8], None), BAD, text)
 
 
+@pytest.mark.parametrize("off,ldw", [(4, 192), (-4, 192), (4 * 192, 192), (4 * (3 * 2 * 2 - 1) * 400 + 4 * 191, 400)])
+def test_eviction_into_weights_that_overlap_in_part_is_refused(off, ldw):
+    """Rows of two layers, three sequences and two kv heads."""
+    kv, batch = _kv(kv_heads=2), _batch(n_seq=3)
+    _refused("ssd_paged_evict", (kv, 2, 1 << 20, batch, batch, A, ldw, 192, 8, 1, 1, A + off, A, None), BAD, "overlap")
+
+
 def test_eviction_into_too_few_pages_or_another_batch_is_refused():
     call = lambda after, keep: (_kv(), 1, 1 << 20, _batch(), after, A, 192, 192, keep, 1, 1, A + 4096, A, None)  # noqa: E731
     _refused("ssd_paged_evict", call(_batch(table_cols=1), 65), BAD, "new table")
