@@ -6,7 +6,9 @@
 // w-th on, with a running reference m, sum l and output O in fp32; the four waves' states are added in LDS. Several groups leave
 // records (m, l, O) that a second launch adds up with weights from their largest m; one group is written out at once.
 // So a row's result depends on its own keys, its query and the span, not on the other rows or sequences.
-// Probabilities are rounded to bf16 as the second product's operand; l sums them before that.
+// Probabilities go into the second product as the sum of two bf16 numbers, since the matrix pipe has time for it and one row's few large
+// weights are not averaged over many (27000 keys of which few matter: 0.0026 from 64 bits with one, 0.0017 with two, the
+// output's own rounding); l sums them as they are.
 //
 // With weights the second launch, knowing every (row, head)'s final m and l, also adds up 2^(s - m) / l over the rows and heads of
 // a kv head. For up to sixteen pairs the first launch leaves it the scores (fp32: 8 bytes a pair and key, written and read, against
@@ -42,8 +44,8 @@ struct PagedAttnArgs {
   float scale_log2;
   float* ws_o;    // [row][head][group][HD]
   float2* ws_ml;  // [row][head][group]: (m, l)
+  float2* ws_t;   // [kv head][group][row][q head of it]: (m, l) once more, as the weights' launch reads them
   float* ws_s;    // [row][head][ld_s]: products q k
-  float2* ws_t;   // [kv head][group][row][q head of it]: (m, l) again, where there are no products
   int64_t ld_s;
   bf16_t* out;
   int64_t ldo;
@@ -119,7 +121,7 @@ __device__ __forceinline__ void paged_fold(PagedFrags<HD>& f, const u32x4_t (&qf
     for (int dt = 0; dt < HD / 16; ++dt) st.o[dt] *= alpha;
   }
   st.m = m;
-  u32x4_t pw[2];
+  u32x4_t pw[2], rest[2];
 #pragma unroll
   for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
@@ -127,12 +129,17 @@ __device__ __forceinline__ void paged_fold(PagedFrags<HD>& f, const u32x4_t (&qf
       const float p0 = __builtin_amdgcn_exp2f(fmaf(s[kt][e], scale_log2, -ms));
       const float p1 = __builtin_amdgcn_exp2f(fmaf(s[kt][e + 1], scale_log2, -ms));
       st.l += p0 + p1;
-      pw[kt >> 1][(kt & 1) * 2 + e / 2] = pack_bf16x2(p0, p1);
+      const uint32_t both = pack_bf16x2(p0, p1);
+      pw[kt >> 1][(kt & 1) * 2 + e / 2] = both;
+      rest[kt >> 1][(kt & 1) * 2 + e / 2] = pack_bf16x2(p0 - __uint_as_float(both << 16), p1 - __uint_as_float(both & 0xffff0000u));
     }
 #pragma unroll
   for (int c = 0; c < 2; ++c)
 #pragma unroll
-    for (int dt = 0; dt < HD / 16; ++dt) st.o[dt] = mfma16x16x32(bits_bf16x8(f.v[dt][c]), bits_bf16x8(pw[c]), st.o[dt]);
+    for (int dt = 0; dt < HD / 16; ++dt) {
+      st.o[dt] = mfma16x16x32(bits_bf16x8(f.v[dt][c]), bits_bf16x8(rest[c]), st.o[dt]);
+      st.o[dt] = mfma16x16x32(bits_bf16x8(f.v[dt][c]), bits_bf16x8(pw[c]), st.o[dt]);
+    }
   next_v();
 }
 
@@ -149,7 +156,8 @@ struct alignas(16) PagedSpans {
 };
 
 // Workgroup (sequence, group, kv head, tile). The tiles of one (sequence, group, kv head) are ids 8 apart: one XCD, whose L2 they share.
-template <int HD, bool SCORES>
+// WK as for the second launch: 1 keeps the scores.
+template <int HD, int WK>
 __global__ __launch_bounds__(256, 2) void paged_fold_kernel(PagedAttnArgs a) {
   __shared__ PagedSpans<HD> lds;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, g = lane >> 4;
@@ -191,7 +199,7 @@ __global__ __launch_bounds__(256, 2) void paged_fold_kernel(PagedAttnArgs a) {
       const bool masked = gone || key0 + PAGE - 1 > lim_lo;
       const int note = gone ? INT32_MAX - PAGE : key0;
       auto scores = [&](const f32x4_t (&s)[4]) {
-        if constexpr (SCORES) {
+        if constexpr (WK == 1) {
           if (c0 + j >= n_cols) return;
           float* dst = a.ws_s + ((int64_t)row * a.heads + head) * a.ld_s + key0;
 #pragma unroll
@@ -261,10 +269,8 @@ __global__ __launch_bounds__(256, 2) void paged_fold_kernel(PagedAttnArgs a) {
       *(f32x4_t*)(a.ws_o + rec * HD + i * 64 + dc * 4) = o;
     }
   }
-  if (dc == 0) {
-    if (!direct || SCORES) a.ws_ml[rec] = make_float2(top, l);
-    if (!SCORES && a.weights) a.ws_t[(((int64_t)kvh * a.n_grps + grp) * a.M + r.r0) * a.rep + c0 + rr] = make_float2(top, l);
-  }
+  if (dc == 0 && !direct) a.ws_ml[rec] = make_float2(top, l);
+  if (WK && dc == 0) a.ws_t[(((int64_t)kvh * a.n_grps + grp) * a.M + r.r0) * a.rep + c0 + rr] = make_float2(top, l);
 }
 
 // Largest reference and the sum l of a (row, head)'s records, `step` apart, by the lanes of a power-of-two group of lg lanes.
@@ -364,16 +370,21 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
     // a pair whose scores are all -inf gives weights of 0
     auto ready = [](float2 t) { return make_float2(t.x == -INFINITY ? 0.f : t.x, t.y == 0.f ? 0.f : 1.f / t.y); };
     auto limit = [&](int p) { return min(r.first + p / a.rep, a.l_cap - 1); };  // the last slot that pair p attends
-    auto records = [&](int p) { return limit(p) < 0 ? 0 : limit(p) / grp_keys + 1; };
+    // totals of the np pairs from p0 on, by lg lanes each
+    auto totals = [&](int p0, int np) {
+      int lg = 16;
+      while (lg > 1 && 256 / lg < np) lg >>= 1;
+      const int mine = min((int)threadIdx.x / lg, np - 1), lim = limit(p0 + mine);
+      const float2 all = paged_total(a.ws_t + ((int64_t)kvh * a.n_grps * a.M + r.r0) * a.rep + p0 + mine, (int64_t)a.M * a.rep,
+                                     lim < 0 ? 0 : lim / grp_keys + 1, threadIdx.x % lg, lg);
+      if (threadIdx.x % lg == 0 && (int)threadIdx.x / lg < np) total[mine] = ready(all);
+      __syncthreads();
+    };
     auto share = [&](float x, float2 t) { return __builtin_amdgcn_exp2f(fmaf(x, a.scale_log2, -t.x)); };
     if constexpr (WK == 1) {
       const int key = ch * 1024 + threadIdx.x * 4;
       f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
-      const int mine = min((int)threadIdx.x >> 4, pairs - 1);
-      const float2 all = paged_total(a.ws_ml + ((int64_t)(r.r0 + mine / a.rep) * a.heads + kvh * a.rep + mine % a.rep) * a.n_grps, 1,
-                                     records(mine), threadIdx.x & 15, 16);
-      if ((threadIdx.x & 15) == 0 && (int)threadIdx.x >> 4 < pairs) total[mine] = ready(all);
-      __syncthreads();
+      totals(0, pairs);
       for (int p = 0; p < pairs; p += 4) {  // four pairs' scores on their way at once; a pair past the last one repeats it and does not count
         f32x4_t x[4];
         int lim[4];
@@ -414,13 +425,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
       for (int p0 = 0; p0 < pairs; p0 += 256) {
         const int np = min(256, pairs - p0);
         if (p0) __syncthreads();
-        int lg = 16;  // lanes a pair
-        while (lg > 1 && 256 / lg < np) lg >>= 1;
-        const int mine = min((int)threadIdx.x / lg, np - 1);
-        const float2 all = paged_total(a.ws_t + ((int64_t)kvh * a.n_grps * a.M + r.r0) * a.rep + p0 + mine, (int64_t)a.M * a.rep,
-                                       records(p0 + mine), threadIdx.x % lg, lg);
-        if (threadIdx.x % lg == 0 && (int)threadIdx.x / lg < np) total[mine] = ready(all);
-        __syncthreads();
+        totals(p0, np);
         if (page < 0) continue;
         for (int c0 = 0; c0 < np; c0 += 16) {
           u32x4_t qf[HD / 32];
@@ -480,7 +485,7 @@ static int launch_paged_join(PagedAttnArgs& a, hipStream_t stream) {
 static int paged_groups(int64_t l_max, int span) { return (int)((l_max + (int64_t)PA_WAVES * span - 1) / ((int64_t)PA_WAVES * span)); }
 static int64_t paged_score_ld(int64_t l_max) { return (l_max + PAGE - 1) / PAGE * PAGE; }
 
-template <int HD, bool SCORES>
+template <int HD, int WK>
 static int launch_paged_attn(PagedAttnArgs a, hipStream_t stream) {
   const int tiles = (int)(((int64_t)a.b.rows_max * a.rep + 15) / 16);
   a.sets = tiles;
@@ -488,13 +493,11 @@ static int launch_paged_attn(PagedAttnArgs a, hipStream_t stream) {
   if (units > INT32_MAX || paged_grid_too_large(grid, 256)) return set_error(SSD_ERANGE, "paged_attention: too many workgroups");
   a.units = (int)units;
   // the second launch's size is checked before the first is enqueued
-  if (paged_grid_too_large((int64_t)a.b.n_seq * (a.b.rows_max * (int64_t)a.heads + (a.weights ? a.c.kv * (int64_t)(a.l_cap / 256 + 1) : 0)), 256))
+  if (paged_grid_too_large((int64_t)a.b.n_seq * (a.b.rows_max * (int64_t)a.heads + (WK ? a.c.kv * (int64_t)(a.l_cap / 256 + 1) : 0)), 256))
     return set_error(SSD_ERANGE, "paged_attention: too many workgroups");
-  SSD_LAUNCH((paged_fold_kernel<HD, SCORES>), dim3((unsigned)grid), dim3(256), 0, stream, a);
+  SSD_LAUNCH((paged_fold_kernel<HD, WK>), dim3((unsigned)grid), dim3(256), 0, stream, a);
   if (int rc = check_launch("paged_attention_fold")) return rc;
-  if constexpr (SCORES) return launch_paged_join<HD, 1>(a, stream);
-  if (a.weights) return launch_paged_join<HD, 2>(a, stream);
-  return a.n_grps > 1 ? launch_paged_join<HD, 0>(a, stream) : SSD_OK;
+  return WK || a.n_grps > 1 ? launch_paged_join<HD, WK>(a, stream) : SSD_OK;
 }
 
 int paged_join(const PagedBatch& b, int M, int heads, int head_dim, int l_cap, int grp_keys, int n_grps, float* ws_o, float2* ws_ml,
@@ -513,7 +516,7 @@ using namespace ssd;
 SSD_API int64_t ssd_paged_attn_ws_floats(int M, int heads, int head_dim, int64_t l_max, int span, int weights) {
   if (M < 0 || heads < 1 || head_dim < 1 || l_max < 1 || l_max > 1 << 30 || span < 64 || span % 64 || span > PA_MAX_SPAN) return -1;
   const int64_t pairs = (int64_t)M * heads, g = paged_groups(l_max, span);
-  return pairs * g * (head_dim + 2) + (pairs * g * 2) % 4 + (weights ? pairs * paged_score_ld(l_max) : 0);
+  return weights ? pairs * g * (head_dim + 4) + pairs * paged_score_ld(l_max) : pairs * g * (head_dim + 2);
 }
 
 SSD_API int ssd_paged_attention_bf16(const SsdPagedKv* cache, const SsdPagedBatch* batch, const uint16_t* q, int64_t ldq, int M,
@@ -546,9 +549,10 @@ SSD_API int ssd_paged_attention_bf16(const SsdPagedKv* cache, const SsdPagedBatc
   a.span_blk = span / PAGE, a.n_grps = paged_groups(l_max, span), a.grp_keys = PA_WAVES * span, a.scale_log2 = scale * 1.4426950408889634f;
   const int64_t recs = (int64_t)M * heads * a.n_grps;
   a.ws_o = ws, a.ws_ml = (float2*)(ws + recs * cache->head_dim);
-  a.ws_s = ws + recs * (cache->head_dim + 2) + (recs * 2) % 4, a.ld_s = paged_score_ld(l_max), a.ws_t = (float2*)a.ws_s;
+  a.ws_t = a.ws_ml + recs, a.ws_s = (float*)(a.ws_t + recs), a.ld_s = paged_score_ld(l_max);
   a.out = out, a.ldo = ldo, a.weights = weights, a.ldw_seq = ldw_seq, a.ldw = ldw, a.decay = decay;
-  const bool scores = weights && (int64_t)a.b.rows_max * a.rep <= PA_SCORES;
-  if (cache->head_dim == 64) return scores ? launch_paged_attn<64, true>(a, stream) : launch_paged_attn<64, false>(a, stream);
-  return scores ? launch_paged_attn<128, true>(a, stream) : launch_paged_attn<128, false>(a, stream);
+  const int wk = !weights ? 0 : (int64_t)a.b.rows_max * a.rep <= PA_SCORES ? 1 : 2;
+  if (cache->head_dim == 64)
+    return wk == 0 ? launch_paged_attn<64, 0>(a, stream) : wk == 1 ? launch_paged_attn<64, 1>(a, stream) : launch_paged_attn<64, 2>(a, stream);
+  return wk == 0 ? launch_paged_attn<128, 0>(a, stream) : wk == 1 ? launch_paged_attn<128, 1>(a, stream) : launch_paged_attn<128, 2>(a, stream);
 }

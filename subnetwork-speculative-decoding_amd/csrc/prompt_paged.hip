@@ -5,7 +5,8 @@
 // heads that share a kv head, a workgroup of four waves has 128 columns of one kv head, 32 a wave, and a block's K and V are copied
 // into LDS once for all of them (global to LDS, 16 bytes a lane, into two buffers each). Blocks are folded with a running
 // reference m, sum l and output O in fp32; the reference follows a column's maximum only when that has grown by more than
-// 2^8. Probabilities are rounded to bf16 as the second product's operand; l sums them before that.
+// 2^8. Probabilities are rounded to bf16 as the second product's operand; l sums them as rounded, so that what a rounding does to a
+// weight that dominates it does to l too.
 //
 // v_mfma_f32_32x32x16_bf16 rather than 16x16x32: the vector pipe stands still for about 8 cycles with every matrix instruction that another
 // wave issues, whatever its size, so half as many of twice the work leave it more (a wave of products beside one of multiply-adds:
@@ -14,12 +15,12 @@
 // What bounds it, 32 heads on 8 kv heads of 128 (8b shapes): a prompt of 16384 rows 1.89 ms, 1160 TFLOP/s, where a large library product reaches
 // 1300: matrix pipe and vector pipe, each about half of a block's 1.9 us for two workgroups a CU, at the clock that the power leaves.
 // Shorter prompts: a tile's beginning and end, about 8 us (rows, pages, first copies; the partly attended blocks; the output), of
-// which a second workgroup on the CU hides half, and the last tiles' end: 4096 rows 145 to 155 us (by box), 16 prompts of 232 to 1500
-// rows 183 to 191.
-// Tried (us of 16 prompts, 191 on that box): tiles dealt to resident workgroups, the next one's first blocks copied before the output 202;
-// the longest tiles of all sequences first 192. Eight waves a workgroup: a prompt of 4096 rows 138 against 147, of 2048 60 against 50,
-// 16 prompts 170 against 160. 64 columns a wave with twice the registers 269 for 157, two groups of waves taking turns at the
-// matrix pipe 155, sums of l by dot products no change.
+// which a second workgroup on the CU hides half, and the last tiles' end: 4096 rows 131 us (1050 TFLOP/s), 16 prompts of 232 to 1500 rows
+// 132; on a slower box 7 % more.
+// Tried (us of 16 prompts with the write of their K and V, 191 on that box): tiles dealt to resident workgroups, the next one's first
+// blocks copied before the output 202; the longest tiles of all sequences first 192. Eight waves a workgroup: a prompt of 4096 rows 138 against 147, of 2048 60 against 50,
+// 16 prompts 170 against 160. 64 columns a wave with twice the registers: 4096 rows 269 for 157; two groups of waves that take
+// turns at the matrix pipe 155.
 #include "paged.h"
 
 #include <algorithm>
@@ -115,6 +116,12 @@ __device__ __forceinline__ void prompt_reference(PromptState<HD>& st, const f32x
   st.m = grow ? mx : st.m;
 }
 
+// l plus two bf16 values, in fp32.
+__device__ __forceinline__ float prompt_sum2(uint32_t two, float l) {
+  typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, two), __builtin_bit_cast(bf16x2_t, 0x3f803f80u), l, false);
+}
+
 template <int HD>
 __device__ __forceinline__ void prompt_exp(PromptState<HD>& st, const f32x16_t (&s)[2], float scale_log2, u32x4_t (&p)[4]) {
   const float ms = st.m == -INFINITY ? 0.f : st.m;  // nothing attended so far: every p is 0
@@ -124,8 +131,9 @@ __device__ __forceinline__ void prompt_exp(PromptState<HD>& st, const f32x16_t (
     for (int r = 0; r < 16; r += 2) {
       const float p0 = __builtin_amdgcn_exp2f(fmaf(s[c][r], scale_log2, -ms));
       const float p1 = __builtin_amdgcn_exp2f(fmaf(s[c][r + 1], scale_log2, -ms));
-      st.l += p0 + p1;
-      p[2 * c + r / 8][r % 8 / 2] = pack_bf16x2(p0, p1);
+      const uint32_t both = pack_bf16x2(p0, p1);
+      st.l = prompt_sum2(both, st.l);
+      p[2 * c + r / 8][r % 8 / 2] = both;
     }
 }
 
