@@ -16,8 +16,8 @@
 // 1300: matrix pipe and vector pipe, each about half of a block's 1.9 us for two workgroups a CU, at the clock that the power leaves.
 // Shorter prompts: a tile's beginning and end, about 8 us (rows, pages, first copies; the partly attended blocks; the output), of
 // which a second workgroup on the CU hides half, and the last tiles' end: 4096 rows 131 us (1050 TFLOP/s), 16 prompts of 232 to 1500 rows
-// 132; on a slower box 7 % more.
-// Tried (us of 16 prompts with the write of their K and V, 191 on that box): tiles dealt to resident workgroups, the next one's first
+// 132; on a slower card 7 % more.
+// Tried (us of 16 prompts with the write of their K and V, 191 on that card): tiles dealt to resident workgroups, the next one's first
 // blocks copied before the output 202; the longest tiles of all sequences first 192. Eight waves a workgroup: a prompt of 4096 rows 138 against 147, of 2048 60 against 50,
 // 16 prompts 170 against 160. 64 columns a wave with twice the registers: 4096 rows 269 for 157; two groups of waves that take
 // turns at the matrix pipe 155.
