@@ -307,9 +307,9 @@ int ssd_paged_read_bf16(const SsdPagedKv* cache, const SsdPagedBatch* batch, int
 
 /* Attention of the batch's rows q [M][heads * head_dim]: row i of a sequence attends slots [0, lengths - n + i], itself the
  * last (the causal mask of ssd/models/subnetwork_draft.py:165-191 for a chunk behind a cache). Zeros for rows that attend
- * nothing, or scores of -inf alone. l_max (1 .. 64 * table_cols): slots from there on are not attended. heads / kv_heads any whole ratio; scale > 0.
- * A V value that is not finite reaches the rows that attend its slot and no other (where some rows attend only part of its
- * 64-slot block it makes their outputs NaN).
+ * nothing, or scores of -inf alone. l_max (1 .. 64 * table_cols): slots from there on are not attended. heads / kv_heads any
+ * whole ratio; scale > 0. A V value that is not finite makes the outputs of the rows that attend its slot NaN or infinite, and
+ * no other's.
  *
  * ssd_paged_attention_bf16 is for few rows a sequence: the length is cut into groups of 4 * span slots (span a multiple of 64 up
  * to 4096), folded by a workgroup each and added up in a fixed order, so a row's result depends on its query, its keys
