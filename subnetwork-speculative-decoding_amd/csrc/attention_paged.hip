@@ -20,7 +20,8 @@
 // row after 131000 keys 97 (5.5), 24 sequences with weights 38; 6 sequences of 16 rows and 1200 to 4001 keys, four tiles that share
 // K and V through L2, 25 and 17 for the join and the weights. One row after 500 keys of the smallest shape 4.8: latency.
 // Tried: two tiles a workgroup, whose registers leave one workgroup a CU (6 sequences of 16 rows 29 us against 25, 2 of 60 rows and
-// 8000 keys 87 against 76).
+// 8000 keys 87 against 76); tiles one after another in a workgroup, K and V on their way for the next while one ends (42 against 41 for
+// two, 50 for three: the tiles' chains are better side by side).
 #include "paged.h"
 
 #include <algorithm>
