@@ -160,7 +160,7 @@ __device__ __forceinline__ uint32_t evict_rank(float f) {
   return f != f ? 0u : (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
 
-constexpr int EV_T = 1024, EV_BINS = 2048;
+constexpr int EV_T = 1024, EV_BINS = 2048, EV_OWN = 8;  // EV_OWN: ranks that a thread keeps
 
 // Exclusive prefix sum of x over the workgroup's threads, and the total; every thread calls it.
 __device__ __forceinline__ int evict_scan(int x, int* wave_sums, int& total) {
@@ -187,7 +187,8 @@ __device__ __forceinline__ int evict_scan(int x, int* wave_sums, int& total) {
 
 // A workgroup per (layer, sequence, kv head) finds the slots that stay. The least rank that stays is found exactly by three
 // histograms of 11, 11 and 10 of its bits; then one pass in slot order writes what ranks above it, and of those that rank with
-// it the lowest slots. What bounds it: the dependent passes over a row; 256 rows of up to 4096 weights 13 us.
+// it the lowest slots. What bounds it: the dependent passes over a row; 256 rows of up to 4096 weights 11 us (13 with loads
+// in every pass).
 __global__ __launch_bounds__(EV_T) void evict_select_kernel(EvictArgs a) {
   __shared__ int hist[EV_BINS], wave_sums[EV_T / 64], found[2];
   const int tid = threadIdx.x, row = blockIdx.x, s = row / a.c.kv % a.b.n_seq;
@@ -200,16 +201,21 @@ __global__ __launch_bounds__(EV_T) void evict_select_kernel(EvictArgs a) {
   uint32_t least = 0;  // ranks above it stay, and `need` of those equal to it
   const bool all = need >= m1 - m0;
   if (!all && need > 0) {
-    uint32_t mask = 0;
+    uint32_t mask = 0, own[EV_OWN];  // the first of this thread's ranks, loaded together
+#pragma unroll
+    for (int i = 0; i < EV_OWN; ++i) own[i] = evict_rank(w[min(m0 + tid + EV_T * i, m1 - 1)]);
 #pragma unroll
     for (int pass = 0; pass < 3; ++pass) {
       const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
       hist[tid] = 0, hist[tid + EV_T] = 0;
       __syncthreads();
-      for (int t = m0 + tid; t < m1; t += EV_T) {
-        const uint32_t u = evict_rank(w[t]);
+      auto count = [&](uint32_t u) {
         if ((u & mask) == least) atomicAdd(&hist[(u >> shift) & (bins - 1)], 1);
-      }
+      };
+#pragma unroll
+      for (int i = 0; i < EV_OWN; ++i)
+        if (m0 + tid + EV_T * i < m1) count(own[i]);
+      for (int t = m0 + tid + EV_T * EV_OWN; t < m1; t += EV_T) count(evict_rank(w[t]));
       __syncthreads();
       // bins from the top: thread i holds bins top - 2i and top - 2i - 1
       const int b1 = EV_BINS - 1 - 2 * tid, h1 = hist[b1], h0 = hist[b1 - 1];
