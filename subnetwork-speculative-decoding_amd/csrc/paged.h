@@ -88,7 +88,6 @@ inline PagedBatch paged_batch(const SsdPagedBatch* b) {
   return PagedBatch{b->table, b->ld_table, b->table_cols, b->n_seq, b->rows_max, b->row_begin, b->lengths};
 }
 
-
 // Adds up every row's records of its length's groups of grp_keys keys (O in ws_o [row][head][group][head_dim], (m, l) in ws_ml) into out.
 int paged_join(const PagedBatch& b, int M, int heads, int head_dim, int l_cap, int grp_keys, int n_grps, float* ws_o, float2* ws_ml,
                bf16_t* out, int64_t ldo, hipStream_t stream);
