@@ -247,8 +247,6 @@ def _prepare_evict(case, r, st, kv, hd):
 
 def _prepare_logprobs(case, r, st):
     M, V = case["rows"], case["vocab"]
-    if own:
-        _package()
     x = r.normal(M, V, dtype=F32).mul_(3.0)
     u = torch.rand(M, V, generator=r.gen(), device="cuda")
     x.masked_fill_(u[:1] < 0.02, float("-inf"))  # columns that no answer may hold
