@@ -841,7 +841,7 @@ def token_logprobs(logits, tokens, top=0, ws=None):
     need = token_logprobs_ws_bytes(m, V, logits.dtype, top)
     if need and ws is None:
         ws = torch.empty(need, dtype=torch.uint8, device=logits.device)
-    pw, size = (None, 0) if ws is None else (_ptr(ws, "ws", torch.uint8, dev), ws.numel())
+    pw, size = (None, 0) if ws is None else (_ptr(ws, "ws", torch.uint8, dev, need), ws.numel())
     ids = torch.empty((m, top), dtype=I32, device=logits.device)
     lps = torch.empty((m, top), dtype=F32, device=logits.device)
     rank, logprobs, entropy = ids.new_empty(m), lps.new_empty(m), lps.new_empty(m)
