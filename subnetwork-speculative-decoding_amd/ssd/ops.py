@@ -756,7 +756,7 @@ def paged_attention(cache, batch, q, heads, l_max, span, ws=None, out=None, scal
         lds = max(lds, shape[1] * ldw) if shape[0] == 1 else lds
     if ws is None:
         ws = torch.empty(max(paged_attn_ws_floats(m, heads, hd, l_max, span, weights is not None), 4), dtype=F32, device=q.device)
-    px = _ptr(ws, "ws", F32, dev, 1)
+    px = _ptr(ws, "ws", F32, dev, 1 if m else 0)
     if m:
         _lib.call("ssd_paged_attention_bf16", cache, batch.desc, pq, ldq, m, heads, l_max, span,
                   hd ** -0.5 if scale is None else float(scale), px, ws.numel(), pw, lds, ldw, float(decay), po, ldo, _stream(dev))
@@ -785,7 +785,7 @@ def paged_prompt(cache, batch, q, heads, l_max, ws=None, out=None, scale=None):
     need = paged_prompt_ws_floats(m, heads, cache.kv_heads, hd, batch.n_seq, l_max)
     if need and ws is None:
         ws = torch.empty(need, dtype=F32, device=q.device)
-    pw, n = (None, 0) if ws is None else (_ptr(ws, "ws", F32, dev, 1), ws.numel())
+    pw, n = (None, 0) if ws is None else (_ptr(ws, "ws", F32, dev, need), ws.numel())
     if m:
         _lib.call("ssd_paged_prompt_bf16", cache, batch.desc, pq, ldq, m, heads, l_max, hd ** -0.5 if scale is None else float(scale), pw, n,
                   po, ldo, _stream(dev))
