@@ -47,7 +47,8 @@ def evict(w, length, keep, recent, first):
 def token_logprobs(logits, tokens, top):
     """(logprobs, entropy, rank, top ids, top logprobs) of finite or -inf logits [M, V], in doubles."""
     x = logits.double()
-    lp = x - torch.logsumexp(x, 1, keepdim=True)
+    d = x - x.amax(1, keepdim=True)  # first: beside a type's lowest value ln V is nothing, in 64 bits too
+    lp = d - d.exp().sum(1, keepdim=True).log()
     order = torch.sort(x, dim=1, descending=True, stable=True).indices
     have = (tokens >= 0) & (tokens < x.shape[1])
     t = torch.where(have, tokens, 0).long()

@@ -7,7 +7,7 @@
 // largest of them; only the few threads whose maximum reaches that bound look at their columns again (from registers, or a wave
 // together), what reaches it is collected, and a value's place is the number of those above it. Equal values rank by column, lowest
 // first. More candidates than the list holds (rows of equal logits) take a pass over the chunk for each place.
-// What bounds it: bytes and the vector pipe (about 13 operations a column): 1800 rows of 50257 fp32 columns 66 us, 5.4 TB/s; 1400
+// What bounds it: bytes and the vector pipe (about 14 operations a column): 1800 rows of 50257 fp32 columns 66 us, 5.4 TB/s; 1400
 // of 128256 bf16 columns 80 without alternatives, 4.5 TB/s, and 83 with 5. For few rows the latency of two launches and their
 // steps: 25 rows of 128256 bf16 columns 6.9 us without alternatives, 13.5 with 5.
 #include "topk.h"
@@ -186,10 +186,12 @@ __global__ __launch_bounds__(256) void lp_chunk_kernel(LogprobArgs a) {
     for (int i = 1; i < 32; ++i) top = lp_max(top, x[i]);
     const float m = lp_max(s.m, top);
     if (__any(m != s.m)) s = lp_rescale(s, m);
-    const float ref = m == -INFINITY ? 0.f : m * LP_LOG2E;
+    const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
-      const float y = fmaxf(fmaf(x[i], LP_LOG2E, -ref), -1e4f);  // -inf: a weight of 0, and 0 times it
+      // The difference first: products with log2 e are rounded by the logits' size, which lp_write's x_c - m would not take back, and
+      // overflow at a type's lowest and largest values. -inf: a weight of 0, and 0 times it.
+      const float y = fmaxf((x[i] - ref) * LP_LOG2E, -1e4f);
       const float e = __builtin_amdgcn_exp2f(y);
       s.z += e;
       s.t = fmaf(e, y, s.t);
