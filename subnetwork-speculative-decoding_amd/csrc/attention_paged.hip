@@ -33,6 +33,7 @@ constexpr int PA_WAVES = 4;
 // anew: 24 sequences of one row and 4000 keys 138 / 166, 6 of 4 rows 52 / 54, of 8 rows 58 / 58, of 16 rows and 1200 to 4001 keys
 // 63 / 58, 2 of 60 rows and 8000 keys 138 / 107).
 constexpr int PA_SCORES = 16;
+constexpr int PA_RUN = 8;  // records that a wave loads at once
 constexpr int PA_MAX_SPAN = 4096;  // a wave's pages are one table word a lane
 
 struct PagedAttnArgs {
@@ -297,8 +298,8 @@ __device__ __forceinline__ float2 paged_total(const float2* ml, int64_t step, in
   return make_float2(m, l);
 }
 
-// Second launch. Workgroups that add up the records: WPP waves a (sequence, row, head), each a run of groups in order, the
-// waves' sums then in order. Workgroups that add up received weights, of a set of slots of a (sequence, kv head), in a fixed order too: WK = 1
+// Second launch. Workgroups that add up the records: WPP waves a (sequence, row, head). PA_RUN groups from each multiple of PA_RUN on are
+// added up in order, then these sums in order, by however many waves: the row's bits follow from its own groups. Workgroups that add up received weights, of a set of slots of a (sequence, kv head), in a fixed order too: WK = 1
 // from the kept scores, a lane four slots; WK = 2 from K, a wave a block, sixteen pairs at a time, the lanes' sums last.
 template <int HD, int WK, int WPP>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
@@ -307,7 +308,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
   // the workgroups that add up weights, which take longer, come first
   if (WK == 0 || (int)blockIdx.x >= a.weight_wgs) {
     constexpr int V = HD / 64;  // dims a lane
-    __shared__ float part[4][HD];
+    __shared__ float part[WPP == 4 ? 64 / PA_RUN : 1][HD];  // sums of runs
     int u = blockIdx.x - (WK ? a.weight_wgs : 0);
     if (WPP == 1) u = u * 4 + w;
     const int h = u % a.heads;
@@ -322,32 +323,36 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
     const float* o = a.ws_o + (row * a.heads + h) * a.n_grps * HD + lane * V;
     const float2 all = paged_total(ml, 1, ng, lane, 64);
     float acc[V] = {};
-    const int run = WPP == 4 ? (ng + 3) / 4 : ng, from = WPP == 4 ? w * run : 0, to = min(from + run, ng);
-    for (int g0 = from; g0 < to; g0 += 64) {
-      const float wg = g0 + lane < to ? paged_weight(ml[g0 + lane].x, all.x) : 0.f;
-      const int n = min(64, to - g0);
-      for (int q = 0; q < n; q += 8) {
-        float x[8][V];
+    for (int g0 = 0; g0 < ng; g0 += 64) {
+      const float wg = g0 + lane < ng ? paged_weight(ml[g0 + lane].x, all.x) : 0.f;
+      const int n = min(64, ng - g0);
+      for (int q = WPP == 4 ? PA_RUN * w : 0; q < n; q += PA_RUN * WPP) {
+        float x[PA_RUN][V], run[V] = {};
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
+        for (int e = 0; e < PA_RUN; ++e)
 #pragma unroll
           for (int v = 0; v < V; ++v) x[e][v] = o[(int64_t)(g0 + min(q + e, n - 1)) * HD + v];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
+        for (int e = 0; e < PA_RUN; ++e) {
           const float t = __shfl(wg, min(q + e, 63));
 #pragma unroll
-          for (int v = 0; v < V; ++v) acc[v] = q + e < n ? fmaf(x[e][v], t, acc[v]) : acc[v];
+          for (int v = 0; v < V; ++v) run[v] = q + e < n ? fmaf(x[e][v], t, run[v]) : run[v];
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          if constexpr (WPP == 4) part[q / PA_RUN][lane * V + v] = run[v];
+          else acc[v] += run[v];
         }
       }
-    }
-    if constexpr (WPP == 4) {
+      if constexpr (WPP == 4) {
+        __syncthreads();
+        for (int q = 0; w == 0 && q < n; q += PA_RUN)
 #pragma unroll
-      for (int v = 0; v < V; ++v) part[w][lane * V + v] = acc[v];
-      __syncthreads();
-      if (w) return;
-#pragma unroll
-      for (int v = 0; v < V; ++v) acc[v] = ((acc[v] + part[1][lane * V + v]) + part[2][lane * V + v]) + part[3][lane * V + v];
+          for (int v = 0; v < V; ++v) acc[v] += part[q / PA_RUN][lane * V + v];
+        if (g0 + 64 < ng) __syncthreads();  // the runs have been read
+      }
     }
+    if (WPP == 4 && w) return;
 #pragma unroll
     for (int v = 0; v < V; ++v) acc[v] = all.y == 0.f ? 0.f : acc[v] / all.y;
     bf16_t* dst = a.out + row * a.ldo + h * HD + lane * V;
