@@ -335,8 +335,8 @@ int ssd_paged_prompt_bf16(const SsdPagedKv* cache, const SsdPagedBatch* batch, c
  * order, to slots 0, 1, ... of the pages in after->table, which must be pages that `batch` does not use, and
  * after->lengths becomes min(lengths, keep) (it may be batch->lengths itself). weights: [layers][n_seq][kv_heads] rows of cap
  * floats, ldw apart, cap >= lengths (slots beyond it count as not there); out_weights, rows alike and elsewhere: the kept
- * ones, then zeros. kept: [layers][n_seq][kv_heads][keep] int32, the slots they came from, then -1. The row_begin and rows_max of both
- * batches are not used. No counterpart in the reference, whose caches only grow. */
+ * ones, then zeros. kept: [layers][n_seq][kv_heads][keep] int32, the slots they came from, then -1. keep may be more than cap, and is at
+ * most 64 * after->table_cols. The row_begin and rows_max of both batches are not used. No counterpart in the reference, whose caches only grow. */
 int ssd_paged_evict(const SsdPagedKv* cache, int layers, int64_t layer_elems, const SsdPagedBatch* batch, const SsdPagedBatch* after,
                     const float* weights, int64_t ldw, int cap, int keep, int recent, int first, float* out_weights, int32_t* kept,
                     hipStream_t stream);

@@ -369,7 +369,6 @@ SSD_API int ssd_paged_evict(const SsdPagedKv* cache, int layers, int64_t layer_e
   if (cap < 1 || ldw < cap) return set_error(SSD_EINVAL, "paged_evict: bad cap=%d ldw=%lld", cap, (long long)ldw);
   if (keep < 1 || recent < 0 || first < 0 || (int64_t)recent + first > keep)
     return set_error(SSD_EINVAL, "paged_evict: keep=%d must hold recent=%d and first=%d", keep, recent, first);
-  if (keep > cap) return set_error(SSD_EINVAL, "paged_evict: keep=%d > %d weights a row", keep, cap);
   if ((int64_t)after->table_cols * PAGE < keep)
     return set_error(SSD_EINVAL, "paged_evict: keep=%d > the %d pages a sequence of the new table", keep, after->table_cols);
   if (batch->n_seq == 0) return SSD_OK;

@@ -1,5 +1,5 @@
-"""A row's bits in the attention of few new rows: they follow from its query, its keys and the span alone, whatever the batch, the
-bound of the lengths and so the number of groups that a call cuts."""
+"""The paged cache's operators at other sizes of a call: a row's bits in the attention of few new rows follow from its query, its keys and
+the span alone, whatever the batch, the bound of the lengths and so the number of groups that a call cuts; eviction that keeps all."""
 
 import pytest
 import torch
@@ -33,3 +33,27 @@ def test_groups_are_added_up_the_same_by_one_wave_and_by_four(groups):
     n = 520  # pairs past the four waves' bound
     many = s.PB(s.table.expand(n, -1).contiguous(), i32([length] * n), i32(sums([1] * n)), 1)
     assert torch.equal(s.cache.attend(0, s.q.cuda().expand(n, -1).contiguous(), many, length), out.expand(n, -1))
+
+
+# ------------------------------------------------------------------------------------------------- eviction
+@pytest.mark.parametrize("keep,cap", [(129, 128), (200, 128), (300, 150), (64, 60)])
+def test_eviction_that_keeps_more_than_the_weights_hold_keeps_all(keep, cap):
+    """A batch whose sequences are all short: every slot stays, in new pages; slots from the weights' end on count as not there."""
+    kv, lens = 2, [100, 0, 128, 37]
+    s = Setup(lens, [1] * 4, kv, kv, 64, seed=42, spare=20).fill()
+    unused = [p for p in range(s.cache.pages) if p not in sum(s.ids, [])]
+    cols = (keep + 63) // 64
+    stay = [min(n, cap, keep) for n in lens]
+    new = i32([[unused.pop() if c * 64 < n else -1 for c in range(cols)] for n in stay])
+    after = s.PB(new, i32([7] * 4), i32(sums(stay)), max(stay))
+    w = torch.rand(1, 4, kv, cap, generator=s.g)
+    kept, moved = s.cache.evict(s.batch, after, w.cuda(), keep, 5, 3)
+    assert after.lengths.tolist() == stay and kept.shape[-1] == keep and moved.shape == w.shape
+    k, v = (x.cpu().view(-1, kv, 64) for x in s.cache.read(0, after, sum(stay)))
+    at = 0
+    for q, n in enumerate(stay):
+        for h in range(kv):
+            assert kept[0, q, h].tolist() == list(range(n)) + [-1] * (keep - n)
+            assert torch.equal(moved[0, q, h].cpu(), torch.cat([w[0, q, h, :n], torch.zeros(cap - n)]))
+        assert torch.equal(k[at:at + n], s.k[q][:n]) and torch.equal(v[at:at + n], s.v[q][:n])
+        at += n
