@@ -319,8 +319,8 @@ int ssd_paged_read_bf16(const SsdPagedKv* cache, const SsdPagedBatch* batch, int
  * softmax weight of t (decay in [0, 1]; 0: the old value is not read); the rest stays, and so do the weights of sequences
  * without rows in the call. Weights are summed in a fixed order.
  * ssd_paged_prompt_bf16 is for many rows a sequence; where they are too few to fill the chip it cuts the length into parts
- * too (ws: ssd_paged_prompt_ws_floats(...) floats, as above; 0: NULL will do). The parts follow from M, the heads, n_seq and
- * l_max, and the results differ by rounding between numbers of parts and from the other's. */
+ * too (ws: ssd_paged_prompt_ws_floats(...) floats, as above, enough for any rows_max; 0: NULL will do). The parts follow from M, the
+ * heads, n_seq, rows_max and l_max, and the results differ by rounding between numbers of parts and from the other's. */
 int64_t ssd_paged_attn_ws_floats(int M, int heads, int head_dim, int64_t l_max, int span, int weights);
 int ssd_paged_attention_bf16(const SsdPagedKv* cache, const SsdPagedBatch* batch, const uint16_t* q, int64_t ldq, int M, int heads,
                              int l_max, int span, float scale, float* ws, int64_t ws_floats, float* weights, int64_t ldw_seq,

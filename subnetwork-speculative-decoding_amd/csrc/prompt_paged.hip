@@ -365,32 +365,44 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedPromptArgs a)
   }
 }
 
-// Workgroups of a call with the length in one part: every sequence's tiles are at most a whole-tile share of the rows and one more.
-static int64_t prompt_tiles(int64_t M, int rep, int n_seq, int kv) { return (M * rep / (32 * PP_WAVES) + n_seq) * kv; }
+// Workgroups of a call with the length in one part, as near as the host can tell: every sequence's tiles are at most those of the
+// longest one's rows, exact for rows of one number, and together at most a whole-tile share of the rows and one more each.
+static int64_t prompt_tiles(int64_t M, int rep, int n_seq, int rows_max, int kv) {
+  constexpr int CW = 32 * PP_WAVES;
+  const int64_t most = (std::min<int64_t>(rows_max, M) * rep + CW - 1) / CW;
+  return std::min(M * rep / CW + n_seq, n_seq * most) * kv;
+}
 
 // Parts of the length: one while the tiles fill the chip's 256 CUs, else as many as bring two workgroups a CU, of eight blocks or more
-// (one / several parts, us: 100 rows of 32 heads after 8000 keys 136 / 37, 500 149 / 87, 40 rows of 15 heads 134 / 22). Two parts
-// pay for their records only over a long length: 4 times 100 rows of 64 heads after 4000 keys 77 / 83.
-static int prompt_splits(int64_t M, int rep, int n_seq, int kv, int64_t l_max) {
-  const int64_t wgs = prompt_tiles(M, rep, n_seq, kv), blocks = (l_max + PAGE - 1) / PAGE;
+// (one / several parts, us: 100 rows of 32 heads after 8000 keys 136 / 37, 500 149 / 87, 40 rows of 15 heads 134 / 22, 16 sequences of 32
+// rows of 32 heads after 8000 keys 151 / 120). Two parts pay for their records only over a long length (4 times 100 rows of 64 heads after
+// 4000 keys 77 / 83; 700 rows of 32 heads after 6500 126 / 116, 900 after 16000 286 / 262), and not where sequences of one tile read K and V
+// once, which is bound by bytes (24 of 32 rows after 8000 168 / 169, 31 192 / 213).
+// The fewer rows the longest sequence can have, the fewer tiles and the more parts: rows_max 0 asks for the most.
+static int prompt_splits(int64_t M, int rep, int n_seq, int rows_max, int kv, int64_t l_max) {
+  const int64_t longest = std::max<int64_t>(rows_max, (M + n_seq - 1) / std::max(n_seq, 1));
+  const int64_t wgs = prompt_tiles(M, rep, n_seq, (int)longest, kv), blocks = (l_max + PAGE - 1) / PAGE;
   if (wgs >= 256) return 1;
   const int64_t n = std::max<int64_t>(1, std::min(512 / std::max<int64_t>(wgs, 1), blocks / 8));
-  return n == 2 && blocks < 96 ? 1 : (int)n;
+  return n == 2 && (blocks < 96 || (rows_max && longest * rep <= 32 * PP_WAVES)) ? 1 : (int)n;
 }
 
 // Of two workgroups on a CU the older one's waves go first, and its tile ends long before the other's (1.7 us a block against 2.4). That is
 // as it should be where a last, part round of tiles follows or the longest tiles begin first and all at once. Where all tiles make two
-// rounds, or one of tiles of like lengths (behind a long past), they had better end together: a wave's priority then goes up and
-// down from block to block. us without / with, heads of 128, by workgroups for the 512 places: prompts of 2048 rows (520) 51 / 54, 2600 (656)
-// 66 / 69, 3400 (856) 103 / 98, 4096 (1032) 141 / 131, 5000 (1256) 196 / 203, 8192 (2056) 486 / 487; 8 pieces of 256 rows after 2000 keys
-// (576) 76 / 74, (1088) 141 / 139; 3 of 500 rows after 6000 (768) 290 / 323, 3 of 256 to 511 (528) 195 / 187. Heads of 64: 2048 rows 35 / 39.
+// rounds, or a little more than one behind pasts of different lengths, they had better end together: a wave's priority then goes up and
+// down from block to block. us without / with, heads of 128, by workgroups for the 512 places. One prompt: 2048 rows (512) 52 / 54, 3000
+// (752) 81 / 84, 3300 (832) 98 / 96, 3600 (904) 115 / 108, 4096 (1024) 143 / 135, 4480 (1120) 166 / 165; of 64 heads 2048 rows (1024) 79 / 74,
+// 2240 (1120) 90 / 91. Two prompts of 2048 rows (1024) 80 / 76, but four of 1024 50 / 54. Five pieces of 512 to 1024 rows behind 0 to 4000
+// keys (960) 183 / 170; 16 of 256 behind 2000 each (1024) 147 / 148. A little over one round, pieces of 64 heads behind 2500 to 5000 keys
+// (528) 150 / 144, (608) 184 / 167; behind 5000 each (528) 231 / 240, (608) 237 / 245: the host cannot tell these apart, and lengths that
+// differ are the rule. A whole round behind 5000 each (512) 166 / 164, behind 2500 to 5000 134 / 139. Heads of 64: 2048 rows 35 / 39.
 static bool prompt_turns(int64_t wgs, int rows_max, int l_max) {
   return (wgs >= 820 && wgs <= 1126) || (wgs > 512 && wgs <= 614 && rows_max <= l_max / 2);  // 1.6 to 2.2 rounds, 1 to 1.2
 }
 
 template <int HD>
 static int launch_paged_prompt(const PagedPromptArgs& a, hipStream_t stream) {
-  const int64_t wgs = prompt_tiles(a.M, a.rep, a.b.n_seq, a.c.kv) * a.splits;
+  const int64_t wgs = prompt_tiles(a.M, a.rep, a.b.n_seq, a.b.rows_max, a.c.kv) * a.splits;
   if (paged_grid_too_large(wgs, 256)) return set_error(SSD_ERANGE, "paged_prompt: too many workgroups");
   if constexpr (HD == 128) {
     if (prompt_turns(wgs, a.b.rows_max, a.l_cap)) SSD_LAUNCH((paged_prompt_kernel<HD, true>), dim3((unsigned)wgs), dim3(256), 0, stream, a);
@@ -409,7 +421,7 @@ using namespace ssd;
 
 SSD_API int64_t ssd_paged_prompt_ws_floats(int M, int heads, int kv_heads, int head_dim, int n_seq, int64_t l_max) {
   if (M < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads || head_dim < 1 || n_seq < 0 || l_max < 1 || l_max > 1 << 30) return -1;
-  const int splits = prompt_splits(M, heads / kv_heads, n_seq, kv_heads, l_max);
+  const int splits = prompt_splits(M, heads / kv_heads, n_seq, 0, kv_heads, l_max);
   return splits == 1 ? 0 : (int64_t)M * heads * splits * (head_dim + 2);
 }
 
@@ -434,10 +446,10 @@ SSD_API int ssd_paged_prompt_bf16(const SsdPagedKv* cache, const SsdPagedBatch* 
   a.Q = q, a.ldq = ldq, a.M = M, a.heads = heads, a.rep = heads / cache->kv_heads, a.l_cap = l_max;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.out = out, a.ldo = ldo;
-  const int64_t need = ssd_paged_prompt_ws_floats(M, heads, cache->kv_heads, cache->head_dim, batch->n_seq, l_max);
+  a.splits = prompt_splits(M, a.rep, batch->n_seq, batch->rows_max, a.c.kv, l_max);
+  const int64_t need = a.splits == 1 ? 0 : (int64_t)M * heads * a.splits * (cache->head_dim + 2);
   if (need && (!ws || ((uintptr_t)ws & 15) || ws_floats < need))
     return set_error(SSD_EINVAL, "paged_prompt: workspace too small or not 16-byte aligned");
-  a.splits = prompt_splits(M, a.rep, batch->n_seq, a.c.kv, l_max);
   a.per = ((l_max + PAGE - 1) / PAGE + a.splits - 1) / a.splits;
   a.ws_o = ws, a.ws_ml = (float2*)(ws + (int64_t)M * heads * a.splits * cache->head_dim);
   return cache->head_dim == 64 ? launch_paged_prompt<64>(a, stream) : launch_paged_prompt<128>(a, stream);

@@ -57,3 +57,35 @@ def test_eviction_that_keeps_more_than_the_weights_hold_keeps_all(keep, cap):
             assert torch.equal(moved[0, q, h].cpu(), torch.cat([w[0, q, h, :n], torch.zeros(cap - n)]))
         assert torch.equal(k[at:at + n], s.k[q][:n]) and torch.equal(v[at:at + n], s.v[q][:n])
         at += n
+
+
+# ------------------------------------------------------------------------------------------------- prompts
+@pytest.mark.parametrize("n,rows,past", [(16, 32, 1200), (7, 32, 700), (3, 64, 1500), (64, 32, 0), (5, 33, 1100)])
+def test_prompts_of_one_length_that_fill_their_tiles(n, rows, past):
+    """As many tiles as the launch counts, none to spare, with the length whole and in parts."""
+    s = Setup([past + rows + i % 3 for i in range(n)], [rows] * n, 4, 1, 64, seed=43).fill()
+    ws = torch.full((s.cache.prompt_floats(n * rows, 4, s.batch),), float("nan"), device="cuda")
+    s.check(s.cache.attend_prompt(0, s.q.cuda(), s.batch, ws=ws))
+
+
+@pytest.mark.parametrize("rows", [[130, 1, 1, 2, 0], [1, 1, 40], [64, 0, 0, 0, 0, 0, 0, 64]])
+def test_prompts_whose_workspace_is_sized_by_the_rows_alone(rows):
+    """Uneven rows, and a bound of them that is far too large."""
+    s = Setup([600 + 100 * i + n for i, n in enumerate(rows)], rows, 4, 1, 64, seed=44).fill()
+    for most in (max(rows), 4096):
+        b = s.PB(s.table, s.lengths, s.begin, most)
+        ws = torch.full((s.cache.prompt_floats(sum(rows), 4, b),), float("nan"), device="cuda")
+        s.check(s.cache.attend_prompt(0, s.q.cuda(), b, ws=ws))
+
+
+def test_prompt_rows_of_no_sequence_and_a_tight_bound():
+    """More rows than the sequences own."""
+    s = Setup([900, 1000], [20, 31], 4, 1, 64, seed=45).fill()
+    q = torch.zeros(300, 256, dtype=torch.bfloat16, device="cuda")
+    q[100:151] = s.q.cuda()
+    out = torch.full_like(q, 7.0)
+    b = s.PB(s.table, s.lengths, i32([100, 120, 151]), 31)
+    ws = torch.full((s.cache.prompt_floats(300, 4, b),), float("nan"), device="cuda")
+    s.cache.attend_prompt(0, q, b, out=out, ws=ws)
+    s.check(out[100:151])
+    assert (out[:100] == 7).all() and (out[151:] == 7).all()

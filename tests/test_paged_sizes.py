@@ -1,0 +1,23 @@
+"""What the host computes for the paged operators' launches and workspaces, on the CPU."""
+
+
+def test_a_prompt_call_counts_the_tiles_that_run():
+    """16 sequences of 32 rows of 4 heads a kv head are 16 tiles of 128 columns a kv head: 128 workgroups for 256 CUs, so the length is
+    cut. One sequence of as many rows makes as many tiles; 32 sequences fill the chip."""
+    from ssd import ops
+
+    floats = lambda m, s: ops.paged_prompt_ws_floats(m, 32, 8, 128, s, 8192)  # noqa: E731
+    four = 32 * 4 * 130  # floats a row: four parts
+    assert floats(16 * 32, 16) == 16 * 32 * four and floats(512, 1) == 512 * four
+    assert floats(15 * 32, 15) == 15 * 32 * four
+    assert floats(32 * 32, 32) == 0 and floats(1024, 1) == 0
+
+
+def test_prompt_workspaces_of_one_sequence_follow_from_its_tiles():
+    from ssd import ops
+
+    for m in (1, 7, 100, 333, 512):
+        one = ops.paged_prompt_ws_floats(m, 32, 8, 128, 1, 16384)
+        tiles = 8 * -(-m * 4 // 128)
+        assert one == (0 if tiles >= 256 else m * 32 * min(512 // tiles, 32) * 130)
+    assert ops.paged_prompt_ws_floats(0, 32, 8, 128, 4, 16384) == 0
