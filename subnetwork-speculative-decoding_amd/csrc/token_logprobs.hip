@@ -357,15 +357,18 @@ __global__ __launch_bounds__(256) void lp_merge_kernel(LogprobArgs a) {
   lp_write(a, row, s, ahead, x.xt, tok, best);
 }
 
-// Chunks of a row. A workgroup takes about 6 us and 0.7 for each batch of 1024 vectors, the second launch 4 to 6, so short rows, and those of
-// many rows, are one chunk; else as many as bring 1024 workgroups, or of one batch each where those are at most twice as many.
-// us at 128256 bf16 columns and 5 alternatives, 1 / 4 / 16 chunks: 1 row 22 / 15 / 12, 64 23 / 17 / 16, 300 35 / 31 / 49, 500
-// 38 / 41 / 74; 300 rows of 32000 columns 16 / 20 / 42.
-static int lp_chunks(int M, int V, int elem) {
-  const int64_t batches = (((int64_t)V * elem + 15) / 16 + 1023) / 1024;
-  if (M >= 400 || batches < 8) return 1;
+// Chunks of a row. A workgroup takes about 6 us and 0.7 to 1.1 for each batch of 32 columns a thread (whatever their type), the second
+// launch 4 to 6, so short rows, and those of many rows, are one chunk; else as many as bring 1024 workgroups, or of one batch each where
+// those are at most 1.4 times as many (us as many / one batch each: 64 rows of 200000 fp32 columns 23 / 26, of 128256 in 13 chunks 21.5 / 18.7,
+// 300 of 65000 30 / 33). us with 5 alternatives, 1 / 4 / 16 chunks: 128256 bf16 columns, 1 row 22 / 15 / 12, 64 27 / 18 / 17, 300
+// 37 / 34 / 50, 399 39 / 41 / 63; fp32 25 / 15 / 12, 30 / 20 / 19, 42 / 44 / 54, 48 / 54 / 68. 50257 columns, 1 / 7 chunks: 25 rows
+// bf16 15 / 12, fp32 16 / 12, 64 15 / 13, 17 / 15, 150 17 / 21, 19 / 22, 300 21 / 29, 23 / 30; 32000 columns, 1 / 4: 25 rows 12 / 12, 12.5 / 12.3.
+constexpr int LP_BATCH = 256 * 32;
+static int lp_chunks(int M, int V) {
+  const int64_t batches = (V + LP_BATCH - 1) / LP_BATCH;
+  if (M >= 400 || batches < (M > 100 ? 8 : 6)) return 1;
   const int64_t want = (1024 + M - 1) / std::max(M, 1);
-  return (int)std::min<int64_t>(2 * want >= batches ? batches : want, LP_CHUNKS);
+  return (int)std::min<int64_t>(7 * want >= 5 * batches ? batches : want, LP_CHUNKS);
 }
 
 }  // namespace ssd
@@ -374,7 +377,7 @@ using namespace ssd;
 
 SSD_API int64_t ssd_token_logprobs_ws_bytes(int M, int V, int dtype, int top) {
   if (M < 0 || V < 1 || V > 1 << 24 || dtype < 0 || dtype > 2 || top < 0 || top > LP_TOP) return -1;
-  const int chunks = lp_chunks(M, V, dtype == 2 ? 4 : 2);
+  const int chunks = lp_chunks(M, V);
   return chunks == 1 ? 0 : (int64_t)M * chunks * lp_record_bytes(top);
 }
 
@@ -393,7 +396,7 @@ SSD_API int ssd_token_logprobs(const void* logits, int dtype, int64_t ld, int M,
   if (ld < V && M > 1) return set_error(SSD_EINVAL, "token_logprobs: row stride %lld < V", (long long)ld);
   if ((uintptr_t)logits % elem) return set_error(SSD_EINVAL, "token_logprobs: logits not aligned to their type");
   LogprobArgs a{};
-  a.x = logits, a.ld = ld, a.M = M, a.V = V, a.chunks = lp_chunks(M, V, elem);
+  a.x = logits, a.ld = ld, a.M = M, a.V = V, a.chunks = lp_chunks(M, V);
   a.vecs = (int)((((int64_t)V * elem + 15) / 16 + a.chunks - 1) / a.chunks);
   a.tok = tokens, a.tok64 = (tokens64 ? 1 : 0), a.top = top, a.ws = (char*)ws;
   a.logprob = logprobs, a.entropy = entropy, a.rank = rank, a.top_ids = top_ids, a.top_lp = top_logprobs;

@@ -1,5 +1,8 @@
 """What the host computes for the paged operators' launches and workspaces, on the CPU."""
 
+import pytest
+import torch
+
 
 def test_a_prompt_call_counts_the_tiles_that_run():
     """16 sequences of 32 rows of 4 heads a kv head are 16 tiles of 128 columns a kv head: 128 workgroups for 256 CUs, so the length is
@@ -21,3 +24,13 @@ def test_prompt_workspaces_of_one_sequence_follow_from_its_tiles():
         tiles = 8 * -(-m * 4 // 128)
         assert one == (0 if tiles >= 256 else m * 32 * min(512 // tiles, 32) * 130)
     assert ops.paged_prompt_ws_floats(0, 32, 8, 128, 4, 16384) == 0
+
+
+@pytest.mark.parametrize("m,v,chunks", [(1, 128256, 16), (25, 128256, 16), (64, 128256, 16), (300, 128256, 4), (400, 128256, 1), (25, 50257, 7),
+                                        (150, 50257, 1), (25, 32000, 1), (25, 200000, 25), (1, 1 << 24, 64), (0, 128256, 16)])
+def test_token_logprobs_cut_rows_by_columns_whatever_their_type(m, v, chunks):
+    """A thread takes 32 columns at a time; a chunk leaves a record of 32 bytes and 8 for each alternative."""
+    from ssd import ops
+
+    for dtype in (torch.bfloat16, torch.float16, torch.float32):
+        assert ops.token_logprobs_ws_bytes(m, v, dtype, 5) == (0 if chunks == 1 else m * chunks * (32 + 40))
