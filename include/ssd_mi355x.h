@@ -317,7 +317,9 @@ int ssd_paged_read_bf16(const SsdPagedKv* cache, const SsdPagedBatch* batch, int
  * time must not share it. With weights (may be NULL): for every slot t in use of sequence s and kv head h,
  * weights[s * ldw_seq + h * ldw + t] becomes decay * itself + the sum over the sequence's rows and h's query heads of the
  * softmax weight of t (decay in [0, 1]; 0: the old value is not read); the rest stays, and so do the weights of sequences
- * without rows in the call. Weights are summed in a fixed order.
+ * without rows in the call. Weights are summed in a fixed order. The workspace's `weights`: 0 without; with, the most (row, query
+ * head) pairs that a kv head has, rows_max * heads / kv_heads (above 16 the scores are not kept; 1 is enough for any). It holds for calls of
+ * up to M rows.
  * ssd_paged_prompt_bf16 is for many rows a sequence; where they are too few to fill the chip it cuts the length into parts
  * too (ws: ssd_paged_prompt_ws_floats(...) floats, as above, enough for any rows_max; 0: NULL will do). The parts follow from M, the
  * heads, n_seq, rows_max and l_max, and the results differ by rounding between numbers of parts and from the other's. */

@@ -521,8 +521,10 @@ using namespace ssd;
 
 SSD_API int64_t ssd_paged_attn_ws_floats(int M, int heads, int head_dim, int64_t l_max, int span, int weights) {
   if (M < 0 || heads < 1 || head_dim < 1 || l_max < 1 || l_max > 1 << 30 || span < 64 || span % 64 || span > PA_MAX_SPAN) return -1;
-  const int64_t pairs = (int64_t)M * heads, g = paged_groups(l_max, span);
-  return weights ? pairs * g * (head_dim + 4) + pairs * paged_score_ld(l_max) : pairs * g * (head_dim + 2);
+  const int64_t pairs = (int64_t)M * heads, recs = paged_groups(l_max, span) * (int64_t)(head_dim + (weights ? 4 : 2));
+  // scores are kept by a call of few pairs a kv head, which one of fewer rows than M may be
+  const int64_t scored = weights == 0 ? 0 : weights <= PA_SCORES ? pairs : (int64_t)std::min(M, PA_SCORES) * heads;
+  return std::max(pairs * recs, scored * (recs + paged_score_ld(l_max)));
 }
 
 SSD_API int ssd_paged_attention_bf16(const SsdPagedKv* cache, const SsdPagedBatch* batch, const uint16_t* q, int64_t ldq, int M,
@@ -541,7 +543,11 @@ SSD_API int ssd_paged_attention_bf16(const SsdPagedKv* cache, const SsdPagedBatc
   const int64_t cols = (int64_t)heads * cache->head_dim;
   if (((uintptr_t)q & 15) || ldq % 8 || ldq < cols || ((uintptr_t)out & 15) || ldo % 8 || ldo < cols)
     return set_error(SSD_EINVAL, "paged_attention: q/out rows must be 16-byte aligned with strides >= heads * head_dim");
-  if (((uintptr_t)ws & 15) || ws_floats < ssd_paged_attn_ws_floats(M, heads, cache->head_dim, l_max, span, weights != nullptr))
+  const int rep = heads / cache->kv_heads;
+  const int wk = !weights ? 0 : (int64_t)std::min(batch->rows_max, M) * rep <= PA_SCORES ? 1 : 2;
+  const int64_t recs = (int64_t)M * heads * paged_groups(l_max, span);
+  if (((uintptr_t)ws & 15) ||
+      ws_floats < recs * (cache->head_dim + (wk ? 4 : 2)) + (wk == 1 ? (int64_t)M * heads * paged_score_ld(l_max) : 0))
     return set_error(SSD_EINVAL, "paged_attention: workspace too small or not 16-byte aligned");
   if (weights && (ldw < l_max || ldw_seq < (int64_t)cache->kv_heads * ldw))
     return set_error(SSD_EINVAL, "paged_attention: weights rows of %lld for l_max %d, sequences %lld apart", (long long)ldw, l_max,
@@ -551,13 +557,11 @@ SSD_API int ssd_paged_attention_bf16(const SsdPagedKv* cache, const SsdPagedBatc
   a.b = paged_batch(batch);
   a.b.rows_max = std::min(a.b.rows_max, M);
   a.c = PagedCache{cache->k, cache->v, cache->pages, cache->kv_heads};
-  a.Q = q, a.ldq = ldq, a.M = M, a.heads = heads, a.rep = heads / cache->kv_heads, a.l_cap = l_max;
+  a.Q = q, a.ldq = ldq, a.M = M, a.heads = heads, a.rep = rep, a.l_cap = l_max;
   a.span_blk = span / PAGE, a.n_grps = paged_groups(l_max, span), a.grp_keys = PA_WAVES * span, a.scale_log2 = scale * 1.4426950408889634f;
-  const int64_t recs = (int64_t)M * heads * a.n_grps;
   a.ws_o = ws, a.ws_ml = (float2*)(ws + recs * cache->head_dim);
   a.ws_t = a.ws_ml + recs, a.ws_s = (float*)(a.ws_t + recs), a.ld_s = paged_score_ld(l_max);
   a.out = out, a.ldo = ldo, a.weights = weights, a.ldw_seq = ldw_seq, a.ldw = ldw, a.decay = decay;
-  const int wk = !weights ? 0 : (int64_t)a.b.rows_max * a.rep <= PA_SCORES ? 1 : 2;
   if (cache->head_dim == 64)
     return wk == 0 ? launch_paged_attn<64, 0>(a, stream) : wk == 1 ? launch_paged_attn<64, 1>(a, stream) : launch_paged_attn<64, 2>(a, stream);
   return wk == 0 ? launch_paged_attn<128, 0>(a, stream) : wk == 1 ? launch_paged_attn<128, 1>(a, stream) : launch_paged_attn<128, 2>(a, stream);

@@ -342,8 +342,9 @@ class PagedKVCache:
         return ops.paged_read(self._layers[i], batch, m, k_out, v_out)
 
     def attend_floats(self, m: int, heads: int, batch: PagedBatch, l_max: Optional[int] = None, weights: bool = False) -> int:
-        """Workspace floats of ``attend`` for ``m`` rows."""
-        return ops.paged_attn_ws_floats(m, heads, self.head_dim, batch.capacity if l_max is None else l_max, self._span(batch), weights)
+        """Workspace floats of ``attend`` for up to ``m`` rows."""
+        pairs = max(min(batch.rows_max, m) * heads // self.kv_heads, 1) if weights else 0
+        return ops.paged_attn_ws_floats(m, heads, self.head_dim, batch.capacity if l_max is None else l_max, self._span(batch), pairs)
 
     def attend(self, i: int, q: torch.Tensor, batch: PagedBatch, l_max: Optional[int] = None, out: Optional[torch.Tensor] = None,
                ws: Optional[torch.Tensor] = None, scale: Optional[float] = None, weights: Optional[torch.Tensor] = None,

@@ -724,7 +724,8 @@ def paged_read(cache, batch, m, k_out=None, v_out=None):
     return k_out, v_out
 
 
-def paged_attn_ws_floats(m: int, heads: int, head_dim: int, l_max: int, span: int, weights: bool = False) -> int:
+def paged_attn_ws_floats(m: int, heads: int, head_dim: int, l_max: int, span: int, weights: int = 0) -> int:
+    """``weights``: 0 without; with, the most (row, query head) pairs of a kv head, or True: enough for any."""
     n = int(_lib.load().ssd_paged_attn_ws_floats(m, heads, head_dim, l_max, span, int(weights)))
     if n < 0:
         raise ValueError(f"paged_attn_ws_floats: bad m={m} heads={heads} l_max={l_max} span={span}")
@@ -755,7 +756,8 @@ def paged_attention(cache, batch, q, heads, l_max, span, ws=None, out=None, scal
         ldw = max(ldw, weights.shape[2]) if shape[1] == 1 else ldw
         lds = max(lds, shape[1] * ldw) if shape[0] == 1 else lds
     if ws is None:
-        ws = torch.empty(max(paged_attn_ws_floats(m, heads, hd, l_max, span, weights is not None), 4), dtype=F32, device=q.device)
+        pairs = 0 if weights is None else max(min(batch.rows_max, m) * (heads // cache.kv_heads), 1)
+        ws = torch.empty(max(paged_attn_ws_floats(m, heads, hd, l_max, span, pairs), 4), dtype=F32, device=q.device)
     px = _ptr(ws, "ws", F32, dev, 1 if m else 0)
     if m:
         _lib.call("ssd_paged_attention_bf16", cache, batch.desc, pq, ldq, m, heads, l_max, span,

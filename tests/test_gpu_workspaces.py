@@ -55,3 +55,37 @@ def test_prompt_workspaces_that_are_too_small_or_not_in_one_run_are_refused():
     torch.cuda.synchronize()
     assert (buf == 7).all()
     assert torch.equal(s.cache.attend_prompt(0, q, s.batch, ws=buf[:need]), s.cache.attend_prompt(0, q, s.batch))
+
+
+@pytest.mark.parametrize("heads,kv,hd", [(32, 8, 128), (15, 5, 128), (16, 16, 64), (20, 1, 64)])
+def test_attention_with_weights_stays_in_its_workspace(heads, kv, hd):
+    """Windows of more pairs than keep scores, and calls of fewer rows in the same workspace."""
+    from test_gpu_paged import Setup, i32
+
+    s = Setup([900, 333, 70], [17, 18, 20], heads, kv, hd, seed=62, span=64).fill()
+    q = s.q.cuda()
+    need = s.cache.attend_floats(55, heads, s.batch, 960, weights=True)
+    buf = torch.full((need + 64,), float("nan"), device="cuda")
+    buf[need:] = 7.0
+    weights = torch.zeros(3, kv, 960, device="cuda")
+    s.check(s.cache.attend(0, q, s.batch, 960, ws=buf[:need], weights=weights), weights, torch.zeros_like(weights))
+    for most in (18, 1):  # rows of the first sequence alone, under the same bound and one of its own
+        for m in (1, 3, 16):
+            if most < m:
+                continue
+            one = s.PB(s.table[:1], i32([900 - 17 + m]), i32([0, m]), most)
+            weights = torch.zeros(1, kv, 960, device="cuda")
+            again = torch.zeros_like(weights)
+            out = s.cache.attend(0, q[:m], one, 960, ws=buf[:need], weights=weights)
+            assert torch.equal(out, s.cache.attend(0, q[:m], one, 960, weights=again)) and torch.equal(weights, again)
+    assert (buf[need:] == 7).all()
+    if 18 * heads // kv > 16:
+        assert need < ws_with_scores(s, heads, hd)
+    with pytest.raises(ValueError, match="workspace"):
+        s.cache.attend(0, q, s.batch, 960, ws=torch.empty(100, device="cuda"), weights=torch.zeros(3, kv, 960, device="cuda"))
+
+
+def ws_with_scores(s, heads, hd):
+    from ssd import ops
+
+    return ops.paged_attn_ws_floats(55, heads, hd, 960, 64, True)

@@ -34,3 +34,17 @@ def test_token_logprobs_cut_rows_by_columns_whatever_their_type(m, v, chunks):
 
     for dtype in (torch.bfloat16, torch.float16, torch.float32):
         assert ops.token_logprobs_ws_bytes(m, v, dtype, 5) == (0 if chunks == 1 else m * chunks * (32 + 40))
+
+
+def test_attention_workspaces_hold_scores_where_they_are_kept():
+    """Scores [row][head][slots] up to 16 (row, head) pairs a kv head. 96 rows of 32 heads, 4032 slots in 8 groups of 512: 64 pairs."""
+    from ssd import ops
+
+    floats = lambda m, pairs: ops.paged_attn_ws_floats(m, 32, 128, 4032, 128, pairs)  # noqa: E731
+    records, scores = 32 * 8 * 132, 32 * 4032  # a row's
+    assert floats(96, 0) == 96 * 32 * 8 * 130
+    assert floats(96, 1) == floats(96, True) == floats(96, 16) == 96 * (records + scores)
+    assert floats(96, 17) == floats(96, 64) == max(96 * records, 16 * (records + scores))
+    sizes = [floats(m, 64) for m in range(1, 97)]
+    assert sizes == sorted(sizes)  # enough for fewer rows, whose call may keep its scores
+    assert sizes[3] >= floats(4, 16)
