@@ -495,11 +495,11 @@ template <int HD, int WK>
 static int launch_paged_attn(PagedAttnArgs a, hipStream_t stream) {
   const int tiles = (int)(((int64_t)a.b.rows_max * a.rep + 15) / 16);
   a.sets = tiles;
-  const int64_t units = (int64_t)a.b.n_seq * a.n_grps * a.c.kv, grid = (units + 7) / 8 * 8 * tiles;
+  const int64_t units = paged_product({a.b.n_seq, a.n_grps, a.c.kv}), grid = paged_product({(units + 7) / 8 * 8, tiles});
   if (units > INT32_MAX || paged_grid_too_large(grid, 256)) return set_error(SSD_ERANGE, "paged_attention: too many workgroups");
   a.units = (int)units;
   // the second launch's size is checked before the first is enqueued
-  if (paged_grid_too_large((int64_t)a.b.n_seq * (a.b.rows_max * (int64_t)a.heads + (WK ? a.c.kv * (int64_t)(a.l_cap / 256 + 1) : 0)), 256))
+  if (paged_grid_too_large(paged_product({a.b.n_seq, a.b.rows_max * (int64_t)a.heads + (WK ? a.c.kv * (int64_t)(a.l_cap / 256 + 1) : 0)}), 256))
     return set_error(SSD_ERANGE, "paged_attention: too many workgroups");
   SSD_LAUNCH((paged_fold_kernel<HD, WK>), dim3((unsigned)grid), dim3(256), 0, stream, a);
   if (int rc = check_launch("paged_attention_fold")) return rc;
@@ -524,7 +524,7 @@ SSD_API int64_t ssd_paged_attn_ws_floats(int M, int heads, int head_dim, int64_t
   const int64_t pairs = (int64_t)M * heads, recs = paged_groups(l_max, span) * (int64_t)(head_dim + (weights ? 4 : 2));
   // scores are kept by a call of few pairs a kv head, which one of fewer rows than M may be
   const int64_t scored = weights == 0 ? 0 : weights <= PA_SCORES ? pairs : (int64_t)std::min(M, PA_SCORES) * heads;
-  return std::max(pairs * recs, scored * (recs + paged_score_ld(l_max)));
+  return std::max(paged_product({pairs, recs}), paged_product({scored, recs + paged_score_ld(l_max)}));
 }
 
 SSD_API int ssd_paged_attention_bf16(const SsdPagedKv* cache, const SsdPagedBatch* batch, const uint16_t* q, int64_t ldq, int M,
@@ -545,9 +545,9 @@ SSD_API int ssd_paged_attention_bf16(const SsdPagedKv* cache, const SsdPagedBatc
     return set_error(SSD_EINVAL, "paged_attention: q/out rows must be 16-byte aligned with strides >= heads * head_dim");
   const int rep = heads / cache->kv_heads;
   const int wk = !weights ? 0 : (int64_t)std::min(batch->rows_max, M) * rep <= PA_SCORES ? 1 : 2;
-  const int64_t recs = (int64_t)M * heads * paged_groups(l_max, span);
-  if (((uintptr_t)ws & 15) ||
-      ws_floats < recs * (cache->head_dim + (wk ? 4 : 2)) + (wk == 1 ? (int64_t)M * heads * paged_score_ld(l_max) : 0))
+  const int64_t recs = paged_product({M, heads, paged_groups(l_max, span)});
+  if (((uintptr_t)ws & 15) || ws_floats < paged_product({recs, cache->head_dim + (wk ? 4 : 2)}) +
+                                              (wk == 1 ? paged_product({M, heads, paged_score_ld(l_max)}) : 0))
     return set_error(SSD_EINVAL, "paged_attention: workspace too small or not 16-byte aligned");
   if (weights && (ldw < l_max || ldw_seq < (int64_t)cache->kv_heads * ldw))
     return set_error(SSD_EINVAL, "paged_attention: weights rows of %lld for l_max %d, sequences %lld apart", (long long)ldw, l_max,

@@ -8,6 +8,8 @@
 #pragma once
 #include "common.h"
 
+#include <initializer_list>
+
 namespace ssd {
 
 constexpr int PAGE = 64;
@@ -80,7 +82,15 @@ __device__ __forceinline__ int paged_page(const PagedBatch& b, int s, int p, int
 }
 
 // A launch holds at most 2^32 - 1 threads.
-__host__ inline bool paged_grid_too_large(int64_t workgroups, int threads) { return workgroups * threads > (int64_t)UINT32_MAX; }
+__host__ inline bool paged_grid_too_large(int64_t workgroups, int threads) { return workgroups > (int64_t)UINT32_MAX / threads; }
+
+// Product of sizes, INT64_MAX / 2 if that is less (a sum of two such does not wrap either).
+__host__ inline int64_t paged_product(std::initializer_list<int64_t> sizes) {
+  int64_t p = 1;
+  for (const int64_t n : sizes)
+    if (__builtin_mul_overflow(p, n, &p) || p > INT64_MAX / 2) return n == 0 ? 0 : INT64_MAX / 2;
+  return p;
+}
 
 // Host checks of the descriptors; 0, or the code of the error they set.
 int paged_check(const SsdPagedKv* c, const SsdPagedBatch* b, const char* what);

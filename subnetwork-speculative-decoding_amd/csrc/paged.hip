@@ -127,7 +127,7 @@ static int paged_rows_call(const SsdPagedKv* c, const SsdPagedBatch* b, uint16_t
     return set_error(SSD_EINVAL, "%s: k/v rows must be 16-byte aligned with strides >= kv_heads * head_dim", what);
   PagedRowArgs a{paged_batch(b), PagedCache{c->k, c->v, c->pages, c->kv_heads}, k, v, ldk, ldv, M, 0};
   a.page_sets = (int)(((int64_t)std::min(b->rows_max, M) + 62) / 64 + 1);
-  const int64_t wgs = (int64_t)b->n_seq * a.page_sets * c->kv_heads;
+  const int64_t wgs = paged_product({b->n_seq, a.page_sets, c->kv_heads});
   if (paged_grid_too_large(wgs, 256)) return set_error(SSD_ERANGE, "%s: too many workgroups", what);
   const dim3 grid((unsigned)wgs), block(256);
   if (write) {
@@ -364,7 +364,7 @@ SSD_API int ssd_paged_evict(const SsdPagedKv* cache, int layers, int64_t layer_e
   if (int rc = paged_check(cache, after, "paged_evict")) return rc;
   if (!weights || !out_weights || !kept) return set_error(SSD_EINVAL, "paged_evict: null pointer");
   if (after->n_seq != batch->n_seq) return set_error(SSD_EINVAL, "paged_evict: %d sequences become %d", batch->n_seq, after->n_seq);
-  const int64_t one = (int64_t)cache->pages * cache->kv_heads * PAGE * cache->head_dim;
+  const int64_t one = paged_product({cache->pages, cache->kv_heads, PAGE, cache->head_dim});
   if (layers < 1 || layer_elems < one) return set_error(SSD_EINVAL, "paged_evict: bad layers=%d layer_elems=%lld", layers, (long long)layer_elems);
   if (cap < 1 || ldw < cap) return set_error(SSD_EINVAL, "paged_evict: bad cap=%d ldw=%lld", cap, (long long)ldw);
   if (keep < 1 || recent < 0 || first < 0 || (int64_t)recent + first > keep)
@@ -378,10 +378,10 @@ SSD_API int ssd_paged_evict(const SsdPagedKv* cache, int layers, int64_t layer_e
   a.layer_elems = (size_t)layer_elems, a.w = weights, a.ldw = ldw, a.w_out = out_weights, a.cap = cap;
   a.keep = keep, a.recent = recent, a.first = first, a.layers = layers, a.kept = kept, a.new_len = after->lengths;
   a.dst_pages = (keep + PAGE - 1) / PAGE;
-  const int64_t rows = (int64_t)layers * batch->n_seq * cache->kv_heads;
-  if (paged_grid_too_large(rows, EV_T) || paged_grid_too_large(rows * a.dst_pages, 256))
+  const int64_t rows = paged_product({layers, batch->n_seq, cache->kv_heads});
+  if (paged_grid_too_large(rows, EV_T) || paged_grid_too_large(paged_product({rows, a.dst_pages}), 256))
     return set_error(SSD_ERANGE, "paged_evict: too many workgroups");
-  const int64_t reach = 4 * (((int64_t)layers * batch->n_seq * cache->kv_heads - 1) * ldw + cap);  // bytes from the first row to the last's end
+  const int64_t reach = paged_product({4, paged_product({rows - 1, ldw}) + cap});  // bytes from the first row to the last's end
   if (std::abs((intptr_t)weights - (intptr_t)out_weights) < reach)
     return set_error(SSD_EINVAL, "paged_evict: out_weights must not overlap weights");
   SSD_LAUNCH(evict_select_kernel, dim3((unsigned)rows), dim3(EV_T), 0, stream, a);

@@ -370,7 +370,7 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedPromptArgs a)
 static int64_t prompt_tiles(int64_t M, int rep, int n_seq, int rows_max, int kv) {
   constexpr int CW = 32 * PP_WAVES;
   const int64_t most = (std::min<int64_t>(rows_max, M) * rep + CW - 1) / CW;
-  return std::min(M * rep / CW + n_seq, n_seq * most) * kv;
+  return paged_product({std::min(M * rep / CW + n_seq, n_seq * most), kv});
 }
 
 // Parts of the length: one while the tiles fill the chip's 256 CUs, else as many as bring two workgroups a CU, of eight blocks or more

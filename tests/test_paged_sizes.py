@@ -48,3 +48,22 @@ def test_attention_workspaces_hold_scores_where_they_are_kept():
     sizes = [floats(m, 64) for m in range(1, 97)]
     assert sizes == sorted(sizes)  # enough for fewer rows, whose call may keep its scores
     assert sizes[3] >= floats(4, 16)
+
+
+def test_launches_whose_size_passes_64_bits_are_refused():
+    from test_paged import BAD, RANGE, A, _batch, _kv, _refused
+
+    most, ld = (1 << 31) - 1, 1 << 40
+    wide = _batch(n_seq=1 << 30, rows_max=300, table_cols=1 << 24, ld_table=1 << 24)
+    for kv in (1 << 30, most):
+        c = _kv(kv_heads=kv)
+        _refused("ssd_paged_write_bf16", (c, wide, A, ld, A, ld, most, None), RANGE, "workgroups")
+        _refused("ssd_paged_read_bf16", (c, wide, most, A, ld, A, ld, None), RANGE, "workgroups")
+        args = (A, ld, 1, kv, 1 << 30, 64, 0.1, A, (1 << 63) - 1, None, 0, 0, 1.0, A, ld, None)
+        _refused("ssd_paged_attention_bf16", (c, wide, *args), RANGE, "workgroups")
+        for layers in (1 << 20, 1 << 30):
+            args = (A, most, most, 1 << 30, 1, 1, A + 4096, A, None)
+            _refused("ssd_paged_evict", (c, layers, (1 << 63) - 1, wide, wide, *args), RANGE, "workgroups")
+    # 2^20 rows of 2^15 heads in 2^22 groups: floats past 64 bits
+    args = (A, ld, 1 << 20, 1 << 15, 1 << 30, 64, 0.1, A, 1 << 40, None, 0, 0, 1.0, A, ld, None)
+    _refused("ssd_paged_attention_bf16", (_kv(head_dim=128), wide, *args), BAD, "workspace")
