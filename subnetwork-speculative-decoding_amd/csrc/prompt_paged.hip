@@ -12,11 +12,11 @@
 // wave issues, whatever its size, so half as many of twice the work leave it more (a wave of products beside one of multiply-adds:
 // 406 ns against 345 for the same work). While a block's scores become probabilities and meet V, the next block's scores are
 // under way; the blocks that some columns attend only part of, one or two a tile, follow without that.
-// What bounds it, 32 heads on 8 kv heads of 128 (8b shapes): a prompt of 16384 rows 1.89 ms, 1160 TFLOP/s, where a large library product reaches
-// 1300: matrix pipe and vector pipe, each about half of a block's 1.9 us for two workgroups a CU, at the clock that the power leaves.
+// What bounds it, 32 heads on 8 kv heads of 128 (8b shapes): a prompt of 16384 rows 1.94 ms, 1130 TFLOP/s, where a large library product reaches
+// 1280: matrix pipe and vector pipe, each about half of a block's 1.9 us for two workgroups a CU, at the clock that the power leaves.
 // Shorter prompts: a tile's beginning and end, about 8 us (rows, pages, first copies; the partly attended blocks; the output), of
-// which a second workgroup on the CU hides half, and the last tiles' end: 4096 rows 131 us (1050 TFLOP/s), 16 prompts of 232 to 1500 rows
-// 132; on a slower card 7 % more.
+// which a second workgroup on the CU hides half, and the last tiles' end: 4096 rows 134 us when a graph repeats the call, 143 among
+// passes with their write (960 TFLOP/s), 16 prompts of up to 1500 rows 155 and 164.
 // Tried (us of 16 prompts with the write of their K and V, 191 on that card): tiles dealt to resident workgroups, the next one's first
 // blocks copied before the output 202; the longest tiles of all sequences first 192. Eight waves a workgroup: a prompt of 4096 rows 138 against 147, of 2048 60 against 50,
 // 16 prompts 170 against 160. 64 columns a wave with twice the registers: 4096 rows 269 for 157; two groups of waves that take
@@ -378,12 +378,16 @@ static int64_t prompt_tiles(int64_t M, int rep, int n_seq, int rows_max, int kv)
 // rows of 32 heads after 8000 keys 151 / 120). Two parts pay for their records only over a long length (4 times 100 rows of 64 heads after
 // 4000 keys 77 / 83; 700 rows of 32 heads after 6500 126 / 116, 900 after 16000 286 / 262), and not where sequences of one tile read K and V
 // once, which is bound by bytes (24 of 32 rows after 8000 168 / 169, 31 192 / 213).
+// Where eight blocks a part leave the CUs' second places part empty, one workgroup a CU is better (192 rows after 4000 in 7 / 5 parts 34 / 30,
+// 320 after 2000 in 4 / 3 34 / 30, six sequences of 32 rows after 4000 in 7 / 5 34 / 32).
 // The fewer rows the longest sequence can have, the fewer tiles and the more parts: rows_max 0 asks for the most.
 static int prompt_splits(int64_t M, int rep, int n_seq, int rows_max, int kv, int64_t l_max) {
   const int64_t longest = std::max<int64_t>(rows_max, (M + n_seq - 1) / std::max(n_seq, 1));
   const int64_t wgs = prompt_tiles(M, rep, n_seq, (int)longest, kv), blocks = (l_max + PAGE - 1) / PAGE;
   if (wgs >= 256) return 1;
-  const int64_t n = std::max<int64_t>(1, std::min(512 / std::max<int64_t>(wgs, 1), blocks / 8));
+  int64_t n = std::max<int64_t>(1, std::min(512 / std::max<int64_t>(wgs, 1), blocks / 8));
+  const int64_t round = 256 / std::max<int64_t>(wgs, 1);
+  if (rows_max && round >= 2 && wgs * n > 256 && wgs * n < 435 && wgs * round >= 205) n = round;
   return n == 2 && (blocks < 96 || (rows_max && longest * rep <= 32 * PP_WAVES)) ? 1 : (int)n;
 }
 
