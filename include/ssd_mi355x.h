@@ -308,7 +308,7 @@ int ssd_paged_read_bf16(const SsdPagedKv* cache, const SsdPagedBatch* batch, int
 /* Attention of the batch's rows q [M][heads * head_dim]: row i of a sequence attends slots [0, lengths - n + i], itself the
  * last (the causal mask of ssd/models/subnetwork_draft.py:165-191 for a chunk behind a cache). Zeros for rows that attend
  * nothing, or scores of -inf alone. l_max (1 .. 64 * table_cols): slots from there on are not attended. heads / kv_heads any
- * whole ratio; scale > 0. A V value that is not finite makes the outputs of the rows that attend its slot NaN or infinite, and
+ * whole ratio; scale > 0. out is not q. A V value that is not finite makes the outputs of the rows that attend its slot NaN or infinite, and
  * no other's.
  *
  * ssd_paged_attention_bf16 is for few rows a sequence: the length is cut into groups of 4 * span slots (span a multiple of 64 up
@@ -335,7 +335,8 @@ int ssd_paged_prompt_bf16(const SsdPagedKv* cache, const SsdPagedBatch* batch, c
  * with more than `keep` slots stay the first `first`, the last `recent`, and of those between as many as complete
  * `keep`, those of the largest weight (equal ones: the lowest slots; NaN below every number); of shorter ones all. They move, in their
  * order, to slots 0, 1, ... of the pages in after->table, which must be pages that `batch` does not use, and
- * after->lengths becomes min(lengths, keep) (it may be batch->lengths itself). weights: [layers][n_seq][kv_heads] rows of cap
+ * after->lengths becomes min(lengths, keep) (it may be batch->lengths itself). What stays keeps the rotation of the position that it was written
+ * at: from here on a slot is not a position. weights: [layers][n_seq][kv_heads] rows of cap
  * floats, ldw apart, cap >= lengths (slots beyond it count as not there); out_weights, rows alike and elsewhere: the kept
  * ones, then zeros. kept: [layers][n_seq][kv_heads][keep] int32, the slots they came from, then -1. keep may be more than cap, and is at
  * most 64 * after->table_cols. The row_begin and rows_max of both batches are not used. No counterpart in the reference, whose caches only grow. */

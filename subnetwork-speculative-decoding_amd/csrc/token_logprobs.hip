@@ -7,9 +7,9 @@
 // largest of them; only the few threads whose maximum reaches that bound look at their columns again (from registers, or a wave
 // together), what reaches it is collected, and a value's place is the number of those above it. Equal values rank by column, lowest
 // first. More candidates than the list holds (rows of equal logits) take a pass over the chunk for each place.
-// What bounds it: bytes and the vector pipe (about 14 operations a column): 1800 rows of 50257 fp32 columns 66 us, 5.4 TB/s; 1400
-// of 128256 bf16 columns 80 without alternatives, 4.5 TB/s, and 83 with 5. For few rows the latency of two launches and their
-// steps: 25 rows of 128256 bf16 columns 6.9 us without alternatives, 13.5 with 5.
+// What bounds it: bytes and the vector pipe (about 14 operations a column): 1800 rows of 50257 fp32 columns 68 us, 5.3 TB/s; 1400
+// of 128256 bf16 columns 77 without alternatives, 4.7 TB/s, and 87 with 5. For few rows the latency of two launches and their
+// steps: 25 rows of 128256 bf16 columns 6.7 us without alternatives, 13.3 with 5.
 #include "topk.h"
 
 #include <algorithm>

@@ -734,7 +734,7 @@ def paged_attn_ws_floats(m: int, heads: int, head_dim: int, l_max: int, span: in
 
 def paged_attention(cache, batch, q, heads, l_max, span, ws=None, out=None, scale=None, weights=None, decay=1.0):
     """Attention of few rows a sequence over the pages (ssd_paged_attention_bf16). ``weights``: fp32 [n_seq, kv_heads, >= l_max],
-    updated in place. ``ws`` (fp32, paged_attn_ws_floats(...)) and ``out`` are made here if None."""
+    updated in place. ``ws`` (fp32, paged_attn_ws_floats(...)) and ``out`` (rows of no sequence unset) are made here if None."""
     dev, hd, m = _batch_dev(cache, batch), cache.head_dim, q.shape[0]
     cols = heads * hd
     pq, ldq = _rows_ptr(q, "q", dev, m, cols)
@@ -774,7 +774,7 @@ def paged_prompt_ws_floats(m: int, heads: int, kv_heads: int, head_dim: int, n_s
 
 def paged_prompt(cache, batch, q, heads, l_max, ws=None, out=None, scale=None):
     """Causal attention of many rows a sequence over the pages (ssd_paged_prompt_bf16). ``ws`` (fp32, paged_prompt_ws_floats(...)) and
-    ``out`` are made here if None."""
+    ``out`` (rows of no sequence unset) are made here if None."""
     dev, hd, m = _batch_dev(cache, batch), cache.head_dim, q.shape[0]
     cols = heads * hd
     pq, ldq = _rows_ptr(q, "q", dev, m, cols)
