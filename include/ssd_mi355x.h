@@ -308,7 +308,7 @@ int ssd_paged_read_bf16(const SsdPagedKv* cache, const SsdPagedBatch* batch, int
 /* Attention of the batch's rows q [M][heads * head_dim]: row i of a sequence attends slots [0, lengths - n + i], itself the
  * last (the causal mask of ssd/models/subnetwork_draft.py:165-191 for a chunk behind a cache). Zeros for rows that attend
  * nothing, or scores of -inf alone. l_max (1 .. 64 * table_cols): slots from there on are not attended. heads / kv_heads any
- * whole ratio; scale > 0. out is not q. A V value that is not finite makes the outputs of the rows that attend its slot NaN or infinite, and
+ * whole ratio; scale > 0. out may be q, but not in a call with weights of more than 16 (row, query head) pairs a kv head. A V value that is not finite makes the outputs of the rows that attend its slot NaN or infinite, and
  * no other's.
  *
  * ssd_paged_attention_bf16 is for few rows a sequence: the length is cut into groups of 4 * span slots (span a multiple of 64 up

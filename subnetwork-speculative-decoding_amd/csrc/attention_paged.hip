@@ -546,6 +546,8 @@ SSD_API int ssd_paged_attention_bf16(const SsdPagedKv* cache, const SsdPagedBatc
     return set_error(SSD_EINVAL, "paged_attention: q/out rows must be 16-byte aligned with strides >= heads * head_dim");
   const int rep = heads / cache->kv_heads;
   const int wk = !weights ? 0 : (int64_t)std::min(batch->rows_max, M) * rep <= PA_SCORES ? 1 : 2;
+  if (wk == 2 && q == out)  // the second launch reads q while it writes out
+    return set_error(SSD_EINVAL, "paged_attention: out must not be q where weights are made from it (more than %d pairs a kv head)", PA_SCORES);
   const int64_t recs = paged_product({M, heads, paged_groups(l_max, span)});
   if (((uintptr_t)ws & 15) || ws_floats < paged_product({recs, cache->head_dim + (wk ? 4 : 2)}) +
                                               (wk == 1 ? paged_product({M, heads, paged_score_ld(l_max)}) : 0))

@@ -354,7 +354,8 @@ class PagedKVCache:
         table's capacity) bounds the lengths: slots from there on are not attended, and a close bound saves empty
         workgroups. ``weights`` fp32 [S, kv_heads, >= l_max]: decay * weights + the softmax weights each slot in use received from the
         call's rows, summed over rows and a kv head's query heads (decay 0: set); sequences without rows keep theirs. ``ws``: fp32, attend_floats(...).
-        Rows of no sequence, and those past ``rows_max``, are left as they were; in an ``out`` made here they are unset. ``out`` is not ``q``."""
+        Rows of no sequence, and those past ``rows_max``, are left as they were; in an ``out`` made here they are unset. ``out`` may be ``q``, but not with
+        weights of more than 16 (row, query head) pairs a kv head."""
         return ops.paged_attention(self._layers[i], batch, q, self._heads(q), l_max, self._span(batch), ws, out, scale, weights, decay)
 
     def prompt_floats(self, m: int, heads: int, batch: PagedBatch, l_max: Optional[int] = None) -> int:
@@ -367,7 +368,7 @@ class PagedKVCache:
         64 (row, query head) pairs a kv head on it is the faster one (us of attend / attend_prompt, 4 heads a kv head: 6 sequences of 8 rows
         after 2500 to 4000 keys 24 / 27, of 16 rows 33 / 29, of 32 rows 49 / 32; 24 of 16 rows after 2000 keys 62 / 41; one of 16 rows after
         4000 12 / 19). Each softmax weight is rounded to one bf16 number here, to two in ``attend``: error of the output 0.0018 and 0.0017 of its
-        norm. ``ws``: fp32, prompt_floats(...). Rows of no sequence and ``out`` as in ``attend``."""
+        norm. ``ws``: fp32, prompt_floats(...). Rows of no sequence as in ``attend``; ``out`` may be ``q``."""
         return ops.paged_prompt(self._layers[i], batch, q, self._heads(q), l_max, ws, out, scale)
 
     def evict(self, batch: PagedBatch, after: PagedBatch, weights: torch.Tensor, keep: int, recent: int = 0, first: int = 0,

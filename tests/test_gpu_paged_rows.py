@@ -89,3 +89,19 @@ def test_prompt_rows_of_no_sequence_and_a_tight_bound():
     s.cache.attend_prompt(0, q, b, out=out, ws=ws)
     s.check(out[100:151])
     assert (out[:100] == 7).all() and (out[151:] == 7).all()
+
+
+# ------------------------------------------------------------------------------------------------- the output in q's place
+@pytest.mark.parametrize("lens,rows", [([70, 500], [1, 2]), ([3000], [1]), ([200, 90, 64], [150, 90, 3]), ([5000], [20])])
+def test_outputs_may_take_the_place_of_q(lens, rows):
+    s = Setup(lens, rows, 8, 2, 128, seed=46, span=64).fill()
+    for f in (s.cache.attend, s.cache.attend_prompt):
+        q = s.q.cuda()
+        want = f(0, q, s.batch)
+        f(0, q, s.batch, out=q)
+        assert torch.equal(q, want)
+    if max(rows) * 4 <= 16:  # scores that are kept
+        q, w = s.q.cuda(), torch.zeros(2, len(lens), 2, s.batch.capacity, device="cuda")
+        want = s.cache.attend(0, q, s.batch, weights=w[0])
+        s.cache.attend(0, q, s.batch, weights=w[1], out=q)
+        assert torch.equal(q, want) and torch.equal(w[0], w[1])

@@ -67,3 +67,10 @@ def test_launches_whose_size_passes_64_bits_are_refused():
     # 2^20 rows of 2^15 heads in 2^22 groups: floats past 64 bits
     args = (A, ld, 1 << 20, 1 << 15, 1 << 30, 64, 0.1, A, 1 << 40, None, 0, 0, 1.0, A, ld, None)
     _refused("ssd_paged_attention_bf16", (_kv(head_dim=128), wide, *args), BAD, "workspace")
+
+
+def test_weights_that_are_made_from_q_again_refuse_it_as_the_output():
+    from test_paged import BAD, A, _batch, _kv, _refused
+
+    args = (A, 256, 20, 4, 64, 64, 0.1, A, 1 << 20, A, 128, 64, 1.0, A, 256, None)
+    _refused("ssd_paged_attention_bf16", (_kv(), _batch(rows_max=9), *args), BAD, "out must not be q")  # 18 pairs of a kv head
