@@ -17,9 +17,9 @@
 // What bounds it: bytes of K and V, each read once where a kv head's pairs are one tile. A wave has one block's K and V in
 // registers and loads the next block's as soon as a product has used the present one's, 32 KB in flight; with 245 registers that
 // is two workgroups a CU. 32 heads on 8 kv heads of 128, us of both launches: 32 sequences of one row and up to 8192 keys
-// 142 (5.2 TB/s), one row after 131000 keys 97 (5.5), 24 sequences of up to 4000 keys with weights 38 with K and V in the caches (32 + 6; 49 from
-// memory); 6 sequences of 16 rows and 1200 to 4001 keys, four tiles that share
-// K and V through L2, 25 and 17 for the join and the weights. One row after 500 keys of the smallest shape 4.8: latency.
+// 142 (5.2 TB/s), one row after 131000 keys 97 (5.5); 24 sequences of up to 4000 keys with weights, 15 heads on 5, 38 with K and V in
+// the caches (32 + 6), 49 from memory; 6 sequences of 16 rows and 1200 to 4001 keys, four tiles that share K and V through L2, 26 and
+// 17 for the join and the weights. One row after 500 keys of the smallest shape 4.8: latency.
 // Tried: two tiles a workgroup, whose registers leave one workgroup a CU (6 sequences of 16 rows 29 us against 25, 2 of 60 rows and
 // 8000 keys 87 against 76); tiles one after another in a workgroup, K and V on their way for the next while one ends (42 against 41 for
 // two, 50 for three: the tiles' chains are better side by side).
@@ -300,8 +300,8 @@ __device__ __forceinline__ float2 paged_total(const float2* ml, int64_t step, in
 }
 
 // Second launch. Workgroups that add up the records: WPP waves a (sequence, row, head). PA_RUN groups from each multiple of PA_RUN on are
-// added up in order, then these sums in order, by however many waves: the row's bits follow from its own groups. Workgroups that add up received weights, of a set of slots of a (sequence, kv head), in a fixed order too: WK = 1
-// from the kept scores, a lane four slots; WK = 2 from K, a wave a block, sixteen pairs at a time, the lanes' sums last.
+// added up in order, then these sums in order, by however many waves: the row's bits follow from its own groups. Workgroups that add up
+// received weights, of a set of slots of a (sequence, kv head), in a fixed order too: WK = 1 from the kept scores, a lane four slots; WK = 2 from K, a wave a block, sixteen pairs at a time, the lanes' sums last.
 template <int HD, int WK, int WPP>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);

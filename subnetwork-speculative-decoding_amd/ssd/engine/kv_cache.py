@@ -377,7 +377,7 @@ class PagedKVCache:
         [layers, S, kv_heads, >= lengths]: the ``first`` and the ``recent`` last slots stay, and those of the largest weight between
         (equal ones: the lowest). What stays moves to the pages of ``after``, which must not be pages of ``batch``, and
         after.lengths becomes min(lengths, keep); if ``keep`` is more than the sequences have, all stay. A slot is not a position any more: K
-        that stays was rotated to the position it was written at, so later rows are rotated to positions that the caller counts on. Returns (kept [layers, S, kv_heads, keep] int32: the slots it came from, then -1;
-        the weights that moved along, then zeros)."""
+        that stays was rotated to the position it was written at, so later rows are rotated to positions that the caller counts on. Returns
+        (kept [layers, S, kv_heads, keep] int32: the slots it came from, then -1; the weights that moved along, then zeros)."""
         return ops.paged_evict(self._layers[0], self.num_slots, self.k.stride(0), batch, after, weights, keep, recent, first, out_weights,
                                kept)
